@@ -353,4 +353,113 @@ struct CombineArgs {
     int32_t out_dtype;
 };
 
+// ---- MXFP4 (mx_numerics.h) --------------------------------------------------
+
+// Rows into row-major codes [rows][ceil(cols / 2)] and scales [rows][ceil(cols / 32)].
+struct MxQuantizeArgs {
+    const void* x;        // f32 or bf16 [rows][cols]
+    uint8_t* codes;
+    uint8_t* scales;
+    uint64_t* nonfinite;  // or null
+    int64_t units;        // groups of eight values, four per block: 4 * rows * ceil(cols / 32)
+    int64_t rows;
+    uint32_t cols;
+    uint32_t row_units;   // 4 ceil(cols / 32)
+    int32_t x_dtype;
+    int32_t flat;         // 1: cols % 32 == 0, so units follow each other in memory
+};
+
+// Rows into the GEMM's tiled form, or (token) the form that is gathered.
+struct MxQuantizeTilesArgs {
+    const void* x;
+    uint8_t* out;         // regions, or codes of the token form
+    uint8_t* scales;      // token form
+    uint64_t* nonfinite;
+    int64_t rows;
+    int32_t cols;
+    int32_t kt, kq;
+    int32_t x_dtype;
+    int32_t token;
+    int32_t pad_;
+};
+
+struct MxDequantizeArgs {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    void* out;
+    int64_t units;
+    uint32_t cols;
+    uint32_t row_units;
+    int32_t out_dtype;
+    int32_t flat;
+};
+
+struct MxTileArgs {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    uint8_t* tiled;
+    int64_t lanes;        // 64 per (row tile, scale piece of four K tiles)
+    int64_t n;
+    int32_t k, kt, kq;
+    int32_t pad_;
+};
+
+// Weight-streaming products (few rows): see mxfp4_stream.hip.
+struct MxStreamArgs {
+    const void* x;           // f32 or bf16 [M][K] (quantized in the kernel), or null
+    const uint8_t* xcodes;   // token form, when x is null
+    const uint8_t* xscales;
+    const uint8_t* w;        // tiled weights (of expert 0)
+    const float* bias;       // [N] (of expert 0) or null
+    void* out;               // [M][N], or per slot; null where the output is quantized
+    uint8_t* hcodes;         // quantized ReLU^2 output in token form
+    uint8_t* hscales;
+    uint64_t* nonfinite;
+    const int32_t* offsets;  // [experts + 1] or null (one product, M rows)
+    const int32_t* perm;     // [routes] or null: row of slot s is perm[s] / gather_div
+    int32_t M, N, K;         // M: rows of x
+    int32_t kt, kq;
+    int32_t x_dtype, out_dtype;
+    int32_t gather_div;
+    int32_t experts;
+    int32_t compact;         // blockIdx.y counts the experts that have routes
+    int32_t units;           // N tiles (N tile pairs) in all, dealt to gridDim.x workgroups
+    int32_t nonfinite_stage;
+};
+
+// LDS-tiled product of two tiled operands (many rows): see mxfp4_gemm.hip.
+struct MxGemmArgs {
+    const uint8_t* a;        // tiled [M][K]
+    const uint8_t* w;        // tiled [N][K]
+    const float* bias;       // [N] or null
+    void* out;               // [M][N]
+    int32_t M, N;
+    int32_t kt, kq;
+    int32_t tiles_m, tiles_n;
+    int32_t out_dtype;
+    int32_t pad_;
+};
+
+// ---- load balance of the router (moe_balance.hip) ---------------------------
+struct BalanceArgs {
+    const float* logits;        // [T][E]
+    const int32_t* indices;     // [T][k]
+    const int32_t* seq;         // [S + 1] token offsets of the sequences, or null (one of all tokens)
+    int32_t* counts;            // [S][E]
+    float* loss;                // [1]
+    const float* dloss;         // [1]
+    float* dlogits;             // [T][E]
+    // workspace: per chunk of a sequence's tokens, in sequence order
+    float* part_p;              // [chunks][E] sums of p
+    int32_t* part_n;            // [chunks][E] routes
+    double* seq_loss;           // [S]
+    uint32_t* arrived;          // [1]
+    int32_t tokens, experts, top_k, sequences;
+    int32_t chunk, chunks;      // tokens per chunk, chunks that the workspace holds
+    int32_t softmax;
+    float coefficient;
+    int32_t group;              // lanes per token: a power of two, 4 experts per lane and turn
+    int32_t pad_;
+};
+
 }  // namespace nh

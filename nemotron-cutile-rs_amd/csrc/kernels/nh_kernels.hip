@@ -7,3 +7,7 @@
 #include "moe.hip"
 #include "gemm_persistent.hip"
 #include "gemm_direct.hip"
+#include "mxfp4_quantize.hip"
+#include "mxfp4_stream.hip"
+#include "mxfp4_gemm.hip"
+#include "moe_balance.hip"

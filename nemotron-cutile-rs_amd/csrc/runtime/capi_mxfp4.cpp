@@ -1,0 +1,423 @@
+// Device entry points of the MXFP4 operators: validate on the host, then enqueue.
+#include <algorithm>
+#include <cstdint>
+
+#include "../kernels/mx_numerics.h"
+#include "nh_runtime.h"
+
+using namespace nh;
+
+namespace {
+
+// Rows that one launch takes straight from x: the kernel quantizes 16.
+constexpr size_t kMxRowsMax = 16;
+constexpr size_t kMxRowsMaxK = 16384;
+
+// K tiles that each of at most eight waves owns: 1, 2, 4, 8, 16 (index 0..4).
+int mx_split(int kt) { return kt <= 8 ? 0 : kt <= 16 ? 1 : kt <= 32 ? 2 : kt <= 64 ? 3 : 4; }
+
+// A row of `cols` values in `rows`: what the conversions address.
+nh_status check_mx_rows(size_t rows, size_t cols, nh_error* err) {
+    size_t t;
+    if (!mul_ok(rows, cols, &t) || t >= (1ull << 48)) return set_error(err, NH_INVALID_SHAPE, "rows * cols overflows");
+    // a workgroup takes 1024 groups of eight values
+    if (rows > (size_t)kMaxGrid || cols > (size_t)kMaxGrid - 64 ||
+        (rows * mx_row_blocks(cols) * 4 + 1023) / 1024 > (size_t)kMaxGrid)
+        return set_error(err, NH_UNSUPPORTED, "rows and cols must be < 2^31 and their product < 2^44");
+    return NH_OK;
+}
+
+unsigned mx_unit_grid(int64_t units) { return (unsigned)((units + 1023) / 1024); }
+
+// The few-row product: fills the launch shape into `a` and launches kernel ids
+// first + split (16 rows at a time) or wide + split.
+nh_status launch_mx_stream(nh_context* ctx, KernelId first, KernelId wide, MxStreamArgs a, size_t rows, bool requant,
+                           unsigned workgroups, unsigned experts, nh_stream stream, nh_error* err) {
+    const int split = mx_split(a.kt), c = 1 << split;
+    const bool w = wide != K_COUNT && rows > 16;
+    const int rb = !w ? 1 : split == 3 ? 2 : 4, t = requant ? 2 : 1, waves = (a.kt + c - 1) / c;
+    // h's units cover its whole K tiles: their blocks past N are written as zeros
+    a.units = requant ? 4 * (int)mx_k_tiles((uint64_t)a.N) : (a.N + 15) / 16;
+    // a run's bias lies in LDS: at most 16 KiB
+    const unsigned least = (unsigned)((a.units + 255 / t) / (256 / t));
+    const unsigned gx = std::max(1u, std::min((unsigned)a.units, std::max(workgroups, least)));
+    const size_t run = (size_t)(a.units + gx - 1) / gx;
+    const size_t lds = (size_t)2 * t * rb * waves * 1024 + (a.bias ? run * t * 16 * 4 : 0);
+    return launch(ctx, (KernelId)((w ? wide : first) + split), gx, 64u * waves, lds, stream, a, err, experts);
+}
+
+nh_status launch_mx_tiles(nh_context* ctx, const void* x, nh_dtype dtype, size_t rows, size_t k, uint8_t* out,
+                          uint8_t* token_scales, uint64_t* nonfinite, nh_stream stream, nh_error* err) {
+    MxQuantizeTilesArgs q{x, out, token_scales, nonfinite, (int64_t)rows, (int32_t)k, (int)mx_k_tiles(k),
+                          (int)mx_k_pieces(k), dtype, token_scales ? 1 : 0, 0};
+    return launch(ctx, K_MX_QUANTIZE_TILES, (unsigned)((rows + 15) / 16 * q.kq), 256, 0, stream, q, err);
+}
+
+nh_status launch_mx_gemm(nh_context* ctx, const uint8_t* a, const uint8_t* w, const float* bias, size_t m, size_t n,
+                         size_t k, void* out, nh_dtype out_dtype, nh_stream stream, nh_error* err) {
+    struct Tile {
+        KernelId id;
+        int b, threads, stages, per_cu;
+    };
+    static const Tile kTiles[] = {{K_MX_GEMM_256, 256, 512, 2, 1}, {K_MX_GEMM_128, 128, 256, 2, 2}, {K_MX_GEMM_64, 64, 256, 4, 2}};
+    const size_t cus = (size_t)ctx->cu_count;
+    const Tile* t = &kTiles[2];
+    for (const Tile& c : kTiles)
+        if (((m + c.b - 1) / c.b) * ((n + c.b - 1) / c.b) >= cus) {
+            t = &c;
+            break;
+        }
+    MxGemmArgs g{a, w, bias, out, (int)m, (int)n, (int)mx_k_tiles(k), (int)mx_k_pieces(k), (int)((m + t->b - 1) / t->b),
+                 (int)((n + t->b - 1) / t->b), out_dtype, 0};
+    const size_t tiles = (size_t)g.tiles_m * g.tiles_n, row_tiles = (size_t)2 * t->b / 16;
+    const size_t lds = (size_t)t->stages * (2 * row_tiles * 1024 + row_tiles * 256) + 1024;
+    const unsigned grid = (unsigned)std::min(tiles, cus * t->per_cu);
+    return launch(ctx, t->id, grid, (unsigned)t->threads, lds, stream, g, err);
+}
+
+}  // namespace
+
+extern "C" {
+
+nh_status nh_quantize_rows_mxfp4(nh_context* ctx, const void* x, nh_dtype dtype, size_t rows, size_t cols,
+                                 uint8_t* codes, uint8_t* scales, uint64_t* nonfinite, nh_stream stream, nh_error* err) {
+    clear_error(err);
+    nh_status st;
+    if ((st = check_dtype(dtype, err)) || (st = check_mx_rows(rows, cols, err))) return st;
+    if ((st = bind_device(ctx, err))) return st;
+    if (rows == 0 || cols == 0) return NH_OK;
+    const int64_t row_units = (int64_t)mx_row_blocks(cols) * 4, units = (int64_t)rows * row_units;
+    MxQuantizeArgs a{x, codes, scales, nonfinite, units, (int64_t)rows, (uint32_t)cols, (uint32_t)row_units, dtype,
+                     cols % kMxBlock == 0 ? 1 : 0};
+    return launch(ctx, K_MX_QUANTIZE, mx_unit_grid(units), 256, 0, stream, a, err);
+}
+
+nh_status nh_dequantize_mxfp4(nh_context* ctx, const uint8_t* codes, const uint8_t* scales, size_t rows, size_t cols,
+                              void* out, nh_dtype out_dtype, nh_stream stream, nh_error* err) {
+    clear_error(err);
+    nh_status st;
+    if ((st = check_dtype(out_dtype, err)) || (st = check_mx_rows(rows, cols, err))) return st;
+    if ((st = bind_device(ctx, err))) return st;
+    if (rows == 0 || cols == 0) return NH_OK;
+    const int64_t row_units = (int64_t)mx_row_blocks(cols) * 4, units = (int64_t)rows * row_units;
+    MxDequantizeArgs a{codes, scales, out, units, (uint32_t)cols, (uint32_t)row_units, out_dtype,
+                       cols % kMxBlock == 0 ? 1 : 0};
+    return launch(ctx, K_MX_DEQUANTIZE, mx_unit_grid(units), 256, 0, stream, a, err);
+}
+
+size_t nh_tiled_mxfp4_weights_bytes(size_t n, size_t k) {
+    if (n == 0 || k == 0 || n > (1ull << 40) || k > (1ull << 40) || (n >> 20) * (k >> 20) >= (1ull << 20)) return 0;
+    return (size_t)mx_tiled_bytes(n, k);
+}
+
+nh_status nh_tile_weights_mxfp4(nh_context* ctx, const uint8_t* codes, const uint8_t* scales, size_t n, size_t k,
+                                uint8_t* tiled, size_t tiled_len, nh_stream stream, nh_error* err) {
+    clear_error(err);
+    const size_t need = nh_tiled_mxfp4_weights_bytes(n, k);
+    if (need == 0) return set_error(err, NH_INVALID_SHAPE, "invalid weight shape n=%zu k=%zu", n, k);
+    if (n >= (1u << 31) || k > (size_t)kMaxGrid - 128) return set_error(err, NH_UNSUPPORTED, "n and k must be < 2^31");
+    if (tiled_len != need) return mismatch(err, "tiled", need, tiled_len);
+    if (!aligned16(tiled)) return set_error(err, NH_UNSUPPORTED, "tiled must be 16-byte aligned");
+    nh_status st = bind_device(ctx, err);
+    if (st) return st;
+    const int kq = (int)mx_k_pieces(k);
+    MxTileArgs a{codes, scales, tiled, (int64_t)((n + 15) / 16) * kq * 64, (int64_t)n, (int32_t)k, (int)mx_k_tiles(k), kq, 0};
+    const int64_t grid = std::min<int64_t>((a.lanes + 255) / 256, 1 << 20);
+    return launch(ctx, K_MX_TILE, (unsigned)grid, 256, 0, stream, a, err);
+}
+
+int nh_supports_linear_mxfp4(size_t m, size_t n, size_t k) {
+    // K up to 2^17 keeps 16 row tiles of codes and scales within a 32-bit
+    // buffer offset, m n below 2^40 the output tiles and their stages within 31 bits
+    return m > 0 && n > 0 && k > 0 && m < (1u << 24) && n < (1u << 28) && k <= (1u << 17) &&
+           (uint64_t)m * n < (1ull << 40) && (uint64_t)m * k < (1ull << 38);
+}
+
+size_t nh_linear_mxfp4_workspace_size(size_t m, size_t n, size_t k) {
+    if (!nh_supports_linear_mxfp4(m, n, k)) return 0;
+    if (m <= kMxRowsMax && k <= kMxRowsMaxK) return 0;
+    return align256((size_t)mx_tiled_bytes(m, k));  // the token form of the rows is no larger
+}
+
+nh_status nh_linear_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, const uint8_t* w, const float* bias,
+                          size_t m, size_t n, size_t k, void* out, nh_dtype out_dtype, void* workspace,
+                          size_t workspace_bytes, uint64_t* nonfinite, nh_stream stream, nh_error* err) {
+    clear_error(err);
+    if (n == 0 || k == 0) return set_error(err, NH_INVALID_SHAPE, "invalid linear shape k=%zu n=%zu", k, n);
+    if (m == 0) return set_error(err, NH_INVALID_ROW_COUNT, "row_count must be non-zero, got 0");
+    nh_status st;
+    if ((st = check_dtype(x_dtype, err)) || (st = check_dtype(out_dtype, err))) return st;
+    if (!nh_supports_linear_mxfp4(m, n, k))
+        return set_error(err, NH_UNSUPPORTED, "shape m=%zu n=%zu k=%zu outside the gfx950 envelope (k <= 131072, "
+                         "m < 2^24, n < 2^28, m * n < 2^40)", m, n, k);
+    if (!aligned16(w)) return set_error(err, NH_UNSUPPORTED, "w must be 16-byte aligned");
+    const size_t need = nh_linear_mxfp4_workspace_size(m, n, k);
+    if (need && (!workspace || workspace_bytes < need)) return mismatch(err, "workspace", need, workspace_bytes);
+    if (need && !aligned16(workspace)) return set_error(err, NH_UNSUPPORTED, "workspace must be 16-byte aligned");
+    // the one-launch form stores outputs while other workgroups still read x
+    if (overlap(out, m * n * (out_dtype == NH_BF16 ? 2 : 4), x, m * k * (x_dtype == NH_BF16 ? 2 : 4)))
+        return set_error(err, NH_INVALID_PARAMS, "out must not overlap x");
+    if ((st = bind_device(ctx, err))) return st;
+    MxStreamArgs a{};
+    a.w = w;
+    a.bias = bias;
+    a.out = out;
+    a.M = (int)m;
+    a.N = (int)n;
+    a.K = (int)k;
+    a.kt = (int)mx_k_tiles(k);
+    a.kq = (int)mx_k_pieces(k);
+    a.x_dtype = x_dtype;
+    a.out_dtype = out_dtype;
+    a.gather_div = 1;
+    const unsigned cus = (unsigned)ctx->cu_count;
+    if (need == 0) {
+        a.x = x;
+        a.nonfinite = nonfinite;
+        return launch_mx_stream(ctx, K_MX_ROWS1, K_COUNT, a, m, false, cus, 1, stream, err);
+    }
+    uint8_t* ws = (uint8_t*)workspace;
+    if (m <= 64 && k <= 8192) {
+        uint8_t* scales = ws + m * mx_token_codes(k);
+        if ((st = launch_mx_tiles(ctx, x, x_dtype, m, k, ws, scales, nonfinite, stream, err))) return st;
+        a.xcodes = ws;
+        a.xscales = scales;
+        return launch_mx_stream(ctx, K_MX_TOK1, K_MX_TOK1_WIDE, a, m, false, cus, 1, stream, err);
+    }
+    if ((st = launch_mx_tiles(ctx, x, x_dtype, m, k, ws, nullptr, nonfinite, stream, err))) return st;
+    return launch_mx_gemm(ctx, ws, w, bias, m, n, k, out, out_dtype, stream, err);
+}
+
+}  // extern "C"
+
+// Workspace of the MoE layer, 256-byte aligned fields; false: sizes overflow.
+static bool mx_moe_layout(size_t T, size_t H, size_t I, size_t E, size_t k, size_t off[11]) {
+    size_t R, t;
+    if (T == 0 || H == 0 || I == 0 || E == 0 || k == 0 || !mul_ok(T, k, &R) || R >= (1ull << 31) || H > (1u << 24) ||
+        I > (1u << 24) || E > (1u << 24) || !mul_ok(R * 4, std::max(H, I), &t) || t >= (1ull << 60))
+        return false;
+    size_t cur = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = cur;
+        cur += align256(bytes);
+        return o;
+    };
+    off[0] = take(R * 4);                        // indices
+    off[1] = take(R * 4);                        // weights
+    off[2] = take((E + 1) * 4);                  // offsets
+    off[3] = take(R * 4);                        // perm
+    off[4] = take(R * 4);                        // pos
+    off[5] = take(T * mx_token_codes(H));        // x in MXFP4, token form
+    off[6] = take(T * mx_token_scales(H));
+    off[7] = take(R * mx_token_codes(I));        // h in MXFP4, token form by slot
+    off[8] = take(R * mx_token_scales(I));
+    off[9] = take(R * H * 4);                    // down output per slot (f32)
+    off[10] = cur;
+    return true;
+}
+
+extern "C" {
+
+int nh_supports_moe_forward_mxfp4(size_t tokens, size_t hidden, size_t inter, size_t experts, size_t top_k) {
+    size_t off[11];
+    if (!mx_moe_layout(tokens, hidden, inter, experts, top_k, off) || top_k > experts) return 0;
+    return experts <= 1024 && top_k <= 64 && tokens <= (size_t)kMaxGrid / 4 && hidden <= 8192 && inter <= 8192;
+}
+
+size_t nh_moe_forward_mxfp4_workspace_size(size_t tokens, size_t hidden, size_t inter, size_t experts, size_t top_k) {
+    size_t off[11];
+    return mx_moe_layout(tokens, hidden, inter, experts, top_k, off) ? off[10] : 0;
+}
+
+void nh_moe_mxfp4_workspace_layout(size_t tokens, size_t hidden, size_t inter, size_t experts, size_t top_k,
+                                   size_t offsets_out[5]) {
+    size_t off[11] = {};
+    mx_moe_layout(tokens, hidden, inter, experts, top_k, off);
+    for (int i = 0; i < 5; ++i) offsets_out[i] = off[i];
+}
+
+nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, const float* logits, size_t tokens,
+                               size_t hidden, size_t inter, size_t experts, size_t top_k, int renormalize,
+                               float scaling, const uint8_t* w_up, const uint8_t* w_down, const nh_moe_biases* biases,
+                               const float* shared, void* out, nh_dtype out_dtype, void* workspace,
+                               size_t workspace_bytes, uint64_t* nonfinite, nh_stream stream, nh_error* err) {
+    clear_error(err);
+    if (tokens == 0) return set_error(err, NH_INVALID_ROW_COUNT, "row_count must be non-zero, got 0");
+    size_t off[11];
+    if (top_k > experts || !mx_moe_layout(tokens, hidden, inter, experts, top_k, off))
+        return set_error(err, NH_INVALID_SHAPE, "invalid MoE shape");
+    if (biases && (biases->shared_up || biases->shared_down))
+        return set_error(err, NH_INVALID_PARAMS, "shared expert biases given without a shared expert");
+    nh_status st;
+    if ((st = check_dtype(x_dtype, err)) || (st = check_dtype(out_dtype, err))) return st;
+    if (!nh_supports_moe_forward_mxfp4(tokens, hidden, inter, experts, top_k))
+        return set_error(err, NH_UNSUPPORTED, "MoE shape outside the gfx950 envelope (experts <= 1024, top_k <= 64, "
+                         "hidden and inter <= 8192)");
+    if (!workspace || workspace_bytes < off[10]) return mismatch(err, "workspace", off[10], workspace_bytes);
+    if (!aligned16(workspace) || !aligned16(w_up) || !aligned16(w_down))
+        return set_error(err, NH_UNSUPPORTED, "weights and workspace must be 16-byte aligned");
+    if ((st = bind_device(ctx, err))) return st;
+    uint8_t* ws = (uint8_t*)workspace;
+    int32_t *idx = (int32_t*)(ws + off[0]), *offsets = (int32_t*)(ws + off[2]), *perm = (int32_t*)(ws + off[3]),
+            *pos = (int32_t*)(ws + off[4]);
+    float *wts = (float*)(ws + off[1]), *d = (float*)(ws + off[9]);
+    const size_t R = tokens * top_k;
+    if ((st = launch_mx_tiles(ctx, x, x_dtype, tokens, hidden, ws + off[5], ws + off[6], nonfinite, stream, err)))
+        return st;
+    if ((st = nh_moe_route_sigmoid_topk(ctx, logits, tokens, experts, top_k, renormalize, scaling, idx, wts, stream, err)))
+        return st;
+    if ((st = nh_moe_permute(ctx, idx, tokens, top_k, experts, offsets, perm, pos, stream, err))) return st;
+    // as many workgroups per expert as give each CU one; slots packed onto the
+    // experts with routes where a tenth has none
+    const double live = expected_experts(experts, R);
+    const unsigned parts = (unsigned)std::max(1.0, (double)ctx->cu_count / std::max(1.0, live) + 0.5);
+    MxStreamArgs a{};
+    a.offsets = offsets;
+    a.experts = (int)experts;
+    a.compact = live < 0.9 * (double)experts ? 1 : 0;
+    const unsigned slots = (unsigned)(a.compact ? std::min(experts, R) : experts);
+    a.xcodes = ws + off[5];
+    a.xscales = ws + off[6];
+    a.w = w_up;
+    a.bias = biases ? biases->up : nullptr;
+    a.hcodes = ws + off[7];
+    a.hscales = ws + off[8];
+    a.nonfinite = nonfinite;
+    a.nonfinite_stage = kStageIntermediate;
+    a.perm = perm;
+    a.gather_div = (int)top_k;
+    a.M = (int)R;
+    a.N = (int)inter;
+    a.K = (int)hidden;
+    a.kt = (int)mx_k_tiles(hidden);
+    a.kq = (int)mx_k_pieces(hidden);
+    if ((st = launch_mx_stream(ctx, K_MX_REQUANT1, K_MX_REQUANT1_WIDE, a, tokens, true, parts, slots, stream, err)))
+        return st;
+    a.xcodes = ws + off[7];
+    a.xscales = ws + off[8];
+    a.w = w_down;
+    a.bias = biases ? biases->down : nullptr;
+    a.hcodes = a.hscales = nullptr;
+    a.perm = nullptr;
+    a.out = d;
+    a.out_dtype = DT_F32;
+    a.N = (int)hidden;
+    a.K = (int)inter;
+    a.kt = (int)mx_k_tiles(inter);
+    a.kq = (int)mx_k_pieces(inter);
+    if ((st = launch_mx_stream(ctx, K_MX_TOK1, K_MX_TOK1_WIDE, a, tokens, false, parts, slots, stream, err))) return st;
+    return nh_moe_combine_shared(ctx, d, pos, wts, shared, tokens, top_k, hidden, out, out_dtype, stream, err);
+}
+
+// ---- load balance of the router ---------------------------------------------
+}  // extern "C"
+
+namespace {
+
+struct BalancePlan {
+    int chunk, chunks, group;
+    size_t part_n, seq_loss, arrived, bytes;  // workspace offsets and size
+};
+
+bool plan_balance(size_t sequences, size_t tokens, size_t experts, BalancePlan* p) {
+    if (sequences == 0 || experts == 0 || sequences >= (1u << 30) || tokens >= (1u << 30) || experts > 1024 ||
+        tokens * experts >= (1ull << 40))
+        return false;
+    // a chunk per CU of 256, of 64 tokens at least
+    p->chunk = (int)std::max<size_t>(64, (tokens + 255) / 256);
+    p->chunks = (int)(tokens / (size_t)p->chunk + sequences);  // each sequence's last one may be short
+    p->group = 1;
+    while (4 * p->group < (int)experts && p->group < 64) p->group *= 2;
+    const size_t part = align256((size_t)p->chunks * experts * 4);
+    p->part_n = part;
+    p->seq_loss = 2 * part;
+    p->arrived = p->seq_loss + align256(sequences * sizeof(double));
+    p->bytes = p->arrived + 256;
+    return true;
+}
+
+nh_status check_balance(size_t sequences, const int32_t* seq_offsets, size_t tokens, size_t experts, size_t top_k,
+                        float coefficient, BalancePlan* p, nh_error* err) {
+    if (experts == 0 || top_k == 0 || sequences == 0 || (!seq_offsets && sequences != 1))
+        return set_error(err, NH_INVALID_SHAPE, "invalid balance shape sequences=%zu experts=%zu top_k=%zu", sequences,
+                         experts, top_k);
+    if (!std::isfinite(coefficient)) return set_error(err, NH_INVALID_PARAMS, "coefficient must be finite");
+    if (!plan_balance(sequences, tokens, experts, p) || top_k > 1024 || tokens * top_k >= (1ull << 31))
+        return set_error(err, NH_UNSUPPORTED, "device balance needs experts <= 1024, sequences and tokens < 2^30, "
+                         "tokens * top_k < 2^31");
+    return NH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t nh_moe_balance_loss_workspace_size(size_t sequences, size_t tokens, size_t experts) {
+    BalancePlan p;
+    return plan_balance(sequences, tokens, experts, &p) ? p.bytes : 0;
+}
+
+nh_status nh_moe_balance_loss(nh_context* ctx, const float* logits, const int32_t* indices, const int32_t* seq_offsets,
+                              size_t sequences, size_t tokens, size_t experts, size_t top_k, int softmax,
+                              float coefficient, int32_t* counts, float* loss, void* workspace, size_t workspace_bytes,
+                              nh_stream stream, nh_error* err) {
+    clear_error(err);
+    BalancePlan p;
+    nh_status st = check_balance(sequences, seq_offsets, tokens, experts, top_k, coefficient, &p, err);
+    if (st) return st;
+    if (!workspace || workspace_bytes < p.bytes) return mismatch(err, "workspace", p.bytes, workspace_bytes);
+    if (!aligned16(workspace)) return set_error(err, NH_UNSUPPORTED, "workspace must be 16-byte aligned");
+    if ((st = bind_device(ctx, err))) return st;
+    uint8_t* ws = (uint8_t*)workspace;
+    BalanceArgs a{};
+    a.logits = logits;
+    a.indices = indices;
+    a.seq = seq_offsets;
+    a.counts = counts;
+    a.loss = loss;
+    a.part_p = (float*)ws;
+    a.part_n = (int32_t*)(ws + p.part_n);
+    a.seq_loss = (double*)(ws + p.seq_loss);
+    a.arrived = (uint32_t*)(ws + p.arrived);
+    a.tokens = (int)tokens;
+    a.experts = (int)experts;
+    a.top_k = (int)top_k;
+    a.sequences = (int)sequences;
+    a.chunk = p.chunk;
+    a.chunks = p.chunks;
+    a.softmax = softmax ? 1 : 0;
+    a.coefficient = coefficient;
+    a.group = p.group;
+    if ((st = launch(ctx, K_BALANCE_PARTIAL, (unsigned)p.chunks, 1024, 17 * experts * 4, stream, a, err))) return st;
+    return launch(ctx, K_BALANCE_REDUCE, (unsigned)sequences, 1024, 128 + 2 * 1024 * 4, stream, a, err);
+}
+
+nh_status nh_moe_balance_loss_backward(nh_context* ctx, const float* logits, const int32_t* counts,
+                                       const int32_t* seq_offsets, size_t sequences, size_t tokens, size_t experts,
+                                       size_t top_k, int softmax, float coefficient, const float* dloss, float* dlogits,
+                                       nh_stream stream, nh_error* err) {
+    clear_error(err);
+    BalancePlan p;
+    nh_status st = check_balance(sequences, seq_offsets, tokens, experts, top_k, coefficient, &p, err);
+    if (st) return st;
+    if ((st = bind_device(ctx, err))) return st;
+    if (tokens == 0) return NH_OK;
+    BalanceArgs a{};
+    a.logits = logits;
+    a.seq = seq_offsets;
+    a.counts = const_cast<int32_t*>(counts);
+    a.dloss = dloss;
+    a.dlogits = dlogits;
+    a.tokens = (int)tokens;
+    a.experts = (int)experts;
+    a.top_k = (int)top_k;
+    a.sequences = (int)sequences;
+    a.softmax = softmax ? 1 : 0;
+    a.coefficient = coefficient;
+    a.group = p.group;
+    const size_t rows = 4 * (64 / (size_t)p.group);  // tokens per workgroup and turn
+    const size_t grid = std::min<size_t>((tokens + rows - 1) / rows, (size_t)ctx->cu_count * 8);
+    return launch(ctx, K_BALANCE_BACKWARD, (unsigned)grid, 256, 0, stream, a, err);
+}
+
+}  // extern "C"

@@ -12,17 +12,10 @@ using namespace nh;
 
 namespace {
 
-constexpr int64_t kMaxGrid = 0x7fffffff;
-
 unsigned grid_for(int64_t items, int per_block) {
     int64_t g = (items + per_block - 1) / per_block;
     g = std::max<int64_t>(1, std::min<int64_t>(g, 1 << 20));
     return (unsigned)g;
-}
-
-// Whether [a, a + an) and [b, b + bn) share bytes.
-bool overlap(const void* a, size_t an, const void* b, size_t bn) {
-    return an != 0 && bn != 0 && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
 }
 
 // Waves per workgroup of the GEMV family: wave w owns K tiles w, w + W, ...,
@@ -157,11 +150,6 @@ size_t gemm_lds_bytes(int bm, int bn, int stages, int ks = 2) {
     return ring + (size_t)(bm + 2 * bn) * 4;
 }
 
-nh_status check_dtype(nh_dtype d, nh_error* err) {
-    if (d != NH_F32 && d != NH_BF16) return set_error(err, NH_INVALID_PARAMS, "unknown dtype %d", (int)d);
-    return NH_OK;
-}
-
 // Shared validation of the W8A8 GEMM family (GemmError::InvalidShape for a
 // zero or overflowing dimension, gemm.rs:192-208; envelope for the rest).
 nh_status check_w8a8_shape(size_t m, size_t n, size_t k, nh_error* err) {
@@ -222,7 +210,6 @@ nh_status launch_quantize(nh_context* ctx, const void* x, nh_dtype dtype, size_t
 
 // Bytes of the activation tiles of m <= 16 rows of k codes.
 size_t act_tiles_bytes(size_t m, size_t k) { return m * (size_t)tiled_k_tiles(k) * 64; }
-size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 nh_status launch_gemv(nh_context* ctx, const int8_t* xq, const float* sx, const int8_t* wq, const float* sw,
                       const float* bias, int M, int N, int K, void* out, nh_dtype out_dtype, bool x_tiled,
@@ -1135,11 +1122,6 @@ nh_status nh_moe_permute(nh_context* ctx, const int32_t* indices, size_t tokens,
 }  // extern "C"
 
 constexpr int kExpertWaves = 8;
-
-// Experts that evenly spread routes reach.
-static double expected_experts(size_t experts, size_t routes) {
-    return experts * (1.0 - std::pow(1.0 - 1.0 / (double)experts, (double)routes));
-}
 
 // Workgroups per expert: as many as give every CU one when the routes reach as
 // many experts as evenly spread ones do, plus three standard deviations (their

@@ -78,6 +78,37 @@ const char* const kKernelSymbols[K_COUNT] = {  // in KernelId order
     "nh_gemm_f32_mfma_short_kernel",       // K_GEMM_F32_MFMA_SHORT
     "nh_gemm_f32_mfma_short_bf16_kernel",  // K_GEMM_F32_MFMA_SHORT_BF16
     "nh_gemm_f32_mfma_short_any_kernel",   // K_GEMM_F32_MFMA_SHORT_ANY
+    "nh_quantize_mxfp4_kernel",            // K_MX_QUANTIZE
+    "nh_quantize_mxfp4_tiles_kernel",      // K_MX_QUANTIZE_TILES
+    "nh_dequantize_mxfp4_kernel",          // K_MX_DEQUANTIZE
+    "nh_tile_mxfp4_kernel",                // K_MX_TILE
+    "nh_mx_stream_rows1_kernel",           // K_MX_ROWS1
+    "nh_mx_stream_rows2_kernel",           // K_MX_ROWS2
+    "nh_mx_stream_rows4_kernel",           // K_MX_ROWS4
+    "nh_mx_stream_rows8_kernel",           // K_MX_ROWS8
+    "nh_mx_stream_rows16_kernel",          // K_MX_ROWS16
+    "nh_mx_stream_tok1_kernel",            // K_MX_TOK1
+    "nh_mx_stream_tok2_kernel",            // K_MX_TOK2
+    "nh_mx_stream_tok4_kernel",            // K_MX_TOK4
+    "nh_mx_stream_tok8_kernel",            // K_MX_TOK8
+    "nh_mx_stream_tok1_wide_kernel",       // K_MX_TOK1_WIDE
+    "nh_mx_stream_tok2_wide_kernel",       // K_MX_TOK2_WIDE
+    "nh_mx_stream_tok4_wide_kernel",       // K_MX_TOK4_WIDE
+    "nh_mx_stream_tok8_wide_kernel",       // K_MX_TOK8_WIDE
+    "nh_mx_stream_requant1_kernel",        // K_MX_REQUANT1
+    "nh_mx_stream_requant2_kernel",        // K_MX_REQUANT2
+    "nh_mx_stream_requant4_kernel",        // K_MX_REQUANT4
+    "nh_mx_stream_requant8_kernel",        // K_MX_REQUANT8
+    "nh_mx_stream_requant1_wide_kernel",   // K_MX_REQUANT1_WIDE
+    "nh_mx_stream_requant2_wide_kernel",   // K_MX_REQUANT2_WIDE
+    "nh_mx_stream_requant4_wide_kernel",   // K_MX_REQUANT4_WIDE
+    "nh_mx_stream_requant8_wide_kernel",   // K_MX_REQUANT8_WIDE
+    "nh_mx_gemm_256x256_kernel",           // K_MX_GEMM_256
+    "nh_mx_gemm_128x128_kernel",           // K_MX_GEMM_128
+    "nh_mx_gemm_64x64_kernel",             // K_MX_GEMM_64
+    "nh_moe_balance_partial_kernel",       // K_BALANCE_PARTIAL
+    "nh_moe_balance_reduce_kernel",        // K_BALANCE_REDUCE
+    "nh_moe_balance_backward_kernel",      // K_BALANCE_BACKWARD
 };
 
 void clear_error(nh_error* err) {
@@ -107,6 +138,11 @@ nh_status mismatch(nh_error* err, const char* argument, uint64_t expected, uint6
 
 nh_status device_error(nh_error* err, hipError_t e, const char* what) {
     return set_error(err, NH_DEVICE_ERROR, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
+}
+
+nh_status check_dtype(nh_dtype d, nh_error* err) {
+    if (d != NH_F32 && d != NH_BF16) return set_error(err, NH_INVALID_PARAMS, "unknown dtype %d", (int)d);
+    return NH_OK;
 }
 
 nh_status bind_device(nh_context* ctx, nh_error* err) {
@@ -341,6 +377,10 @@ static const struct {
     {"moe_permute_host", 0},     {"moe_grouped_gemm_w8a8_host", 0}, {"moe_combine_host", 0},
     {"tile_weights_i8", 1},      {"tile_weights_i8_host", 0},  {"gemm_f32", 1},
     {"mlp_w8a8", 1},             {"gemm_w8a8_tiled_a", 1},
+    {"quantize_rows_mxfp4", 1},  {"dequantize_mxfp4", 1},       {"tile_weights_mxfp4", 1},
+    {"linear_mxfp4", 1},         {"moe_forward_mxfp4", 1},      {"moe_balance_loss", 1},
+    {"quantize_rows_mxfp4_host", 0}, {"dequantize_mxfp4_host", 0}, {"tile_weights_mxfp4_host", 0},
+    {"linear_mxfp4_host", 0},    {"moe_forward_mxfp4_host", 0}, {"moe_balance_loss_host", 0},
 };
 
 int nh_kernel_count(void) { return (int)(sizeof(kRegistry) / sizeof(kRegistry[0])); }

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime_api.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstddef>
 #include <cstdint>
@@ -81,6 +82,37 @@ enum KernelId : int {
     K_GEMM_F32_MFMA_SHORT,       // the f64 matrix-core GEMMs at K <= 128
     K_GEMM_F32_MFMA_SHORT_BF16,
     K_GEMM_F32_MFMA_SHORT_ANY,
+    K_MX_QUANTIZE,               // MXFP4: rows to row-major codes and scales
+    K_MX_QUANTIZE_TILES,         // rows to the tiled or the token form
+    K_MX_DEQUANTIZE,
+    K_MX_TILE,                   // row-major codes to the tiled form
+    K_MX_ROWS1,                  // weight-streaming product of up to 16 rows, quantized inside; 1, 2, .. K tiles per wave
+    K_MX_ROWS2,
+    K_MX_ROWS4,
+    K_MX_ROWS8,
+    K_MX_ROWS16,
+    K_MX_TOK1,                   // ... of codes in the token form, 16 rows at a time
+    K_MX_TOK2,
+    K_MX_TOK4,
+    K_MX_TOK8,
+    K_MX_TOK1_WIDE,              // ... 64 rows at a time (32 at 8 K tiles per wave)
+    K_MX_TOK2_WIDE,
+    K_MX_TOK4_WIDE,
+    K_MX_TOK8_WIDE,
+    K_MX_REQUANT1,               // ... with ReLU^2 and quantization of the output
+    K_MX_REQUANT2,
+    K_MX_REQUANT4,
+    K_MX_REQUANT8,
+    K_MX_REQUANT1_WIDE,
+    K_MX_REQUANT2_WIDE,
+    K_MX_REQUANT4_WIDE,
+    K_MX_REQUANT8_WIDE,
+    K_MX_GEMM_256,               // LDS-tiled product of two tiled operands
+    K_MX_GEMM_128,
+    K_MX_GEMM_64,
+    K_BALANCE_PARTIAL,           // router balance: sums per chunk of tokens
+    K_BALANCE_REDUCE,
+    K_BALANCE_BACKWARD,
     K_COUNT
 };
 
@@ -165,6 +197,20 @@ nh_status launch(nh_context* ctx, KernelId id, unsigned gx, unsigned bx, size_t 
                                          params, nullptr);
     if (e != hipSuccess) return device_error(err, e, kKernelSymbols[id]);
     return NH_OK;
+}
+
+nh_status check_dtype(nh_dtype d, nh_error* err);
+constexpr int64_t kMaxGrid = 0x7fffffff;
+inline size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+
+// Experts that evenly spread routes reach.
+inline double expected_experts(size_t experts, size_t routes) {
+    return experts * (1.0 - std::pow(1.0 - 1.0 / (double)experts, (double)routes));
+}
+
+// Whether [a, a + an) and [b, b + bn) share bytes.
+inline bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+    return an != 0 && bn != 0 && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
 }
 
 inline bool mul_ok(size_t a, size_t b, size_t* out) { return !__builtin_mul_overflow(a, b, out); }

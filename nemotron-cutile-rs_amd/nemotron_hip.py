@@ -156,6 +156,29 @@ _SIGNATURES = {
     "nh_linear_w4a8_workspace_size": (SZ, [SZ, SZ, SZ]),
     "nh_linear_w4a8": (ST, [P, P, C.c_int, P, C.c_float, C.c_uint32, P, SZ, SZ, SZ, P, C.c_int, P, SZ, P, P, E]),
     "nh_linear_w4a8_host": (ST, [P, C.c_int, P, SZ, C.c_float, C.c_uint32, P, SZ, SZ, SZ, P, C.c_int, E]),
+    "nh_quantize_rows_mxfp4": (ST, [P, P, C.c_int, SZ, SZ, P, P, P, P, E]),
+    "nh_quantize_rows_mxfp4_host": (ST, [P, C.c_int, SZ, SZ, P, P, E]),
+    "nh_dequantize_mxfp4": (ST, [P, P, P, SZ, SZ, P, C.c_int, P, E]),
+    "nh_dequantize_mxfp4_host": (ST, [P, P, SZ, SZ, P, C.c_int, E]),
+    "nh_tiled_mxfp4_weights_bytes": (SZ, [SZ, SZ]),
+    "nh_tile_weights_mxfp4": (ST, [P, P, P, SZ, SZ, P, SZ, P, E]),
+    "nh_tile_weights_mxfp4_host": (ST, [P, P, SZ, SZ, P, SZ, E]),
+    "nh_supports_linear_mxfp4": (C.c_int, [SZ, SZ, SZ]),
+    "nh_linear_mxfp4_workspace_size": (SZ, [SZ, SZ, SZ]),
+    "nh_linear_mxfp4": (ST, [P, P, C.c_int, P, P, SZ, SZ, SZ, P, C.c_int, P, SZ, P, P, E]),
+    "nh_linear_mxfp4_host": (ST, [P, C.c_int, P, P, SZ, SZ, SZ, P, C.c_int, E]),
+    "nh_supports_moe_forward_mxfp4": (C.c_int, [SZ, SZ, SZ, SZ, SZ]),
+    "nh_moe_forward_mxfp4_workspace_size": (SZ, [SZ, SZ, SZ, SZ, SZ]),
+    "nh_moe_mxfp4_workspace_layout": (None, [SZ, SZ, SZ, SZ, SZ, C.POINTER(SZ)]),
+    "nh_moe_forward_mxfp4": (ST, [P, P, C.c_int, P, SZ, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, MB, P, P, C.c_int, P,
+                                  SZ, P, P, E]),
+    "nh_moe_forward_mxfp4_host": (ST, [P, C.c_int, P, SZ, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, MB, P, P, C.c_int,
+                                       E]),
+    "nh_moe_balance_loss_workspace_size": (SZ, [SZ, SZ, SZ]),
+    "nh_moe_balance_loss": (ST, [P, P, P, P, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, P, SZ, P, E]),
+    "nh_moe_balance_loss_backward": (ST, [P, P, P, P, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, P, E]),
+    "nh_moe_balance_loss_host": (ST, [P, P, P, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, E]),
+    "nh_moe_balance_loss_backward_host": (ST, [P, P, P, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, E]),
     "nh_safetensors_tensor_info": (ST, [C.c_char_p, C.c_char_p, C.POINTER(TensorInfo), E]),
     "nh_safetensors_read": (ST, [P, C.c_char_p, C.c_char_p, P, SZ, E]),
     "nh_load_linear_i8": (ST, [P, C.c_char_p, C.c_char_p, C.c_char_p, SZ, SZ, P, SZ, P, SZ, P, E]),
@@ -361,6 +384,14 @@ def tile_weights(ctx, wq_dev, n, k, stream=None):
     nbytes = lib().nh_tiled_weights_bytes(n, k)
     out = ctx.empty(nbytes, np.int8)
     call("nh_tile_weights_i8", ctx.handle, wq_dev.ptr, n, k, out.ptr, nbytes, stream)
+    return out
+
+
+def tile_weights_mxfp4(ctx, codes_dev, scales_dev, n, k, stream=None):
+    """Device MXFP4 codes and scales of an [n][k] matrix -> a new device buffer in the tiled form."""
+    nbytes = lib().nh_tiled_mxfp4_weights_bytes(n, k)
+    out = ctx.empty(nbytes, np.uint8)
+    call("nh_tile_weights_mxfp4", ctx.handle, codes_dev.ptr, scales_dev.ptr, n, k, out.ptr, nbytes, stream)
     return out
 
 

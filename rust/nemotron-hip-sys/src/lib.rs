@@ -1140,6 +1140,308 @@ extern "C" {
         err: *mut nh_error,
     ) -> nh_status;
 
+    /// MXFP4: 4-bit floating point in blocks with a shared scale --- OCP microscaling: e2m1 elements (0,
+    /// 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) in blocks of 32 consecutive values of a row, each with
+    /// one e8m0 scale byte E standing for 2^(E - 127) (255: NaN). 4.25 bits a value, and the product runs
+    /// on the matrix cores' native MXFP4 form. No counterpart in the reference. Quantization: E = max(0,
+    /// exponent field of the block's largest |x| - 2), so the largest lies in [4, 8) of the scale and
+    /// saturates past 6; elements are rounded to nearest, ties to the even mantissa, the sign of a zero
+    /// kept. A block that holds a NaN or an infinity gets E = 255 and codes 0: it reads back as NaN, and
+    /// every output that it takes part in is NaN. (As elsewhere, an optional `nonfinite` word records the
+    /// first such value.) Row-major form: codes [rows][ceil(cols / 2)], two per byte, low nibble first;
+    /// scales [rows][ceil(cols / 32)]. A row's last block may be part of one. x, codes and scales may start
+    /// at any address of their element type. Tiled form (weights of the products): per 16 rows one region
+    /// of KT = ceil(k / 128) tiles of 1024 bytes of codes, byte 16*(16*g + r) + b of tile kt holding
+    /// W[16*nt + r][128*kt + 32*g + 2*b] (low nibble) and the value behind it, then ceil(KT / 4) pieces of
+    /// 256 scale bytes, byte 4*(16*g + r) + j of piece q being the scale of row r's block 4*(4*q + j) + g;
+    /// zeros outside the matrix. 16-byte aligned.
+    pub fn nh_quantize_rows_mxfp4(
+        ctx: *mut nh_context,
+        x: *const c_void,
+        dtype: nh_dtype,
+        rows: usize,
+        cols: usize,
+        codes: *mut u8,
+        scales: *mut u8,
+        nonfinite: *mut u64,
+        stream: nh_stream,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// Host twin, bit-identical; NH_NON_FINITE_INPUT on the first bad element, before anything is written.
+    pub fn nh_quantize_rows_mxfp4_host(
+        x: *const c_void,
+        dtype: nh_dtype,
+        rows: usize,
+        cols: usize,
+        codes: *mut u8,
+        scales: *mut u8,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// The values, exact in f32 and bf16 (a scale byte of 254 can overflow to infinity; 255 gives NaN).
+    pub fn nh_dequantize_mxfp4(
+        ctx: *mut nh_context,
+        codes: *const u8,
+        scales: *const u8,
+        rows: usize,
+        cols: usize,
+        out: *mut c_void,
+        out_dtype: nh_dtype,
+        stream: nh_stream,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    pub fn nh_dequantize_mxfp4_host(
+        codes: *const u8,
+        scales: *const u8,
+        rows: usize,
+        cols: usize,
+        out: *mut c_void,
+        out_dtype: nh_dtype,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// Bytes of the tiled form (0 for an invalid shape), and the conversion.
+    pub fn nh_tiled_mxfp4_weights_bytes(n: usize, k: usize) -> usize;
+
+    pub fn nh_tile_weights_mxfp4(
+        ctx: *mut nh_context,
+        codes: *const u8,
+        scales: *const u8,
+        n: usize,
+        k: usize,
+        tiled: *mut u8,
+        tiled_len: usize,
+        stream: nh_stream,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    pub fn nh_tile_weights_mxfp4_host(
+        codes: *const u8,
+        scales: *const u8,
+        n: usize,
+        k: usize,
+        tiled: *mut u8,
+        tiled_len: usize,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// Linear layer over tiled MXFP4 weights: y = Q(x) W^T (+ bias), x (f32 or bf16 rows of any k)
+    /// quantized as above, products exact, sums in f32. Up to 16 rows of k <= 16384 are one launch that
+    /// streams the weights once and touches no workspace; otherwise a launch quantizes the rows into the
+    /// workspace (nh_linear_mxfp4_workspace_size bytes, 16-byte aligned) ahead of the product.
+    /// Deterministic. Errors: INVALID_SHAPE (n or k == 0), INVALID_ROW_COUNT (m == 0), INVALID_PARAMS
+    /// (dtype), LENGTH_MISMATCH "workspace", UNSUPPORTED outside nh_supports_linear_mxfp4 or for a
+    /// misaligned w or workspace.
+    pub fn nh_supports_linear_mxfp4(m: usize, n: usize, k: usize) -> c_int;
+
+    pub fn nh_linear_mxfp4_workspace_size(m: usize, n: usize, k: usize) -> usize;
+
+    pub fn nh_linear_mxfp4(
+        ctx: *mut nh_context,
+        x: *const c_void,
+        x_dtype: nh_dtype,
+        w: *const u8,
+        bias: *const f32,
+        m: usize,
+        n: usize,
+        k: usize,
+        out: *mut c_void,
+        out_dtype: nh_dtype,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        nonfinite: *mut u64,
+        stream: nh_stream,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// Host twin (w tiled, as on the device): sums in f64, rounded once, so within the device's f32
+    /// summation error of it. NH_NON_FINITE_INPUT "input".
+    pub fn nh_linear_mxfp4_host(
+        x: *const c_void,
+        x_dtype: nh_dtype,
+        w: *const u8,
+        bias: *const f32,
+        m: usize,
+        n: usize,
+        k: usize,
+        out: *mut c_void,
+        out_dtype: nh_dtype,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// MoE layer over MXFP4 experts, from given logits: routing and permutation as nh_moe_forward_w8a8,
+    /// then per route h = ReLU^2(Q(x) W_up^T + b_up) and Q(h) W_down^T + b_down, combined with the routes'
+    /// weights in route order (nh_moe_combine_shared: `shared`, f32 [tokens][hidden] or NULL, is added
+    /// first, e.g. a shared expert's output). w_up is `experts` tiled [inter][hidden] matrices at a stride
+    /// of nh_tiled_mxfp4_weights_bytes(inter, hidden), w_down tiled [hidden][inter] ones. biases: up and
+    /// down (the shared ones must be NULL). h stays on the device in MXFP4 (a NaN in it marks its block,
+    /// and `nonfinite` reports it as "intermediate"). The workspace starts with the fields of
+    /// nh_moe_workspace_layout at other offsets (nh_moe_mxfp4_workspace_layout). Errors as
+    /// nh_moe_forward_w8a8.
+    pub fn nh_supports_moe_forward_mxfp4(
+        tokens: usize,
+        hidden: usize,
+        inter: usize,
+        experts: usize,
+        top_k: usize,
+    ) -> c_int;
+
+    pub fn nh_moe_forward_mxfp4_workspace_size(
+        tokens: usize,
+        hidden: usize,
+        inter: usize,
+        experts: usize,
+        top_k: usize,
+    ) -> usize;
+
+    /// byte offsets in the workspace of: [0] indices i32[T*k], [1] weights f32[T*k], [2] offsets i32[E+1],
+    /// [3] perm i32[T*k], [4] pos i32[T*k].
+    pub fn nh_moe_mxfp4_workspace_layout(
+        tokens: usize,
+        hidden: usize,
+        inter: usize,
+        experts: usize,
+        top_k: usize,
+        offsets_out: *mut usize,
+    );
+
+    pub fn nh_moe_forward_mxfp4(
+        ctx: *mut nh_context,
+        x: *const c_void,
+        x_dtype: nh_dtype,
+        logits: *const f32,
+        tokens: usize,
+        hidden: usize,
+        inter: usize,
+        experts: usize,
+        top_k: usize,
+        renormalize: c_int,
+        scaling: f32,
+        w_up: *const u8,
+        w_down: *const u8,
+        biases: *const nh_moe_biases,
+        shared: *const f32,
+        out: *mut c_void,
+        out_dtype: nh_dtype,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        nonfinite: *mut u64,
+        stream: nh_stream,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// Host twin (f64 sums rounded to f32); NH_NON_FINITE_INPUT "input" or "intermediate".
+    pub fn nh_moe_forward_mxfp4_host(
+        x: *const c_void,
+        x_dtype: nh_dtype,
+        logits: *const f32,
+        tokens: usize,
+        hidden: usize,
+        inter: usize,
+        experts: usize,
+        top_k: usize,
+        renormalize: c_int,
+        scaling: f32,
+        w_up: *const u8,
+        w_down: *const u8,
+        biases: *const nh_moe_biases,
+        shared: *const f32,
+        out: *mut c_void,
+        out_dtype: nh_dtype,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// load balance of the router, for training it -- From the logits [tokens][experts] and the routes
+    /// chosen on them (indices [tokens][top_k], e.g. of nh_moe_route_sigmoid_topk; an id outside [0,
+    /// experts) counts nowhere): the routes per expert, and the balance loss L = coefficient / S * sum_s
+    /// sum_e f_se P_se, f_se = experts / (top_k n_s) * counts_se, P_se = 1 / n_s * sum of p_te over the n_s
+    /// tokens of sequence s, with p = softmax(logits) (softmax != 0) or sigmoid(logits) over the row's sum
+    /// of sigmoids. seq_offsets (S + 1 non-decreasing i32, on the device) cut the tokens into sequences
+    /// [seq_offsets[s], seq_offsets[s + 1]); NULL, with sequences = 1, is one of all tokens. Tokens outside
+    /// every sequence (padding) count nowhere; an empty sequence adds 0. A row of -inf alone has no
+    /// probabilities and adds 0; a NaN logit makes the loss NaN. counts is i32 [S][experts], loss one f32.
+    /// Sums in f32 and f64 of a fixed order: results do not change from run to run. The workspace
+    /// (nh_moe_balance_loss_workspace_size bytes, 16-byte aligned) is free again once the call has run.
+    /// Errors: INVALID_SHAPE (experts, top_k or sequences == 0; sequences != 1 without offsets),
+    /// INVALID_PARAMS (a coefficient that is not finite), LENGTH_MISMATCH "workspace", UNSUPPORTED (experts
+    /// > 1024, sizes past 2^31, alignment). No counterpart in the reference.
+    pub fn nh_moe_balance_loss_workspace_size(
+        sequences: usize,
+        tokens: usize,
+        experts: usize,
+    ) -> usize;
+
+    pub fn nh_moe_balance_loss(
+        ctx: *mut nh_context,
+        logits: *const f32,
+        indices: *const i32,
+        seq_offsets: *const i32,
+        sequences: usize,
+        tokens: usize,
+        experts: usize,
+        top_k: usize,
+        softmax: c_int,
+        coefficient: f32,
+        counts: *mut i32,
+        loss: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: nh_stream,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// Its gradient: dlogits [tokens][experts] = dloss (one f32 on the device) * dL/dlogits, from the
+    /// counts of the forward call (the counts themselves take no gradient). Every row is written; rows
+    /// outside every sequence are 0.
+    pub fn nh_moe_balance_loss_backward(
+        ctx: *mut nh_context,
+        logits: *const f32,
+        counts: *const i32,
+        seq_offsets: *const i32,
+        sequences: usize,
+        tokens: usize,
+        experts: usize,
+        top_k: usize,
+        softmax: c_int,
+        coefficient: f32,
+        dloss: *const f32,
+        dlogits: *mut f32,
+        stream: nh_stream,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    /// Host twins (sums in f64).
+    pub fn nh_moe_balance_loss_host(
+        logits: *const f32,
+        indices: *const i32,
+        seq_offsets: *const i32,
+        sequences: usize,
+        tokens: usize,
+        experts: usize,
+        top_k: usize,
+        softmax: c_int,
+        coefficient: f32,
+        counts: *mut i32,
+        loss: *mut f32,
+        err: *mut nh_error,
+    ) -> nh_status;
+
+    pub fn nh_moe_balance_loss_backward_host(
+        logits: *const f32,
+        counts: *const i32,
+        seq_offsets: *const i32,
+        sequences: usize,
+        tokens: usize,
+        experts: usize,
+        top_k: usize,
+        softmax: c_int,
+        coefficient: f32,
+        dloss: *const f32,
+        dlogits: *mut f32,
+        err: *mut nh_error,
+    ) -> nh_status;
     pub fn nh_safetensors_tensor_info(
         path: *const c_char,
         name: *const c_char,
