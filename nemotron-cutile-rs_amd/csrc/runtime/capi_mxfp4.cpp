@@ -57,20 +57,23 @@ nh_status launch_mx_gemm(nh_context* ctx, const uint8_t* a, const uint8_t* w, co
                          size_t k, void* out, nh_dtype out_dtype, nh_stream stream, nh_error* err) {
     struct Tile {
         KernelId id;
-        int b, threads, stages, per_cu;
+        int bm, bn, threads, ks, stages, per_cu;
     };
-    static const Tile kTiles[] = {{K_MX_GEMM_256, 256, 512, 2, 1}, {K_MX_GEMM_128, 128, 256, 2, 2}, {K_MX_GEMM_64, 64, 256, 4, 2}};
+    static const Tile kTiles[] = {{K_MX_GEMM_256, 256, 256, 512, 1, 4, 1}, {K_MX_GEMM_256_128, 256, 128, 512, 1, 5, 1},
+                                  {K_MX_GEMM_128, 128, 128, 256, 1, 4, 2}, {K_MX_GEMM_64, 64, 64, 256, 4, 2, 2}};
     const size_t cus = (size_t)ctx->cu_count;
-    const Tile* t = &kTiles[2];
+    const Tile* t = &kTiles[3];
     for (const Tile& c : kTiles)
-        if (((m + c.b - 1) / c.b) * ((n + c.b - 1) / c.b) >= cus) {
+        if (((m + c.bm - 1) / c.bm) * ((n + c.bn - 1) / c.bn) >= cus) {
             t = &c;
             break;
         }
-    MxGemmArgs g{a, w, bias, out, (int)m, (int)n, (int)mx_k_tiles(k), (int)mx_k_pieces(k), (int)((m + t->b - 1) / t->b),
-                 (int)((n + t->b - 1) / t->b), out_dtype, 0};
-    const size_t tiles = (size_t)g.tiles_m * g.tiles_n, row_tiles = (size_t)2 * t->b / 16;
-    const size_t lds = (size_t)t->stages * (2 * row_tiles * 1024 + row_tiles * 256) + 1024;
+    MxGemmArgs g{a, w, bias, out, (int)m, (int)n, (int)mx_k_tiles(k), (int)mx_k_pieces(k), (int)((m + t->bm - 1) / t->bm),
+                 (int)((n + t->bn - 1) / t->bn), out_dtype, 0};
+    // the ring's stages, the pieces of scales that they span (mx_gemm_pieces), a spare KiB
+    const size_t tiles = (size_t)g.tiles_m * g.tiles_n, row_tiles = (size_t)(t->bm + t->bn) / 16;
+    const size_t pieces = t->ks == 4 ? t->stages : t->stages / 2 + 1;
+    const size_t lds = row_tiles * ((size_t)t->stages * t->ks * 1024 + pieces * 256) + 1024;
     const unsigned grid = (unsigned)std::min(tiles, cus * t->per_cu);
     return launch(ctx, t->id, grid, (unsigned)t->threads, lds, stream, g, err);
 }

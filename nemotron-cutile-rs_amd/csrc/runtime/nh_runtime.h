@@ -108,6 +108,7 @@ enum KernelId : int {
     K_MX_REQUANT4_WIDE,
     K_MX_REQUANT8_WIDE,
     K_MX_GEMM_256,               // LDS-tiled product of two tiled operands
+    K_MX_GEMM_256_128,
     K_MX_GEMM_128,
     K_MX_GEMM_64,
     K_BALANCE_PARTIAL,           // router balance: sums per chunk of tokens

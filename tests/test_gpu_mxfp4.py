@@ -210,7 +210,8 @@ def test_linear_exact(ctx, m, n, k, kind):
     want = x.astype(np.float32) @ w.T.astype(np.float32)  # exact, as the kernel's
     if bias is not None:
         want = want + bias
-    assert np.array_equal(got, R.to_bf16_bits(want) if bf16 else want), f"{(got != want).sum()} differ"
+    want = R.to_bf16_bits(want) if bf16 else want
+    assert np.array_equal(got, want), f"{(got != want).sum()} differ"
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 300, 4096), (16, 64, 2701), (40, 100, 3000), (200, 300, 2701), (1100, 1030, 512)])
