@@ -423,7 +423,10 @@ struct MxStreamArgs {
     int32_t gather_div;
     int32_t experts;
     int32_t compact;         // blockIdx.y counts the experts that have routes
-    int32_t units;           // N tiles (N tile pairs) in all, dealt to gridDim.x workgroups
+    int32_t run, longer;     // units (N tiles, or pairs of them) per workgroup; the first `longer` take one more
+    int32_t waves, groups;   // per group and in all: blockDim = 64 waves groups
+    int32_t row_blocks;      // RB of the kernel
+    int32_t pad_;
     int32_t nonfinite_stage;
 };
 

@@ -13,8 +13,10 @@ namespace {
 constexpr size_t kMxRowsMax = 16;
 constexpr size_t kMxRowsMaxK = 16384;
 
-// K tiles that each of at most eight waves owns: 1, 2, 4, 8, 16 (index 0..4).
-int mx_split(int kt) { return kt <= 8 ? 0 : kt <= 16 ? 1 : kt <= 32 ? 2 : kt <= 64 ? 3 : 4; }
+// K tiles that each of a group's waves owns (at most eight waves): 2, 4, 8, 16
+// (index 0..3).  More per wave where K leaves a wave too few loads to hide
+// their latency, and the other waves go to groups of their own.
+int mx_split(int kt) { return kt <= 8 ? 0 : kt <= 32 ? 1 : kt <= 64 ? 2 : 3; }
 
 // A row of `cols` values in `rows`: what the conversions address.
 nh_status check_mx_rows(size_t rows, size_t cols, nh_error* err) {
@@ -29,21 +31,25 @@ nh_status check_mx_rows(size_t rows, size_t cols, nh_error* err) {
 
 unsigned mx_unit_grid(int64_t units) { return (unsigned)((units + 1023) / 1024); }
 
-// The few-row product: fills the launch shape into `a` and launches kernel ids
-// first + split (16 rows at a time) or wide + split.
-nh_status launch_mx_stream(nh_context* ctx, KernelId first, KernelId wide, MxStreamArgs a, size_t rows, bool requant,
+// The few-row product: fills the launch shape into `a` and launches kernel
+// first + split (16 rows at a time), or with as many rows, which are codes, the
+// forms of 32 and 64 that follow it (K past 4096 has none of 64).
+nh_status launch_mx_stream(nh_context* ctx, KernelId first, MxStreamArgs a, size_t rows, bool requant,
                            unsigned workgroups, unsigned experts, nh_stream stream, nh_error* err) {
-    const int split = mx_split(a.kt), c = 1 << split;
-    const bool w = wide != K_COUNT && rows > 16;
-    const int rb = !w ? 1 : split == 3 ? 2 : 4, t = requant ? 2 : 1, waves = (a.kt + c - 1) / c;
+    const int split = mx_split(a.kt), c = 2 << split, t = requant ? 2 : 1;
+    const int form = rows <= 16 ? 0 : rows <= 32 || split == 2 ? 1 : 2;
+    a.row_blocks = 1 << form;
+    a.waves = (a.kt + c - 1) / c;
+    a.groups = 8 / a.waves;
     // h's units cover its whole K tiles: their blocks past N are written as zeros
-    a.units = requant ? 4 * (int)mx_k_tiles((uint64_t)a.N) : (a.N + 15) / 16;
+    const unsigned units = requant ? 4 * (unsigned)mx_k_tiles((uint64_t)a.N) : (unsigned)((a.N + 15) / 16);
     // a run's bias lies in LDS: at most 16 KiB
-    const unsigned least = (unsigned)((a.units + 255 / t) / (256 / t));
-    const unsigned gx = std::max(1u, std::min((unsigned)a.units, std::max(workgroups, least)));
-    const size_t run = (size_t)(a.units + gx - 1) / gx;
-    const size_t lds = (size_t)2 * t * rb * waves * 1024 + (a.bias ? run * t * 16 * 4 : 0);
-    return launch(ctx, (KernelId)((w ? wide : first) + split), gx, 64u * waves, lds, stream, a, err, experts);
+    const unsigned least = (units + 255 / t) / (256 / t);
+    const unsigned gx = std::max(1u, std::min(units, std::max(workgroups, least)));
+    a.run = (int)(units / gx);
+    a.longer = (int)(units % gx);
+    const size_t lds = (size_t)2 * t * a.row_blocks * a.waves * a.groups * 1024 + (a.bias ? (size_t)(a.run + 1) * t * 16 * 4 : 0);
+    return launch(ctx, (KernelId)(first + 3 * form + split), gx, 64u * a.waves * a.groups, lds, stream, a, err, experts);
 }
 
 nh_status launch_mx_tiles(nh_context* ctx, const void* x, nh_dtype dtype, size_t rows, size_t k, uint8_t* out,
@@ -177,7 +183,11 @@ nh_status nh_linear_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
     if (need == 0) {
         a.x = x;
         a.nonfinite = nonfinite;
-        return launch_mx_stream(ctx, K_MX_ROWS1, K_COUNT, a, m, false, cus, 1, stream, err);
+        // rows that start at 16-byte boundaries and hold whole blocks load
+        // without a branch, up to what fits the registers
+        const bool straight = k % kMxBlock == 0 && aligned16(x) && k <= (x_dtype == NH_BF16 ? 8192 : 4096);
+        const KernelId id = !straight ? K_MX_ANY_2 : x_dtype == NH_BF16 ? K_MX_BF16_2 : K_MX_F32_2;
+        return launch_mx_stream(ctx, id, a, m, false, cus, 1, stream, err);
     }
     uint8_t* ws = (uint8_t*)workspace;
     if (m <= 64 && k <= 8192) {
@@ -185,7 +195,7 @@ nh_status nh_linear_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
         if ((st = launch_mx_tiles(ctx, x, x_dtype, m, k, ws, scales, nonfinite, stream, err))) return st;
         a.xcodes = ws;
         a.xscales = scales;
-        return launch_mx_stream(ctx, K_MX_TOK1, K_MX_TOK1_WIDE, a, m, false, cus, 1, stream, err);
+        return launch_mx_stream(ctx, K_MX_TOK2, a, m, false, cus, 1, stream, err);
     }
     if ((st = launch_mx_tiles(ctx, x, x_dtype, m, k, ws, nullptr, nonfinite, stream, err))) return st;
     return launch_mx_gemm(ctx, ws, w, bias, m, n, k, out, out_dtype, stream, err);
@@ -294,7 +304,7 @@ nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype,
     a.K = (int)hidden;
     a.kt = (int)mx_k_tiles(hidden);
     a.kq = (int)mx_k_pieces(hidden);
-    if ((st = launch_mx_stream(ctx, K_MX_REQUANT1, K_MX_REQUANT1_WIDE, a, tokens, true, parts, slots, stream, err)))
+    if ((st = launch_mx_stream(ctx, K_MX_REQUANT2, a, tokens, true, parts, slots, stream, err)))
         return st;
     a.xcodes = ws + off[7];
     a.xscales = ws + off[8];
@@ -308,7 +318,7 @@ nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype,
     a.K = (int)inter;
     a.kt = (int)mx_k_tiles(inter);
     a.kq = (int)mx_k_pieces(inter);
-    if ((st = launch_mx_stream(ctx, K_MX_TOK1, K_MX_TOK1_WIDE, a, tokens, false, parts, slots, stream, err))) return st;
+    if ((st = launch_mx_stream(ctx, K_MX_TOK2, a, tokens, false, parts, slots, stream, err))) return st;
     return nh_moe_combine_shared(ctx, d, pos, wts, shared, tokens, top_k, hidden, out, out_dtype, stream, err);
 }
 

@@ -82,27 +82,31 @@ const char* const kKernelSymbols[K_COUNT] = {  // in KernelId order
     "nh_quantize_mxfp4_tiles_kernel",      // K_MX_QUANTIZE_TILES
     "nh_dequantize_mxfp4_kernel",          // K_MX_DEQUANTIZE
     "nh_tile_mxfp4_kernel",                // K_MX_TILE
-    "nh_mx_stream_rows1_kernel",           // K_MX_ROWS1
-    "nh_mx_stream_rows2_kernel",           // K_MX_ROWS2
-    "nh_mx_stream_rows4_kernel",           // K_MX_ROWS4
-    "nh_mx_stream_rows8_kernel",           // K_MX_ROWS8
-    "nh_mx_stream_rows16_kernel",          // K_MX_ROWS16
-    "nh_mx_stream_tok1_kernel",            // K_MX_TOK1
-    "nh_mx_stream_tok2_kernel",            // K_MX_TOK2
-    "nh_mx_stream_tok4_kernel",            // K_MX_TOK4
-    "nh_mx_stream_tok8_kernel",            // K_MX_TOK8
-    "nh_mx_stream_tok1_wide_kernel",       // K_MX_TOK1_WIDE
-    "nh_mx_stream_tok2_wide_kernel",       // K_MX_TOK2_WIDE
-    "nh_mx_stream_tok4_wide_kernel",       // K_MX_TOK4_WIDE
-    "nh_mx_stream_tok8_wide_kernel",       // K_MX_TOK8_WIDE
-    "nh_mx_stream_requant1_kernel",        // K_MX_REQUANT1
-    "nh_mx_stream_requant2_kernel",        // K_MX_REQUANT2
-    "nh_mx_stream_requant4_kernel",        // K_MX_REQUANT4
-    "nh_mx_stream_requant8_kernel",        // K_MX_REQUANT8
-    "nh_mx_stream_requant1_wide_kernel",   // K_MX_REQUANT1_WIDE
-    "nh_mx_stream_requant2_wide_kernel",   // K_MX_REQUANT2_WIDE
-    "nh_mx_stream_requant4_wide_kernel",   // K_MX_REQUANT4_WIDE
-    "nh_mx_stream_requant8_wide_kernel",   // K_MX_REQUANT8_WIDE
+    "nh_mx_stream_bf16_2_kernel",             // K_MX_BF16_2
+    "nh_mx_stream_bf16_4_kernel",             // K_MX_BF16_4
+    "nh_mx_stream_bf16_8_kernel",             // K_MX_BF16_8
+    "nh_mx_stream_f32_2_kernel",              // K_MX_F32_2
+    "nh_mx_stream_f32_4_kernel",              // K_MX_F32_4
+    "nh_mx_stream_any_2_kernel",              // K_MX_ANY_2
+    "nh_mx_stream_any_4_kernel",              // K_MX_ANY_4
+    "nh_mx_stream_any_8_kernel",              // K_MX_ANY_8
+    "nh_mx_stream_any_16_kernel",             // K_MX_ANY_16
+    "nh_mx_stream_tok2_kernel",               // K_MX_TOK2
+    "nh_mx_stream_tok4_kernel",               // K_MX_TOK4
+    "nh_mx_stream_tok8_kernel",               // K_MX_TOK8
+    "nh_mx_stream_tok2_32_kernel",            // K_MX_TOK2_32
+    "nh_mx_stream_tok4_32_kernel",            // K_MX_TOK4_32
+    "nh_mx_stream_tok8_32_kernel",            // K_MX_TOK8_32
+    "nh_mx_stream_tok2_64_kernel",            // K_MX_TOK2_64
+    "nh_mx_stream_tok4_64_kernel",            // K_MX_TOK4_64
+    "nh_mx_stream_requant2_kernel",           // K_MX_REQUANT2
+    "nh_mx_stream_requant4_kernel",           // K_MX_REQUANT4
+    "nh_mx_stream_requant8_kernel",           // K_MX_REQUANT8
+    "nh_mx_stream_requant2_32_kernel",        // K_MX_REQUANT2_32
+    "nh_mx_stream_requant4_32_kernel",        // K_MX_REQUANT4_32
+    "nh_mx_stream_requant8_32_kernel",        // K_MX_REQUANT8_32
+    "nh_mx_stream_requant2_64_kernel",        // K_MX_REQUANT2_64
+    "nh_mx_stream_requant4_64_kernel",        // K_MX_REQUANT4_64
     "nh_mx_gemm_256x256_kernel",           // K_MX_GEMM_256
     "nh_mx_gemm_256x128_kernel",           // K_MX_GEMM_256_128
     "nh_mx_gemm_128x128_kernel",           // K_MX_GEMM_128

@@ -86,27 +86,31 @@ enum KernelId : int {
     K_MX_QUANTIZE_TILES,         // rows to the tiled or the token form
     K_MX_DEQUANTIZE,
     K_MX_TILE,                   // row-major codes to the tiled form
-    K_MX_ROWS1,                  // weight-streaming product of up to 16 rows, quantized inside; 1, 2, .. K tiles per wave
-    K_MX_ROWS2,
-    K_MX_ROWS4,
-    K_MX_ROWS8,
-    K_MX_ROWS16,
-    K_MX_TOK1,                   // ... of codes in the token form, 16 rows at a time
-    K_MX_TOK2,
+    K_MX_BF16_2,                 // weight-streaming product of up to 16 rows, quantized inside; 2, 4, .. K tiles per wave
+    K_MX_BF16_4,
+    K_MX_BF16_8,
+    K_MX_F32_2,
+    K_MX_F32_4,
+    K_MX_ANY_2,                  // rows of any alignment and width
+    K_MX_ANY_4,
+    K_MX_ANY_8,
+    K_MX_ANY_16,
+    K_MX_TOK2,                   // ... of codes in the token form, 16 rows at a time
     K_MX_TOK4,
     K_MX_TOK8,
-    K_MX_TOK1_WIDE,              // ... 64 rows at a time (32 at 8 K tiles per wave)
-    K_MX_TOK2_WIDE,
-    K_MX_TOK4_WIDE,
-    K_MX_TOK8_WIDE,
-    K_MX_REQUANT1,               // ... with ReLU^2 and quantization of the output
-    K_MX_REQUANT2,
+    K_MX_TOK2_32,                // 32 rows
+    K_MX_TOK4_32,
+    K_MX_TOK8_32,
+    K_MX_TOK2_64,                // 64 rows
+    K_MX_TOK4_64,
+    K_MX_REQUANT2,               // ... with ReLU^2 and quantization of the output
     K_MX_REQUANT4,
     K_MX_REQUANT8,
-    K_MX_REQUANT1_WIDE,
-    K_MX_REQUANT2_WIDE,
-    K_MX_REQUANT4_WIDE,
-    K_MX_REQUANT8_WIDE,
+    K_MX_REQUANT2_32,
+    K_MX_REQUANT4_32,
+    K_MX_REQUANT8_32,
+    K_MX_REQUANT2_64,
+    K_MX_REQUANT4_64,
     K_MX_GEMM_256,               // LDS-tiled product of two tiled operands
     K_MX_GEMM_256_128,
     K_MX_GEMM_128,
