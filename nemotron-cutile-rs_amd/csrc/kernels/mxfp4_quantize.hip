@@ -59,12 +59,13 @@ extern "C" __global__ __launch_bounds__(256) void nh_quantize_mxfp4_kernel(MxQua
 // 16 rows x 512 columns (one scale piece) per workgroup.  Rows are read whole
 // waves at a time (1 KiB of bf16), the codes meet in LDS in tile order and
 // leave as whole tiles (or 256 bytes of a row in the token form).
-extern "C" __global__ __launch_bounds__(256) void nh_quantize_mxfp4_tiles_kernel(MxQuantizeTilesArgs a) {
-    __shared__ __align__(16) uint32_t codes[4 * 256];  // [K tile][lane][4]
-    __shared__ uint8_t scales[256];                    // [lane][K tile]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t rt = blockIdx.x / a.kq;
-    const int q = (int)(blockIdx.x - rt * a.kq);
+// (256 of the workgroup's threads, `tid` of them; every thread of the workgroup
+// calls it, for one barrier.)
+__device__ __forceinline__ void mx_quantize_tiles(const MxQuantizeTilesArgs& a, int64_t block, int tid, uint32_t* codes,
+                                                  uint8_t* scales) {
+    const int lane = tid & 63, wave = tid >> 6;
+    const int64_t rt = block / a.kq;
+    const int q = (int)(block - rt * a.kq);
     const int c = q * 512 + lane * 8;
     v4i v[4][2];
     int count[4];
@@ -99,6 +100,12 @@ extern "C" __global__ __launch_bounds__(256) void nh_quantize_mxfp4_tiles_kernel
             *(uint32_t*)(a.scales + (rt * 16 + rs) * ((int64_t)a.kq * 16) + q * 16 + g * 4) =
                 *(const uint32_t*)(scales + (g * 16 + rs) * 4);
     }
+}
+
+extern "C" __global__ __launch_bounds__(256) void nh_quantize_mxfp4_tiles_kernel(MxQuantizeTilesArgs a) {
+    __shared__ __align__(16) uint32_t codes[4 * 256];  // [K tile][lane][4]
+    __shared__ __align__(4) uint8_t scales[256];       // [lane][K tile]
+    mx_quantize_tiles(a, blockIdx.x, threadIdx.x, codes, scales);
 }
 
 // Codes and scales back to values: exact in f32, and in bf16 (two significant
@@ -188,5 +195,47 @@ extern "C" __global__ __launch_bounds__(256) void nh_tile_mxfp4_kernel(MxTileArg
             *(v4i*)(region + (int64_t)(4 * q + j) * 1024 + lane * 16) = w;
         }
         *(uint32_t*)(region + (int64_t)a.kt * 1024 + q * 256 + lane * 4) = s;
+    }
+}
+
+// The MoE layer ahead of its experts, in one launch: workgroups of 16 waves
+// route a token per wave (nh_moe_route_sigmoid_topk), the others quantize the
+// tokens into the token form; neither waits for the other.  With few routes the
+// one that routes also sorts them by expert (nh_moe_permute: stable, by route
+// id), every thread counting against all routes in LDS.
+extern "C" __global__ __launch_bounds__(1024) void nh_mx_moe_prep_kernel(MxMoePrepArgs a) {
+    __shared__ __align__(16) uint32_t codes[4][4 * 256];
+    __shared__ __align__(4) uint8_t scales[4][256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if ((int)blockIdx.x >= a.route_blocks) {  // uniform
+        const int64_t block = ((int64_t)blockIdx.x - a.route_blocks) * 4 + (tid >> 8);
+        mx_quantize_tiles(a.q, block, tid & 255, codes[tid >> 8], scales[tid >> 8]);  // past the rows: nothing
+        return;
+    }
+    for (int token = (int)blockIdx.x * 16 + wave; token < a.r.tokens; token += 16 * a.route_blocks) {
+        if (a.r.experts <= 128)
+            route_kernel_body<2>(a.r, token, lane);
+        else if (a.r.experts <= 256)
+            route_kernel_body<4>(a.r, token, lane);
+        else
+            route_kernel_body<kMaxExpertsPerLane>(a.r, token, lane);
+    }
+    if (!a.permute) return;
+    __syncthreads();  // the routes' stores are done
+    const int R = a.p.routes, E = a.p.experts;
+    int* ids = (int*)codes;
+    if (tid < R) ids[tid] = a.p.indices[tid];
+    __syncthreads();
+    if (tid < R) {  // routing gives ids in [0, E)
+        const int e = ids[tid];
+        int slot = 0;
+        for (int i = 0; i < R; ++i) slot += ids[i] < e || (ids[i] == e && i < tid);
+        a.p.pos[tid] = slot;
+        a.p.perm[slot] = tid;
+    }
+    for (int e = tid; e <= E; e += 1024) {
+        int n = 0;
+        for (int i = 0; i < R; ++i) n += ids[i] < e;
+        a.p.offsets[e] = n;
     }
 }

@@ -430,6 +430,15 @@ struct MxStreamArgs {
     int32_t nonfinite_stage;
 };
 
+// The MoE layer's routing, and the quantization of its tokens, side by side.
+struct MxMoePrepArgs {
+    MxQuantizeTilesArgs q;
+    RouteArgs r;
+    PermuteArgs p;
+    int32_t route_blocks;    // workgroups that route, 16 tokens each; the others quantize four blocks each
+    int32_t permute;         // 1: the one workgroup that routes also sorts the routes
+};
+
 // LDS-tiled product of two tiled operands (many rows): see mxfp4_gemm.hip.
 struct MxGemmArgs {
     const uint8_t* a;        // tiled [M][K]

@@ -275,15 +275,35 @@ nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype,
             *pos = (int32_t*)(ws + off[4]);
     float *wts = (float*)(ws + off[1]), *d = (float*)(ws + off[9]);
     const size_t R = tokens * top_k;
-    if ((st = launch_mx_tiles(ctx, x, x_dtype, tokens, hidden, ws + off[5], ws + off[6], nonfinite, stream, err)))
+    // routing beside the tokens' quantization; the routes of a few tokens are
+    // sorted in the same launch (one workgroup routes 16 tokens at a time)
+    MxMoePrepArgs prep{};
+    prep.q = MxQuantizeTilesArgs{x, ws + off[5], ws + off[6], nonfinite, (int64_t)tokens, (int32_t)hidden,
+                                 (int)mx_k_tiles(hidden), (int)mx_k_pieces(hidden), x_dtype, 1, 0};
+    prep.r.scores = logits;
+    prep.r.indices = idx;
+    prep.r.weights = wts;
+    prep.r.tokens = (int)tokens;
+    prep.r.experts = (int)experts;
+    prep.r.top_k = (int)top_k;
+    prep.r.renormalize = renormalize ? 1 : 0;
+    prep.r.scaling = scaling;
+    prep.p = PermuteArgs{idx, offsets, perm, pos, (int)R, (int)experts};
+    prep.permute = tokens <= 32 && R <= 512 ? 1 : 0;
+    prep.route_blocks = prep.permute ? 1 : (int)((tokens + 15) / 16);
+    const size_t blocks = (tokens + 15) / 16 * (size_t)prep.q.kq;
+    if ((st = launch(ctx, K_MX_MOE_PREP, (unsigned)(prep.route_blocks + (blocks + 3) / 4), 1024, 0, stream, prep, err)))
         return st;
-    if ((st = nh_moe_route_sigmoid_topk(ctx, logits, tokens, experts, top_k, renormalize, scaling, idx, wts, stream, err)))
-        return st;
-    if ((st = nh_moe_permute(ctx, idx, tokens, top_k, experts, offsets, perm, pos, stream, err))) return st;
-    // as many workgroups per expert as give each CU one; slots packed onto the
-    // experts with routes where a tenth has none
-    const double live = expected_experts(experts, R);
-    const unsigned parts = (unsigned)std::max(1.0, (double)ctx->cu_count / std::max(1.0, live) + 0.5);
+    if (!prep.permute && (st = nh_moe_permute(ctx, idx, tokens, top_k, experts, offsets, perm, pos, stream, err))) return st;
+    // As many workgroups per expert as give every CU one when the routes reach
+    // as many experts as evenly spread ones do and three standard deviations
+    // more (a few past the CUs cost a second round: 8 tokens over 128 experts in
+    // 6 parts each took 67 or 82 us by the input); slots packed onto the
+    // experts with routes where a tenth has none.
+    const double live = expected_experts(experts, R), load = (double)R / (double)experts, q = std::exp(-load);
+    const double var = (double)experts * (q - (1.0 + load) * q * q);
+    const double most = std::min({(double)experts, (double)R, live + 3.0 * std::sqrt(std::max(0.0, var))});
+    const unsigned parts = (unsigned)std::max(1.0, (double)ctx->cu_count / most);
     MxStreamArgs a{};
     a.offsets = offsets;
     a.experts = (int)experts;

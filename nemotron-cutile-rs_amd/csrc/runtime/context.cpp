@@ -80,6 +80,7 @@ const char* const kKernelSymbols[K_COUNT] = {  // in KernelId order
     "nh_gemm_f32_mfma_short_any_kernel",   // K_GEMM_F32_MFMA_SHORT_ANY
     "nh_quantize_mxfp4_kernel",            // K_MX_QUANTIZE
     "nh_quantize_mxfp4_tiles_kernel",      // K_MX_QUANTIZE_TILES
+    "nh_mx_moe_prep_kernel",               // K_MX_MOE_PREP
     "nh_dequantize_mxfp4_kernel",          // K_MX_DEQUANTIZE
     "nh_tile_mxfp4_kernel",                // K_MX_TILE
     "nh_mx_stream_bf16_2_kernel",             // K_MX_BF16_2

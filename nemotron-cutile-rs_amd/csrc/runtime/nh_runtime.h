@@ -84,6 +84,7 @@ enum KernelId : int {
     K_GEMM_F32_MFMA_SHORT_ANY,
     K_MX_QUANTIZE,               // MXFP4: rows to row-major codes and scales
     K_MX_QUANTIZE_TILES,         // rows to the tiled or the token form
+    K_MX_MOE_PREP,               // routing (and few routes' permutation) beside the tokens' quantization
     K_MX_DEQUANTIZE,
     K_MX_TILE,                   // row-major codes to the tiled form
     K_MX_BF16_2,                 // weight-streaming product of up to 16 rows, quantized inside; 2, 4, .. K tiles per wave
