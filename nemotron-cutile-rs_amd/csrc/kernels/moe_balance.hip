@@ -64,24 +64,38 @@ __device__ __forceinline__ int balance_chunk(const BalanceArgs& a, int b, int la
     return -1;
 }
 
-__device__ __forceinline__ float group_max(float v, int group) {
-    for (int off = group >> 1; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, kWave));
+// Maximum and sum over the lanes of a token (G consecutive lanes, every one of
+// them gets it): lane moves within rows of 16, then swaps of rows and halves.
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float v) {
+    return f32_from_bits((uint32_t)__builtin_amdgcn_update_dpp((int)f32_bits(v), (int)f32_bits(v), CTRL, 0xf, 0xf, false));
+}
+
+template <int G, class Op>
+__device__ __forceinline__ float group_reduce(float v, Op op) {
+    if constexpr (G >= 2) v = op(v, dpp_move<0xb1>(v));    // quad_perm 1,0,3,2
+    if constexpr (G >= 4) v = op(v, dpp_move<0x4e>(v));    // quad_perm 2,3,0,1
+    if constexpr (G >= 8) v = op(v, dpp_move<0x141>(v));   // row_half_mirror
+    if constexpr (G >= 16) v = op(v, dpp_move<0x140>(v));  // row_mirror
+    if constexpr (G >= 32) {
+        const auto t = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
+        v = op(f32_from_bits(t[0]), f32_from_bits(t[1]));
+    }
+    if constexpr (G >= 64) {
+        const auto t = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
+        v = op(f32_from_bits(t[0]), f32_from_bits(t[1]));
+    }
     return v;
 }
 
-__device__ __forceinline__ float group_sum(float v, int group) {
-    for (int off = group >> 1; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-    return v;
-}
-
-// A token's logits: lane j of the group holds experts 4 (j + i group) .. + 3 in
-// turn i; experts past E are -inf.
-template <int S>
+// A token's logits: lane j of its G holds experts 4 (j + i G) .. + 3 in turn i;
+// experts past E, and every one where !ok, are -inf.
+template <int G, int S>
 __device__ __forceinline__ void balance_row(const BalanceArgs& a, int64_t token, int j, bool ok, float (&z)[S][4]) {
     const int E = a.experts;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-        const int e = 4 * (j + i * a.group);
+        const int e = 4 * (j + i * G);
         const float* at = a.logits + token * E + e;
 #pragma unroll
         for (int q = 0; q < 4; ++q) z[i][q] = -__builtin_inff();
@@ -96,16 +110,18 @@ __device__ __forceinline__ void balance_row(const BalanceArgs& a, int64_t token,
 }
 
 // The row's probabilities in place of its logits; slope: d of each (sigmoid).
-template <int S, bool SLOPE>
-__device__ __forceinline__ void balance_probabilities(const BalanceArgs& a, float (&z)[S][4], float (&slope)[S][4]) {
+// v_exp_f32 and v_rcp_f32 are within an ulp, the argument's rounding is what
+// counts: |z| 2^-24 of a probability.  An exp of a NaN is one, so is its row.
+template <int G, int S, bool SOFTMAX, bool SLOPE>
+__device__ __forceinline__ void balance_probabilities(float (&z)[S][4], float (&slope)[S][4]) {
     float m = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) m = fmaxf(m, z[i][q]);
-    m = group_max(m, a.group);
+    m = group_reduce<G>(m, [](float x, float y) { return fmaxf(x, y); });
     const bool none = m == -__builtin_inff();
-    if (!a.softmax) m = fminf(m, 0.0f);
+    if (!SOFTMAX) m = fminf(m, 0.0f);
     if (none) m = 0.0f;
     float sum = 0.0f;
 #pragma unroll
@@ -113,83 +129,143 @@ __device__ __forceinline__ void balance_probabilities(const BalanceArgs& a, floa
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float v = z[i][q];
-            if (a.softmax) {
+            if constexpr (SOFTMAX) {
                 z[i][q] = __expf(v - m);
             } else {
-                const float d = 1.0f + __expf(-fabsf(v));
-                z[i][q] = __expf(fminf(v, 0.0f) - m) / d;
-                if constexpr (SLOPE) slope[i][q] = __expf(-fmaxf(v, 0.0f)) / d;
-                if (v != v) z[i][q] = v;  // the minimum drops a NaN
+                const float t = __expf(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + t);
+                // exp(min(v, 0) - m): t itself unless the row's sigmoids are all below 1/2
+                z[i][q] = r * (m < 0.0f ? __expf(v - m) : v >= 0.0f ? 1.0f : t);
+                if constexpr (SLOPE) slope[i][q] = r * (v >= 0.0f ? t : 1.0f);
             }
             sum += z[i][q];
         }
-    sum = group_sum(sum, a.group);
-    const float r = none && !(sum != sum) ? 0.0f : 1.0f / sum;
+    sum = group_reduce<G>(sum, [](float x, float y) { return x + y; });
+    const float r = none && !(sum != sum) ? 0.0f : __builtin_amdgcn_rcpf(sum);
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) z[i][q] *= r;
 }
 
-template <int S>
-__device__ __forceinline__ void balance_partial(const BalanceArgs& a, int* lds) {
+// Rows that a wave has in flight per lane group: loads and lane moves of one
+// row are a chain, and several interleave (131072 x 128, forward and backward:
+// 72 us one row at a time through LDS-crossbar moves, 53 so).  One past 256
+// experts, where four rows' registers leave few waves.
+constexpr int balance_rows(int turns) { return turns == 1 ? 4 : 1; }
+
+template <int G, int S, bool SOFTMAX>
+__device__ __forceinline__ void balance_partial(const BalanceArgs& a, int* lds, int lo, int hi) {
     const int E = a.experts, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int lo, hi, first;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.arrived = 0;
-    const int s = balance_chunk(a, blockIdx.x, lane, lo, hi, first);
-    if (s < 0) return;  // uniform
     int* hist = lds;                    // [E]
     float* psum = (float*)(lds + E);    // [waves][E]
     for (int e = threadIdx.x; e < E; e += blockDim.x) hist[e] = 0;
     __syncthreads();
-    const int64_t r1 = (int64_t)hi * a.top_k;
-    for (int64_t r = (int64_t)lo * a.top_k + threadIdx.x; r < r1; r += blockDim.x) {
-        const int e = a.indices[r];
-        if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
-    }
-    const int rows = 64 / a.group, j = lane & (a.group - 1), row = lane / a.group;
+    // the chunk's routes: the first loads go out ahead of the logits, and count behind them
+    const int64_t r0 = (int64_t)lo * a.top_k + threadIdx.x, r1 = (int64_t)hi * a.top_k;
+    constexpr int kEarly = 4;
+    int early[kEarly];
+#pragma unroll
+    for (int u = 0; u < kEarly; ++u) early[u] = r0 + u * 64 * kBalanceWaves < r1 ? a.indices[r0 + u * 64 * kBalanceWaves] : -1;
+    constexpr int rows = 64 / G, kBalanceRows = balance_rows(S);
+    const int j = lane & (G - 1), row = lane / G;
     float acc[S][4];
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) acc[i][q] = 0.0f;
-    for (int t0 = lo + wave * rows; t0 < hi; t0 += kBalanceWaves * rows) {
-        const bool ok = t0 + row < hi;
-        float z[S][4], none[S][4];
-        balance_row<S>(a, t0 + row, j, ok, z);
-        balance_probabilities<S, false>(a, z, none);
+    for (int t0 = lo + wave * rows * kBalanceRows; t0 < hi; t0 += kBalanceWaves * rows * kBalanceRows) {
+        float z[kBalanceRows][S][4], none[S][4];
 #pragma unroll
-        for (int i = 0; i < S; ++i)
+        for (int u = 0; u < kBalanceRows; ++u) {
+            const int t = t0 + u * rows + row;
+            balance_row<G, S>(a, t, j, t < hi, z[u]);
+        }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[i][q] += z[i][q];
+        for (int u = 0; u < kBalanceRows; ++u) balance_probabilities<G, S, SOFTMAX, false>(z[u], none);
+#pragma unroll
+        for (int u = 0; u < kBalanceRows; ++u)
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[i][q] += z[u][i][q];
     }
+    auto count = [&](int e) {
+        if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
+    };
+#pragma unroll
+    for (int u = 0; u < kEarly; ++u) count(early[u]);
+    for (int64_t r = r0 + kEarly * 64 * kBalanceWaves; r < r1; r += 64 * kBalanceWaves) count(a.indices[r]);
     // the wave's rows, then the waves in order
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             float v = acc[i][q];
-            for (int off = 32; off >= a.group; off >>= 1) v += __shfl_xor(v, off, kWave);
-            const int e = 4 * (j + i * a.group) + q;
+#pragma unroll
+            for (int off = 32; off >= G; off >>= 1) v += __shfl_xor(v, off, kWave);
+            const int e = 4 * (j + i * G) + q;
             if (row == 0 && e < E) psum[wave * E + e] = v;
         }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += blockDim.x) {
-        float v = psum[e];
-        for (int w = 1; w < kBalanceWaves; ++w) v += psum[w * E + e];
-        a.part_p[(int64_t)blockIdx.x * E + e] = v;
-        a.part_n[(int64_t)blockIdx.x * E + e] = hist[e];
-    }
 }
+
+// A body per lanes a token has (and turns, past 256 experts) and kind of probability.
+#define NH_BALANCE_FORMS(call)                      \
+    switch (a.experts <= 256 ? a.group : 0) {       \
+        case 1: call(1, 1); break;                  \
+        case 2: call(2, 1); break;                  \
+        case 4: call(4, 1); break;                  \
+        case 8: call(8, 1); break;                  \
+        case 16: call(16, 1); break;                \
+        case 32: call(32, 1); break;                \
+        case 64: call(64, 1); break;                \
+        default: call(64, 4); break;                \
+    }
 
 }  // namespace
 
+// One chunk of a sequence's tokens per workgroup; with one chunk in all
+// (a.single) the counts and the loss at once.
 extern "C" __global__ __launch_bounds__(64 * kBalanceWaves) void nh_moe_balance_partial_kernel(BalanceArgs a) {
     extern __shared__ int balance_lds[];
-    if (a.experts <= 256)
-        balance_partial<1>(a, balance_lds);
-    else
-        balance_partial<4>(a, balance_lds);
+    const int E = a.experts, lane = threadIdx.x & 63;
+    if (blockIdx.x == 0 && threadIdx.x == 0 && !a.single) *a.arrived = 0;
+    int lo, hi, first;
+    if (a.single) {
+        balance_bounds(a, 0, lo, hi);
+    } else if (balance_chunk(a, blockIdx.x, lane, lo, hi, first) < 0) {
+        return;  // uniform
+    }
+#define NH_CALL(G, S)                                               \
+    if (a.softmax) balance_partial<G, S, true>(a, balance_lds, lo, hi); \
+    else balance_partial<G, S, false>(a, balance_lds, lo, hi)
+    NH_BALANCE_FORMS(NH_CALL)
+#undef NH_CALL
+    const int* hist = balance_lds;
+    const float* psum = (const float*)(balance_lds + E);
+    double dot = 0.0;
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        float v = psum[e];
+        for (int w = 1; w < kBalanceWaves; ++w) v += psum[w * E + e];
+        if (a.single) {
+            a.counts[e] = hist[e];
+            dot += (double)v * (double)hist[e];
+        } else {
+            a.part_p[(int64_t)blockIdx.x * E + e] = v;
+            a.part_n[(int64_t)blockIdx.x * E + e] = hist[e];
+        }
+    }
+    if (!a.single) return;
+    dot = wave_sum_f64(dot);
+    __syncthreads();  // the partial sums are read
+    double* red = (double*)(balance_lds + (E & ~1));
+    if (lane == 0) red[threadIdx.x >> 6] = dot;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    double sum = 0.0;
+    for (int w = 0; w < kBalanceWaves; ++w) sum += red[w];
+    const double n = (double)(hi - lo);
+    a.loss[0] = hi > lo ? (float)((double)a.coefficient * sum * (double)E / ((double)a.top_k * n * n)) : 0.0f;
 }
 
 // One workgroup per sequence: its chunks' sums in order, its counts and loss;
@@ -215,10 +291,21 @@ extern "C" __global__ __launch_bounds__(1024) void nh_moe_balance_reduce_kernel(
     float v = 0.0f;
     int c = 0;
     if (part < parts) {
-#pragma unroll 8
-        for (int i = part; i < chunks; i += parts) {
-            v += a.part_p[(int64_t)(before + i) * E + col];
-            c += a.part_n[(int64_t)(before + i) * E + col];
+        constexpr int kAhead = 16;  // loads in flight; past the chunks the last one's, unused
+        for (int i0 = part; i0 < chunks; i0 += parts * kAhead) {
+            float pv[kAhead];
+            int pn[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int64_t at = (int64_t)(before + min(i0 + u * parts, chunks - 1)) * E + col;
+                pv[u] = a.part_p[at];
+                pn[u] = a.part_n[at];
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                v += i0 + u * parts < chunks ? pv[u] : 0.0f;
+                c += i0 + u * parts < chunks ? pn[u] : 0;
+            }
         }
         ps[part * cols + col] = v;
         ns[part * cols + col] = c;
@@ -258,64 +345,60 @@ extern "C" __global__ __launch_bounds__(1024) void nh_moe_balance_reduce_kernel(
 
 namespace {
 
-template <int S>
-__device__ __forceinline__ void balance_backward(const BalanceArgs& a) {
-    const int E = a.experts, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int rows = 64 / a.group, j = lane & (a.group - 1), row = lane / a.group;
-    const int64_t waves = (int64_t)gridDim.x * (blockDim.x >> 6);
-    const float up = a.dloss[0] * a.coefficient / (float)a.sequences;
-    int s = -1, lo = 0, hi = 0;  // the group's sequence, its f and scale
-    float f[S][4], scale = 0.0f;
-    for (int64_t t0 = ((int64_t)blockIdx.x * (blockDim.x >> 6) + wave) * rows; t0 < a.tokens; t0 += waves * rows) {
-        const int t = (int)t0 + row;
-        const bool ok = t < a.tokens;
-        float z[S][4], slope[S][4];
-        balance_row<S>(a, t, j, ok, z);
-        if (s < 0 || t >= hi) {
-            // the first sequence that ends behind t
-            int b = 0, e = a.sequences - 1;
-            while (b < e) {
-                const int m = (b + e) >> 1;
-                if (balance_bounds(a, m, lo, hi), hi > t) e = m;
-                else b = m + 1;
-            }
-            s = b;
-            const int n = balance_bounds(a, s, lo, hi);
-            scale = n > 0 ? up / (float)n : 0.0f;
-            const float per = n > 0 ? (float)E / ((float)a.top_k * (float)n) : 0.0f;
+template <int G, int S, bool SOFTMAX>
+__device__ __forceinline__ void balance_backward(const BalanceArgs& a, int s, int lo, int hi, int n) {
+    const int E = a.experts, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    constexpr int rows = 64 / G, kBalanceRows = balance_rows(S);
+    const int j = lane & (G - 1), row = lane / G;
+    // f and the gradient's scale, of the sequence
+    const float scale = a.dloss[0] * a.coefficient / ((float)a.sequences * (float)n);
+    const float per = (float)E / ((float)a.top_k * (float)n);
+    float f[S][4];
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int e = 4 * (j + i * G) + q;
+            f[i][q] = e < E ? (float)a.counts[(int64_t)s * E + e] * per : 0.0f;
+        }
+    for (int t0 = lo + wave * rows * kBalanceRows; t0 < hi; t0 += waves * rows * kBalanceRows) {
+        float z[kBalanceRows][S][4], slope[kBalanceRows][S][4], fp[kBalanceRows];
+#pragma unroll
+        for (int u = 0; u < kBalanceRows; ++u) {
+            const int t = t0 + u * rows + row;
+            balance_row<G, S>(a, t, j, t < hi, z[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kBalanceRows; ++u) balance_probabilities<G, S, SOFTMAX, true>(z[u], slope[u]);
+#pragma unroll
+        for (int u = 0; u < kBalanceRows; ++u) {
+            fp[u] = 0.0f;
 #pragma unroll
             for (int i = 0; i < S; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int x = 4 * (j + i * a.group) + q;
-                    f[i][q] = x < E ? (float)a.counts[(int64_t)s * E + x] * per : 0.0f;
-                }
+                for (int q = 0; q < 4; ++q) fp[u] += f[i][q] * z[u][i][q];
+            fp[u] = group_reduce<G>(fp[u], [](float x, float y) { return x + y; });
         }
-        balance_probabilities<S, true>(a, z, slope);
-        float fp = 0.0f;
 #pragma unroll
-        for (int i = 0; i < S; ++i)
+        for (int u = 0; u < kBalanceRows; ++u) {
+            const int t = t0 + u * rows + row;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) fp += f[i][q] * z[i][q];
-        fp = group_sum(fp, a.group);
-        const bool in = t >= lo && t < hi;
+            for (int i = 0; i < S; ++i) {
+                const int e = 4 * (j + i * G);
+                float d[4];
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const int e = 4 * (j + i * a.group);
-            float d[4];
+                for (int q = 0; q < 4; ++q) {
+                    d[q] = scale * z[u][i][q] * (f[i][q] - fp[u]);
+                    if constexpr (!SOFTMAX) d[q] *= slope[u][i][q];
+                }
+                float* at = a.dlogits + (int64_t)t * E + e;
+                if (t < hi && e + 3 < E) {
+                    __builtin_memcpy(at, d, 16);
+                } else if (t < hi) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                d[q] = scale * z[i][q] * (f[i][q] - fp);
-                if (!a.softmax) d[q] *= slope[i][q];
-                if (!in) d[q] = 0.0f;  // behind the last sequence
-            }
-            float* at = a.dlogits + (int64_t)t * E + e;
-            if (ok && e + 3 < E) {
-                __builtin_memcpy(at, d, 16);
-            } else if (ok) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (e + q < E) at[q] = d[q];
+                    for (int q = 0; q < 4; ++q)
+                        if (e + q < E) at[q] = d[q];
+                }
             }
         }
     }
@@ -323,9 +406,27 @@ __device__ __forceinline__ void balance_backward(const BalanceArgs& a) {
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(256) void nh_moe_balance_backward_kernel(BalanceArgs a) {
-    if (a.experts <= 256)
-        balance_backward<1>(a);
-    else
-        balance_backward<4>(a);
+// One chunk of a sequence's tokens per workgroup; the last a.padding workgroups
+// clear the rows before the first sequence and behind the last.
+extern "C" __global__ __launch_bounds__(256, 4) void nh_moe_balance_backward_kernel(BalanceArgs a) {
+    int lo, hi, first = 0;
+    if ((int)blockIdx.x >= a.chunks) {
+        balance_bounds(a, 0, lo, first);
+        balance_bounds(a, a.sequences - 1, first, hi);
+        const int64_t head = (int64_t)lo * a.experts, tail = (int64_t)hi * a.experts, end = (int64_t)a.tokens * a.experts;
+        const int64_t step = (int64_t)a.padding * blockDim.x;
+        const int64_t at = (int64_t)(blockIdx.x - a.chunks) * blockDim.x + threadIdx.x;
+        for (int64_t i = at; i < head; i += step) a.dlogits[i] = 0.0f;
+        for (int64_t i = tail + at; i < end; i += step) a.dlogits[i] = 0.0f;
+        return;
+    }
+    const int s = balance_chunk(a, blockIdx.x, threadIdx.x & 63, lo, hi, first);
+    if (s < 0) return;  // uniform
+    int l, h;
+    const int n = balance_bounds(a, s, l, h);
+#define NH_CALL(G, S)                                               \
+    if (a.softmax) balance_backward<G, S, true>(a, s, lo, hi, n); \
+    else balance_backward<G, S, false>(a, s, lo, hi, n)
+    NH_BALANCE_FORMS(NH_CALL)
+#undef NH_CALL
 }

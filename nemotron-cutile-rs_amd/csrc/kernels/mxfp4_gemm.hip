@@ -242,13 +242,11 @@ __device__ __forceinline__ void mx_gemm(const MxGemmArgs& a, int8_t* smem) {
 
 }  // namespace
 
-// LDS: NH_MX_GEMM_LDS (launch_mx_gemm)
 #define NH_MX_GEMM(name, BM, BN, WGM, WGN, KS, NS)                                            \
     extern "C" __global__ __launch_bounds__(64 * WGM * WGN, 2) void name(MxGemmArgs a) {      \
         extern __shared__ __align__(1024) int8_t smem[];                                      \
         mx_gemm<BM, BN, WGM, WGN, KS, NS>(a, smem);                                           \
     }
 NH_MX_GEMM(nh_mx_gemm_256x256_kernel, 256, 256, 2, 4, 1, 4)
-NH_MX_GEMM(nh_mx_gemm_256x128_kernel, 256, 128, 4, 2, 1, 5)
 NH_MX_GEMM(nh_mx_gemm_128x128_kernel, 128, 128, 2, 2, 1, 4)
 NH_MX_GEMM(nh_mx_gemm_64x64_kernel, 64, 64, 2, 2, 4, 2)

@@ -40,7 +40,7 @@ extern "C" __global__ __launch_bounds__(256) void nh_quantize_mxfp4_kernel(MxQua
                 block[t] = row * (a.row_units >> 2) + (c >> 5);
             }
         }
-        mx_load8(a.x, value[t], count[t], a.x_dtype, v[t]);
+        mx_load8<true>(a.x, value[t], count[t], a.x_dtype, v[t]);
     }
 #pragma unroll
     for (int t = 0; t < kMxTurns; ++t) {
@@ -73,7 +73,7 @@ __device__ __forceinline__ void mx_quantize_tiles(const MxQuantizeTilesArgs& a, 
     for (int i = 0; i < 4; ++i) {
         const int64_t row = rt * 16 + wave * 4 + i;
         count[i] = row < a.rows && c < a.cols ? min(8, a.cols - c) : 0;
-        mx_load8(a.x, row * a.cols + c, count[i], a.x_dtype, v[i]);
+        mx_load8<true>(a.x, row * a.cols + c, count[i], a.x_dtype, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

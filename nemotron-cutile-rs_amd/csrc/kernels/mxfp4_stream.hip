@@ -328,7 +328,7 @@ __device__ __forceinline__ void mx_stream(const MxStreamArgs& a, int8_t* lds) {
     p.seg0 = 0;
     p.seg1 = a.M;
     if (a.offsets) {
-        e = blockIdx.y;
+        e = (int)(blockIdx.y / (unsigned)a.row_parts);
         if (a.compact) {
             e = nth_active_expert(a.offsets, a.experts, e, p.lane, p.seg0, p.seg1);
         } else {
@@ -353,9 +353,11 @@ __device__ __forceinline__ void mx_stream(const MxStreamArgs& a, int8_t* lds) {
         }
     }
     // the bias lies behind the partial tiles of RB row blocks
-    for (int m0 = p.seg0; m0 < p.seg1; m0 += 16 * RB) {
+    // workgroups of an expert's row parts take its passes in turn
+    const int step = 16 * RB * a.row_parts;
+    for (int m0 = p.seg0 + 16 * RB * (int)(blockIdx.y % (unsigned)a.row_parts); m0 < p.seg1; m0 += step) {
         mx_pass<C, RB, D, SRC, EPI>(a, p, m0, lds);
-        if (m0 + 16 * RB < p.seg1) lds_publish();  // the last sums are read before the next pass writes partials
+        if (m0 + step < p.seg1) lds_publish();  // the last sums are read before the next pass writes partials
     }
 }
 

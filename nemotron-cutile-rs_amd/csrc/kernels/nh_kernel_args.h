@@ -426,7 +426,7 @@ struct MxStreamArgs {
     int32_t run, longer;     // units (N tiles, or pairs of them) per workgroup; the first `longer` take one more
     int32_t waves, groups;   // per group and in all: blockDim = 64 waves groups
     int32_t row_blocks;      // RB of the kernel
-    int32_t pad_;
+    int32_t row_parts;       // blockIdx.y = expert * row_parts + part: passes of 16 RB rows dealt to workgroups
     int32_t nonfinite_stage;
 };
 
@@ -471,6 +471,8 @@ struct BalanceArgs {
     int32_t softmax;
     float coefficient;
     int32_t group;              // lanes per token: a power of two, 4 experts per lane and turn
+    int32_t single;             // forward: one workgroup has every token of the one sequence
+    int32_t padding;            // backward: workgroups that clear the rows outside every sequence
     int32_t pad_;
 };
 

@@ -31,13 +31,16 @@ nh_status check_mx_rows(size_t rows, size_t cols, nh_error* err) {
 
 unsigned mx_unit_grid(int64_t units) { return (unsigned)((units + 1023) / 1024); }
 
+// Rows that one pass of the few-row product takes (codes).
+int mx_pass_rows(size_t rows, int kt) { return rows <= 16 ? 16 : rows <= 32 || mx_split(kt) == 2 ? 32 : 64; }
+
 // The few-row product: fills the launch shape into `a` and launches kernel
 // first + split (16 rows at a time), or with as many rows, which are codes, the
 // forms of 32 and 64 that follow it (K past 4096 has none of 64).
 nh_status launch_mx_stream(nh_context* ctx, KernelId first, MxStreamArgs a, size_t rows, bool requant,
                            unsigned workgroups, unsigned experts, nh_stream stream, nh_error* err) {
     const int split = mx_split(a.kt), c = 2 << split, t = requant ? 2 : 1;
-    const int form = rows <= 16 ? 0 : rows <= 32 || split == 2 ? 1 : 2;
+    const int pass = mx_pass_rows(rows, a.kt), form = pass == 16 ? 0 : pass == 32 ? 1 : 2;
     a.row_blocks = 1 << form;
     a.waves = (a.kt + c - 1) / c;
     a.groups = 8 / a.waves;
@@ -61,23 +64,38 @@ nh_status launch_mx_tiles(nh_context* ctx, const void* x, nh_dtype dtype, size_t
 
 nh_status launch_mx_gemm(nh_context* ctx, const uint8_t* a, const uint8_t* w, const float* bias, size_t m, size_t n,
                          size_t k, void* out, nh_dtype out_dtype, nh_stream stream, nh_error* err) {
+    // Tiles by time: a round of workgroups takes so many us per K tile with every
+    // CU at its full number of them, or with one per CU at most, and so many for
+    // its outputs.  From 72 products of 80..2048 rows, 1024..21504 columns, K
+    // 512..8192, each with every tile; the choice is within 8% of the best of
+    // them but where few tiles meet a long K (2048 x 8192 -> 4096: 256 / 128 / 64
+    // tiles take 68.5 / 57.5 / 72.9 us; 8192 -> 8192 76 / 98 / 127; 300 x 8192 ->
+    // 4096 62 / 37 / 21).
     struct Tile {
         KernelId id;
-        int bm, bn, threads, ks, stages, per_cu;
+        int b, threads, ks, stages, per_cu;
+        double full, one, store;
     };
-    static const Tile kTiles[] = {{K_MX_GEMM_256, 256, 256, 512, 1, 4, 1}, {K_MX_GEMM_256_128, 256, 128, 512, 1, 5, 1},
-                                  {K_MX_GEMM_128, 128, 128, 256, 1, 4, 2}, {K_MX_GEMM_64, 64, 64, 256, 4, 2, 2}};
+    static const Tile kTiles[] = {{K_MX_GEMM_256, 256, 512, 1, 4, 1, 0.8, 0.8, 6.0},
+                                  {K_MX_GEMM_128, 128, 256, 1, 4, 2, 0.72, 0.42, 3.4},
+                                  {K_MX_GEMM_64, 64, 256, 4, 2, 2, 0.31, 0.18, 1.1}};
     const size_t cus = (size_t)ctx->cu_count;
-    const Tile* t = &kTiles[3];
-    for (const Tile& c : kTiles)
-        if (((m + c.bm - 1) / c.bm) * ((n + c.bn - 1) / c.bn) >= cus) {
+    const double kt = (double)mx_k_tiles(k);
+    const Tile* t = nullptr;
+    double least = 0.0;
+    for (const Tile& c : kTiles) {
+        const size_t tiles = ((m + c.b - 1) / c.b) * ((n + c.b - 1) / c.b), round = cus * c.per_cu, rest = tiles % round;
+        const double time = (double)(tiles / round) * (kt * c.full + c.store) +
+                            (rest == 0 ? 0.0 : kt * (rest <= cus ? c.one : c.full) + c.store);
+        if (!t || time < least) {
             t = &c;
-            break;
+            least = time;
         }
-    MxGemmArgs g{a, w, bias, out, (int)m, (int)n, (int)mx_k_tiles(k), (int)mx_k_pieces(k), (int)((m + t->bm - 1) / t->bm),
-                 (int)((n + t->bn - 1) / t->bn), out_dtype, 0};
+    }
+    MxGemmArgs g{a, w, bias, out, (int)m, (int)n, (int)mx_k_tiles(k), (int)mx_k_pieces(k), (int)((m + t->b - 1) / t->b),
+                 (int)((n + t->b - 1) / t->b), out_dtype, 0};
     // the ring's stages, the pieces of scales that they span (mx_gemm_pieces), a spare KiB
-    const size_t tiles = (size_t)g.tiles_m * g.tiles_n, row_tiles = (size_t)(t->bm + t->bn) / 16;
+    const size_t tiles = (size_t)g.tiles_m * g.tiles_n, row_tiles = (size_t)2 * t->b / 16;
     const size_t pieces = t->ks == 4 ? t->stages : t->stages / 2 + 1;
     const size_t lds = row_tiles * ((size_t)t->stages * t->ks * 1024 + pieces * 256) + 1024;
     const unsigned grid = (unsigned)std::min(tiles, cus * t->per_cu);
@@ -179,6 +197,7 @@ nh_status nh_linear_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
     a.x_dtype = x_dtype;
     a.out_dtype = out_dtype;
     a.gather_div = 1;
+    a.row_parts = 1;
     const unsigned cus = (unsigned)ctx->cu_count;
     if (need == 0) {
         a.x = x;
@@ -303,12 +322,23 @@ nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype,
     const double live = expected_experts(experts, R), load = (double)R / (double)experts, q = std::exp(-load);
     const double var = (double)experts * (q - (1.0 + load) * q * q);
     const double most = std::min({(double)experts, (double)R, live + 3.0 * std::sqrt(std::max(0.0, var))});
-    const unsigned parts = (unsigned)std::max(1.0, (double)ctx->cu_count / most);
+    // An expert's passes go to workgroups of their own where the mean expert has
+    // several (700 tokens, 2 of 8 experts, 4096 x 1792: 97 us one after another, 85).
+    auto plan = [&](MxStreamArgs& a, size_t n, size_t k, unsigned* parts, unsigned* slots) {
+        a.N = (int)n;
+        a.K = (int)k;
+        a.kt = (int)mx_k_tiles(k);
+        a.kq = (int)mx_k_pieces(k);
+        const double pass = mx_pass_rows(tokens, a.kt);
+        a.row_parts = load <= pass ? 1 : (int)std::min(std::ceil((load + 2.0 * std::sqrt(load)) / pass), 32.0);
+        *parts = (unsigned)std::max(1.0, (double)ctx->cu_count / (most * a.row_parts));
+        *slots = (unsigned)(a.compact ? std::min(experts, R) : experts) * (unsigned)a.row_parts;
+    };
+    unsigned parts, slots;
     MxStreamArgs a{};
     a.offsets = offsets;
     a.experts = (int)experts;
     a.compact = live < 0.9 * (double)experts ? 1 : 0;
-    const unsigned slots = (unsigned)(a.compact ? std::min(experts, R) : experts);
     a.xcodes = ws + off[5];
     a.xscales = ws + off[6];
     a.w = w_up;
@@ -320,10 +350,7 @@ nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype,
     a.perm = perm;
     a.gather_div = (int)top_k;
     a.M = (int)R;
-    a.N = (int)inter;
-    a.K = (int)hidden;
-    a.kt = (int)mx_k_tiles(hidden);
-    a.kq = (int)mx_k_pieces(hidden);
+    plan(a, inter, hidden, &parts, &slots);
     if ((st = launch_mx_stream(ctx, K_MX_REQUANT2, a, tokens, true, parts, slots, stream, err)))
         return st;
     a.xcodes = ws + off[7];
@@ -334,10 +361,7 @@ nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype,
     a.perm = nullptr;
     a.out = d;
     a.out_dtype = DT_F32;
-    a.N = (int)hidden;
-    a.K = (int)inter;
-    a.kt = (int)mx_k_tiles(inter);
-    a.kq = (int)mx_k_pieces(inter);
+    plan(a, hidden, inter, &parts, &slots);
     if ((st = launch_mx_stream(ctx, K_MX_TOK2, a, tokens, false, parts, slots, stream, err))) return st;
     return nh_moe_combine_shared(ctx, d, pos, wts, shared, tokens, top_k, hidden, out, out_dtype, stream, err);
 }
@@ -421,7 +445,12 @@ nh_status nh_moe_balance_loss(nh_context* ctx, const float* logits, const int32_
     a.softmax = softmax ? 1 : 0;
     a.coefficient = coefficient;
     a.group = p.group;
-    if ((st = launch(ctx, K_BALANCE_PARTIAL, (unsigned)p.chunks, 1024, 17 * experts * 4, stream, a, err))) return st;
+    // a few rows, one sequence: one workgroup and launch (64 x 128: 13.9 us forward
+    // and backward in three launches, 10.8 in two)
+    a.single = sequences == 1 && tokens * experts <= 256 * 128 ? 1 : 0;
+    const size_t lds = 17 * experts * 4 + 256;
+    if (a.single) return launch(ctx, K_BALANCE_PARTIAL, 1, 1024, lds, stream, a, err);
+    if ((st = launch(ctx, K_BALANCE_PARTIAL, (unsigned)p.chunks, 1024, lds, stream, a, err))) return st;
     return launch(ctx, K_BALANCE_REDUCE, (unsigned)sequences, 1024, 128 + 2 * 1024 * 4, stream, a, err);
 }
 
@@ -448,9 +477,11 @@ nh_status nh_moe_balance_loss_backward(nh_context* ctx, const float* logits, con
     a.softmax = softmax ? 1 : 0;
     a.coefficient = coefficient;
     a.group = p.group;
-    const size_t rows = 4 * (64 / (size_t)p.group);  // tokens per workgroup and turn
-    const size_t grid = std::min<size_t>((tokens + rows - 1) / rows, (size_t)ctx->cu_count * 8);
-    return launch(ctx, K_BALANCE_BACKWARD, (unsigned)grid, 256, 0, stream, a, err);
+    // chunks for four workgroups of four waves per CU, of 32 tokens at least
+    a.chunk = (int)std::max<size_t>(32, (tokens + 4 * (size_t)ctx->cu_count - 1) / (4 * (size_t)ctx->cu_count));
+    a.chunks = (int)(tokens / (size_t)a.chunk + sequences);
+    a.padding = seq_offsets ? 64 : 0;
+    return launch(ctx, K_BALANCE_BACKWARD, (unsigned)(a.chunks + a.padding), 256, 0, stream, a, err);
 }
 
 }  // extern "C"

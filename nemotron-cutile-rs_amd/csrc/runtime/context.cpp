@@ -109,7 +109,6 @@ const char* const kKernelSymbols[K_COUNT] = {  // in KernelId order
     "nh_mx_stream_requant2_64_kernel",        // K_MX_REQUANT2_64
     "nh_mx_stream_requant4_64_kernel",        // K_MX_REQUANT4_64
     "nh_mx_gemm_256x256_kernel",           // K_MX_GEMM_256
-    "nh_mx_gemm_256x128_kernel",           // K_MX_GEMM_256_128
     "nh_mx_gemm_128x128_kernel",           // K_MX_GEMM_128
     "nh_mx_gemm_64x64_kernel",             // K_MX_GEMM_64
     "nh_moe_balance_partial_kernel",       // K_BALANCE_PARTIAL

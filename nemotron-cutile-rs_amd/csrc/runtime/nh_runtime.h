@@ -113,7 +113,6 @@ enum KernelId : int {
     K_MX_REQUANT2_64,
     K_MX_REQUANT4_64,
     K_MX_GEMM_256,               // LDS-tiled product of two tiled operands
-    K_MX_GEMM_256_128,
     K_MX_GEMM_128,
     K_MX_GEMM_64,
     K_BALANCE_PARTIAL,           // router balance: sums per chunk of tokens
