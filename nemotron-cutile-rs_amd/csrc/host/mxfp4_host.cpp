@@ -2,6 +2,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <exception>
+#include <new>
 #include <vector>
 
 #include "../kernels/mx_numerics.h"
@@ -34,6 +36,16 @@ nh_status find_nonfinite(const void* x, nh_dtype d, size_t n, const char* what, 
         return set_error(err, NH_NON_FINITE_INPUT, "non-finite %s value %g at index %zu", what, (double)v, i);
     }
     return NH_OK;
+}
+
+// Runs the body of a twin; memory that is not there is an error, no exception.
+template <class Body>
+nh_status guarded(nh_error* err, Body body) {
+    try {
+        return body();
+    } catch (const std::exception&) {  // std::bad_alloc, std::length_error
+        return set_error(err, NH_DEVICE_ERROR, "out of host memory");
+    }
 }
 
 // One block of `count` values: its scale byte, and their codes.
@@ -148,13 +160,16 @@ nh_status nh_linear_mxfp4_host(const void* x, nh_dtype x_dtype, const uint8_t* w
     if (!mul_ok(m, k, &mk) || !mul_ok(m, n, &mn) || nh_tiled_mxfp4_weights_bytes(n, k) == 0)
         return set_error(err, NH_INVALID_SHAPE, "linear shape m=%zu n=%zu k=%zu overflows", m, n, k);
     if ((st = find_nonfinite(x, x_dtype, mk, "input", err))) return st;
-    std::vector<float> xv(mk), row(k);
-    for (size_t i = 0; i < m; ++i) requantize_row(x, x_dtype, i, k, xv.data() + i * k);
-    for (size_t j = 0; j < n; ++j) {
-        tiled_row(w, j, k, row.data());
-        for (size_t i = 0; i < m; ++i) store_f32(out, i * n + j, dot(xv.data() + i * k, row.data(), k, bias, j), out_dtype);
-    }
-    return NH_OK;
+    return guarded(err, [&]() -> nh_status {
+        std::vector<float> xv(mk), row(k);
+        for (size_t i = 0; i < m; ++i) requantize_row(x, x_dtype, i, k, xv.data() + i * k);
+        for (size_t j = 0; j < n; ++j) {
+            tiled_row(w, j, k, row.data());
+            for (size_t i = 0; i < m; ++i)
+                store_f32(out, i * n + j, dot(xv.data() + i * k, row.data(), k, bias, j), out_dtype);
+        }
+        return NH_OK;
+    });
 }
 
 nh_status nh_moe_forward_mxfp4_host(const void* x, nh_dtype x_dtype, const float* logits, size_t tokens, size_t hidden,
@@ -173,40 +188,46 @@ nh_status nh_moe_forward_mxfp4_host(const void* x, nh_dtype x_dtype, const float
     nh_status st;
     if ((st = check_dtype(x_dtype, err)) || (st = check_dtype(out_dtype, err))) return st;
     if ((st = find_nonfinite(x, x_dtype, tokens * hidden, "input", err))) return st;
-    std::vector<int32_t> idx(routes), offsets(experts + 1), perm(routes), pos(routes);
-    std::vector<float> wts(routes), xv(tokens * hidden), h(routes * inter), hq(inter), d(routes * hidden), row;
-    if ((st = nh_moe_route_sigmoid_topk_host(logits, tokens * experts, tokens, experts, top_k, renormalize, scaling,
-                                             idx.data(), routes, wts.data(), routes, err)))
-        return st;
-    if ((st = nh_moe_permute_host(idx.data(), tokens, top_k, experts, offsets.data(), perm.data(), pos.data(), err)))
-        return st;
-    for (size_t t = 0; t < tokens; ++t) requantize_row(x, x_dtype, t, hidden, xv.data() + t * hidden);
-    const float *b_up = biases ? biases->up : nullptr, *b_down = biases ? biases->down : nullptr;
-    row.resize(std::max(hidden, inter));
-    for (size_t e = 0; e < experts; ++e) {
-        const size_t s0 = (size_t)offsets[e], s1 = (size_t)offsets[e + 1];
-        if (s0 == s1) continue;
-        for (size_t j = 0; j < inter; ++j) {
-            tiled_row(w_up + e * nh_tiled_mxfp4_weights_bytes(inter, hidden), j, hidden, row.data());
-            for (size_t s = s0; s < s1; ++s)
-                h[s * inter + j] = relu2(dot(xv.data() + (size_t)perm[s] / top_k * hidden, row.data(), hidden,
-                                             b_up ? b_up + e * inter : nullptr, j));
+    return guarded(err, [&]() -> nh_status {
+        std::vector<int32_t> idx(routes), offsets(experts + 1), perm(routes), pos(routes);
+        std::vector<float> wts(routes), xv(tokens * hidden), h(routes * inter), hq(inter), d(routes * hidden), row;
+        if ((st = nh_moe_route_sigmoid_topk_host(logits, tokens * experts, tokens, experts, top_k, renormalize, scaling,
+                                                 idx.data(), routes, wts.data(), routes, err)))
+            return st;
+        if ((st = nh_moe_permute_host(idx.data(), tokens, top_k, experts, offsets.data(), perm.data(), pos.data(), err)))
+            return st;
+        for (size_t t = 0; t < tokens; ++t) requantize_row(x, x_dtype, t, hidden, xv.data() + t * hidden);
+        const float *b_up = biases ? biases->up : nullptr, *b_down = biases ? biases->down : nullptr;
+        row.resize(std::max(hidden, inter));
+        for (size_t e = 0; e < experts; ++e) {
+            const size_t s0 = (size_t)offsets[e], s1 = (size_t)offsets[e + 1];
+            if (s0 == s1) continue;
+            for (size_t j = 0; j < inter; ++j) {
+                tiled_row(w_up + e * nh_tiled_mxfp4_weights_bytes(inter, hidden), j, hidden, row.data());
+                for (size_t s = s0; s < s1; ++s) {
+                    // a NaN (of a weight's block with no value) stays one, as on the device
+                    const float y = dot(xv.data() + (size_t)perm[s] / top_k * hidden, row.data(), hidden,
+                                        b_up ? b_up + e * inter : nullptr, j);
+                    h[s * inter + j] = y != y ? y : relu2(y);
+                }
+            }
         }
-    }
-    if ((st = find_nonfinite(h.data(), NH_F32, h.size(), "intermediate", err))) return st;
-    for (size_t s = 0; s < routes; ++s) {
-        requantize_row(h.data(), NH_F32, s, inter, hq.data());
-        std::copy(hq.begin(), hq.end(), h.begin() + s * inter);
-    }
-    for (size_t e = 0; e < experts; ++e) {
-        const size_t s0 = (size_t)offsets[e], s1 = (size_t)offsets[e + 1];
-        for (size_t j = 0; s0 < s1 && j < hidden; ++j) {
-            tiled_row(w_down + e * nh_tiled_mxfp4_weights_bytes(hidden, inter), j, inter, row.data());
-            for (size_t s = s0; s < s1; ++s)
-                d[s * hidden + j] = dot(h.data() + s * inter, row.data(), inter, b_down ? b_down + e * hidden : nullptr, j);
+        if ((st = find_nonfinite(h.data(), NH_F32, h.size(), "intermediate", err))) return st;
+        for (size_t s = 0; s < routes; ++s) {
+            requantize_row(h.data(), NH_F32, s, inter, hq.data());
+            std::copy(hq.begin(), hq.end(), h.begin() + s * inter);
         }
-    }
-    return nh_moe_combine_shared_host(d.data(), pos.data(), wts.data(), shared, tokens, top_k, hidden, out, out_dtype, err);
+        for (size_t e = 0; e < experts; ++e) {
+            const size_t s0 = (size_t)offsets[e], s1 = (size_t)offsets[e + 1];
+            for (size_t j = 0; s0 < s1 && j < hidden; ++j) {
+                tiled_row(w_down + e * nh_tiled_mxfp4_weights_bytes(hidden, inter), j, inter, row.data());
+                for (size_t s = s0; s < s1; ++s)
+                    d[s * hidden + j] =
+                        dot(h.data() + s * inter, row.data(), inter, b_down ? b_down + e * hidden : nullptr, j);
+            }
+        }
+        return nh_moe_combine_shared_host(d.data(), pos.data(), wts.data(), shared, tokens, top_k, hidden, out, out_dtype, err);
+    });
 }
 
 }  // extern "C"
@@ -264,29 +285,31 @@ nh_status nh_moe_balance_loss_host(const float* logits, const int32_t* indices, 
     clear_error(err);
     nh_status st = check_balance(sequences, seq_offsets, tokens, experts, top_k, coefficient, err);
     if (st) return st;
-    std::vector<double> p(experts), slope(experts), sums(experts);
-    double total = 0.0;
-    for (size_t s = 0; s < sequences; ++s) {
-        size_t lo, hi;
-        bounds(seq_offsets, s, tokens, &lo, &hi);
-        std::fill(sums.begin(), sums.end(), 0.0);
-        int32_t* c = counts + s * experts;
-        std::fill(c, c + experts, 0);
-        for (size_t t = lo; t < hi; ++t) {
-            probabilities(logits + t * experts, experts, softmax, p.data(), slope.data());
-            for (size_t e = 0; e < experts; ++e) sums[e] += p[e];
-            for (size_t j = 0; j < top_k; ++j) {
-                const int32_t e = indices[t * top_k + j];
-                if (e >= 0 && (size_t)e < experts) ++c[e];
+    return guarded(err, [&]() -> nh_status {
+        std::vector<double> p(experts), slope(experts), sums(experts);
+        double total = 0.0;
+        for (size_t s = 0; s < sequences; ++s) {
+            size_t lo, hi;
+            bounds(seq_offsets, s, tokens, &lo, &hi);
+            std::fill(sums.begin(), sums.end(), 0.0);
+            int32_t* c = counts + s * experts;
+            std::fill(c, c + experts, 0);
+            for (size_t t = lo; t < hi; ++t) {
+                probabilities(logits + t * experts, experts, softmax, p.data(), slope.data());
+                for (size_t e = 0; e < experts; ++e) sums[e] += p[e];
+                for (size_t j = 0; j < top_k; ++j) {
+                    const int32_t e = indices[t * top_k + j];
+                    if (e >= 0 && (size_t)e < experts) ++c[e];
+                }
             }
+            double dot = 0.0;
+            const double n = (double)(hi - lo);
+            for (size_t e = 0; e < experts; ++e) dot += (double)c[e] * sums[e];
+            if (hi > lo) total += (double)coefficient / (double)sequences * dot * (double)experts / ((double)top_k * n * n);
         }
-        double dot = 0.0;
-        const double n = (double)(hi - lo);
-        for (size_t e = 0; e < experts; ++e) dot += (double)c[e] * sums[e];
-        if (hi > lo) total += (double)coefficient / (double)sequences * dot * (double)experts / ((double)top_k * n * n);
-    }
-    *loss = (float)total;
-    return NH_OK;
+        *loss = (float)total;
+        return NH_OK;
+    });
 }
 
 nh_status nh_moe_balance_loss_backward_host(const float* logits, const int32_t* counts, const int32_t* seq_offsets,
@@ -296,21 +319,23 @@ nh_status nh_moe_balance_loss_backward_host(const float* logits, const int32_t* 
     nh_status st = check_balance(sequences, seq_offsets, tokens, experts, top_k, coefficient, err);
     if (st) return st;
     std::fill(dlogits, dlogits + tokens * experts, 0.0f);
-    std::vector<double> p(experts), slope(experts);
-    for (size_t s = 0; s < sequences; ++s) {
-        size_t lo, hi;
-        bounds(seq_offsets, s, tokens, &lo, &hi);
-        const double n = (double)(hi - lo), per = (double)experts / ((double)top_k * n);
-        for (size_t t = lo; t < hi; ++t) {
-            probabilities(logits + t * experts, experts, softmax, p.data(), slope.data());
-            double fp = 0.0;
-            for (size_t e = 0; e < experts; ++e) fp += (double)counts[s * experts + e] * per * p[e];
-            for (size_t e = 0; e < experts; ++e)
-                dlogits[t * experts + e] = (float)((double)*dloss * (double)coefficient / ((double)sequences * n) * p[e] *
-                                                   ((double)counts[s * experts + e] * per - fp) * slope[e]);
+    return guarded(err, [&]() -> nh_status {
+        std::vector<double> p(experts), slope(experts);
+        for (size_t s = 0; s < sequences; ++s) {
+            size_t lo, hi;
+            bounds(seq_offsets, s, tokens, &lo, &hi);
+            const double n = (double)(hi - lo), per = (double)experts / ((double)top_k * n);
+            for (size_t t = lo; t < hi; ++t) {
+                probabilities(logits + t * experts, experts, softmax, p.data(), slope.data());
+                double fp = 0.0;
+                for (size_t e = 0; e < experts; ++e) fp += (double)counts[s * experts + e] * per * p[e];
+                for (size_t e = 0; e < experts; ++e)
+                    dlogits[t * experts + e] = (float)((double)*dloss * (double)coefficient / ((double)sequences * n) * p[e] *
+                                                       ((double)counts[s * experts + e] * per - fp) * slope[e]);
+            }
         }
-    }
-    return NH_OK;
+        return NH_OK;
+    });
 }
 
 }  // extern "C"
