@@ -514,10 +514,11 @@ nh_status nh_tile_weights_mxfp4_host(const uint8_t *codes, const uint8_t *scales
  * 16 rows of k <= 16384 are one launch that streams the weights once and
  * touches no workspace; otherwise a launch quantizes the rows into the
  * workspace (nh_linear_mxfp4_workspace_size bytes, 16-byte aligned) ahead of
- * the product.  Deterministic.  Errors: INVALID_SHAPE (n or k == 0),
- * INVALID_ROW_COUNT (m == 0), INVALID_PARAMS (dtype), LENGTH_MISMATCH
- * "workspace", UNSUPPORTED outside nh_supports_linear_mxfp4 or for a
- * misaligned w or workspace. */
+ * the product; calls that may run at once need a workspace each.  out must
+ * not overlap x.  Deterministic.  Errors: INVALID_SHAPE (n or k == 0),
+ * INVALID_ROW_COUNT (m == 0), INVALID_PARAMS (dtype, a null operand, out over
+ * x), LENGTH_MISMATCH "workspace", UNSUPPORTED outside
+ * nh_supports_linear_mxfp4 or for a misaligned w or workspace. */
 int nh_supports_linear_mxfp4(size_t m, size_t n, size_t k);
 size_t nh_linear_mxfp4_workspace_size(size_t m, size_t n, size_t k);
 nh_status nh_linear_mxfp4(nh_context *ctx, const void *x, nh_dtype x_dtype, const uint8_t *w, const float *bias,
@@ -534,10 +535,10 @@ nh_status nh_linear_mxfp4_host(const void *x, nh_dtype x_dtype, const uint8_t *w
  * first, e.g. a shared expert's output).  w_up is `experts` tiled
  * [inter][hidden] matrices at a stride of nh_tiled_mxfp4_weights_bytes(inter,
  * hidden), w_down tiled [hidden][inter] ones.  biases: up and down (the shared
- * ones must be NULL).  h stays on the device in MXFP4 (a NaN in it marks its
- * block, and `nonfinite` reports it as "intermediate").  The workspace starts
- * with the fields of nh_moe_workspace_layout at other offsets
- * (nh_moe_mxfp4_workspace_layout).  Errors as nh_moe_forward_w8a8. */
+ * ones must be NULL).  h stays on the device in MXFP4 (a NaN or an infinity in
+ * it marks its block, and `nonfinite` reports it as "intermediate").  The
+ * workspace holds what nh_moe_workspace_layout names, at the offsets of
+ * nh_moe_mxfp4_workspace_layout.  Errors as nh_moe_forward_w8a8. */
 int nh_supports_moe_forward_mxfp4(size_t tokens, size_t hidden, size_t inter, size_t experts, size_t top_k);
 size_t nh_moe_forward_mxfp4_workspace_size(size_t tokens, size_t hidden, size_t inter, size_t experts, size_t top_k);
 /* byte offsets in the workspace of: [0] indices i32[T*k], [1] weights
@@ -573,8 +574,8 @@ nh_status nh_moe_forward_mxfp4_host(const void *x, nh_dtype x_dtype, const float
  * bytes, 16-byte aligned) is free again once the call has run.  Errors:
  * INVALID_SHAPE (experts, top_k or sequences == 0; sequences != 1 without
  * offsets), INVALID_PARAMS (a coefficient that is not finite), LENGTH_MISMATCH
- * "workspace", UNSUPPORTED (experts > 1024, sizes past 2^31, alignment).  No
- * counterpart in the reference. */
+ * "workspace", UNSUPPORTED (experts > 1024, sequences > 16384, sizes past 2^31,
+ * alignment).  No counterpart in the reference. */
 size_t nh_moe_balance_loss_workspace_size(size_t sequences, size_t tokens, size_t experts);
 nh_status nh_moe_balance_loss(nh_context *ctx, const float *logits, const int32_t *indices, const int32_t *seq_offsets,
                               size_t sequences, size_t tokens, size_t experts, size_t top_k, int softmax,

@@ -126,6 +126,12 @@ __device__ __forceinline__ void mx_gemm(const MxGemmArgs& a, int8_t* smem) {
         if (bf16 && mt + BM <= a.M && nt + BN <= a.N && FN % 2 == 0) {
             const int g = lane >> 4;
             uint16_t* row = (uint16_t*)a.out + (int64_t)m0 * a.N + n0 + (g & 1) * 16 + (g >> 1) * 8;
+            float bv[FN][4];
+            if (a.bias)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) bv[j][r] = a.bias[n0 + j * 16 + 4 * g + r];
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -138,7 +144,7 @@ __device__ __forceinline__ void mx_gemm(const MxGemmArgs& a, int8_t* smem) {
                         for (int r = 0; r < 4; ++r) y[r] = acc[i][j + h][r];
                         if (a.bias) {
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) y[r] = y[r] + a.bias[n0 + (j + h) * 16 + 4 * g + r];
+                            for (int r = 0; r < 4; ++r) y[r] = y[r] + bv[j + h][r];
                         }
                         w[2 * h] = f32x2_to_bf16x2(y[0], y[1]);
                         w[2 * h + 1] = f32x2_to_bf16x2(y[2], y[3]);

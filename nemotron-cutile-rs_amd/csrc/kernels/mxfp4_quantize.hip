@@ -56,11 +56,15 @@ extern "C" __global__ __launch_bounds__(256) void nh_quantize_mxfp4_kernel(MxQua
     }
 }
 
-// 16 rows x 512 columns (one scale piece) per workgroup.  Rows are read whole
+// 16 rows x 512 columns (one scale piece) per workgroup.  ONCE (many rows): past
+// the caches, which then keep the codes for the product (2048 x 4096 -> 21504:
+// 111.0 us, 112.9 without; 512 x 4096 -> 4096, where x itself is still there: 14.0
+// against 13.6).  Rows are read whole
 // waves at a time (1 KiB of bf16), the codes meet in LDS in tile order and
 // leave as whole tiles (or 256 bytes of a row in the token form).
 // (256 of the workgroup's threads, `tid` of them; every thread of the workgroup
 // calls it, for one barrier.)
+template <bool ONCE>
 __device__ __forceinline__ void mx_quantize_tiles(const MxQuantizeTilesArgs& a, int64_t block, int tid, uint32_t* codes,
                                                   uint8_t* scales) {
     const int lane = tid & 63, wave = tid >> 6;
@@ -73,7 +77,7 @@ __device__ __forceinline__ void mx_quantize_tiles(const MxQuantizeTilesArgs& a, 
     for (int i = 0; i < 4; ++i) {
         const int64_t row = rt * 16 + wave * 4 + i;
         count[i] = row < a.rows && c < a.cols ? min(8, a.cols - c) : 0;
-        mx_load8<true>(a.x, row * a.cols + c, count[i], a.x_dtype, v[i]);
+        mx_load8<ONCE>(a.x, row * a.cols + c, count[i], a.x_dtype, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -105,7 +109,10 @@ __device__ __forceinline__ void mx_quantize_tiles(const MxQuantizeTilesArgs& a, 
 extern "C" __global__ __launch_bounds__(256) void nh_quantize_mxfp4_tiles_kernel(MxQuantizeTilesArgs a) {
     __shared__ __align__(16) uint32_t codes[4 * 256];  // [K tile][lane][4]
     __shared__ __align__(4) uint8_t scales[256];       // [lane][K tile]
-    mx_quantize_tiles(a, blockIdx.x, threadIdx.x, codes, scales);
+    if (a.once)
+        mx_quantize_tiles<true>(a, blockIdx.x, threadIdx.x, codes, scales);
+    else
+        mx_quantize_tiles<false>(a, blockIdx.x, threadIdx.x, codes, scales);
 }
 
 // Codes and scales back to values: exact in f32, and in bf16 (two significant
@@ -209,7 +216,7 @@ extern "C" __global__ __launch_bounds__(1024) void nh_mx_moe_prep_kernel(MxMoePr
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if ((int)blockIdx.x >= a.route_blocks) {  // uniform
         const int64_t block = ((int64_t)blockIdx.x - a.route_blocks) * 4 + (tid >> 8);
-        mx_quantize_tiles(a.q, block, tid & 255, codes[tid >> 8], scales[tid >> 8]);  // past the rows: nothing
+        mx_quantize_tiles<false>(a.q, block, tid & 255, codes[tid >> 8], scales[tid >> 8]);  // past the rows: nothing
         return;
     }
     for (int token = (int)blockIdx.x * 16 + wave; token < a.r.tokens; token += 16 * a.route_blocks) {

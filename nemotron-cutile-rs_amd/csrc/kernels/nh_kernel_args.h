@@ -380,7 +380,7 @@ struct MxQuantizeTilesArgs {
     int32_t kt, kq;
     int32_t x_dtype;
     int32_t token;
-    int32_t pad_;
+    int32_t once;         // x is not read again soon: past the caches
 };
 
 struct MxDequantizeArgs {

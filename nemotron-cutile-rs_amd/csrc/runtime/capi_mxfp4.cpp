@@ -1,6 +1,7 @@
 // Device entry points of the MXFP4 operators: validate on the host, then enqueue.
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 
 #include "../kernels/mx_numerics.h"
 #include "nh_runtime.h"
@@ -17,6 +18,13 @@ constexpr size_t kMxRowsMaxK = 16384;
 // (index 0..3).  More per wave where K leaves a wave too few loads to hide
 // their latency, and the other waves go to groups of their own.
 int mx_split(int kt) { return kt <= 8 ? 0 : kt <= 32 ? 1 : kt <= 64 ? 2 : 3; }
+
+// An operand that a call reads or writes has to be there.
+nh_status check_given(std::initializer_list<const void*> operands, nh_error* err) {
+    for (const void* p : operands)
+        if (!p) return set_error(err, NH_INVALID_PARAMS, "null operand");
+    return NH_OK;
+}
 
 // A row of `cols` values in `rows`: what the conversions address.
 nh_status check_mx_rows(size_t rows, size_t cols, nh_error* err) {
@@ -58,7 +66,7 @@ nh_status launch_mx_stream(nh_context* ctx, KernelId first, MxStreamArgs a, size
 nh_status launch_mx_tiles(nh_context* ctx, const void* x, nh_dtype dtype, size_t rows, size_t k, uint8_t* out,
                           uint8_t* token_scales, uint64_t* nonfinite, nh_stream stream, nh_error* err) {
     MxQuantizeTilesArgs q{x, out, token_scales, nonfinite, (int64_t)rows, (int32_t)k, (int)mx_k_tiles(k),
-                          (int)mx_k_pieces(k), dtype, token_scales ? 1 : 0, 0};
+                          (int)mx_k_pieces(k), dtype, token_scales ? 1 : 0, rows * k >= (4u << 20) ? 1 : 0};
     return launch(ctx, K_MX_QUANTIZE_TILES, (unsigned)((rows + 15) / 16 * q.kq), 256, 0, stream, q, err);
 }
 
@@ -111,6 +119,7 @@ nh_status nh_quantize_rows_mxfp4(nh_context* ctx, const void* x, nh_dtype dtype,
     clear_error(err);
     nh_status st;
     if ((st = check_dtype(dtype, err)) || (st = check_mx_rows(rows, cols, err))) return st;
+    if (rows != 0 && cols != 0 && (st = check_given({x, codes, scales}, err))) return st;
     if ((st = bind_device(ctx, err))) return st;
     if (rows == 0 || cols == 0) return NH_OK;
     const int64_t row_units = (int64_t)mx_row_blocks(cols) * 4, units = (int64_t)rows * row_units;
@@ -124,6 +133,7 @@ nh_status nh_dequantize_mxfp4(nh_context* ctx, const uint8_t* codes, const uint8
     clear_error(err);
     nh_status st;
     if ((st = check_dtype(out_dtype, err)) || (st = check_mx_rows(rows, cols, err))) return st;
+    if (rows != 0 && cols != 0 && (st = check_given({codes, scales, out}, err))) return st;
     if ((st = bind_device(ctx, err))) return st;
     if (rows == 0 || cols == 0) return NH_OK;
     const int64_t row_units = (int64_t)mx_row_blocks(cols) * 4, units = (int64_t)rows * row_units;
@@ -145,8 +155,8 @@ nh_status nh_tile_weights_mxfp4(nh_context* ctx, const uint8_t* codes, const uin
     if (n >= (1u << 31) || k > (size_t)kMaxGrid - 128) return set_error(err, NH_UNSUPPORTED, "n and k must be < 2^31");
     if (tiled_len != need) return mismatch(err, "tiled", need, tiled_len);
     if (!aligned16(tiled)) return set_error(err, NH_UNSUPPORTED, "tiled must be 16-byte aligned");
-    nh_status st = bind_device(ctx, err);
-    if (st) return st;
+    nh_status st;
+    if ((st = check_given({codes, scales, tiled}, err)) || (st = bind_device(ctx, err))) return st;
     const int kq = (int)mx_k_pieces(k);
     MxTileArgs a{codes, scales, tiled, (int64_t)((n + 15) / 16) * kq * 64, (int64_t)n, (int32_t)k, (int)mx_k_tiles(k), kq, 0};
     const int64_t grid = std::min<int64_t>((a.lanes + 255) / 256, 1 << 20);
@@ -177,6 +187,7 @@ nh_status nh_linear_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
     if (!nh_supports_linear_mxfp4(m, n, k))
         return set_error(err, NH_UNSUPPORTED, "shape m=%zu n=%zu k=%zu outside the gfx950 envelope (k <= 131072, "
                          "m < 2^24, n < 2^28, m * n < 2^40)", m, n, k);
+    if ((st = check_given({x, w, out}, err))) return st;
     if (!aligned16(w)) return set_error(err, NH_UNSUPPORTED, "w must be 16-byte aligned");
     const size_t need = nh_linear_mxfp4_workspace_size(m, n, k);
     if (need && (!workspace || workspace_bytes < need)) return mismatch(err, "workspace", need, workspace_bytes);
@@ -285,6 +296,7 @@ nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype,
     if (!nh_supports_moe_forward_mxfp4(tokens, hidden, inter, experts, top_k))
         return set_error(err, NH_UNSUPPORTED, "MoE shape outside the gfx950 envelope (experts <= 1024, top_k <= 64, "
                          "hidden and inter <= 8192)");
+    if ((st = check_given({x, logits, w_up, w_down, out}, err))) return st;
     if (!workspace || workspace_bytes < off[10]) return mismatch(err, "workspace", off[10], workspace_bytes);
     if (!aligned16(workspace) || !aligned16(w_up) || !aligned16(w_down))
         return set_error(err, NH_UNSUPPORTED, "weights and workspace must be 16-byte aligned");
@@ -377,7 +389,8 @@ struct BalancePlan {
 };
 
 bool plan_balance(size_t sequences, size_t tokens, size_t experts, BalancePlan* p) {
-    if (sequences == 0 || experts == 0 || sequences >= (1u << 30) || tokens >= (1u << 30) || experts > 1024 ||
+    // every workgroup walks the offsets, 64 at a time
+    if (sequences == 0 || experts == 0 || sequences > 16384 || tokens >= (1u << 30) || experts > 1024 ||
         tokens * experts >= (1ull << 40))
         return false;
     // a chunk per CU of 256, of 64 tokens at least
@@ -400,8 +413,8 @@ nh_status check_balance(size_t sequences, const int32_t* seq_offsets, size_t tok
                          experts, top_k);
     if (!std::isfinite(coefficient)) return set_error(err, NH_INVALID_PARAMS, "coefficient must be finite");
     if (!plan_balance(sequences, tokens, experts, p) || top_k > 1024 || tokens * top_k >= (1ull << 31))
-        return set_error(err, NH_UNSUPPORTED, "device balance needs experts <= 1024, sequences and tokens < 2^30, "
-                         "tokens * top_k < 2^31");
+        return set_error(err, NH_UNSUPPORTED, "device balance needs experts <= 1024, sequences <= 16384, "
+                         "tokens < 2^30 and tokens * top_k < 2^31");
     return NH_OK;
 }
 
@@ -422,6 +435,8 @@ nh_status nh_moe_balance_loss(nh_context* ctx, const float* logits, const int32_
     BalancePlan p;
     nh_status st = check_balance(sequences, seq_offsets, tokens, experts, top_k, coefficient, &p, err);
     if (st) return st;
+    if ((st = check_given({counts, loss}, err))) return st;
+    if (tokens != 0 && (st = check_given({logits, indices}, err))) return st;
     if (!workspace || workspace_bytes < p.bytes) return mismatch(err, "workspace", p.bytes, workspace_bytes);
     if (!aligned16(workspace)) return set_error(err, NH_UNSUPPORTED, "workspace must be 16-byte aligned");
     if ((st = bind_device(ctx, err))) return st;
@@ -462,6 +477,7 @@ nh_status nh_moe_balance_loss_backward(nh_context* ctx, const float* logits, con
     BalancePlan p;
     nh_status st = check_balance(sequences, seq_offsets, tokens, experts, top_k, coefficient, &p, err);
     if (st) return st;
+    if (tokens != 0 && (st = check_given({logits, counts, dloss, dlogits}, err))) return st;
     if ((st = bind_device(ctx, err))) return st;
     if (tokens == 0) return NH_OK;
     BalanceArgs a{};
