@@ -191,7 +191,8 @@ LINEAR = [(1, 16, 32), (1, 1, 1), (3, 17, 33), (16, 48, 1024), (16, 40, 1025), (
           (16, 272, 4096), (1, 4099, 2701), (5, 64, 4097), (9, 130, 8192), (4, 16, 8200), (16, 35, 16384), (1, 5000, 512),
           (3, 40, 16385), (16, 16, 20000), (17, 16, 128), (17, 40, 1000), (64, 33, 2000), (50, 70, 4095), (33, 100, 4096),
           (64, 50, 8192), (31, 19, 5000), (64, 24, 9000), (65, 64, 512), (65, 1, 1), (100, 130, 300), (300, 515, 130),
-          (129, 200, 2701), (1040, 2050, 256), (1040, 2047, 700), (4100, 4100, 128), (4097, 4200, 384), (2050, 17000, 64)]
+          (129, 200, 2701), (1040, 2050, 256), (1040, 2047, 700), (4100, 4100, 128), (4097, 4200, 384), (2050, 17000, 64),
+          (20, 50, 3000), (1030, 8000, 128), (520, 16300, 1100), (2040, 16300, 384)]
 
 
 @pytest.mark.parametrize("m,n,k", LINEAR)
@@ -280,7 +281,8 @@ def route(logits, k, renormalize, scaling):
 # rows per expert from none to past one pass of 64; widths ragged against 32, 128 and 512; all five splits of K
 MOE = [(1, 64, 32, 8, 2), (3, 100, 70, 4, 1), (8, 1040, 200, 16, 6), (16, 333, 129, 3, 3), (17, 96, 33, 8, 2), (40, 256, 130, 60, 4),
        (70, 128, 96, 2, 1), (200, 160, 64, 2, 2), (33, 512, 1100, 5, 2), (20, 2100, 40, 4, 2), (5, 4200, 50, 4, 2), (24, 60, 4200, 3, 2),
-       (12, 48, 2200, 3, 2), (9, 8192, 32, 2, 1), (90, 7000, 36, 2, 2)]
+       (12, 48, 2200, 3, 2), (9, 8192, 32, 2, 1), (90, 7000, 36, 2, 2), (6, 60, 4200, 3, 2), (40, 2100, 40, 4, 2),
+       (10, 64, 32, 200, 4), (40, 32, 32, 300, 8)]
 
 
 @pytest.mark.parametrize("t,h,i,e,k", MOE)
@@ -347,6 +349,87 @@ def test_moe_layer_bf16_against_the_host_twin(ctx):
     # of about 1e-5 each to change a code, so one that does (a step of its block) stays within a row's tenth
     off = np.linalg.norm(got - want, axis=1) / np.linalg.norm(want, axis=1)
     assert (off < 0.1).all() and np.median(off) < 2.0 ** -8
+
+
+def test_moe_weights_without_a_value(ctx):
+    """A weight block of scale 255: a NaN column of h is a bad intermediate, a NaN column of the experts' output is none."""
+    t, h, i, e, k = 6, 96, 64, 4, 2
+    note("moe weight scale 255")
+    _, x, logits, ups, downs = moe_case(ctx, t, h, i, e, k, 5)
+    idx, _ = route(logits, k, 0, 1.0)
+    du, dd = tile_all(ctx, ups).numpy(), tile_all(ctx, downs).numpy()
+    need = NH.lib().nh_moe_forward_mxfp4_workspace_size(t, h, i, e, k)
+    bad_expert = int(idx[0, 0])
+    hit = (idx == bad_expert).any(axis=1)
+    assert hit.any() and not hit.all()
+    for which in ("up", "down"):
+        w = {"up": du.copy(), "down": dd.copy()}
+        n, cols = (i, h) if which == "up" else (h, i)
+        per = w[which].size // e
+        # row 5 of the expert's second 16 (r = 5 of row tile 1): block 1 of its one K tile, piece byte 4 lane
+        region = 1024 + 256
+        w[which][bad_expert * per + region + 1024 + 4 * (16 * 1 + 5)] = 255
+        up, down = ctx.upload(w["up"]), ctx.upload(w["down"])
+        ws, dx, dl = ctx.upload(np.full(need, 0xFF, np.uint8)), ctx.upload(x), ctx.upload(logits)
+        out, word = Guarded(ctx, (t, h), np.float32), ctx.upload(np.zeros(1, np.uint64))
+        NH.call("nh_moe_forward_mxfp4", ctx.handle, dx.ptr, NH.F32, dl.ptr, t, h, i, e, k, 0, 1.0, up.ptr, down.ptr, None, None,
+                out.ptr, NH.F32, ws.ptr, need, word.ptr, None)
+        ctx.synchronize()
+        got, (st, err) = out.numpy(), NH.call_status("nh_take_nonfinite", ctx.handle, word.ptr, None)
+        host = np.empty((t, h), np.float32)
+        hst, herr = NH.call_status("nh_moe_forward_mxfp4_host", x.ctypes.data, NH.F32, logits.ctypes.data, t, h, i, e, k, 0, 1.0,
+                                   w["up"].ctypes.data, w["down"].ctypes.data, None, None, host.ctypes.data, NH.F32)
+        if which == "up":
+            assert st == hst == NH.NON_FINITE_INPUT and err.argument == herr.argument == b"intermediate"
+            assert err.index == herr.index and err.index % i == 21
+            assert np.isnan(got[hit]).all() and np.isfinite(got[~hit]).all()
+        else:
+            assert st == hst == NH.OK
+            assert np.isnan(got[hit, 21]).all() and np.isnan(host[hit, 21]).all()
+            got[hit, 21] = 0
+            assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("m", [3, 40, 200])
+def test_linear_in_flight_twice_and_replayed(ctx, m):
+    """Calls in flight on two streams with a workspace each, eager and as graphs replayed over new rows."""
+    n, k = 300, 700
+    note(f"linear on two streams, captured and replayed, m={m}")
+    rng = np.random.default_rng(4)
+    w = R.grid_matrix(rng, n, k, 0)
+    tiled, _ = weights(ctx, w)
+    need = NH.lib().nh_linear_mxfp4_workspace_size(m, n, k)
+    graphs, runs = NH.HipGraphs(), []
+
+    class Run:
+        def __init__(self):
+            self.stream = NH.P()
+            NH.call("nh_stream_create", ctx.handle, C.byref(self.stream))
+            self.dx = ctx.empty((m, k), np.float32)
+            self.out, self.ws = Guarded(ctx, (m, n), np.float32), ctx.upload(np.full(max(need, 16), 0xFF, np.uint8))
+            self.graph = graphs.capture(self.stream, self.issue)
+            self.new_rows()
+
+        def new_rows(self):
+            self.x = R.grid_matrix(rng, m, k, 0).astype(np.float32)
+            self.dx.copy_from(self.x)
+
+        def issue(self):
+            NH.call("nh_linear_mxfp4", ctx.handle, self.dx.ptr, NH.F32, tiled.ptr, None, m, n, k, self.out.ptr, NH.F32,
+                    self.ws.ptr, need, None, self.stream)
+
+    runs = [Run(), Run()]
+    ctx.synchronize()
+    for turn in range(4):
+        for r in runs * 2:
+            r.issue() if turn == 0 else graphs.launch(r.graph[1], r.stream)
+        for r in runs:
+            ctx.synchronize(r.stream)
+            assert np.array_equal(r.out.numpy(), r.x @ w.T.astype(np.float32)), turn
+            r.new_rows()
+    for r in runs:
+        graphs.destroy(*r.graph)
+        NH.call("nh_stream_destroy", ctx.handle, r.stream)
 
 
 def test_moe_bad_values_stay_in_their_rows(ctx):

@@ -1,12 +1,15 @@
 """MXFP4 and the router's balance loss without a GPU: the host twins against plain 64-bit forms, the refusals of the
 device entry points, and which kernels a call launches."""
 import ctypes as C
+import os
+import re
 
 import numpy as np
 import pytest
 
 import mx_reference as R
 import nemotron_hip as NH
+import test_gpu_mxfp4 as G
 from dispatch import BIAS, OUT, S, W, W2, WS, X, Recorder
 
 
@@ -272,3 +275,100 @@ def test_linear_without_a_workspace_is_one_launch(rec):
         for m in (1, 16):
             assert len(mx_kernels(rec, m, 4096, k)) == 1
     assert [v[0] for v in mx_kernels(rec, 17, 4096, 4096)][0] == "quantize_mxfp4_tiles"
+
+
+def moe_launches(rec, t, h, i, e, k):
+    ws = NH.lib().nh_moe_forward_mxfp4_workspace_size(t, h, i, e, k)
+    return rec.launches("nh_moe_forward_mxfp4", X, NH.F32, S, t, h, i, e, k, 1, 1.0, W, W2, None, None, OUT, NH.F32, WS, ws, None,
+                        None)
+
+
+def test_every_kernel_is_reached_by_the_device_tests(rec):
+    """The products' and the layer's shapes of the device tests launch every MXFP4 kernel between them."""
+    seen = {v[0] for m, n, k in G.LINEAR for dt in (NH.F32, NH.BF16) for v in mx_kernels(rec, m, n, k, dt)}
+    seen |= {v[0] for shape in G.MOE for v in moe_launches(rec, *shape)}
+    src = open(os.path.join(os.path.dirname(NH.__file__), "csrc", "runtime", "context.cpp")).read()
+    names = set(re.findall(r'"nh_(mx_\w+)_kernel"', src))
+    assert len(names) > 25 and names <= seen, names - seen
+
+
+# Tiles by the rounds they take (launch_mx_gemm): large ones where they fill the chip, small ones where K is long and they do not.
+@pytest.mark.parametrize("m,n,k,tile,grid", [(2048, 21504, 4096, "256x256", 256), (8192, 8192, 8192, "256x256", 256),
+                                             (2048, 4096, 4096, "128x128", 512), (300, 4096, 8192, "64x64", 320),
+                                             (65, 64, 512, "64x64", 2), (1 << 23, 16, 128, "64x64", 512)])
+def test_gemm_tiles(rec, m, n, k, tile, grid):
+    assert mx_kernels(rec, m, n, k)[-1] == (f"mx_gemm_{tile}", grid, 1)
+
+
+# Each pass of an expert's rows has a workgroup of its own where the mean expert has several; a round of the 256 CUs at most.
+@pytest.mark.parametrize("shape", [(8, 2048, 1792, 128, 6), (500, 2688, 1856, 128, 6), (700, 4096, 1792, 8, 2), (1, 4096, 1792, 8, 2)])
+def test_moe_workgroups(rec, shape):
+    for name, gx, gy in moe_launches(rec, *shape):
+        if name.startswith("mx_stream"):
+            assert gx * min(gy, shape[0] * shape[4]) <= 256
+
+
+# One workgroup for few logits of one sequence, else a chunk per workgroup and a workgroup per sequence.
+def test_balance_launches(rec):
+    def launches(t, e, s=1, seq=None):
+        ws = NH.lib().nh_moe_balance_loss_workspace_size(s, t, e)
+        a = rec.launches("nh_moe_balance_loss", X, W, seq, s, t, e, 2, 0, 0.1, OUT, BIAS, WS, ws, None)
+        b = rec.launches("nh_moe_balance_loss_backward", X, OUT, seq, s, t, e, 2, 0, 0.1, BIAS, OUT, None)
+        return a, [v[0] for v in b]
+    back = ["moe_balance_backward"]
+    assert launches(256, 128) == ([("moe_balance_partial", 1, 1)], back)
+    assert launches(257, 128) == ([("moe_balance_partial", 5, 1), ("moe_balance_reduce", 1, 1)], back)
+    assert launches(64, 128, 3, S) == ([("moe_balance_partial", 4, 1), ("moe_balance_reduce", 3, 1)], back)
+    assert launches(131072, 128) == ([("moe_balance_partial", 257, 1), ("moe_balance_reduce", 1, 1)], back)
+
+
+def test_null_operands_are_refused(rec):
+    """Found before a launch: on a recording context, which would note it."""
+    def refused(name, args, operands):
+        for at in operands:
+            st, err = NH.call_status(name, rec.ctx, *(None if i == at else v for i, v in enumerate(args)))
+            assert st == NH.INVALID_PARAMS and err.message == b"null operand", (name, at)
+        assert NH.call_status(name, rec.ctx, *args)[0] == NH.OK
+    ws = NH.lib().nh_moe_forward_mxfp4_workspace_size(4, 64, 32, 8, 2)
+    bws = NH.lib().nh_moe_balance_loss_workspace_size(1, 64, 8)
+    refused("nh_quantize_rows_mxfp4", (X, NH.F32, 4, 64, OUT, S, None, None), (0, 4, 5))
+    refused("nh_dequantize_mxfp4", (X, S, 4, 64, OUT, NH.F32, None), (0, 1, 4))
+    refused("nh_linear_mxfp4", (X, NH.F32, W, None, 4, 64, 256, OUT, NH.F32, None, 0, None, None), (0, 2, 7))
+    refused("nh_moe_forward_mxfp4", (X, NH.F32, S, 4, 64, 32, 8, 2, 1, 1.0, W, W2, None, None, OUT, NH.F32, WS, ws, None, None),
+            (0, 2, 10, 11, 14))
+    refused("nh_moe_balance_loss", (X, W, None, 1, 64, 8, 2, 0, 0.1, OUT, BIAS, WS, bws, None), (0, 1, 9, 10))
+    refused("nh_moe_balance_loss_backward", (X, W, None, 1, 64, 8, 2, 0, 0.1, BIAS, OUT, None), (0, 1, 9, 10))
+    assert NH.call_status("nh_moe_balance_loss", rec.ctx, None, None, None, 1, 0, 8, 2, 0, 0.1, OUT, BIAS, WS, bws, None)[0] == NH.OK
+
+
+def test_many_sequences_are_refused(rec):
+    """Every workgroup walks the offsets."""
+    size = NH.lib().nh_moe_balance_loss_workspace_size
+    assert size(16384, 1 << 20, 128) > 0 == size(16385, 1 << 20, 128)
+    st, _ = NH.call_status("nh_moe_balance_loss", rec.ctx, X, W, S, 16385, 1 << 20, 128, 2, 0, 0.1, OUT, BIAS, WS, 1 << 40, None)
+    assert st == NH.UNSUPPORTED
+
+
+def test_host_twins_without_memory_are_an_error():
+    """A size that no allocation meets comes back as a status, never as an exception through the C entry."""
+    logits, idx = np.zeros((1, 4), np.float32), np.zeros((1, 1), np.int32)
+    counts, loss = np.zeros((1, 4), np.int32), np.zeros(1, np.float32)
+    st, err = NH.call_status("nh_moe_balance_loss_host", logits.ctypes.data, idx.ctypes.data, None, 1, 0, 1 << 60, 1, 0, 0.1,
+                             counts.ctypes.data, loss.ctypes.data)
+    assert st == NH.DEVICE_ERROR and err.message == b"out of host memory"
+
+
+def test_moe_host_of_weights_without_a_value():
+    """A weight block of scale 255 makes h NaN in its column: an intermediate with no value, as on the device."""
+    t, h, i, e, k = 2, 64, 32, 2, 1
+    rng = np.random.default_rng(0)
+    x, logits = rng.standard_normal((t, h)).astype(np.float32), np.array([[1, -1], [-1, 1]], np.float32)
+    tiles = [tile_host(*R.quantize(rng.standard_normal(s))[:2], *s) for s in ((i, h), (i, h), (h, i), (h, i))]
+    up, down = np.concatenate(tiles[:2]), np.concatenate(tiles[2:])
+    out = np.empty((t, h), np.float32)
+    args = (x.ctypes.data, NH.F32, logits.ctypes.data, t, h, i, e, k, 0, 1.0, up.ctypes.data, down.ctypes.data, None, None,
+            out.ctypes.data, NH.F32)
+    assert NH.call_status("nh_moe_forward_mxfp4_host", *args)[0] == NH.OK
+    up[tiles[0].size + 1024 + 4 * 3] = 255  # expert 1, row 3, block 0
+    st, err = NH.call_status("nh_moe_forward_mxfp4_host", *args)
+    assert st == NH.NON_FINITE_INPUT and err.argument == b"intermediate" and err.index == i + 3
