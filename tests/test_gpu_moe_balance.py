@@ -86,6 +86,19 @@ def test_balance(ctx, t, e, k, seq, softmax):
     assert (got[2][~inside] == 0).all()  # every row is written, padding with zeros
 
 
+@pytest.mark.parametrize("count", [65, 300, 1500])
+def test_balance_of_many_sequences(ctx, count):
+    """More sequences than one step over the offsets takes, some of them empty, with rows before and behind."""
+    t, e, k = 2000, 24, 3
+    note(f"balance of {count} sequences")
+    rng = np.random.default_rng(count)
+    seq = np.sort(rng.integers(5, t - 7, count + 1)).astype(np.int32)
+    z = (rng.standard_normal((t, e)) * 2).astype(np.float32)
+    idx = routes(rng, t, e, k)
+    got, want = run(ctx, z, idx, seq.tolist(), 0), R.balance(z, idx, seq.tolist(), 0, 0.5, 1.5)
+    check(got, want, z, seq.tolist(), 0, 1.5)
+
+
 @pytest.mark.parametrize("softmax", [0, 1])
 def test_balance_of_extreme_rows(ctx, softmax):
     note(f"balance extremes softmax={softmax}")
