@@ -15,6 +15,12 @@
 //    into a ring of their own, and are held as one dword per fragment.
 //  * Tiles are dealt so that an XCD's workgroups hold neighbours of a
 //    column-major order over the row tiles: they share weight panels in its L2.
+// 2048 x 4096 -> 21504 takes 107 to 113 us by card, 7 of them the rows'
+// quantization: 3.2 to 3.4 PFLOP/s.  The MFMAs alone, the CUs' load path and the
+// LDS reads take about 50 us each and overlap in part: without loads 93 of 113,
+// without seven of eight MFMAs 89, without the outputs' stores 96.  300 x
+// 2701 -> 4099, 325 tiles of 64 x 64, takes 10.5: two or fewer workgroups per CU
+// wait for each stage's loads.
 #include "mxfp4_device.h"
 
 using namespace nh;

@@ -8,6 +8,8 @@
 // saturating, the scale's exponent subtracted): bit-identical to mx_code for
 // every bf16 value under every scale byte a block of it can have, and on 2^24
 // f32 values of all exponents with ties, checked on the device.
+// 16384 x 4096 f32: to codes 56 us and back 52 (304 MB each: 5.4 and 5.8 TB/s);
+// a row of 8192 2.3 us each way, which is a launch.
 #include "mxfp4_device.h"
 
 using namespace nh;
