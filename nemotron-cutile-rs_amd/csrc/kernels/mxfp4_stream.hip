@@ -256,7 +256,8 @@ __device__ __forceinline__ void mx_pass(const MxStreamArgs& a, const MxPlace& p,
             const int u = p.u_begin + p.group + (s / T) * p.groups;
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                if (((s / T) * RB + rb) % W != p.wave) continue;
+                // (a group past the run's last unit has no outputs, and no bias in LDS)
+                if (u >= p.u_end || ((s / T) * RB + rb) % W != p.wave) continue;
                 const int row = m0 + rb * 16 + r16;
                 float y[T][4];
 #pragma unroll
@@ -273,7 +274,7 @@ __device__ __forceinline__ void mx_pass(const MxStreamArgs& a, const MxPlace& p,
 #pragma unroll
                     for (int n = 0; n < 4; ++n) y[i][n] = a.bias ? sum[n] + sbias[ln + n] : sum[n];
                 }
-                if (row >= p.seg1 || u >= p.u_end) continue;
+                if (row >= p.seg1) continue;
                 if constexpr (EPI == kMxOut) {
                     const int n = u * 16 + 4 * g;
                     const int64_t o = (int64_t)row * a.N + n;

@@ -1,0 +1,84 @@
+"""MXFP4 products and experts at the edges of their launch: runs of units that the waves' groups do not share evenly."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import mx_reference as R
+import nemotron_hip as NH
+from test_gpu_mxfp4 import Guarded, U, moe_case, note, route, run_linear, tile_all, weights
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = NH.Context(0)
+    yield c
+    c.close()
+
+
+# K of up to 512 leaves four or eight groups of waves, and a run of one or two units of 16 columns: the groups behind
+# the run's last unit have no outputs and no bias to read.  128 bytes of bias lie in LDS where four groups would have read
+# 256, eight 512.
+@pytest.mark.parametrize("m,n,k", [(1, 4112, 512), (16, 4112, 100), (3, 16, 128), (2, 8209, 500), (40, 4112, 512)])
+def test_bias_of_groups_without_a_unit(ctx, m, n, k):
+    note(f"bias, idle groups m={m} n={n} k={k}")
+    rng = np.random.default_rng(n + k)
+    x, w, bias = R.grid_matrix(rng, m, k, 0), R.grid_matrix(rng, n, k, 0), R.grid_matrix(rng, 1, n, 0)[0]
+    tiled, _ = weights(ctx, w)
+    assert np.array_equal(run_linear(ctx, x, tiled, n, bias), x @ w.T + bias)  # sums of quarters, exact in f32
+
+
+def moe(ctx, x, logits, du, dd, h, i, k, biases=None, out_dtype=NH.F32):
+    """The layer on f32 rows, renormalised routes: (output, non-finite status)."""
+    t, e = logits.shape
+    dx, dl = ctx.upload(x), ctx.upload(logits)
+    need = NH.lib().nh_moe_forward_mxfp4_workspace_size(t, h, i, e, k)
+    ws = ctx.upload(np.full(need, 0xFF, np.uint8))
+    out, word = Guarded(ctx, (t, h), np.float32), ctx.upload(np.zeros(1, np.uint64))
+    NH.call("nh_moe_forward_mxfp4", ctx.handle, dx.ptr, NH.F32, dl.ptr, t, h, i, e, k, 1, 1.0, du.ptr, dd.ptr, biases, None,
+            out.ptr, out_dtype, ws.ptr, need, word.ptr, None)
+    ctx.synchronize()
+    return out.numpy(), NH.call_status("nh_take_nonfinite", ctx.handle, word.ptr, None)[0]
+
+
+def moe_want(x, logits, ups, downs, k, bu=None, bd=None):
+    """The layer in 64 bits, and the size of its sums.  The sums before h are exact in f32, so h is the kernel's."""
+    idx, wts = route(logits, k, 1, 1.0)
+    t, h = x.shape
+    want, size = np.zeros((t, h)), np.zeros((t, h))
+    for n in range(logits.shape[1]):
+        tok, j = np.nonzero(idx == n)
+        if tok.size == 0:
+            continue
+        y = (x[tok].astype(np.float32) @ ups[n].T + (0 if bu is None else bu[n])).astype(np.float32)
+        hv = R.quantize((np.maximum(y, 0) ** 2).astype(np.float32))[2]
+        d, s = hv @ downs[n].T.astype(np.float64), np.abs(hv) @ np.abs(downs[n]).T.astype(np.float64)
+        if bd is not None:
+            d, s = d + bd[n], s + np.abs(bd[n])
+        w = wts[tok, j].astype(np.float64)[:, None]
+        want[tok] += w * d
+        size[tok] += w * s
+    return want, size
+
+
+def check_moe(ctx, t, h, i, e, k, logits, bias, seed):
+    rng, x, _, ups, downs = moe_case(ctx, t, h, i, e, k, seed)
+    bu, bd = (R.grid_matrix(rng, e, i, 0), R.grid_matrix(rng, e, h, 0)) if bias else (None, None)
+    du, dd = tile_all(ctx, ups), tile_all(ctx, downs)
+    dbu, dbd = (ctx.upload(bu), ctx.upload(bd)) if bias else (None, None)
+    biases = C.byref(NH.MoeBiases(dbu.ptr, dbd.ptr, None, None)) if bias else None
+    got, st = moe(ctx, x, logits, du, dd, h, i, k, biases)
+    want, size = moe_want(x, logits, ups, downs, k, bu, bd)
+    assert st == NH.OK
+    # i products, eight parts, a bias; the weight's product and the sum over the routes
+    assert (np.abs(got - want) <= (i + 10 + 2 * k) * U * size).all()
+
+
+# Two units of h (its one K tile has four) and three of the output in an expert's run, eight groups on them.
+@pytest.mark.parametrize("t,h,i,e,k", [(2, 40, 50, 4, 2), (20, 48, 130, 200, 1)])
+def test_expert_bias_of_groups_without_a_unit(ctx, t, h, i, e, k):
+    note(f"moe bias, idle groups t={t} h={h} i={i}")
+    logits = np.random.default_rng(t).standard_normal((t, e)).astype(np.float32)
+    check_moe(ctx, t, h, i, e, k, logits, True, t + 1)
