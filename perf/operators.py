@@ -360,20 +360,30 @@ def _nh():
 
 
 class _Bound:
-    """Entry points with their arguments bound to a layer's buffers, as a serving loop keeps them."""
+    """Entry points with their arguments bound to a layer's buffers, as a serving loop keeps them: all but the stream,
+    which is the one that is current when a pass runs."""
 
     def __init__(self, state):
         NH, ctx = _nh()
         self.NH, self.ctx, self.err, self.calls, self.keep = NH, ctx.handle, NH.NhError(), [], []
-        self.stream = torch.cuda.current_stream().cuda_stream
         self.outs = getattr(self, "_" + state["case"]["op"])(state["case"], state)
 
     def add(self, name, *args):
         fn = getattr(self.NH.lib(), name)
         simple = (ctypes.c_size_t, ctypes.c_int, ctypes.c_float, ctypes.c_void_p)
-        args = (self.ctx, *[a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args], self.stream)
+        args = (self.ctx, *[a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args])
         conv = [t(a) if t in simple and not isinstance(a, t) else a for t, a in zip(fn.argtypes, args)]
-        self.calls.append((fn, (*conv, ctypes.byref(self.err))))
+        self.calls.append((fn, conv))
+
+    def run(self):
+        """One pass on the current stream.  Its outputs and its workspace are the state's: a state's passes run one
+        after the other, and the next one overwrites what this one returns."""
+        stream, err = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), ctypes.byref(self.err)
+        for fn, args in self.calls:
+            status = fn(*args, stream, err)
+            if status:
+                self.NH.check(status, self.err)
+        return self.outs
 
     def empty(self, shape, dtype):
         self.keep.append(torch.empty(shape, dtype=dtype, device="cuda"))
@@ -427,11 +437,7 @@ def _run_own(state):
     bound = state.get("bound")
     if bound is None:
         bound = state["bound"] = _Bound(state)
-    for fn, args in bound.calls:
-        status = fn(*args)
-        if status:
-            bound.NH.check(status, bound.err)
-    return bound.outs
+    return bound.run()
 
 
 # ---- cost and expected values -----------------------------------------------
