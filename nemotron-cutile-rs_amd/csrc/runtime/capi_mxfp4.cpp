@@ -26,14 +26,17 @@ nh_status check_given(std::initializer_list<const void*> operands, nh_error* err
     return NH_OK;
 }
 
+// A launch holds fewer than 2^32 threads in a dimension.
+bool launchable(uint64_t workgroups, uint64_t threads) { return workgroups * threads < (1ull << 32); }
+
 // A row of `cols` values in `rows`: what the conversions address.
 nh_status check_mx_rows(size_t rows, size_t cols, nh_error* err) {
     size_t t;
     if (!mul_ok(rows, cols, &t) || t >= (1ull << 48)) return set_error(err, NH_INVALID_SHAPE, "rows * cols overflows");
-    // a workgroup takes 1024 groups of eight values
+    // a workgroup of 256 takes 1024 groups of eight values (so indices stay within the 38 bits of a non-finite word)
     if (rows > (size_t)kMaxGrid || cols > (size_t)kMaxGrid - 64 ||
-        (rows * mx_row_blocks(cols) * 4 + 1023) / 1024 > (size_t)kMaxGrid)
-        return set_error(err, NH_UNSUPPORTED, "rows and cols must be < 2^31 and their product < 2^44");
+        !launchable((rows * mx_row_blocks(cols) * 4 + 1023) / 1024, 256))
+        return set_error(err, NH_UNSUPPORTED, "rows and cols must be < 2^31 and rows * ceil(cols / 32) <= 2^32 - 256");
     return NH_OK;
 }
 
@@ -165,9 +168,11 @@ nh_status nh_tile_weights_mxfp4(nh_context* ctx, const uint8_t* codes, const uin
 
 int nh_supports_linear_mxfp4(size_t m, size_t n, size_t k) {
     // K up to 2^17 keeps 16 row tiles of codes and scales within a 32-bit
-    // buffer offset, m n below 2^40 the output tiles and their stages within 31 bits
+    // buffer offset, m n below 2^40 the output tiles and their stages within 31 bits;
+    // the rows' quantization has a workgroup of 256 per 16 rows and 512 columns
     return m > 0 && n > 0 && k > 0 && m < (1u << 24) && n < (1u << 28) && k <= (1u << 17) &&
-           (uint64_t)m * n < (1ull << 40) && (uint64_t)m * k < (1ull << 38);
+           (uint64_t)m * n < (1ull << 40) && (uint64_t)m * k < (1ull << 38) &&
+           launchable((m + 15) / 16 * mx_k_pieces(k), 256);
 }
 
 size_t nh_linear_mxfp4_workspace_size(size_t m, size_t n, size_t k) {
@@ -186,7 +191,7 @@ nh_status nh_linear_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
     if ((st = check_dtype(x_dtype, err)) || (st = check_dtype(out_dtype, err))) return st;
     if (!nh_supports_linear_mxfp4(m, n, k))
         return set_error(err, NH_UNSUPPORTED, "shape m=%zu n=%zu k=%zu outside the gfx950 envelope (k <= 131072, "
-                         "m < 2^24, n < 2^28, m * n < 2^40)", m, n, k);
+                         "m < 2^24, n < 2^28, m * n < 2^40, ceil(m / 16) * ceil(k / 512) < 2^24)", m, n, k);
     if ((st = check_given({x, w, out}, err))) return st;
     if (!aligned16(w)) return set_error(err, NH_UNSUPPORTED, "w must be 16-byte aligned");
     const size_t need = nh_linear_mxfp4_workspace_size(m, n, k);
@@ -233,6 +238,11 @@ nh_status nh_linear_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
 
 }  // extern "C"
 
+// Workgroups (of 1024) that the MoE layer's prep launch routes and quantizes with.
+static bool mx_moe_permutes(size_t T, size_t R) { return T <= 32 && R <= 512; }
+static size_t mx_moe_route_blocks(size_t T, size_t R) { return mx_moe_permutes(T, R) ? 1 : (T + 15) / 16; }
+static size_t mx_moe_quantize_blocks(size_t T, size_t H) { return ((T + 15) / 16 * mx_k_pieces(H) + 3) / 4; }
+
 // Workspace of the MoE layer, 256-byte aligned fields; false: sizes overflow.
 static bool mx_moe_layout(size_t T, size_t H, size_t I, size_t E, size_t k, size_t off[11]) {
     size_t R, t;
@@ -264,7 +274,11 @@ extern "C" {
 int nh_supports_moe_forward_mxfp4(size_t tokens, size_t hidden, size_t inter, size_t experts, size_t top_k) {
     size_t off[11];
     if (!mx_moe_layout(tokens, hidden, inter, experts, top_k, off) || top_k > experts) return 0;
-    return experts <= 1024 && top_k <= 64 && tokens <= (size_t)kMaxGrid / 4 && hidden <= 8192 && inter <= 8192;
+    // one launch routes and quantizes; a non-finite word has 38 bits for an index into x or h
+    const uint64_t routes = (uint64_t)tokens * top_k;
+    return experts <= 1024 && top_k <= 64 && hidden <= 8192 && inter <= 8192 &&
+           launchable(mx_moe_route_blocks(tokens, routes) + mx_moe_quantize_blocks(tokens, hidden), 1024) &&
+           routes * inter < (1ull << 38);
 }
 
 size_t nh_moe_forward_mxfp4_workspace_size(size_t tokens, size_t hidden, size_t inter, size_t experts, size_t top_k) {
@@ -295,7 +309,8 @@ nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype,
     if ((st = check_dtype(x_dtype, err)) || (st = check_dtype(out_dtype, err))) return st;
     if (!nh_supports_moe_forward_mxfp4(tokens, hidden, inter, experts, top_k))
         return set_error(err, NH_UNSUPPORTED, "MoE shape outside the gfx950 envelope (experts <= 1024, top_k <= 64, "
-                         "hidden and inter <= 8192)");
+                         "hidden and inter <= 8192, ceil(tokens / 16) * (1 + ceil(hidden / 512) / 4) < 2^22, "
+                         "tokens * top_k * inter < 2^38)");
     if ((st = check_given({x, logits, w_up, w_down, out}, err))) return st;
     if (!workspace || workspace_bytes < off[10]) return mismatch(err, "workspace", off[10], workspace_bytes);
     if (!aligned16(workspace) || !aligned16(w_up) || !aligned16(w_down))
@@ -320,10 +335,10 @@ nh_status nh_moe_forward_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype,
     prep.r.renormalize = renormalize ? 1 : 0;
     prep.r.scaling = scaling;
     prep.p = PermuteArgs{idx, offsets, perm, pos, (int)R, (int)experts};
-    prep.permute = tokens <= 32 && R <= 512 ? 1 : 0;
-    prep.route_blocks = prep.permute ? 1 : (int)((tokens + 15) / 16);
-    const size_t blocks = (tokens + 15) / 16 * (size_t)prep.q.kq;
-    if ((st = launch(ctx, K_MX_MOE_PREP, (unsigned)(prep.route_blocks + (blocks + 3) / 4), 1024, 0, stream, prep, err)))
+    prep.permute = mx_moe_permutes(tokens, R) ? 1 : 0;
+    prep.route_blocks = (int)mx_moe_route_blocks(tokens, R);
+    if ((st = launch(ctx, K_MX_MOE_PREP, (unsigned)(prep.route_blocks + mx_moe_quantize_blocks(tokens, hidden)), 1024, 0,
+                     stream, prep, err)))
         return st;
     if (!prep.permute && (st = nh_moe_permute(ctx, idx, tokens, top_k, experts, offsets, perm, pos, stream, err))) return st;
     // As many workgroups per expert as give every CU one when the routes reach
