@@ -1306,10 +1306,10 @@ nh_status nh_moe_combine_shared(nh_context* ctx, const float* slot_out, const in
     // four columns per thread when every row starts 16-byte aligned (8 bytes for bf16 out)
     const bool vec4 = hidden % 4 == 0 && aligned16(slot_out) && aligned16(shared) &&
                       ((uintptr_t)out % (out_dtype == NH_BF16 ? 8 : 16)) == 0;
+    const unsigned rows = (unsigned)std::min<size_t>(tokens, 65535);
     if (vec4)
-        return launch(ctx, K_COMBINE4, (unsigned)((hidden / 4 + 255) / 256), 256, 0, stream, a, err,
-                      (unsigned)tokens);
-    return launch(ctx, K_COMBINE, (unsigned)((hidden + 255) / 256), 256, 0, stream, a, err, (unsigned)tokens);
+        return launch(ctx, K_COMBINE4, (unsigned)((hidden / 4 + 255) / 256), 256, 0, stream, a, err, rows);
+    return launch(ctx, K_COMBINE, (unsigned)((hidden + 255) / 256), 256, 0, stream, a, err, rows);
 }
 
 // Workspace of the fused MoE layer, 256-byte aligned fields.

@@ -82,3 +82,11 @@ def test_expert_bias_of_groups_without_a_unit(ctx, t, h, i, e, k):
     note(f"moe bias, idle groups t={t} h={h} i={i}")
     logits = np.random.default_rng(t).standard_normal((t, e)).astype(np.float32)
     check_moe(ctx, t, h, i, e, k, logits, True, t + 1)
+
+
+# More tokens than a grid's 16 bits; the mean expert has 32 parts of its rows to give out, and each takes many passes.
+def test_experts_of_many_tokens(ctx):
+    t, h, i, e, k = 70001, 40, 36, 2, 1
+    note(f"moe t={t}")
+    logits = np.random.default_rng(8).standard_normal((t, e)).astype(np.float32)
+    check_moe(ctx, t, h, i, e, k, logits, False, 8)

@@ -79,6 +79,13 @@ def test_accepted_sizes_launch(rec):
         if NH.call_status("nh_quantize_rows_mxfp4", rec.ctx, X, NH.F32, rows, cols, OUT, S, None, None)[0] == NH.OK:
             launches += rec.launches("nh_dequantize_mxfp4", X, S, rows, cols, OUT, NH.F32, None)
         for kernel, gx, gy in launches:
-            assert gx * workgroup(kernel) < 1 << 32 and gy < 1 << 32, (kernel, gx, gy)
+            assert gx * workgroup(kernel) < 1 << 32 and gy <= 65535, (kernel, gx, gy)
             seen.add(kernel)
     assert {"mx_moe_prep", "quantize_mxfp4_tiles", "dequantize_mxfp4", "mx_gemm_64x64"} <= seen
+
+
+@pytest.mark.parametrize("hidden", [40, 41])
+def test_combine_of_more_tokens_than_a_grid_has_rows(rec, hidden):
+    for tokens, rows in ((1, 1), (65535, 65535), (65536, 65535), ((1 << 31) - 1, 65535)):
+        (_, gx, gy), = rec.launches("nh_moe_combine", X, W, S, tokens, 1, hidden, OUT, NH.F32, None)
+        assert (gx, gy) == (1, rows)
