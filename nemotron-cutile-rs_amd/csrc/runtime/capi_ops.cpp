@@ -1306,10 +1306,18 @@ nh_status nh_moe_combine_shared(nh_context* ctx, const float* slot_out, const in
     // four columns per thread when every row starts 16-byte aligned (8 bytes for bf16 out)
     const bool vec4 = hidden % 4 == 0 && aligned16(slot_out) && aligned16(shared) &&
                       ((uintptr_t)out % (out_dtype == NH_BF16 ? 8 : 16)) == 0;
-    const unsigned rows = (unsigned)std::min<size_t>(tokens, 65535);
-    if (vec4)
-        return launch(ctx, K_COMBINE4, (unsigned)((hidden / 4 + 255) / 256), 256, 0, stream, a, err, rows);
-    return launch(ctx, K_COMBINE, (unsigned)((hidden + 255) / 256), 256, 0, stream, a, err, rows);
+    const KernelId id = vec4 ? K_COMBINE4 : K_COMBINE;
+    const unsigned gx = (unsigned)(((vec4 ? hidden / 4 : hidden) + 255) / 256);
+    constexpr size_t kRows = 65535;  // tokens of a launch: what a grid holds in y
+    for (size_t t0 = 0; t0 < tokens; t0 += kRows) {
+        a.pos = pos + t0 * top_k;
+        a.weights = weights + t0 * top_k;
+        a.out = (uint8_t*)out + t0 * hidden * (out_dtype == NH_BF16 ? 2 : 4);
+        a.shared = shared ? shared + t0 * hidden : nullptr;
+        st = launch(ctx, id, gx, 256, 0, stream, a, err, (unsigned)std::min(kRows, tokens - t0));
+        if (st) return st;
+    }
+    return NH_OK;
 }
 
 // Workspace of the fused MoE layer, 256-byte aligned fields.

@@ -90,3 +90,24 @@ def test_experts_of_many_tokens(ctx):
     note(f"moe t={t}")
     logits = np.random.default_rng(8).standard_normal((t, e)).astype(np.float32)
     check_moe(ctx, t, h, i, e, k, logits, False, 8)
+
+
+@pytest.mark.parametrize("hidden,bf16", [(40, False), (40, True), (9, True), (9, False)])
+@pytest.mark.parametrize("with_shared", [False, True])
+def test_combine_of_many_tokens(ctx, hidden, bf16, with_shared):
+    note(f"combine of 140001 tokens hidden={hidden} bf16={bf16} shared={with_shared}")
+    t, k = 140001, 2
+    rng = np.random.default_rng(hidden)
+    d, w = rng.standard_normal((t * k, hidden), dtype=np.float32), rng.standard_normal((t, k), dtype=np.float32)
+    shared = rng.standard_normal((t, hidden), dtype=np.float32)
+    pos = rng.permutation(t * k).astype(np.int32).reshape(t, k)
+    pos[[5, 65535, 139999], 1] = -1  # dropped routes
+    dev = [ctx.upload(v) for v in (d, pos, w, shared)]
+    out = Guarded(ctx, (t, hidden), np.uint16 if bf16 else np.float32)
+    NH.call("nh_moe_combine_shared", ctx.handle, dev[0].ptr, dev[1].ptr, dev[2].ptr, dev[3].ptr if with_shared else None, t, k,
+            hidden, out.ptr, NH.BF16 if bf16 else NH.F32, None)
+    ctx.synchronize()
+    want = shared.copy() if with_shared else np.zeros((t, hidden), np.float32)
+    for j in range(k):
+        want = np.where(pos[:, j:j + 1] < 0, want, want + w[:, j:j + 1] * d[pos[:, j]])
+    assert np.array_equal(out.numpy(), R.to_bf16_bits(want) if bf16 else want)
