@@ -310,9 +310,9 @@ extern "C" __global__ __launch_bounds__(1024) void nh_moe_balance_reduce_kernel(
     // threads by expert and by residue of the chunk
     const int cols = min(E, 1024), parts = 1024 / cols, col = threadIdx.x % cols, part = threadIdx.x / cols;
     double* red = (double*)balance_lds;      // [16]
-    float* ps = (float*)(red + 16);          // [parts][cols]
+    double* ps = red + 16;                   // [parts][cols]
     int* ns = (int*)(ps + 1024);             // [parts][cols]
-    float v = 0.0f;
+    double v = 0.0;                          // a long sequence has 257 chunks, past 512 experts all of them in one thread
     int c = 0;
     if (part < parts) {
         constexpr int kAhead = 16;  // loads in flight; past the chunks the last one's, unused
@@ -327,7 +327,7 @@ extern "C" __global__ __launch_bounds__(1024) void nh_moe_balance_reduce_kernel(
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                v += i0 + u * parts < chunks ? pv[u] : 0.0f;
+                v += i0 + u * parts < chunks ? (double)pv[u] : 0.0;
                 c += i0 + u * parts < chunks ? pn[u] : 0;
             }
         }
@@ -340,7 +340,7 @@ extern "C" __global__ __launch_bounds__(1024) void nh_moe_balance_reduce_kernel(
         double p = 0.0;
         int total = 0;
         for (int i = 0; i < parts; ++i) {
-            p += (double)ps[i * cols + threadIdx.x];
+            p += ps[i * cols + threadIdx.x];
             total += ns[i * cols + threadIdx.x];
         }
         a.counts[(int64_t)s * E + threadIdx.x] = total;

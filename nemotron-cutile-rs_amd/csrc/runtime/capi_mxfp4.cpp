@@ -481,7 +481,7 @@ nh_status nh_moe_balance_loss(nh_context* ctx, const float* logits, const int32_
     const size_t lds = 17 * experts * 4 + 256;
     if (a.single) return launch(ctx, K_BALANCE_PARTIAL, 1, 1024, lds, stream, a, err);
     if ((st = launch(ctx, K_BALANCE_PARTIAL, (unsigned)p.chunks, 1024, lds, stream, a, err))) return st;
-    return launch(ctx, K_BALANCE_REDUCE, (unsigned)sequences, 1024, 128 + 2 * 1024 * 4, stream, a, err);
+    return launch(ctx, K_BALANCE_REDUCE, (unsigned)sequences, 1024, 128 + 1024 * 12, stream, a, err);
 }
 
 nh_status nh_moe_balance_loss_backward(nh_context* ctx, const float* logits, const int32_t* counts,
