@@ -131,11 +131,25 @@ __device__ __forceinline__ void balance_row(const BalanceArgs& a, int64_t token,
     }
 }
 
-// The row's probabilities in place of its logits; slope: d of each (sigmoid).
-// v_exp_f32 and v_rcp_f32 are within an ulp, the argument's rounding is what
-// counts: |z| 2^-24 of a probability.  An exp of a NaN is one, so is its row.
+// exp(x), x <= 0 or a NaN: 2^t, t = x log2 e as rounded, times 1 + (x - t ln 2),
+// ln 2 in two parts: off by the 2^-23 of v_exp_f32 and a rounding whatever x
+// (2^t alone by |x| 2^-24).  v_exp_f32 gives 0 below the normal range.  x stops
+// at -128 (2^-184): an infinity's difference would be a NaN.
+__device__ __forceinline__ float exp_nonpositive(float x) {
+    constexpr float kLn2 = 0x1.62e43p-1f, kLn2Rest = -0x1.05c61p-29f;
+    x = __builtin_elementwise_maximum(x, -128.0f);  // a NaN stays one
+    const float t = x * 0x1.715476p+0f;
+    const float r = __builtin_fmaf(-t, kLn2Rest, __builtin_fmaf(-t, kLn2, x));
+    const float p = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(p, r, p);
+}
+
+// The row's u in place of its logits, returning 1 / sum u (p = u / sum u); slope:
+// d of each (sigmoid).  p is off by the rounding of the difference from the row's
+// largest logit (2^-24 of it; none in a sigmoid), the 2^-23 of v_exp_f32 and of
+// v_rcp_f32, and a few half steps.  An exp of a NaN is one, so is its row.
 template <int G, int S, bool SOFTMAX, bool SLOPE>
-__device__ __forceinline__ void balance_probabilities(float (&z)[S][4], float (&slope)[S][4]) {
+__device__ __forceinline__ float balance_probabilities(float (&z)[S][4], float (&slope)[S][4]) {
     float m = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < S; ++i)
@@ -152,21 +166,17 @@ __device__ __forceinline__ void balance_probabilities(float (&z)[S][4], float (&
         for (int q = 0; q < 4; ++q) {
             const float v = z[i][q];
             if constexpr (SOFTMAX) {
-                z[i][q] = __expf(v - m);
+                z[i][q] = exp_nonpositive(v - m);
             } else {
-                const float t = __expf(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + t);
+                const float t = exp_nonpositive(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + t);
                 // exp(min(v, 0) - m): t itself unless the row's sigmoids are all below 1/2
-                z[i][q] = r * (m < 0.0f ? __expf(v - m) : v >= 0.0f ? 1.0f : t);
+                z[i][q] = r * (m < 0.0f ? exp_nonpositive(v - m) : v >= 0.0f ? 1.0f : t);
                 if constexpr (SLOPE) slope[i][q] = r * (v >= 0.0f ? t : 1.0f);
             }
             sum += z[i][q];
         }
     sum = group_reduce<G>(sum, [](float x, float y) { return x + y; });
-    const float r = none && !(sum != sum) ? 0.0f : __builtin_amdgcn_rcpf(sum);
-#pragma unroll
-    for (int i = 0; i < S; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) z[i][q] *= r;
+    return none && !(sum != sum) ? 0.0f : __builtin_amdgcn_rcpf(sum);
 }
 
 // Rows that a wave has in flight per lane group: loads and lane moves of one
@@ -203,13 +213,13 @@ __device__ __forceinline__ void balance_partial(const BalanceArgs& a, int* lds, 
             balance_row<G, S>(a, t, j, t < hi, z[u]);
         }
 #pragma unroll
-        for (int u = 0; u < kBalanceRows; ++u) balance_probabilities<G, S, SOFTMAX, false>(z[u], none);
-#pragma unroll
-        for (int u = 0; u < kBalanceRows; ++u)
+        for (int u = 0; u < kBalanceRows; ++u) {
+            const float r = balance_probabilities<G, S, SOFTMAX, false>(z[u], none);
 #pragma unroll
             for (int i = 0; i < S; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) acc[i][q] += z[u][i][q];
+                for (int q = 0; q < 4; ++q) acc[i][q] = __builtin_fmaf(z[u][i][q], r, acc[i][q]);
+        }
     }
     auto count = [&](int e) {
         if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
@@ -231,17 +241,20 @@ __device__ __forceinline__ void balance_partial(const BalanceArgs& a, int* lds, 
     __syncthreads();
 }
 
-// A body per lanes a token has (and turns, past 256 experts) and kind of probability.
-#define NH_BALANCE_FORMS(call)                      \
-    switch (a.experts <= 256 ? a.group : 0) {       \
-        case 1: call(1, 1); break;                  \
-        case 2: call(2, 1); break;                  \
-        case 4: call(4, 1); break;                  \
-        case 8: call(8, 1); break;                  \
-        case 16: call(16, 1); break;                \
-        case 32: call(32, 1); break;                \
-        case 64: call(64, 1); break;                \
-        default: call(64, 4); break;                \
+// A body per lanes a token has (and turns, past 256 experts) and kind of
+// probability.  (32768 x 512, sigmoid, forward and backward: 42 and 35 us in four
+// turns, half of them of nothing, 36 and 30 in two.)
+#define NH_BALANCE_FORMS(call)                                             \
+    switch (a.experts <= 256 ? a.group : a.experts <= 512 ? 128 : 256) {   \
+        case 1: call(1, 1); break;                                         \
+        case 2: call(2, 1); break;                                         \
+        case 4: call(4, 1); break;                                         \
+        case 8: call(8, 1); break;                                         \
+        case 16: call(16, 1); break;                                       \
+        case 32: call(32, 1); break;                                       \
+        case 64: call(64, 1); break;                                       \
+        case 128: call(64, 2); break;                                      \
+        default: call(64, 4); break;                                       \
     }
 
 }  // namespace
@@ -398,7 +411,13 @@ __device__ __forceinline__ void balance_backward(const BalanceArgs& a, int s, in
             balance_row<G, S>(a, t, j, t < hi, z[u]);
         }
 #pragma unroll
-        for (int u = 0; u < kBalanceRows; ++u) balance_probabilities<G, S, SOFTMAX, true>(z[u], slope[u]);
+        for (int u = 0; u < kBalanceRows; ++u) {
+            const float r = balance_probabilities<G, S, SOFTMAX, true>(z[u], slope[u]);
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) z[u][i][q] *= r;
+        }
 #pragma unroll
         for (int u = 0; u < kBalanceRows; ++u) {
             fp[u] = 0.0f;
