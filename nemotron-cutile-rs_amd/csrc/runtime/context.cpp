@@ -384,8 +384,10 @@ static const struct {
     {"mlp_w8a8", 1},             {"gemm_w8a8_tiled_a", 1},
     {"quantize_rows_mxfp4", 1},  {"dequantize_mxfp4", 1},       {"tile_weights_mxfp4", 1},
     {"linear_mxfp4", 1},         {"moe_forward_mxfp4", 1},      {"moe_balance_loss", 1},
+    {"moe_balance_loss_backward", 1},
     {"quantize_rows_mxfp4_host", 0}, {"dequantize_mxfp4_host", 0}, {"tile_weights_mxfp4_host", 0},
     {"linear_mxfp4_host", 0},    {"moe_forward_mxfp4_host", 0}, {"moe_balance_loss_host", 0},
+    {"moe_balance_loss_backward_host", 0},
 };
 
 int nh_kernel_count(void) { return (int)(sizeof(kRegistry) / sizeof(kRegistry[0])); }
