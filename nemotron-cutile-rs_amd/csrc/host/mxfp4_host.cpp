@@ -98,6 +98,7 @@ nh_status nh_quantize_rows_mxfp4_host(const void* x, nh_dtype dtype, size_t rows
     size_t n;
     if (st) return st;
     if (!mul_ok(rows, cols, &n)) return set_error(err, NH_INVALID_SHAPE, "rows * cols overflows");
+    if (n != 0 && (st = check_given({x, codes, scales}, err))) return st;
     if ((st = find_nonfinite(x, dtype, n, "input", err))) return st;
     float v[kMxBlock];
     uint8_t c[kMxBlock];
@@ -120,6 +121,7 @@ nh_status nh_dequantize_mxfp4_host(const uint8_t* codes, const uint8_t* scales, 
     size_t n;
     if (st) return st;
     if (!mul_ok(rows, cols, &n)) return set_error(err, NH_INVALID_SHAPE, "rows * cols overflows");
+    if (n != 0 && (st = check_given({codes, scales, out}, err))) return st;
     const size_t rc = mx_row_codes(cols), rb = mx_row_blocks(cols);
     for (size_t r = 0; r < rows; ++r)
         for (size_t c = 0; c < cols; ++c)
@@ -134,6 +136,7 @@ nh_status nh_tile_weights_mxfp4_host(const uint8_t* codes, const uint8_t* scales
     const size_t need = nh_tiled_mxfp4_weights_bytes(n, k);
     if (need == 0) return set_error(err, NH_INVALID_SHAPE, "invalid weight shape n=%zu k=%zu", n, k);
     if (tiled_len != need) return mismatch(err, "tiled", need, tiled_len);
+    if (nh_status st = check_given({codes, scales, tiled}, err)) return st;
     std::memset(tiled, 0, need);
     const size_t rc = mx_row_codes(k), rb = mx_row_blocks(k);
     for (size_t r = 0; r < n; ++r) {
@@ -159,6 +162,7 @@ nh_status nh_linear_mxfp4_host(const void* x, nh_dtype x_dtype, const uint8_t* w
     size_t mk, mn;
     if (!mul_ok(m, k, &mk) || !mul_ok(m, n, &mn) || nh_tiled_mxfp4_weights_bytes(n, k) == 0)
         return set_error(err, NH_INVALID_SHAPE, "linear shape m=%zu n=%zu k=%zu overflows", m, n, k);
+    if ((st = check_given({x, w, out}, err))) return st;
     if ((st = find_nonfinite(x, x_dtype, mk, "input", err))) return st;
     return guarded(err, [&]() -> nh_status {
         std::vector<float> xv(mk), row(k);
@@ -187,6 +191,7 @@ nh_status nh_moe_forward_mxfp4_host(const void* x, nh_dtype x_dtype, const float
         return set_error(err, NH_INVALID_PARAMS, "shared expert biases given without a shared expert");
     nh_status st;
     if ((st = check_dtype(x_dtype, err)) || (st = check_dtype(out_dtype, err))) return st;
+    if ((st = check_given({x, logits, w_up, w_down, out}, err))) return st;
     if ((st = find_nonfinite(x, x_dtype, tokens * hidden, "input", err))) return st;
     return guarded(err, [&]() -> nh_status {
         std::vector<int32_t> idx(routes), offsets(experts + 1), perm(routes), pos(routes);
@@ -285,6 +290,8 @@ nh_status nh_moe_balance_loss_host(const float* logits, const int32_t* indices, 
     clear_error(err);
     nh_status st = check_balance(sequences, seq_offsets, tokens, experts, top_k, coefficient, err);
     if (st) return st;
+    if ((st = check_given({counts, loss}, err))) return st;
+    if (tokens != 0 && (st = check_given({logits, indices}, err))) return st;
     return guarded(err, [&]() -> nh_status {
         std::vector<double> p(experts), slope(experts), sums(experts);
         double total = 0.0;
@@ -318,6 +325,7 @@ nh_status nh_moe_balance_loss_backward_host(const float* logits, const int32_t* 
     clear_error(err);
     nh_status st = check_balance(sequences, seq_offsets, tokens, experts, top_k, coefficient, err);
     if (st) return st;
+    if (tokens != 0 && (st = check_given({logits, counts, dloss, dlogits}, err))) return st;
     std::fill(dlogits, dlogits + tokens * experts, 0.0f);
     return guarded(err, [&]() -> nh_status {
         std::vector<double> p(experts), slope(experts);

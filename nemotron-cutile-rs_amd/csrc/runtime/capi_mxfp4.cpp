@@ -1,7 +1,6 @@
 // Device entry points of the MXFP4 operators: validate on the host, then enqueue.
 #include <algorithm>
 #include <cstdint>
-#include <initializer_list>
 
 #include "../kernels/mx_numerics.h"
 #include "nh_runtime.h"
@@ -18,13 +17,6 @@ constexpr size_t kMxRowsMaxK = 16384;
 // (index 0..3).  More per wave where K leaves a wave too few loads to hide
 // their latency, and the other waves go to groups of their own.
 int mx_split(int kt) { return kt <= 8 ? 0 : kt <= 32 ? 1 : kt <= 64 ? 2 : 3; }
-
-// An operand that a call reads or writes has to be there.
-nh_status check_given(std::initializer_list<const void*> operands, nh_error* err) {
-    for (const void* p : operands)
-        if (!p) return set_error(err, NH_INVALID_PARAMS, "null operand");
-    return NH_OK;
-}
 
 // A launch holds fewer than 2^32 threads in a dimension.
 bool launchable(uint64_t workgroups, uint64_t threads) { return workgroups * threads < (1ull << 32); }

@@ -150,6 +150,12 @@ nh_status check_dtype(nh_dtype d, nh_error* err) {
     return NH_OK;
 }
 
+nh_status check_given(std::initializer_list<const void*> operands, nh_error* err) {
+    for (const void* p : operands)
+        if (!p) return set_error(err, NH_INVALID_PARAMS, "null operand");
+    return NH_OK;
+}
+
 nh_status bind_device(nh_context* ctx, nh_error* err) {
     if (!ctx) return set_error(err, NH_INVALID_PARAMS, "null context");
     if (ctx->record) return NH_OK;

@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 
 #include "../kernels/nh_kernel_args.h"
 #include "../kernels/nh_numerics.h"
@@ -205,6 +206,8 @@ nh_status launch(nh_context* ctx, KernelId id, unsigned gx, unsigned bx, size_t 
 }
 
 nh_status check_dtype(nh_dtype d, nh_error* err);
+// An operand that a call reads or writes has to be there.
+nh_status check_given(std::initializer_list<const void*> operands, nh_error* err);
 constexpr int64_t kMaxGrid = 0x7fffffff;
 inline size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 

@@ -3,6 +3,8 @@ import ctypes as C
 import os
 import re
 
+import numpy as np
+
 import nemotron_hip as NH
 
 HEADER = os.path.join(os.path.dirname(__file__), "..", "include", "nemotron_hip.h")
@@ -18,3 +20,29 @@ def test_registry_lists_every_entry_point():
     assert len(entries) == 14
     for e in entries:
         assert names.get(e) == (0 if e.endswith("_host") else 1), e
+
+
+def test_host_twins_refuse_null_operands():
+    """As the device's entry points do; the operands that a call has no use for may be NULL."""
+    t, h, i, e, k = 4, 64, 32, 8, 2
+    keep = [np.zeros(1 << 16, d) for d in (np.float32, np.float32, np.uint8, np.uint8, np.int32, np.float32)]
+    f, out, b, s, ids, up = (v.ctypes.data for v in keep)
+    size = NH.lib().nh_tiled_mxfp4_weights_bytes(t, h)
+
+    def refused(name, args, operands):
+        for at in operands:
+            st, err = NH.call_status(name, *(None if n == at else v for n, v in enumerate(args)))
+            assert st == NH.INVALID_PARAMS and err.message == b"null operand", (name, at)
+        assert NH.call_status(name, *args)[0] == NH.OK, name
+
+    refused("nh_quantize_rows_mxfp4_host", (f, NH.F32, t, h, b, s), (0, 4, 5))
+    refused("nh_dequantize_mxfp4_host", (b, s, t, h, out, NH.F32), (0, 1, 4))
+    refused("nh_tile_weights_mxfp4_host", (b, s, t, h, out, size), (0, 1, 4))
+    refused("nh_linear_mxfp4_host", (f, NH.F32, b, None, t, 16, h, out, NH.F32), (0, 2, 7))
+    refused("nh_moe_forward_mxfp4_host", (f, NH.F32, f, t, h, i, e, k, 1, 1.0, b, b, None, None, out, NH.F32), (0, 2, 10, 11, 14))
+    refused("nh_moe_balance_loss_host", (f, ids, None, 1, t, e, k, 0, 0.1, s, out), (0, 1, 9, 10))
+    refused("nh_moe_balance_loss_backward_host", (f, ids, None, 1, t, e, k, 0, 0.1, up, out), (0, 1, 9, 10))
+    assert NH.call_status("nh_quantize_rows_mxfp4_host", None, NH.F32, 0, h, None, None)[0] == NH.OK
+    assert NH.call_status("nh_dequantize_mxfp4_host", None, None, t, 0, None, NH.F32)[0] == NH.OK
+    assert NH.call_status("nh_moe_balance_loss_host", None, None, None, 1, 0, e, k, 0, 0.1, s, out)[0] == NH.OK
+    assert NH.call_status("nh_moe_balance_loss_backward_host", None, None, None, 1, 0, e, k, 0, 0.1, None, None)[0] == NH.OK
