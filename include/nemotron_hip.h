@@ -573,9 +573,12 @@ nh_status nh_moe_forward_mxfp4_host(const void *x, nh_dtype x_dtype, const float
  * not change from run to run.  The workspace (nh_moe_balance_loss_workspace_size
  * bytes, 16-byte aligned) is free again once the call has run.  Errors:
  * INVALID_SHAPE (experts, top_k or sequences == 0; sequences != 1 without
- * offsets), INVALID_PARAMS (a coefficient that is not finite), LENGTH_MISMATCH
- * "workspace", UNSUPPORTED (experts > 1024, sequences > 16384, sizes past 2^31,
- * alignment).  No counterpart in the reference. */
+ * offsets), INVALID_PARAMS (a coefficient that is not finite, a null operand),
+ * LENGTH_MISMATCH "workspace", UNSUPPORTED outside
+ * nh_supports_moe_balance_loss (experts <= 1024, sequences <= 16384, tokens
+ * < 2^30, tokens * top_k < 2^31) or for a misaligned workspace.  No counterpart
+ * in the reference. */
+int nh_supports_moe_balance_loss(size_t sequences, size_t tokens, size_t experts, size_t top_k);
 size_t nh_moe_balance_loss_workspace_size(size_t sequences, size_t tokens, size_t experts);
 nh_status nh_moe_balance_loss(nh_context *ctx, const float *logits, const int32_t *indices, const int32_t *seq_offsets,
                               size_t sequences, size_t tokens, size_t experts, size_t top_k, int softmax,

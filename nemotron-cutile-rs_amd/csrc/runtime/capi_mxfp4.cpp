@@ -419,15 +419,21 @@ nh_status check_balance(size_t sequences, const int32_t* seq_offsets, size_t tok
         return set_error(err, NH_INVALID_SHAPE, "invalid balance shape sequences=%zu experts=%zu top_k=%zu", sequences,
                          experts, top_k);
     if (!std::isfinite(coefficient)) return set_error(err, NH_INVALID_PARAMS, "coefficient must be finite");
-    if (!plan_balance(sequences, tokens, experts, p) || top_k > 1024 || tokens * top_k >= (1ull << 31))
+    if (!nh_supports_moe_balance_loss(sequences, tokens, experts, top_k))
         return set_error(err, NH_UNSUPPORTED, "device balance needs experts <= 1024, sequences <= 16384, "
                          "tokens < 2^30 and tokens * top_k < 2^31");
+    plan_balance(sequences, tokens, experts, p);
     return NH_OK;
 }
 
 }  // namespace
 
 extern "C" {
+
+int nh_supports_moe_balance_loss(size_t sequences, size_t tokens, size_t experts, size_t top_k) {
+    BalancePlan p;
+    return plan_balance(sequences, tokens, experts, &p) && top_k > 0 && top_k <= 1024 && tokens * top_k < (1ull << 31);
+}
 
 size_t nh_moe_balance_loss_workspace_size(size_t sequences, size_t tokens, size_t experts) {
     BalancePlan p;

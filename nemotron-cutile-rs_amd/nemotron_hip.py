@@ -174,6 +174,7 @@ _SIGNATURES = {
                                   SZ, P, P, E]),
     "nh_moe_forward_mxfp4_host": (ST, [P, C.c_int, P, SZ, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, MB, P, P, C.c_int,
                                        E]),
+    "nh_supports_moe_balance_loss": (C.c_int, [SZ, SZ, SZ, SZ]),
     "nh_moe_balance_loss_workspace_size": (SZ, [SZ, SZ, SZ]),
     "nh_moe_balance_loss": (ST, [P, P, P, P, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, P, SZ, P, E]),
     "nh_moe_balance_loss_backward": (ST, [P, P, P, P, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, P, E]),

@@ -1365,8 +1365,16 @@ extern "C" {
     /// Sums in f32 and f64 of a fixed order: results do not change from run to run. The workspace
     /// (nh_moe_balance_loss_workspace_size bytes, 16-byte aligned) is free again once the call has run.
     /// Errors: INVALID_SHAPE (experts, top_k or sequences == 0; sequences != 1 without offsets),
-    /// INVALID_PARAMS (a coefficient that is not finite), LENGTH_MISMATCH "workspace", UNSUPPORTED (experts
-    /// > 1024, sizes past 2^31, alignment). No counterpart in the reference.
+    /// INVALID_PARAMS (a coefficient that is not finite, a null operand), LENGTH_MISMATCH "workspace",
+    /// UNSUPPORTED outside nh_supports_moe_balance_loss (experts <= 1024, sequences <= 16384, tokens < 2^30,
+    /// tokens * top_k < 2^31) or for a misaligned workspace. No counterpart in the reference.
+    pub fn nh_supports_moe_balance_loss(
+        sequences: usize,
+        tokens: usize,
+        experts: usize,
+        top_k: usize,
+    ) -> c_int;
+
     pub fn nh_moe_balance_loss_workspace_size(
         sequences: usize,
         tokens: usize,

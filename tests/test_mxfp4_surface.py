@@ -46,3 +46,21 @@ def test_host_twins_refuse_null_operands():
     assert NH.call_status("nh_dequantize_mxfp4_host", None, None, t, 0, None, NH.F32)[0] == NH.OK
     assert NH.call_status("nh_moe_balance_loss_host", None, None, None, 1, 0, e, k, 0, 0.1, s, out)[0] == NH.OK
     assert NH.call_status("nh_moe_balance_loss_backward_host", None, None, None, 1, 0, e, k, 0, 0.1, None, None)[0] == NH.OK
+
+
+def test_balance_has_an_envelope():
+    """nh_supports_moe_balance_loss is 1 exactly where neither call is refused, and where the workspace has a size."""
+    lib = NH.lib()
+    p = 1 << 40  # an operand that no call here gets to: there is no context
+    for s, t, e, k in ((1, 64, 8, 2), (16384, 1 << 20, 1024, 8), (16385, 64, 8, 2), (1, 64, 1025, 2), (1, 1 << 30, 8, 1),
+                       (1, (1 << 30) - 1, 8, 2), (1, (1 << 30) - 1, 8, 3), (1, 0, 8, 2), (1, 64, 8, 1024), (1, 64, 8, 1025),
+                       (0, 64, 8, 2), (1, 64, 0, 2), (1, 64, 8, 0), (2, (1 << 64) - 1, 1, 1)):
+        yes = lib.nh_supports_moe_balance_loss(s, t, e, k)
+        size = lib.nh_moe_balance_loss_workspace_size(s, t, e)
+        a = NH.call_status("nh_moe_balance_loss", None, p, p, p, s, t, e, k, 0, 0.1, p, p, p, size, None)
+        b = NH.call_status("nh_moe_balance_loss_backward", None, p, p, p, s, t, e, k, 0, 0.1, p, p, None)
+        for st, err in (a, b):
+            if yes:
+                assert size > 0 and err.message == b"null context", (s, t, e, k)
+            else:
+                assert st in (NH.UNSUPPORTED, NH.INVALID_SHAPE) and err.message != b"null context", (s, t, e, k)
