@@ -538,7 +538,8 @@ nh_status nh_linear_mxfp4_host(const void *x, nh_dtype x_dtype, const uint8_t *w
  * ones must be NULL).  h stays on the device in MXFP4 (a NaN or an infinity in
  * it marks its block, and `nonfinite` reports it as "intermediate").  The
  * workspace holds what nh_moe_workspace_layout names, at the offsets of
- * nh_moe_mxfp4_workspace_layout.  Errors as nh_moe_forward_w8a8. */
+ * nh_moe_mxfp4_workspace_layout; calls that may run at once need one each.
+ * Errors as nh_moe_forward_w8a8, and INVALID_PARAMS for a null operand. */
 int nh_supports_moe_forward_mxfp4(size_t tokens, size_t hidden, size_t inter, size_t experts, size_t top_k);
 size_t nh_moe_forward_mxfp4_workspace_size(size_t tokens, size_t hidden, size_t inter, size_t experts, size_t top_k);
 /* byte offsets in the workspace of: [0] indices i32[T*k], [1] weights

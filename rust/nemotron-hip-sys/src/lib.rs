@@ -1227,13 +1227,13 @@ extern "C" {
         err: *mut nh_error,
     ) -> nh_status;
 
-    /// Linear layer over tiled MXFP4 weights: y = Q(x) W^T (+ bias), x (f32 or bf16 rows of any k)
-    /// quantized as above, products exact, sums in f32. Up to 16 rows of k <= 16384 are one launch that
-    /// streams the weights once and touches no workspace; otherwise a launch quantizes the rows into the
-    /// workspace (nh_linear_mxfp4_workspace_size bytes, 16-byte aligned) ahead of the product.
-    /// Deterministic. Errors: INVALID_SHAPE (n or k == 0), INVALID_ROW_COUNT (m == 0), INVALID_PARAMS
-    /// (dtype), LENGTH_MISMATCH "workspace", UNSUPPORTED outside nh_supports_linear_mxfp4 or for a
-    /// misaligned w or workspace.
+    /// Linear layer over tiled MXFP4 weights: y = Q(x) W^T (+ bias), x (f32 or bf16 rows of any k) quantized
+    /// as above, products exact, sums in f32. Up to 16 rows of k <= 16384 are one launch that streams the
+    /// weights once and touches no workspace; otherwise a launch quantizes the rows into the workspace
+    /// (nh_linear_mxfp4_workspace_size bytes, 16-byte aligned) ahead of the product; calls that may run at
+    /// once need a workspace each. out must not overlap x. Deterministic. Errors: INVALID_SHAPE (n or k ==
+    /// 0), INVALID_ROW_COUNT (m == 0), INVALID_PARAMS (dtype, a null operand, out over x), LENGTH_MISMATCH
+    /// "workspace", UNSUPPORTED outside nh_supports_linear_mxfp4 or for a misaligned w or workspace.
     pub fn nh_supports_linear_mxfp4(m: usize, n: usize, k: usize) -> c_int;
 
     pub fn nh_linear_mxfp4_workspace_size(m: usize, n: usize, k: usize) -> usize;
@@ -1271,15 +1271,15 @@ extern "C" {
         err: *mut nh_error,
     ) -> nh_status;
 
-    /// MoE layer over MXFP4 experts, from given logits: routing and permutation as nh_moe_forward_w8a8,
-    /// then per route h = ReLU^2(Q(x) W_up^T + b_up) and Q(h) W_down^T + b_down, combined with the routes'
-    /// weights in route order (nh_moe_combine_shared: `shared`, f32 [tokens][hidden] or NULL, is added
-    /// first, e.g. a shared expert's output). w_up is `experts` tiled [inter][hidden] matrices at a stride
-    /// of nh_tiled_mxfp4_weights_bytes(inter, hidden), w_down tiled [hidden][inter] ones. biases: up and
-    /// down (the shared ones must be NULL). h stays on the device in MXFP4 (a NaN in it marks its block,
-    /// and `nonfinite` reports it as "intermediate"). The workspace starts with the fields of
-    /// nh_moe_workspace_layout at other offsets (nh_moe_mxfp4_workspace_layout). Errors as
-    /// nh_moe_forward_w8a8.
+    /// MoE layer over MXFP4 experts, from given logits: routing and permutation as nh_moe_forward_w8a8, then
+    /// per route h = ReLU^2(Q(x) W_up^T + b_up) and Q(h) W_down^T + b_down, combined with the routes'
+    /// weights in route order (nh_moe_combine_shared: shared, f32 [tokens][hidden] or NULL, is added first,
+    /// e.g. a shared expert's output). w_up is experts tiled [inter][hidden] matrices at a stride of
+    /// nh_tiled_mxfp4_weights_bytes(inter, hidden), w_down tiled [hidden][inter] ones. biases: up and down
+    /// (the shared ones must be NULL). h stays on the device in MXFP4 (a NaN or an infinity in it marks its
+    /// block, and nonfinite reports it as "intermediate"). The workspace holds what nh_moe_workspace_layout
+    /// names, at the offsets of nh_moe_mxfp4_workspace_layout; calls that may run at once need one each.
+    /// Errors as nh_moe_forward_w8a8, and INVALID_PARAMS for a null operand.
     pub fn nh_supports_moe_forward_mxfp4(
         tokens: usize,
         hidden: usize,

@@ -64,3 +64,16 @@ def test_balance_has_an_envelope():
                 assert size > 0 and err.message == b"null context", (s, t, e, k)
             else:
                 assert st in (NH.UNSUPPORTED, NH.INVALID_SHAPE) and err.message != b"null context", (s, t, e, k)
+
+
+def test_rust_comments_are_the_headers():
+    """Each MXFP4 and balance declaration of the Rust crate stands under its header comment, word for word."""
+    words = lambda t: re.findall(r"\w+", t)  # noqa: E731
+    header, crate = open(HEADER).read(), open(os.path.join(os.path.dirname(HEADER), "..", "rust", "nemotron-hip-sys", "src",
+                                                           "lib.rs")).read()
+    comments = re.findall(r"/\*((?:[^*]|\*(?!/))*)\*/\n[^;{}/]*?\b(nh_\w*(?:mxfp4|balance)\w*)\s*\(", header)
+    assert len(comments) > 10
+    for text, name in comments:
+        rust = re.search(r"((?:    ///[^\n]*\n)+)    pub fn " + name + r"\b", crate)
+        assert rust, name
+        assert words(rust.group(1)) == words(re.sub(r"\n \*", "\n", text)), name
