@@ -111,3 +111,15 @@ def test_combine_of_many_tokens(ctx, hidden, bf16, with_shared):
     for j in range(k):
         want = np.where(pos[:, j:j + 1] < 0, want, want + w[:, j:j + 1] * d[pos[:, j]])
     assert np.array_equal(out.numpy(), R.to_bf16_bits(want) if bf16 else want)
+
+
+# The launches are dealt for evenly spread routes; here every token agrees on the same experts, the mean expert has
+# several passes of rows (t = 300), or none is compacted away (128 experts, six of them with routes).
+@pytest.mark.parametrize("t,h,i,e,k,liked", [(300, 136, 70, 8, 2, (3, 5)), (300, 136, 70, 8, 2, (0, 7)),
+                                             (100, 128, 64, 128, 6, (1, 2, 64, 65, 126, 127)), (700, 160, 96, 4, 1, (3,)),
+                                             (20, 64, 40, 16, 3, (0, 1, 15)), (33, 4200, 36, 6, 1, (2,))])
+def test_experts_of_routes_that_agree(ctx, t, h, i, e, k, liked):
+    note(f"moe skew t={t} e={e} k={k} liked={liked}")
+    logits = np.random.default_rng(t + e).standard_normal((t, e)).astype(np.float32)
+    logits[:, list(liked)] += 20
+    check_moe(ctx, t, h, i, e, k, logits, True, t)
