@@ -9,13 +9,32 @@ using namespace nh;
 
 namespace {
 
-// Rows that one launch takes straight from x: the kernel quantizes 16.
+// Rows that one launch takes straight from x: what the kernel quantizes, an
+// MFMA operand of 16 rows, and holds, eight waves of 16 K tiles.
 constexpr size_t kMxRowsMax = 16;
 constexpr size_t kMxRowsMaxK = 16384;
 
+// Rows of codes that stream the weights, and the others go to the GEMM.  The
+// streaming form holds K to 8192, 32 rows a pass past 4096 and 64 below, and
+// reads the weights once a pass; the GEMM's time is a chain of stages along K
+// while it has few tiles.  us, streamed / GEMM, each with its quantization
+// (192 products of 17..64 rows, K 512..8192, 256..32768 columns: the choice is
+// within 9% of the better one; streaming them all took up to 1.8 times as long):
+//   64 rows -> 4096:  K 1024 11.1 / 7.6, 2048 12.6 / 9.5, 2688 10.0 / 11.4, 4096 12.8 / 13.2, 8192 20.1 / 20.9
+//   64 rows -> 16384: K 2688 14.1 / 12.7, 4096 18.1 / 15.4, 8192 34.3 / 24.6
+//   32 rows -> 8192:  K 1024 9.5 / 8.2, 2048 10.3 / 10.1, 4096 11.2 / 14.0, 8192 15.8 / 22.2
+//   128 rows -> 4096: K 4096 20.4 / 13.3
+bool mx_streams(size_t m, size_t n, size_t k) {
+    return m <= 64 && k > 2048 && k <= 8192 && (m <= 32 || n * (k <= 4096 ? 1 : 2) <= 8192);
+}
+
 // K tiles that each of a group's waves owns (at most eight waves): 2, 4, 8, 16
 // (index 0..3).  More per wave where K leaves a wave too few loads to hide
-// their latency, and the other waves go to groups of their own.
+// their latency, and the other waves go to groups of their own.  32, 64 and 128
+// K tiles are what eight waves of 4, 8 and 16 hold (fewer waves of more are
+// slower: 4096 -> 16384 at m = 1 10.7 us by fours, 11.5 by eights); 8 is where
+// twos and fours cross (1 x 1024 -> 4096 6.2 and 6.5, -> 16384 7.2 and 7.0; 2048
+// -> 16384 8.6 and 7.8).
 int mx_split(int kt) { return kt <= 8 ? 0 : kt <= 32 ? 1 : kt <= 64 ? 2 : 3; }
 
 // A launch holds fewer than 2^32 threads in a dimension.
@@ -34,7 +53,9 @@ nh_status check_mx_rows(size_t rows, size_t cols, nh_error* err) {
 
 unsigned mx_unit_grid(int64_t units) { return (unsigned)((units + 1023) / 1024); }
 
-// Rows that one pass of the few-row product takes (codes).
+// Rows that one pass of the few-row product takes (codes): as few as hold them
+// all (17 x 4096 -> 16384: 19.6 us in passes of 16, 13.9 of 32, 14.9 of 64; 40
+// rows 26.1, 21.9, 16.4).
 int mx_pass_rows(size_t rows, int kt) { return rows <= 16 ? 16 : rows <= 32 || mx_split(kt) == 2 ? 32 : 64; }
 
 // The few-row product: fills the launch shape into `a` and launches kernel
@@ -217,7 +238,7 @@ nh_status nh_linear_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
         return launch_mx_stream(ctx, id, a, m, false, cus, 1, stream, err);
     }
     uint8_t* ws = (uint8_t*)workspace;
-    if (m <= 64 && k <= 8192) {
+    if (mx_streams(m, n, k)) {
         uint8_t* scales = ws + m * mx_token_codes(k);
         if ((st = launch_mx_tiles(ctx, x, x_dtype, m, k, ws, scales, nonfinite, stream, err))) return st;
         a.xcodes = ws;

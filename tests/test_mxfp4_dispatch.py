@@ -1,0 +1,25 @@
+"""Which form of an MXFP4 operator a size takes, on both sides of each rule (without a GPU)."""
+import pytest
+
+import nemotron_hip as NH
+from dispatch import OUT, S, W, W2, WS, X, Recorder
+
+
+@pytest.fixture(scope="module")
+def rec():
+    r = Recorder()
+    yield r
+    r.close()
+
+
+# Rows of codes: streamed where K is long and the columns few, 32 or 64 rows a pass; else the GEMM.
+@pytest.mark.parametrize("m,n,k,kernel", [
+    (17, 4096, 2048, "mx_gemm_64x64"), (17, 4096, 2049, "mx_stream_tok4_32"), (32, 32768, 4096, "mx_stream_tok4_32"),
+    (32, 32768, 8192, "mx_stream_tok8_32"), (32, 4096, 8193, "mx_gemm_64x64"), (33, 8192, 4096, "mx_stream_tok4_64"),
+    (33, 8193, 4096, "mx_gemm_64x64"), (64, 8192, 2049, "mx_stream_tok4_64"), (64, 4096, 4097, "mx_stream_tok8_32"),
+    (64, 4097, 4097, "mx_gemm_64x64"), (64, 4096, 1024, "mx_gemm_64x64"), (65, 4096, 4096, "mx_gemm_64x64"),
+    (16, 4096, 1024, "mx_stream_bf16_2"), (16, 4096, 4096, "mx_stream_bf16_4")])
+def test_streamed_or_tiled(rec, m, n, k, kernel):
+    ws = NH.lib().nh_linear_mxfp4_workspace_size(m, n, k)
+    launches = rec.kernels("nh_linear_mxfp4", X, NH.BF16, W, None, m, n, k, OUT, NH.BF16, WS if ws else None, ws, None, None)
+    assert launches == (["quantize_mxfp4_tiles"] if ws else []) + [kernel]
