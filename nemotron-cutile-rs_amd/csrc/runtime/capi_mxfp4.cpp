@@ -252,7 +252,12 @@ nh_status nh_linear_mxfp4(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
 }  // extern "C"
 
 // Workgroups (of 1024) that the MoE layer's prep launch routes and quantizes with.
-static bool mx_moe_permutes(size_t T, size_t R) { return T <= 32 && R <= 512; }
+// One that routes alone, 16 tokens at a time, also sorts the routes, every thread
+// against all of them, while that takes less than a launch of its own (layers of
+// 128 small experts: 8 tokens with 6 routes each 23.3 us, 24.6 with the launch; 16
+// with 4 23.6 and 24.4; 8 with 16 32.9 and 31.4; 32 with 6, in two turns, 35.5 and
+// 28.5).
+static bool mx_moe_permutes(size_t T, size_t R) { return T <= 16 && R <= 64; }
 static size_t mx_moe_route_blocks(size_t T, size_t R) { return mx_moe_permutes(T, R) ? 1 : (T + 15) / 16; }
 static size_t mx_moe_quantize_blocks(size_t T, size_t H) { return ((T + 15) / 16 * mx_k_pieces(H) + 3) / 4; }
 

@@ -23,3 +23,14 @@ def test_streamed_or_tiled(rec, m, n, k, kernel):
     ws = NH.lib().nh_linear_mxfp4_workspace_size(m, n, k)
     launches = rec.kernels("nh_linear_mxfp4", X, NH.BF16, W, None, m, n, k, OUT, NH.BF16, WS if ws else None, ws, None, None)
     assert launches == (["quantize_mxfp4_tiles"] if ws else []) + [kernel]
+
+
+# The MoE layer's routes: sorted by the workgroup that routes them, one turn of 16 tokens and 64 routes at most.
+@pytest.mark.parametrize("t,k,inside", [(1, 64, True), (8, 8, True), (16, 4, True), (16, 5, False), (17, 1, False), (8, 9, False),
+                                        (32, 2, False)])
+def test_routes_sorted_in_the_first_launch(rec, t, k, inside):
+    ws = NH.lib().nh_moe_forward_mxfp4_workspace_size(t, 512, 256, 128, k)
+    launches = rec.launches("nh_moe_forward_mxfp4", X, NH.F32, S, t, 512, 256, 128, k, 1, 1.0, W, W2, None, None, OUT, NH.F32, WS,
+                            ws, None, None)
+    assert launches[0][0] == "mx_moe_prep" and ("permute" in launches[1][0]) == (not inside)
+    assert launches[0][1] == (1 if inside else -(-t // 16)) + -(--(-t // 16) // 4)
