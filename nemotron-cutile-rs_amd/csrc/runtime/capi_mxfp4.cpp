@@ -499,9 +499,10 @@ nh_status nh_moe_balance_loss(nh_context* ctx, const float* logits, const int32_
     a.softmax = softmax ? 1 : 0;
     a.coefficient = coefficient;
     a.group = p.group;
-    // a few rows, one sequence: one workgroup and launch (64 x 128: 13.9 us forward
-    // and backward in three launches, 10.8 in two)
-    a.single = sequences == 1 && tokens * experts <= 256 * 128 ? 1 : 0;
+    // a few rows and routes, one sequence: one workgroup and launch (64 x 128 5.8 us,
+    // 8.3 in two; 192 x 128 8.4 and 9.1, 256 x 128 10.3 and 9.1; 4096 x 8 10.1 and 10.7
+    // with 2 routes each, 13.6 and 10.5 with 8; 16384 x 1 24 and 27, 32768 x 1 44 and 27)
+    a.single = sequences == 1 && tokens * experts <= 256 * 128 && tokens * top_k <= 16384 ? 1 : 0;
     const size_t lds = 17 * experts * 4 + 256;
     if (a.single) return launch(ctx, K_BALANCE_PARTIAL, 1, 1024, lds, stream, a, err);
     if ((st = launch(ctx, K_BALANCE_PARTIAL, (unsigned)p.chunks, 1024, lds, stream, a, err))) return st;

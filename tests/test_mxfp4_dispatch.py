@@ -34,3 +34,12 @@ def test_routes_sorted_in_the_first_launch(rec, t, k, inside):
                             ws, None, None)
     assert launches[0][0] == "mx_moe_prep" and ("permute" in launches[1][0]) == (not inside)
     assert launches[0][1] == (1 if inside else -(-t // 16)) + -(--(-t // 16) // 4)
+
+
+# The balance loss: one workgroup for few logits and routes of one sequence.
+@pytest.mark.parametrize("t,e,k,one", [(256, 128, 8, True), (257, 128, 8, False), (4096, 8, 4, True), (4096, 8, 5, False),
+                                       (16384, 1, 1, True), (16385, 1, 1, False), (32, 1024, 8, True), (0, 1024, 8, True)])
+def test_balance_in_one_workgroup(rec, t, e, k, one):
+    ws = NH.lib().nh_moe_balance_loss_workspace_size(1, t, e)
+    launches = rec.kernels("nh_moe_balance_loss", X, W, None, 1, t, e, k, 0, 0.1, OUT, S, WS, ws, None)
+    assert launches == ["moe_balance_partial"] + ([] if one else ["moe_balance_reduce"])
