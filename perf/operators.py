@@ -378,7 +378,8 @@ class _Bound:
     def run(self):
         """One pass on the current stream.  Its outputs and its workspace are the state's: a state's passes run one
         after the other, and the next one overwrites what this one returns."""
-        stream, err = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), ctypes.byref(self.err)
+        # the handle alone: the object of torch.cuda.current_stream() costs 3 us, which is a launch
+        stream, err = ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(0)), ctypes.byref(self.err)
         for fn, args in self.calls:
             status = fn(*args, stream, err)
             if status:
