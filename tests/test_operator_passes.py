@@ -53,20 +53,20 @@ def test_a_pass_goes_to_the_current_stream(operators, monkeypatch, case):
         def lib(cls):
             return cls.library
 
-    class Anything:
-        handle, cuda_stream = NH.P(), 0
+    class Program:
+        handle, stream = NH.P(), 0
 
-    empty, current = torch.empty, Anything()
-    monkeypatch.setattr(operators, "_library", (Binding, Anything()))
+    empty = torch.empty
+    monkeypatch.setattr(operators, "_library", (Binding, Program))
     monkeypatch.setattr(torch, "empty", lambda shape, dtype, device=None: empty(shape, dtype=dtype))
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda: current)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: Program.stream, raising=False)
     t = torch.zeros(8)
     state = {"case": case, **{v: t for v in ("x", "logits", "indices", "offsets", "dloss", "bias", "tiled", "tiled_up",
                                              "tiled_down", "codes", "scales")}}
     state["indices"] = torch.zeros((case.get("tokens", 1), 2), dtype=torch.int32)
     calls = 0
     for handle in (0x1000, 0x2000, 0x1000):
-        current.cuda_stream = handle
+        Program.stream = handle
         operators.run(state)
         seen = Binding.library.streams[calls:]
         assert seen and all(s == handle for s in seen)
