@@ -18,8 +18,8 @@
 // four consecutive experts (one 16-byte load) per lane and turn, so a row meets
 // in log2(group) lane moves and a wave takes 64 / group rows at once.
 // Every sum has a fixed order: results do not change from run to run.
-// 131072 x 128: 18 us for the loss's partial sums (67 MB, 3.7 TB/s), 6 to join
-// them, 25 for the gradient (134 MB, 5.4 TB/s); 64 x 128 5.3 and 4.8.
+// 131072 x 128: 22.5 us for the loss's partial sums (67 MB, 3.0 TB/s), 6.6 to join
+// them, 26 for the gradient (134 MB, 5.2 TB/s); 64 x 128 5.7 and 5.1.
 #include "nh_device.h"
 
 using namespace nh;
@@ -52,7 +52,7 @@ __device__ __forceinline__ int wave_scan_i32(int v) {
 
 // Offsets of 64 sequences each that a walk over them has in flight (131072 x 128
 // in 1024 sequences, forward and backward: 234 us one at a time through
-// LDS-crossbar scans, 130 so).
+// LDS-crossbar scans, 117 so).
 constexpr int kSequenceLoads = 4;
 
 __device__ __forceinline__ int balance_chunks(const BalanceArgs& a, int n) { return (n + a.chunk - 1) / a.chunk; }

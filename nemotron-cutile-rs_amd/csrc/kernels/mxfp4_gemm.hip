@@ -19,8 +19,9 @@
 // quantization: 3.2 to 3.4 PFLOP/s.  The MFMAs alone, the CUs' load path and the
 // LDS reads take about 50 us each and overlap in part: without loads 93 of 113,
 // without seven of eight MFMAs 89, without the outputs' stores 96.  300 x
-// 2701 -> 4099, 325 tiles of 64 x 64, takes 10.5: two or fewer workgroups per CU
-// wait for each stage's loads.
+// 2701 -> 4099, 325 tiles of 64 x 64, takes 11: two or fewer workgroups per CU
+// wait for each stage's loads.  So does a long K over few tiles: 1 x 21504 -> 4096,
+// 64 of them, takes 30 us where its weights are 9.
 #include "mxfp4_device.h"
 
 using namespace nh;

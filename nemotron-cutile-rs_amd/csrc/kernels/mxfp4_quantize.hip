@@ -8,8 +8,9 @@
 // saturating, the scale's exponent subtracted): bit-identical to mx_code for
 // every bf16 value under every scale byte a block of it can have, and on 2^24
 // f32 values of all exponents with ties, checked on the device.
-// 16384 x 4096 f32: to codes 56 us and back 52 (304 MB each: 5.4 and 5.8 TB/s);
-// a row of 8192 2.3 us each way, which is a launch.
+// 16384 x 4096 f32: to codes 57 us and back 54 (304 MB each: 5.3 and 5.6 TB/s),
+// their codes into the tiled form 14 (71 MB, 5.1 TB/s); 613 x 2701 bf16, rows that
+// start off alignment, 4.7 and 4.5; a row of 4096 2.5 and 2.3, which is a launch.
 #include "mxfp4_device.h"
 
 using namespace nh;

@@ -20,7 +20,10 @@
 //
 // One row of 4096 -> 16384 takes 9.8 us (36 MB), eight of 4096 -> 131072 47
 // (289 MB, 6.1 TB/s); 128 experts of 2688 x 1856 reached by 500 tokens, 6 routes
-// each, 68 us up and 71 down (342 MB each, 4.9 TB/s).
+// each, 70 us up and 73 down (342 MB each, 4.9 and 4.7 TB/s).  Rows of any
+// alignment, of f32 past K = 4096 or of bf16 past 8192 issue the weights behind
+// their quantization: 8 x 2701 -> 4099 10.5 us, 1 x 8192 f32 -> 4096 16, 1 x 16384
+// -> 4096 30.
 #include "mxfp4_device.h"
 
 using namespace nh;
