@@ -600,6 +600,115 @@ nh_status nh_moe_balance_loss_backward_host(const float *logits, const int32_t *
                                             size_t sequences, size_t tokens, size_t experts, size_t top_k, int softmax,
                                             float coefficient, const float *dloss, float *dlogits, nh_error *err);
 
+/* ---- rows by expert, and back ---------------------------------------------
+ * What stands around experts of any kind, in f32 or bf16, and the gradients
+ * that training through them needs.  Route (t, j) of token t has slot
+ * s = pos[t * top_k + j] (nh_moe_permute), w_tj = weights[t * top_k + j] (f32;
+ * NULL: 1).  A slot outside [0, slots) stands for a route that was not placed:
+ * it takes no part.  No two routes may have one slot.  Slots that no route has
+ * are left as they were.  x, out and their gradients are [tokens][hidden] of
+ * one type, rows and their gradient [slots][hidden] of another or the same, all
+ * at any address of their element type.  Sums run in f32, over j in order, and
+ * are rounded once: results do not change from run to run.  Errors:
+ * INVALID_SHAPE (top_k or hidden == 0), INVALID_PARAMS (dtype, a null operand, an
+ * output over an input but where it says so), UNSUPPORTED outside
+ * nh_supports_moe_rows (tokens * top_k, slots and hidden < 2^31, tokens * hidden
+ * and slots * hidden < 2^40).  No counterpart in the reference.
+ *
+ * Dispatch: rows[s] = w_tj x[t]. */
+int nh_supports_moe_rows(size_t tokens, size_t top_k, size_t hidden, size_t slots);
+nh_status nh_moe_dispatch(nh_context *ctx, const void *x, nh_dtype x_dtype, const int32_t *pos, const float *weights,
+                          size_t tokens, size_t top_k, size_t hidden, size_t slots, void *rows, nh_dtype rows_dtype,
+                          nh_stream stream, nh_error *err);
+/* Its gradient: dx[t] = sum_j w_tj drows[s], and dweights[t, j] = <drows[s], x[t]>
+ * (f32, 0 for a route that was not placed) unless it is NULL (x may then be). */
+nh_status nh_moe_dispatch_backward(nh_context *ctx, const void *drows, nh_dtype rows_dtype, const void *x,
+                                   nh_dtype x_dtype, const int32_t *pos, const float *weights, size_t tokens,
+                                   size_t top_k, size_t hidden, size_t slots, void *dx, float *dweights,
+                                   nh_stream stream, nh_error *err);
+/* Combine: out[t] = shared[t] + sum_j w_tj rows[s]; shared, of out's type, may be NULL (0) or out itself. */
+nh_status nh_moe_combine_rows(nh_context *ctx, const void *rows, nh_dtype rows_dtype, const int32_t *pos,
+                              const float *weights, const void *shared, size_t tokens, size_t top_k, size_t hidden,
+                              size_t slots, void *out, nh_dtype out_dtype, nh_stream stream, nh_error *err);
+/* Its gradient: drows[s] = w_tj dout[t], and dweights[t, j] = <rows[s], dout[t]>
+ * unless it is NULL (rows may then be).  drows may be rows itself. */
+nh_status nh_moe_combine_rows_backward(nh_context *ctx, const void *dout, nh_dtype out_dtype, const void *rows,
+                                       nh_dtype rows_dtype, const int32_t *pos, const float *weights, size_t tokens,
+                                       size_t top_k, size_t hidden, size_t slots, void *drows, float *dweights,
+                                       nh_stream stream, nh_error *err);
+/* Host twins (sums in f64). */
+nh_status nh_moe_dispatch_host(const void *x, nh_dtype x_dtype, const int32_t *pos, const float *weights, size_t tokens,
+                               size_t top_k, size_t hidden, size_t slots, void *rows, nh_dtype rows_dtype,
+                               nh_error *err);
+nh_status nh_moe_dispatch_backward_host(const void *drows, nh_dtype rows_dtype, const void *x, nh_dtype x_dtype,
+                                        const int32_t *pos, const float *weights, size_t tokens, size_t top_k,
+                                        size_t hidden, size_t slots, void *dx, float *dweights, nh_error *err);
+nh_status nh_moe_combine_rows_host(const void *rows, nh_dtype rows_dtype, const int32_t *pos, const float *weights,
+                                   const void *shared, size_t tokens, size_t top_k, size_t hidden, size_t slots,
+                                   void *out, nh_dtype out_dtype, nh_error *err);
+nh_status nh_moe_combine_rows_backward_host(const void *dout, nh_dtype out_dtype, const void *rows, nh_dtype rows_dtype,
+                                            const int32_t *pos, const float *weights, size_t tokens, size_t top_k,
+                                            size_t hidden, size_t slots, void *drows, float *dweights, nh_error *err);
+
+/* ---- low-rank adapters beside a linear layer -------------------------------
+ * Fine-tunes of one frozen projection (nh_linear_w8a8, _w4a8, _mxfp4 or any
+ * other), many in a call: row i belongs to adapter l = adapter_ids[i], or to
+ * none where that is outside [0, adapters), and
+ *   out_i = base_i + s_l B_l h_i,   h_i = A_l x_i,
+ * a = A [adapters][rank][k] and b = B [adapters][n][rank], both f32 or both
+ * bf16 (w_dtype), scales s [adapters] f32 (NULL: 1), base [m][n] of out's type:
+ * the projection's output, or NULL (0); out itself may be base.  Rows without an
+ * adapter get their base.  h_out, f32 [m][rank], receives h for the backward
+ * pass (0 in rows without an adapter) unless it is NULL.  For experts'
+ * adapters, x holds the dispatched rows and adapter_ids their experts.
+ *
+ * Products of bf16 values are exact; h and every sum are f32, of a fixed order:
+ * results do not change from run to run.  The order depends on m and on how many
+ * rows share an adapter, so a row's last bits may differ between batches.  Where x
+ * and the matrices are bf16, B_l's products take h in bf16 parts of 16 significant
+ * bits (24 for an f32 out); an infinity in B_l then makes its outputs infinite or
+ * NaN.  Operands start at any address of their element type.  The workspace
+ * (nh_linear_lora_workspace_size bytes, 16-byte aligned) is free again once the
+ * call has run; calls that may run at once need one each.  Errors: INVALID_SHAPE
+ * (n, k, rank or adapters == 0), INVALID_ROW_COUNT (m == 0), INVALID_PARAMS
+ * (dtype, a null operand, out over x or partly over base), LENGTH_MISMATCH
+ * "workspace", UNSUPPORTED outside nh_supports_linear_lora (m < 2^24, n and k <=
+ * 2^20, m n and m k < 2^40, rank <= 128, adapters <= 1024) or for a misaligned
+ * workspace.  No counterpart in the reference. */
+int nh_supports_linear_lora(size_t m, size_t n, size_t k, size_t rank, size_t adapters);
+size_t nh_linear_lora_workspace_size(size_t m, size_t n, size_t k, size_t rank, size_t adapters);
+nh_status nh_linear_lora(nh_context *ctx, const void *x, nh_dtype x_dtype, const int32_t *adapter_ids, const void *a,
+                         const void *b, nh_dtype w_dtype, const float *scales, size_t m, size_t n, size_t k, size_t rank,
+                         size_t adapters, const void *base, void *out, nh_dtype out_dtype, float *h_out,
+                         void *workspace, size_t workspace_bytes, nh_stream stream, nh_error *err);
+/* Its gradients, with dh_i = s_l B_l^T dout_i:
+ *   dx_i = dx_base_i + A_l^T dh_i   [m][k] of x's type (dx_base: the projection's
+ *                                   own, or NULL for 0; dx itself may be dx_base),
+ *   da_l = sum_i dh_i x_i^T         f32 [adapters][rank][k],
+ *   db_l = s_l sum_i dout_i h_i^T   f32 [adapters][n][rank].
+ * Each of dx, da and db may be NULL (not all), then it is not computed and x (da,
+ * db), a (dx, db without h) and b (dx, da) may be NULL where nothing asks for
+ * them.  h is nh_linear_lora's h_out, or NULL: computed again (for db).  With
+ * accumulate != 0 da and db are added to; otherwise adapters without rows get
+ * zeros.  Workspace nh_linear_lora_backward_workspace_size bytes, errors as
+ * above (dx over x or dout, or partly over dx_base). */
+size_t nh_linear_lora_backward_workspace_size(size_t m, size_t n, size_t k, size_t rank, size_t adapters);
+nh_status nh_linear_lora_backward(nh_context *ctx, const void *x, nh_dtype x_dtype, const int32_t *adapter_ids,
+                                  const void *a, const void *b, nh_dtype w_dtype, const float *scales, const float *h,
+                                  const void *dout, nh_dtype dout_dtype, size_t m, size_t n, size_t k, size_t rank,
+                                  size_t adapters, const void *dx_base, void *dx, float *da, float *db, int accumulate,
+                                  void *workspace, size_t workspace_bytes, nh_stream stream, nh_error *err);
+/* Host twins (sums in f64, h rounded to f32), any shape. */
+nh_status nh_linear_lora_host(const void *x, nh_dtype x_dtype, const int32_t *adapter_ids, const void *a, const void *b,
+                              nh_dtype w_dtype, const float *scales, size_t m, size_t n, size_t k, size_t rank,
+                              size_t adapters, const void *base, void *out, nh_dtype out_dtype, float *h_out,
+                              nh_error *err);
+nh_status nh_linear_lora_backward_host(const void *x, nh_dtype x_dtype, const int32_t *adapter_ids, const void *a,
+                                       const void *b, nh_dtype w_dtype, const float *scales, const float *h,
+                                       const void *dout, nh_dtype dout_dtype, size_t m, size_t n, size_t k, size_t rank,
+                                       size_t adapters, const void *dx_base, void *dx, float *da, float *db,
+                                       int accumulate, nh_error *err);
+
 /* ---- safetensors weights into device memory -----------------------------
  * One .safetensors file: the 8-byte little-endian header length, the JSON
  * header, the data section (WeightManifest::load_tensor and

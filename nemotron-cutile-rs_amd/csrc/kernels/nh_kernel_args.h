@@ -476,4 +476,64 @@ struct BalanceArgs {
     int32_t pad_;
 };
 
+// ---- rows by expert, and back (moe_rows.hip) --------------------------------
+struct MoeRowsArgs {
+    const void* tokens;      // [T][H]: what is dispatched, or the gradient of what was combined; scatter form only
+    const void* rows_in;     // [slots][H]: what is joined, or what the weights' gradients are products with
+    const void* shared;      // [T][H] of the tokens' type or null: joined first
+    const int32_t* pos;      // [T][k] route -> slot, outside [0, slots): the route has none
+    const float* weights;    // [T][k] or null: 1
+    void* rows_out;          // [slots][H], scatter form
+    void* out;               // [T][H], gather form
+    float* dweights;         // [T][k] or null
+    const void* dot;         // [T][H] or null: gather form, dweights = <row, dot>
+    int64_t token0;          // first token of this launch
+    int64_t slots;
+    int32_t top_k, hidden;
+    int32_t threads;         // blockDim
+    int32_t pad_;
+};
+
+// ---- low-rank adapters beside a linear layer (lora.hip) ---------------------
+// Rows gathered by adapter: `tile` consecutive slots hold rows of one adapter.
+struct LoraPlanArgs {
+    const int32_t* ids;      // [m] adapter of a row; outside [0, adapters): none
+    int32_t* slot_row;       // [tiles * 64] row of a slot, -1: none
+    int32_t* tile_adapter;   // [tiles]; `adapters` itself: rows without one
+    int32_t* items;          // [items][4]: adapter, first tile, tiles, partial sum that it writes (-1: the result)
+    int32_t* per_adapter;    // [adapters][2]: items, first partial sum
+    int32_t* counts;         // [2]: tiles, items
+    int32_t m, adapters;
+    int32_t item_tiles;      // most tiles of an item
+    int32_t pad_;
+};
+
+struct LoraArgs {
+    const void* x;           // [m][C] activations (shrink, outer), f32 or bf16
+    const void* w;           // [adapters] matrices of rank x C: [rank][C], or [C][rank] (w_cols)
+    const int32_t* ids;
+    const int32_t* slot_row;
+    const int32_t* tile_adapter;
+    const int32_t* counts;
+    const int32_t* items;
+    const int32_t* per_adapter;
+    const float* scales;     // [adapters] or null: 1
+    const float* h;          // [m][rank]: given low-rank values (finish)
+    float* part;             // [splits][m][rank_pad] sums over parts of C
+    float* h_out;            // [m][rank] or null
+    const void* base;        // [m][C] or null: 0
+    void* out;               // [m][C]
+    void* ht;                // outer: low-rank values [rank_pad][slots] (f32), or three such planes of bf16
+    float* gpart;            // outer: partial sums [partials][rank * C]
+    float* grad;             // [adapters] matrices, laid out as w
+    int64_t slots;           // of ht
+    int32_t m, C, rank, rank_pad, adapters;
+    int32_t x_dtype, w_dtype, out_dtype;
+    int32_t w_cols;          // 1: w is [C][rank]
+    int32_t splits;          // parts of C that shrink sums apart
+    int32_t per_wave;        // columns of C per wave (shrink, expand), a multiple of 32
+    int32_t scaled;          // finish, expand: times the adapter's scale
+    int32_t accumulate;
+};
+
 }  // namespace nh

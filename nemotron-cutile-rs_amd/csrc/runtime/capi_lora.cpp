@@ -1,0 +1,289 @@
+// Device entry points of the low-rank adapters: validate on the host, then enqueue.
+#include <algorithm>
+#include <cstdint>
+
+#include "nh_runtime.h"
+
+using namespace nh;
+
+namespace {
+
+constexpr size_t kTileRows = 64;    // of the plan
+constexpr size_t kDirectRows = 64;  // rows that need no plan: one ballot sees all of them
+
+size_t bytes_of(nh_dtype d) { return d == NH_BF16 ? 2 : 4; }
+int rank_form(size_t rank) { return rank <= 16 ? 0 : rank <= 32 ? 1 : rank <= 64 ? 2 : 3; }
+size_t rank_pad(size_t rank) { return (size_t)16 << rank_form(rank); }
+size_t most_tiles(size_t m, size_t adapters) { return m / kTileRows + std::min(m, adapters + 1); }
+
+// How shrink cuts C: columns per wave (four waves a workgroup) and parts.
+struct Split {
+    size_t per_wave, parts;
+};
+
+Split shrink_split(size_t m, size_t c) {
+    const size_t tiles = m <= kDirectRows ? m : (m + kTileRows - 1) / kTileRows;
+    size_t parts = std::max<size_t>(1, std::min<size_t>(16, (512 + tiles - 1) / tiles));
+    size_t per_wave = std::max<size_t>(128, ((c + 4 * parts - 1) / (4 * parts) + 31) / 32 * 32);
+    return {per_wave, (c + 4 * per_wave - 1) / (4 * per_wave)};
+}
+
+// Columns that a wave of expand takes: a workgroup's low-rank values are summed
+// anew by each of a tile's workgroups.
+size_t expand_columns(size_t m) { return m <= 16 ? 32 : m <= kDirectRows ? 64 : 128; }
+
+// Most tiles of an outer item: about 32 items of an evenly dealt batch.
+size_t item_tiles(size_t m) { return std::max<size_t>(1, (m / kTileRows + 31) / 32); }
+
+struct Layout {
+    size_t slot_row, tile_adapter, counts, items, per_adapter;
+    size_t part_x, part_d, ht_h, ht_d, gpart_a, gpart_b;
+    size_t slots, items_most, bytes;
+};
+
+Layout lora_layout(size_t m, size_t n, size_t k, size_t rank, size_t adapters, bool backward) {
+    Layout l{};
+    size_t cur = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = cur;
+        cur += align256(bytes);
+        return o;
+    };
+    const size_t rp = rank_pad(rank), tiles = most_tiles(m, adapters);
+    l.slots = tiles * kTileRows;
+    if (m > kDirectRows || backward) {
+        l.slot_row = take(l.slots * 4);
+        l.tile_adapter = take(tiles * 4);
+        l.counts = take(8);
+    }
+    l.part_x = take(shrink_split(m, k).parts * m * rp * 4);
+    if (backward) {
+        const size_t it = item_tiles(m);
+        // of adapters with more than `it` tiles: t / it + 1 < 2 t / it items each, and over 64 it rows, so
+        // fewer than 3 per 64 it rows
+        const size_t partials = std::min(2 * (tiles / it) + 2, 3 * (m / (kTileRows * it) + 1));
+        l.items_most = tiles / it + std::min(m, adapters) + 1;
+        l.items = take(l.items_most * 16);
+        l.per_adapter = take(adapters * 8);
+        l.part_d = take(shrink_split(m, n).parts * m * rp * 4);
+        l.ht_h = take(rp * l.slots * 6);
+        l.ht_d = take(rp * l.slots * 6);
+        l.gpart_a = take(partials * rank * k * 4);
+        l.gpart_b = take(partials * rank * n * 4);
+    }
+    l.bytes = cur;
+    return l;
+}
+
+nh_status check_lora(size_t m, size_t n, size_t k, size_t rank, size_t adapters, std::initializer_list<nh_dtype> dtypes,
+                     nh_error* err) {
+    if (n == 0 || k == 0 || rank == 0 || adapters == 0)
+        return set_error(err, NH_INVALID_SHAPE, "invalid adapter shape k=%zu n=%zu rank=%zu adapters=%zu", k, n, rank, adapters);
+    if (m == 0) return set_error(err, NH_INVALID_ROW_COUNT, "row_count must be non-zero, got 0");
+    for (nh_dtype d : dtypes)
+        if (nh_status st = check_dtype(d, err)) return st;
+    if (!nh_supports_linear_lora(m, n, k, rank, adapters))
+        return set_error(err, NH_UNSUPPORTED, "shape m=%zu n=%zu k=%zu rank=%zu adapters=%zu outside the gfx950 envelope "
+                         "(m < 2^24, n and k <= 2^20, m * n and m * k < 2^40, rank <= 128, adapters <= 1024)", m, n, k,
+                         rank, adapters);
+    return NH_OK;
+}
+
+nh_status check_workspace(const void* workspace, size_t given, size_t need, nh_error* err) {
+    if (!workspace || given < need) return mismatch(err, "workspace", need, given);
+    if (!aligned16(workspace)) return set_error(err, NH_UNSUPPORTED, "workspace must be 16-byte aligned");
+    return NH_OK;
+}
+
+// One call's launches over its rows.
+struct Lora {
+    nh_context* ctx;
+    nh_stream stream;
+    nh_error* err;
+    size_t m, rank, adapters;
+    bool direct;
+    LoraArgs common;
+
+    nh_status plan(const Layout& l, uint8_t* ws, const int32_t* ids, bool items) {
+        LoraPlanArgs p{};
+        p.ids = ids;
+        p.slot_row = (int32_t*)(ws + l.slot_row);
+        p.tile_adapter = (int32_t*)(ws + l.tile_adapter);
+        p.counts = (int32_t*)(ws + l.counts);
+        p.items = items ? (int32_t*)(ws + l.items) : nullptr;
+        p.per_adapter = items ? (int32_t*)(ws + l.per_adapter) : nullptr;
+        p.m = (int)m;
+        p.adapters = (int)adapters;
+        p.item_tiles = (int)item_tiles(m);
+        return launch(ctx, K_LORA_PLAN, 1, 1024, 17 * (adapters + 1) * 4, stream, p, err);
+    }
+
+    KernelId form(KernelId first, bool bf16) const {
+        return (KernelId)(first + (bf16 ? 0 : 8) + (direct ? 0 : 4) + rank_form(rank));
+    }
+    unsigned tiles() const { return (unsigned)(direct ? m : most_tiles(m, adapters)); }
+
+    // part = x w^T by parts of C
+    nh_status shrink(const void* x, nh_dtype xd, const void* w, nh_dtype wd, bool w_cols, size_t c, float* part) {
+        LoraArgs a = common;
+        const Split s = shrink_split(m, c);
+        a.x = x;
+        a.w = w;
+        a.part = part;
+        a.C = (int)c;
+        a.x_dtype = xd;
+        a.w_dtype = wd;
+        a.w_cols = w_cols;
+        a.per_wave = (int)s.per_wave;
+        const size_t lds = (size_t)4 * (direct ? 16 : kTileRows) * rank_pad(rank) * 4;
+        return launch(ctx, form(K_LORA_SHRINK, xd == NH_BF16 && wd == NH_BF16), tiles(), 256, lds, stream, a, err,
+                      (unsigned)s.parts);
+    }
+
+    // out = base + (s) h w, h the sum of `splits` parts
+    nh_status expand(const float* part, size_t splits, const void* w, nh_dtype wd, bool w_cols, size_t c, const void* base,
+                     void* out, nh_dtype od, float* h_out, bool scaled) {
+        LoraArgs a = common;
+        a.part = const_cast<float*>(part);
+        a.splits = (int)splits;
+        a.w = w;
+        a.base = base;
+        a.out = out;
+        a.h_out = h_out;
+        a.C = (int)c;
+        a.w_dtype = wd;
+        a.out_dtype = od;
+        a.w_cols = w_cols;
+        a.scaled = scaled;
+        a.per_wave = (int)expand_columns(m);
+        return launch(ctx, form(K_LORA_EXPAND, wd == NH_BF16), tiles(), 256, 0, stream, a, err,
+                      (unsigned)((c + 4 * a.per_wave - 1) / (4 * a.per_wave)));
+    }
+
+    // low-rank values by slot
+    nh_status finish(const float* h, const float* part, size_t splits, bool scaled, bool bf16, void* ht) {
+        LoraArgs a = common;
+        a.h = h;
+        a.part = const_cast<float*>(part);
+        a.splits = (int)splits;
+        a.ht = ht;
+        a.scaled = scaled;
+        a.x_dtype = bf16 ? DT_BF16 : DT_F32;
+        return launch(ctx, K_LORA_FINISH, tiles(), 256, 0, stream, a, err);
+    }
+
+    // grad = ht x over the rows, laid out [rank][c], or [c][rank] (w_cols)
+    nh_status outer(const void* x, nh_dtype xd, const void* ht, bool w_cols, size_t c, float* gpart, float* grad,
+                    bool accumulate, size_t items) {
+        LoraArgs a = common;
+        a.x = x;
+        a.ht = const_cast<void*>(ht);
+        a.gpart = gpart;
+        a.grad = grad;
+        a.C = (int)c;
+        a.x_dtype = xd;
+        a.w_cols = w_cols;
+        a.accumulate = accumulate;
+        nh_status st = launch(ctx, (KernelId)(K_LORA_OUTER + (xd == NH_BF16 ? 0 : 4) + rank_form(rank)),
+                              (unsigned)((c + 255) / 256), 256, 0, stream, a, err, (unsigned)items);
+        if (st) return st;
+        return launch(ctx, K_LORA_REDUCE, (unsigned)((rank * c + 255) / 256), 256, 0, stream, a, err, (unsigned)adapters);
+    }
+};
+
+Lora make_lora(nh_context* ctx, const int32_t* ids, const float* scales, size_t m, size_t rank, size_t adapters,
+               bool direct, const Layout& l, uint8_t* ws, nh_stream stream, nh_error* err) {
+    Lora c{ctx, stream, err, m, rank, adapters, direct, {}};
+    c.common.ids = ids;
+    c.common.scales = scales;
+    c.common.slot_row = (int32_t*)(ws + l.slot_row);
+    c.common.tile_adapter = (int32_t*)(ws + l.tile_adapter);
+    c.common.counts = (int32_t*)(ws + l.counts);
+    c.common.items = (int32_t*)(ws + l.items);
+    c.common.per_adapter = (int32_t*)(ws + l.per_adapter);
+    c.common.slots = (int64_t)l.slots;
+    c.common.m = (int)m;
+    c.common.rank = (int)rank;
+    c.common.rank_pad = (int)rank_pad(rank);
+    c.common.adapters = (int)adapters;
+    return c;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nh_supports_linear_lora(size_t m, size_t n, size_t k, size_t rank, size_t adapters) {
+    return m > 0 && n > 0 && k > 0 && rank > 0 && adapters > 0 && m < (1u << 24) && n <= (1u << 20) && k <= (1u << 20) &&
+           (uint64_t)m * n < (1ull << 40) && (uint64_t)m * k < (1ull << 40) && rank <= 128 && adapters <= 1024;
+}
+
+size_t nh_linear_lora_workspace_size(size_t m, size_t n, size_t k, size_t rank, size_t adapters) {
+    return nh_supports_linear_lora(m, n, k, rank, adapters) ? lora_layout(m, n, k, rank, adapters, false).bytes : 0;
+}
+
+size_t nh_linear_lora_backward_workspace_size(size_t m, size_t n, size_t k, size_t rank, size_t adapters) {
+    return nh_supports_linear_lora(m, n, k, rank, adapters) ? lora_layout(m, n, k, rank, adapters, true).bytes : 0;
+}
+
+nh_status nh_linear_lora(nh_context* ctx, const void* x, nh_dtype x_dtype, const int32_t* adapter_ids, const void* a,
+                         const void* b, nh_dtype w_dtype, const float* scales, size_t m, size_t n, size_t k, size_t rank,
+                         size_t adapters, const void* base, void* out, nh_dtype out_dtype, float* h_out,
+                         void* workspace, size_t workspace_bytes, nh_stream stream, nh_error* err) {
+    clear_error(err);
+    nh_status st;
+    if ((st = check_lora(m, n, k, rank, adapters, {x_dtype, w_dtype, out_dtype}, err)) ||
+        (st = check_given({x, adapter_ids, a, b, out}, err)))
+        return st;
+    const size_t out_bytes = m * n * bytes_of(out_dtype);
+    if (overlap(out, out_bytes, x, m * k * bytes_of(x_dtype)) || (base != out && overlap(out, out_bytes, base, base ? out_bytes : 0)))
+        return set_error(err, NH_INVALID_PARAMS, "out must not overlap x, nor base in part");
+    const Layout l = lora_layout(m, n, k, rank, adapters, false);
+    if ((st = check_workspace(workspace, workspace_bytes, l.bytes, err)) || (st = bind_device(ctx, err))) return st;
+    uint8_t* ws = (uint8_t*)workspace;
+    Lora c = make_lora(ctx, adapter_ids, scales, m, rank, adapters, m <= kDirectRows, l, ws, stream, err);
+    float* part = (float*)(ws + l.part_x);
+    if (!c.direct && (st = c.plan(l, ws, adapter_ids, false))) return st;
+    if ((st = c.shrink(x, x_dtype, a, w_dtype, false, k, part))) return st;
+    return c.expand(part, shrink_split(m, k).parts, b, w_dtype, true, n, base, out, out_dtype, h_out, true);
+}
+
+nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dtype, const int32_t* adapter_ids,
+                                  const void* a, const void* b, nh_dtype w_dtype, const float* scales, const float* h,
+                                  const void* dout, nh_dtype dout_dtype, size_t m, size_t n, size_t k, size_t rank,
+                                  size_t adapters, const void* dx_base, void* dx, float* da, float* db, int accumulate,
+                                  void* workspace, size_t workspace_bytes, nh_stream stream, nh_error* err) {
+    clear_error(err);
+    nh_status st;
+    if ((st = check_lora(m, n, k, rank, adapters, {x_dtype, w_dtype, dout_dtype}, err)) ||
+        (st = check_given({adapter_ids, dout}, err)))
+        return st;
+    if (!dx && !da && !db) return set_error(err, NH_INVALID_PARAMS, "null operand");
+    const bool again = db && !h;  // h is computed here
+    if (((da || again) && (st = check_given({x}, err))) || ((dx || again) && (st = check_given({a}, err))) ||
+        ((dx || da) && (st = check_given({b}, err))))
+        return st;
+    const size_t x_bytes = m * k * bytes_of(x_dtype);
+    if (dx && (overlap(dx, x_bytes, x, x ? x_bytes : 0) || overlap(dx, x_bytes, dout, m * n * bytes_of(dout_dtype)) ||
+               (dx_base != dx && overlap(dx, x_bytes, dx_base, dx_base ? x_bytes : 0))))
+        return set_error(err, NH_INVALID_PARAMS, "dx must not overlap x or dout, nor dx_base in part");
+    const Layout l = lora_layout(m, n, k, rank, adapters, true);
+    if ((st = check_workspace(workspace, workspace_bytes, l.bytes, err)) || (st = bind_device(ctx, err))) return st;
+    uint8_t* ws = (uint8_t*)workspace;
+    Lora c = make_lora(ctx, adapter_ids, scales, m, rank, adapters, false, l, ws, stream, err);
+    float *part_x = (float*)(ws + l.part_x), *part_d = (float*)(ws + l.part_d);
+    const size_t parts_x = shrink_split(m, k).parts, parts_d = shrink_split(m, n).parts;
+    if ((st = c.plan(l, ws, adapter_ids, true))) return st;
+    if (again && (st = c.shrink(x, x_dtype, a, w_dtype, false, k, part_x))) return st;
+    if ((dx || da) && (st = c.shrink(dout, dout_dtype, b, w_dtype, true, n, part_d))) return st;
+    if (dx && (st = c.expand(part_d, parts_d, a, w_dtype, false, k, dx_base, dx, x_dtype, nullptr, true))) return st;
+    if (da && ((st = c.finish(nullptr, part_d, parts_d, true, x_dtype == NH_BF16, ws + l.ht_d)) ||
+               (st = c.outer(x, x_dtype, ws + l.ht_d, false, k, (float*)(ws + l.gpart_a), da, accumulate != 0, l.items_most))))
+        return st;
+    if (db && ((st = c.finish(h, part_x, parts_x, true, dout_dtype == NH_BF16, ws + l.ht_h)) ||
+               (st = c.outer(dout, dout_dtype, ws + l.ht_h, true, n, (float*)(ws + l.gpart_b), db, accumulate != 0, l.items_most))))
+        return st;
+    return NH_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,156 @@
+// Device entry points of the rows by expert: validate on the host, then enqueue.
+#include <algorithm>
+#include <cstdint>
+
+#include "nh_runtime.h"
+
+using namespace nh;
+
+namespace {
+
+size_t bytes_of(nh_dtype d) { return d == NH_BF16 ? 2 : 4; }
+
+nh_status check_rows(nh_dtype token, nh_dtype row, size_t tokens, size_t top_k, size_t hidden, size_t slots,
+                     nh_error* err) {
+    nh_status st;
+    if (top_k == 0 || hidden == 0)
+        return set_error(err, NH_INVALID_SHAPE, "invalid rows shape top_k=%zu hidden=%zu", top_k, hidden);
+    if ((st = check_dtype(token, err)) || (st = check_dtype(row, err))) return st;
+    if (!nh_supports_moe_rows(tokens, top_k, hidden, slots))
+        return set_error(err, NH_UNSUPPORTED, "device rows need tokens * top_k, slots and hidden < 2^31, "
+                         "tokens * hidden and slots * hidden < 2^40");
+    return NH_OK;
+}
+
+// One workgroup per token; eight values a thread, as many threads as take the row
+// in the fewest turns of at most 512.
+nh_status launch_rows(nh_context* ctx, KernelId first, MoeRowsArgs a, nh_dtype token, nh_dtype row, size_t tokens,
+                      nh_stream stream, nh_error* err) {
+    const KernelId id = (KernelId)(first + (token == NH_BF16 ? 2 : 0) + (row == NH_BF16 ? 1 : 0));
+    const size_t vectors = ((size_t)a.hidden + 7) / 8, turns = (vectors + 511) / 512;
+    a.threads = (int)(((vectors + turns - 1) / turns + 63) / 64 * 64);
+    const size_t most = ((1ull << 32) - 1) / (size_t)a.threads;  // workgroups of a launch: fewer than 2^32 threads
+    for (size_t t0 = 0; t0 < tokens; t0 += most) {
+        a.token0 = (int64_t)t0;
+        const nh_status st = launch(ctx, id, (unsigned)std::min(most, tokens - t0), (unsigned)a.threads, 0, stream, a, err);
+        if (st) return st;
+    }
+    return NH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nh_supports_moe_rows(size_t tokens, size_t top_k, size_t hidden, size_t slots) {
+    size_t routes;
+    return top_k > 0 && hidden > 0 && hidden <= (size_t)kMaxGrid && slots <= (size_t)kMaxGrid && tokens <= (size_t)kMaxGrid &&
+           mul_ok(tokens, top_k, &routes) && routes <= (size_t)kMaxGrid && tokens * hidden < (1ull << 40) &&
+           slots * hidden < (1ull << 40);
+}
+
+nh_status nh_moe_dispatch(nh_context* ctx, const void* x, nh_dtype x_dtype, const int32_t* pos, const float* weights,
+                          size_t tokens, size_t top_k, size_t hidden, size_t slots, void* rows, nh_dtype rows_dtype,
+                          nh_stream stream, nh_error* err) {
+    clear_error(err);
+    nh_status st = check_rows(x_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
+    if (st) return st;
+    if (tokens != 0 && slots != 0 && (st = check_given({x, pos, rows}, err))) return st;
+    if (overlap(rows, slots * hidden * bytes_of(rows_dtype), x, tokens * hidden * bytes_of(x_dtype)))
+        return set_error(err, NH_INVALID_PARAMS, "rows must not overlap x");
+    if ((st = bind_device(ctx, err))) return st;
+    if (tokens == 0 || slots == 0) return NH_OK;
+    MoeRowsArgs a{};
+    a.tokens = x;
+    a.pos = pos;
+    a.weights = weights;
+    a.rows_out = rows;
+    a.slots = (int64_t)slots;
+    a.top_k = (int)top_k;
+    a.hidden = (int)hidden;
+    return launch_rows(ctx, K_MOE_SCATTER, a, x_dtype, rows_dtype, tokens, stream, err);
+}
+
+nh_status nh_moe_dispatch_backward(nh_context* ctx, const void* drows, nh_dtype rows_dtype, const void* x,
+                                   nh_dtype x_dtype, const int32_t* pos, const float* weights, size_t tokens,
+                                   size_t top_k, size_t hidden, size_t slots, void* dx, float* dweights,
+                                   nh_stream stream, nh_error* err) {
+    clear_error(err);
+    nh_status st = check_rows(x_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
+    if (st) return st;
+    if (tokens != 0 && ((st = check_given({pos, dx}, err)) || (slots != 0 && (st = check_given({drows}, err))) ||
+                        (dweights && (st = check_given({x}, err)))))
+        return st;
+    const size_t token_bytes = tokens * hidden * bytes_of(x_dtype);
+    if (overlap(dx, token_bytes, drows, slots * hidden * bytes_of(rows_dtype)) || (dweights && overlap(dx, token_bytes, x, token_bytes)))
+        return set_error(err, NH_INVALID_PARAMS, "dx must not overlap drows or x");
+    if ((st = bind_device(ctx, err))) return st;
+    if (tokens == 0) return NH_OK;
+    MoeRowsArgs a{};
+    a.rows_in = drows;
+    a.dot = x;
+    a.pos = pos;
+    a.weights = weights;
+    a.out = dx;
+    a.dweights = dweights;
+    a.slots = (int64_t)slots;
+    a.top_k = (int)top_k;
+    a.hidden = (int)hidden;
+    return launch_rows(ctx, K_MOE_GATHER, a, x_dtype, rows_dtype, tokens, stream, err);
+}
+
+nh_status nh_moe_combine_rows(nh_context* ctx, const void* rows, nh_dtype rows_dtype, const int32_t* pos,
+                              const float* weights, const void* shared, size_t tokens, size_t top_k, size_t hidden,
+                              size_t slots, void* out, nh_dtype out_dtype, nh_stream stream, nh_error* err) {
+    clear_error(err);
+    nh_status st = check_rows(out_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
+    if (st) return st;
+    if (tokens != 0 && ((st = check_given({pos, out}, err)) || (slots != 0 && (st = check_given({rows}, err))))) return st;
+    const size_t token_bytes = tokens * hidden * bytes_of(out_dtype);
+    if (overlap(out, token_bytes, rows, slots * hidden * bytes_of(rows_dtype)) ||
+        (shared && shared != out && overlap(out, token_bytes, shared, token_bytes)))
+        return set_error(err, NH_INVALID_PARAMS, "out must not overlap rows, nor shared in part");
+    if ((st = bind_device(ctx, err))) return st;
+    if (tokens == 0) return NH_OK;
+    MoeRowsArgs a{};
+    a.rows_in = rows;
+    a.shared = shared;
+    a.pos = pos;
+    a.weights = weights;
+    a.out = out;
+    a.slots = (int64_t)slots;
+    a.top_k = (int)top_k;
+    a.hidden = (int)hidden;
+    return launch_rows(ctx, K_MOE_GATHER, a, out_dtype, rows_dtype, tokens, stream, err);
+}
+
+nh_status nh_moe_combine_rows_backward(nh_context* ctx, const void* dout, nh_dtype out_dtype, const void* rows,
+                                       nh_dtype rows_dtype, const int32_t* pos, const float* weights, size_t tokens,
+                                       size_t top_k, size_t hidden, size_t slots, void* drows, float* dweights,
+                                       nh_stream stream, nh_error* err) {
+    clear_error(err);
+    nh_status st = check_rows(out_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
+    if (st) return st;
+    if (tokens != 0 && ((st = check_given({dout, pos}, err)) || (slots != 0 && (st = check_given({drows}, err))) ||
+                        (dweights && slots != 0 && (st = check_given({rows}, err)))))
+        return st;
+    const size_t row_bytes = slots * hidden * bytes_of(rows_dtype);
+    if (overlap(drows, row_bytes, dout, tokens * hidden * bytes_of(out_dtype)) ||
+        (dweights && rows != drows && overlap(drows, row_bytes, rows, row_bytes)))
+        return set_error(err, NH_INVALID_PARAMS, "drows must not overlap dout, nor rows in part");
+    if ((st = bind_device(ctx, err))) return st;
+    if (tokens == 0) return NH_OK;
+    MoeRowsArgs a{};
+    a.tokens = dout;
+    a.rows_in = rows;
+    a.pos = pos;
+    a.weights = weights;
+    a.rows_out = drows;
+    a.dweights = dweights;
+    a.slots = (int64_t)slots;
+    a.top_k = (int)top_k;
+    a.hidden = (int)hidden;
+    return launch_rows(ctx, K_MOE_SCATTER, a, out_dtype, rows_dtype, tokens, stream, err);
+}
+
+}  // extern "C"

@@ -114,6 +114,57 @@ const char* const kKernelSymbols[K_COUNT] = {  // in KernelId order
     "nh_moe_balance_partial_kernel",       // K_BALANCE_PARTIAL
     "nh_moe_balance_reduce_kernel",        // K_BALANCE_REDUCE
     "nh_moe_balance_backward_kernel",      // K_BALANCE_BACKWARD
+    "nh_moe_scatter_rows_f32_f32_kernel",  // K_MOE_SCATTER
+    "nh_moe_scatter_rows_f32_bf16_kernel",
+    "nh_moe_scatter_rows_bf16_f32_kernel",
+    "nh_moe_scatter_rows_bf16_bf16_kernel",
+    "nh_moe_gather_rows_f32_f32_kernel",  // K_MOE_GATHER
+    "nh_moe_gather_rows_f32_bf16_kernel",
+    "nh_moe_gather_rows_bf16_f32_kernel",
+    "nh_moe_gather_rows_bf16_bf16_kernel",
+    "nh_lora_plan_kernel",  // K_LORA_PLAN
+    "nh_lora_finish_kernel",  // K_LORA_FINISH
+    "nh_lora_reduce_kernel",  // K_LORA_REDUCE
+    "nh_lora_shrink_bf16_1_1_kernel",  // K_LORA_SHRINK
+    "nh_lora_shrink_bf16_1_2_kernel",
+    "nh_lora_shrink_bf16_1_4_kernel",
+    "nh_lora_shrink_bf16_1_8_kernel",
+    "nh_lora_shrink_bf16_4_1_kernel",
+    "nh_lora_shrink_bf16_4_2_kernel",
+    "nh_lora_shrink_bf16_4_4_kernel",
+    "nh_lora_shrink_bf16_4_8_kernel",
+    "nh_lora_shrink_f32_1_1_kernel",
+    "nh_lora_shrink_f32_1_2_kernel",
+    "nh_lora_shrink_f32_1_4_kernel",
+    "nh_lora_shrink_f32_1_8_kernel",
+    "nh_lora_shrink_f32_4_1_kernel",
+    "nh_lora_shrink_f32_4_2_kernel",
+    "nh_lora_shrink_f32_4_4_kernel",
+    "nh_lora_shrink_f32_4_8_kernel",
+    "nh_lora_expand_bf16_1_1_kernel",  // K_LORA_EXPAND
+    "nh_lora_expand_bf16_1_2_kernel",
+    "nh_lora_expand_bf16_1_4_kernel",
+    "nh_lora_expand_bf16_1_8_kernel",
+    "nh_lora_expand_bf16_4_1_kernel",
+    "nh_lora_expand_bf16_4_2_kernel",
+    "nh_lora_expand_bf16_4_4_kernel",
+    "nh_lora_expand_bf16_4_8_kernel",
+    "nh_lora_expand_f32_1_1_kernel",
+    "nh_lora_expand_f32_1_2_kernel",
+    "nh_lora_expand_f32_1_4_kernel",
+    "nh_lora_expand_f32_1_8_kernel",
+    "nh_lora_expand_f32_4_1_kernel",
+    "nh_lora_expand_f32_4_2_kernel",
+    "nh_lora_expand_f32_4_4_kernel",
+    "nh_lora_expand_f32_4_8_kernel",
+    "nh_lora_outer_bf16_1_kernel",  // K_LORA_OUTER
+    "nh_lora_outer_bf16_2_kernel",
+    "nh_lora_outer_bf16_4_kernel",
+    "nh_lora_outer_bf16_8_kernel",
+    "nh_lora_outer_f32_1_kernel",
+    "nh_lora_outer_f32_2_kernel",
+    "nh_lora_outer_f32_4_kernel",
+    "nh_lora_outer_f32_8_kernel",
 };
 
 void clear_error(nh_error* err) {
@@ -394,6 +445,10 @@ static const struct {
     {"quantize_rows_mxfp4_host", 0}, {"dequantize_mxfp4_host", 0}, {"tile_weights_mxfp4_host", 0},
     {"linear_mxfp4_host", 0},    {"moe_forward_mxfp4_host", 0}, {"moe_balance_loss_host", 0},
     {"moe_balance_loss_backward_host", 0},
+    {"moe_dispatch", 1},         {"moe_dispatch_backward", 1},  {"moe_combine_rows", 1},
+    {"moe_combine_rows_backward", 1}, {"linear_lora", 1},       {"linear_lora_backward", 1},
+    {"moe_dispatch_host", 0},    {"moe_dispatch_backward_host", 0}, {"moe_combine_rows_host", 0},
+    {"moe_combine_rows_backward_host", 0}, {"linear_lora_host", 0}, {"linear_lora_backward_host", 0},
 };
 
 int nh_kernel_count(void) { return (int)(sizeof(kRegistry) / sizeof(kRegistry[0])); }

@@ -119,7 +119,15 @@ enum KernelId : int {
     K_BALANCE_PARTIAL,           // router balance: sums per chunk of tokens
     K_BALANCE_REDUCE,
     K_BALANCE_BACKWARD,
-    K_COUNT
+    K_MOE_SCATTER,               // rows by expert: the tokens' and the rows' types, f32 f32, f32 bf16, bf16 f32, bf16 bf16
+    K_MOE_GATHER = K_MOE_SCATTER + 4,
+    K_LORA_PLAN = K_MOE_GATHER + 4,
+    K_LORA_FINISH,
+    K_LORA_REDUCE,
+    K_LORA_SHRINK,               // bf16 (f32: + 8) of 16 rows (64: + 4), ranks to 16, 32, 64, 128
+    K_LORA_EXPAND = K_LORA_SHRINK + 16,
+    K_LORA_OUTER = K_LORA_EXPAND + 16,  // bf16 (f32: + 4), ranks to 16, 32, 64, 128
+    K_COUNT = K_LORA_OUTER + 8
 };
 
 extern const char* const kKernelSymbols[K_COUNT];

@@ -180,6 +180,24 @@ _SIGNATURES = {
     "nh_moe_balance_loss_backward": (ST, [P, P, P, P, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, P, E]),
     "nh_moe_balance_loss_host": (ST, [P, P, P, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, E]),
     "nh_moe_balance_loss_backward_host": (ST, [P, P, P, SZ, SZ, SZ, SZ, C.c_int, C.c_float, P, P, E]),
+    "nh_supports_moe_rows": (C.c_int, [SZ, SZ, SZ, SZ]),
+    "nh_moe_dispatch": (ST, [P, P, C.c_int, P, P, SZ, SZ, SZ, SZ, P, C.c_int, P, E]),
+    "nh_moe_dispatch_backward": (ST, [P, P, C.c_int, P, C.c_int, P, P, SZ, SZ, SZ, SZ, P, P, P, E]),
+    "nh_moe_combine_rows": (ST, [P, P, C.c_int, P, P, P, SZ, SZ, SZ, SZ, P, C.c_int, P, E]),
+    "nh_moe_combine_rows_backward": (ST, [P, P, C.c_int, P, C.c_int, P, P, SZ, SZ, SZ, SZ, P, P, P, E]),
+    "nh_moe_dispatch_host": (ST, [P, C.c_int, P, P, SZ, SZ, SZ, SZ, P, C.c_int, E]),
+    "nh_moe_dispatch_backward_host": (ST, [P, C.c_int, P, C.c_int, P, P, SZ, SZ, SZ, SZ, P, P, E]),
+    "nh_moe_combine_rows_host": (ST, [P, C.c_int, P, P, P, SZ, SZ, SZ, SZ, P, C.c_int, E]),
+    "nh_moe_combine_rows_backward_host": (ST, [P, C.c_int, P, C.c_int, P, P, SZ, SZ, SZ, SZ, P, P, E]),
+    "nh_supports_linear_lora": (C.c_int, [SZ, SZ, SZ, SZ, SZ]),
+    "nh_linear_lora_workspace_size": (SZ, [SZ, SZ, SZ, SZ, SZ]),
+    "nh_linear_lora": (ST, [P, P, C.c_int, P, P, P, C.c_int, P, SZ, SZ, SZ, SZ, SZ, P, P, C.c_int, P, P, SZ, P, E]),
+    "nh_linear_lora_backward_workspace_size": (SZ, [SZ, SZ, SZ, SZ, SZ]),
+    "nh_linear_lora_backward": (ST, [P, P, C.c_int, P, P, P, C.c_int, P, P, P, C.c_int, SZ, SZ, SZ, SZ, SZ, P, P, P, P,
+                                     C.c_int, P, SZ, P, E]),
+    "nh_linear_lora_host": (ST, [P, C.c_int, P, P, P, C.c_int, P, SZ, SZ, SZ, SZ, SZ, P, P, C.c_int, P, E]),
+    "nh_linear_lora_backward_host": (ST, [P, C.c_int, P, P, P, C.c_int, P, P, P, C.c_int, SZ, SZ, SZ, SZ, SZ, P, P, P, P,
+                                          C.c_int, E]),
     "nh_safetensors_tensor_info": (ST, [C.c_char_p, C.c_char_p, C.POINTER(TensorInfo), E]),
     "nh_safetensors_read": (ST, [P, C.c_char_p, C.c_char_p, P, SZ, E]),
     "nh_load_linear_i8": (ST, [P, C.c_char_p, C.c_char_p, C.c_char_p, SZ, SZ, P, SZ, P, SZ, P, E]),
