@@ -342,10 +342,16 @@ class _Bound:
         self.add("nh_moe_dispatch_backward", s["drows"], d, None, d, s["pos"], None, t, k, h, t * k, dx, None)
         return {"dy": dy, "dweights": dweights, "dx": dx}
 
+    def onto(self, case, base):
+        """Where a call's result goes.  The plain form adds to an f32 base where it stands, but for the rows that it
+        takes one by one: so do the calls."""
+        one_by_one = case["op"] == "lora" and case["m"] <= case["adapters"]
+        return base if case["x"] == "f32" and not one_by_one else self.empty(base.shape, base.dtype)
+
     def _forward(self, case, s, h):
         sizes = [case[v] for v in ("m", "n", "k", "rank", "adapters")]
         d, w = self.dtype(case["x"]), self.dtype(case["w"])
-        out = self.empty((case["m"], case["n"]), DT[case["x"]])
+        out = self.onto(case, s["base"])
         ws = self.workspace("nh_linear_lora_workspace_size", *sizes)
         self.add("nh_linear_lora", s["x"], d, s["ids"], s["a"], s["b"], w, s["scales"], *sizes, s["base"], out, d, h, *ws)
         return out
@@ -357,7 +363,7 @@ class _Bound:
         sizes = [case[v] for v in ("m", "n", "k", "rank", "adapters")]
         m, n, k, r, count = sizes
         d, w = self.dtype(case["x"]), self.dtype(case["w"])
-        h, dx = self.empty((m, r), torch.float32), self.empty((m, k), DT[case["x"]])
+        h, dx = self.empty((m, r), torch.float32), self.onto(case, s["dx_base"])
         da, db = self.empty((count, r, k), torch.float32), self.empty((count, n, r), torch.float32)
         out = self._forward(case, s, h)
         ws = self.workspace("nh_linear_lora_backward_workspace_size", *sizes)
