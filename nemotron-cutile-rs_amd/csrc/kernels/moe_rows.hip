@@ -11,8 +11,13 @@
 //
 // Bound by the rows' bytes: each value of a row is read or written once, each of
 // a token once.  One workgroup per token, so that pos and the weights are
-// uniform and a weight's gradient is one sum of the workgroup; eight consecutive
-// values per thread and turn, as many threads as take the row in the fewest turns.
+// uniform and a weight's gradient is one sum of the workgroup; 16 bytes of a row
+// per thread and turn, all of a token's routes in flight, as many threads as take
+// the row in the fewest turns.  Rows of 64 MiB and more in all go past the caches,
+// which they would only sweep.  8192 x 2688 bf16, 6 routes each: dispatch (308 MB)
+// 55 us, 64 through the caches; combine (308 MB) 59, 86 so; combine backward with
+// the weights' gradients (573 MB) 108; dispatch backward 59: 5.2 to 5.6 TB/s, the
+// rate of a copy.
 // Sums run in f32, over j in route order; results do not change from run to run.
 #include "nh_device.h"
 
@@ -22,92 +27,132 @@ namespace {
 
 constexpr int kRowRoutes = 8;  // routes in flight
 
-// Eight values of a row from column c on, `n` of them there (0: none is read).
-template <int DT>
-__device__ __forceinline__ void row_load8(const void* p, int64_t at, int n, float (&v)[8]) {
-    if constexpr (DT == DT_BF16) {
-        const uint16_t* q = (const uint16_t*)p + at;
-        if (n >= 8) {
-            v4i x;
-            __builtin_memcpy(&x, q, 16);
-            unpack_bf16x8(x, v);
-        } else {
+// What a thread has of a row: V consecutive values, as they lie in memory.
+template <int DT, int V>
+struct RowPart {
+    static constexpr int bytes = V * (DT == DT_BF16 ? 2 : 4), words = bytes / 4;
+    uint32_t u[words];
+
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < n ? bf16_to_f32(q[i]) : 0.0f;
-        }
-    } else {
-        const float* q = (const float*)p + at;
-        if (n >= 8) {
-            __builtin_memcpy(v, q, 32);
-        } else {
+        for (int i = 0; i < words; ++i) u[i] = 0u;
+    }
+
+    __device__ __forceinline__ void load(const void* p, int64_t at) {
+        __builtin_memcpy(u, (const uint8_t*)p + at * (bytes / V), bytes);
+    }
+
+    // past the caches where `far`
+    __device__ __forceinline__ void load(const void* p, int64_t at, bool far) {
+        static_assert(bytes == 16, "one load");
+        if (!far) return load(p, at);
+        typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(2)));
+        const v4u v = __builtin_nontemporal_load((const v4u*)((const uint8_t*)p + at * (bytes / V)));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < n ? q[i] : 0.0f;
+        for (int i = 0; i < 4; ++i) u[i] = v[i];
+    }
+
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (DT == DT_BF16) return f32_from_bits(i & 1 ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16);
+        else return f32_from_bits(u[i]);
+    }
+};
+
+template <int DT, int V>
+__device__ __forceinline__ void row_store(void* p, int64_t at, const float (&v)[V], bool far = false) {
+    constexpr int words = DT == DT_BF16 ? V / 2 : V;
+    uint32_t x[words];
+#pragma unroll
+    for (int i = 0; i < words; ++i) {
+        if constexpr (DT == DT_BF16) x[i] = f32x2_to_bf16x2(v[2 * i], v[2 * i + 1]);
+        else x[i] = f32_bits(v[i]);
+    }
+    uint8_t* q = (uint8_t*)p + at * (DT == DT_BF16 ? 2 : 4);
+    if constexpr (words == 4) {
+        typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(2)));
+        if (far) {
+            __builtin_nontemporal_store(v4u{x[0], x[1], x[2], x[3]}, (v4u*)q);
+            return;
         }
     }
+    __builtin_memcpy(q, x, 4 * words);
 }
 
-template <int DT>
-__device__ __forceinline__ void row_store8(void* p, int64_t at, int n, const float (&v)[8]) {
-    if constexpr (DT == DT_BF16) {
-        uint16_t* q = (uint16_t*)p + at;
-        if (n >= 8) {
-            const uint32_t x[4] = {f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]),
-                                   f32x2_to_bf16x2(v[6], v[7])};
-            __builtin_memcpy(q, x, 16);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < n) q[i] = f32_to_bf16(v[i]);
-        }
-    } else {
-        float* q = (float*)p + at;
-        if (n >= 8) {
-            __builtin_memcpy(q, v, 32);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < n) q[i] = v[i];
-        }
-    }
-}
-
-// The routes j0 .. of token t: their slots (-1: none) and weights.
+// The routes j0 .. of token t: their slots, and weights; -1 and 0 where there is none.
 __device__ __forceinline__ void row_routes(const MoeRowsArgs& a, int64_t t, int j0, int (&slot)[kRowRoutes],
                                            float (&w)[kRowRoutes]) {
+    int s[kRowRoutes];
+    float given[kRowRoutes];
+#pragma unroll
+    for (int j = 0; j < kRowRoutes; ++j) s[j] = j0 + j < a.top_k ? a.pos[t * a.top_k + j0 + j] : -1;
+#pragma unroll
+    for (int j = 0; j < kRowRoutes; ++j) given[j] = a.weights && j0 + j < a.top_k ? a.weights[t * a.top_k + j0 + j] : 1.0f;
 #pragma unroll
     for (int j = 0; j < kRowRoutes; ++j) {
-        slot[j] = -1;
-        w[j] = 1.0f;
-        if (j0 + j >= a.top_k) continue;
-        const int s = a.pos[t * a.top_k + j0 + j];
-        if (s >= 0 && s < a.slots) slot[j] = s;
-        if (a.weights) w[j] = a.weights[t * a.top_k + j0 + j];
+        const bool there = s[j] >= 0 && s[j] < a.slots;
+        slot[j] = __builtin_amdgcn_readfirstlane(there ? s[j] : -1);
+        w[j] = f32_from_bits((uint32_t)__builtin_amdgcn_readfirstlane((int)f32_bits(there ? given[j] : 0.0f)));
     }
 }
 
-// The workgroup's sums of d, one per route, to dweights.
+// The workgroup's sums of d, one per route, to dweights: the wave's eight sums in
+// ten lane moves, each of the first three halving how many values a lane has.
 __device__ __forceinline__ void row_dweights(const MoeRowsArgs& a, int64_t t, int j0, const float (&d)[kRowRoutes],
                                              float (&red)[16][kRowRoutes]) {
+    static_assert(kRowRoutes == 8, "three halvings");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    float v4[4], v2[2], v;
 #pragma unroll
-    for (int j = 0; j < kRowRoutes; ++j) {
-        float v = d[j];
+    for (int i = 0; i < 4; ++i) v4[i] = (lane & 32 ? d[i + 4] : d[i]) + __shfl_xor(lane & 32 ? d[i] : d[i + 4], 32, kWave);
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-        if (lane == 0) red[wave][j] = v;
-    }
+    for (int i = 0; i < 2; ++i) v2[i] = (lane & 16 ? v4[i + 2] : v4[i]) + __shfl_xor(lane & 16 ? v4[i] : v4[i + 2], 16, kWave);
+    v = (lane & 8 ? v2[1] : v2[0]) + __shfl_xor(lane & 8 ? v2[0] : v2[1], 8, kWave);
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+    if ((lane & 7) == 0) red[wave][(lane >> 5 & 1) * 4 + (lane >> 4 & 1) * 2 + (lane >> 3 & 1)] = v;
     __syncthreads();
     if ((int)threadIdx.x < kRowRoutes && j0 + (int)threadIdx.x < a.top_k) {
-        float v = red[0][threadIdx.x];
-        for (int w = 1; w < waves; ++w) v += red[w][threadIdx.x];
-        a.dweights[t * a.top_k + j0 + threadIdx.x] = v;
+        float sum = red[0][threadIdx.x];
+        for (int w = 1; w < waves; ++w) sum += red[w][threadIdx.x];
+        a.dweights[t * a.top_k + j0 + threadIdx.x] = sum;
     }
     __syncthreads();
+}
+
+// d[j] += <rows_in[slot j], v[t]> over the thread's columns [c, c + V), or those of them up to H.
+template <int TOKEN, int ROW, int V>
+__device__ __forceinline__ void row_dots(const MoeRowsArgs& a, const void* v, int64_t t, int c, const int (&slot)[kRowRoutes],
+                                         float (&d)[kRowRoutes]) {
+    const int H = a.hidden;
+    if (H - c >= V) {
+        RowPart<TOKEN, V> x;
+        RowPart<ROW, V> y[kRowRoutes];
+        x.load(v, t * H + c);
+#pragma unroll
+        for (int j = 0; j < kRowRoutes; ++j) {
+            y[j].clear();
+            if (slot[j] >= 0) y[j].load(a.rows_in, (int64_t)slot[j] * H + c, a.far);
+        }
+#pragma unroll
+        for (int j = 0; j < kRowRoutes; ++j)
+            if (slot[j] >= 0) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) d[j] = __builtin_fmaf(y[j].value(i), x.value(i), d[j]);
+            }
+    } else {
+        for (int i = c; i < H; ++i) {
+            const float x = load_as_f32(v, t * H + i, TOKEN);
+#pragma unroll
+            for (int j = 0; j < kRowRoutes; ++j)
+                if (slot[j] >= 0) d[j] = __builtin_fmaf(load_as_f32(a.rows_in, (int64_t)slot[j] * H + i, ROW), x, d[j]);
+        }
+    }
 }
 
 template <int TOKEN, int ROW>
 __device__ __forceinline__ void scatter_rows(const MoeRowsArgs& a) {
     __shared__ float red[16][kRowRoutes];
+    constexpr int V = ROW == DT_BF16 ? 8 : 4;
     const int64_t t = a.token0 + blockIdx.x;
     const int H = a.hidden;
     for (int j0 = 0; j0 < a.top_k; j0 += kRowRoutes) {
@@ -116,29 +161,28 @@ __device__ __forceinline__ void scatter_rows(const MoeRowsArgs& a) {
         row_routes(a, t, j0, slot, w);
 #pragma unroll
         for (int j = 0; j < kRowRoutes; ++j) d[j] = 0.0f;
-        for (int c = 8 * threadIdx.x; c < H; c += 8 * blockDim.x) {
-            const int n = H - c;
-            float v[8], y[kRowRoutes][8];
-            row_load8<TOKEN>(a.tokens, t * H + c, n, v);
-            if (a.dweights) {
-#pragma unroll
-                for (int j = 0; j < kRowRoutes; ++j)
-                    if (slot[j] >= 0) row_load8<ROW>(a.rows_in, (int64_t)slot[j] * H + c, n, y[j]);
+        for (int c = V * threadIdx.x; c < H; c += V * blockDim.x) {
+            // rows_in may be rows_out: the thread's own values, read first
+            if (a.dweights) row_dots<TOKEN, ROW, V>(a, a.tokens, t, c, slot, d);
+            if (H - c >= V) {
+                RowPart<TOKEN, V> v;
+                v.load(a.tokens, t * H + c);
 #pragma unroll
                 for (int j = 0; j < kRowRoutes; ++j)
                     if (slot[j] >= 0) {
+                        float o[V];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) d[j] = __builtin_fmaf(y[j][i], v[i], d[j]);
+                        for (int i = 0; i < V; ++i) o[i] = w[j] * v.value(i);
+                        row_store<ROW, V>(a.rows_out, (int64_t)slot[j] * H + c, o, a.far);
                     }
-            }
+            } else {
+                for (int i = c; i < H; ++i) {
+                    const float v = load_as_f32(a.tokens, t * H + i, TOKEN);
 #pragma unroll
-            for (int j = 0; j < kRowRoutes; ++j)
-                if (slot[j] >= 0) {
-                    float o[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = a.weights ? w[j] * v[i] : v[i];
-                    row_store8<ROW>(a.rows_out, (int64_t)slot[j] * H + c, n, o);
+                    for (int j = 0; j < kRowRoutes; ++j)
+                        if (slot[j] >= 0) store_out(a.rows_out, (int64_t)slot[j] * H + i, w[j] * v, ROW);
                 }
+            }
         }
         if (a.dweights) row_dweights(a, t, j0, d, red);
     }
@@ -147,54 +191,65 @@ __device__ __forceinline__ void scatter_rows(const MoeRowsArgs& a) {
 template <int TOKEN, int ROW>
 __device__ __forceinline__ void gather_rows(const MoeRowsArgs& a) {
     __shared__ float red[16][kRowRoutes];
+    constexpr int V = ROW == DT_BF16 ? 8 : 4;
     const int64_t t = a.token0 + blockIdx.x;
     const int H = a.hidden;
+    int slot[kRowRoutes];
+    float w[kRowRoutes];
     if (a.dweights) {
         for (int j0 = 0; j0 < a.top_k; j0 += kRowRoutes) {
-            int slot[kRowRoutes];
-            float w[kRowRoutes], d[kRowRoutes];
+            float d[kRowRoutes];
             row_routes(a, t, j0, slot, w);
 #pragma unroll
             for (int j = 0; j < kRowRoutes; ++j) d[j] = 0.0f;
-            for (int c = 8 * threadIdx.x; c < H; c += 8 * blockDim.x) {
-                float v[8];
-                row_load8<TOKEN>(a.dot, t * H + c, H - c, v);
-#pragma unroll
-                for (int j = 0; j < kRowRoutes; ++j)
-                    if (slot[j] >= 0) {
-                        float y[8];
-                        row_load8<ROW>(a.rows_in, (int64_t)slot[j] * H + c, H - c, y);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) d[j] = __builtin_fmaf(y[i], v[i], d[j]);
-                    }
-            }
+            for (int c = V * threadIdx.x; c < H; c += V * blockDim.x) row_dots<TOKEN, ROW, V>(a, a.dot, t, c, slot, d);
             row_dweights(a, t, j0, d, red);
         }
     }
-    for (int c = 8 * threadIdx.x; c < H; c += 8 * blockDim.x) {
-        const int n = H - c;
-        float sum[8];
-        if (a.shared) {
-            row_load8<TOKEN>(a.shared, t * H + c, n, sum);
-        } else {
+    row_routes(a, t, 0, slot, w);
+    for (int c = V * threadIdx.x; c < H; c += V * blockDim.x) {
+        float sum[V];
+        const bool whole = H - c >= V;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+        for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+        if (a.shared) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (c + i < H) sum[i] = load_as_f32(a.shared, t * H + c + i, TOKEN);
         }
         for (int j0 = 0; j0 < a.top_k; j0 += kRowRoutes) {
-            int slot[kRowRoutes];
-            float w[kRowRoutes], y[kRowRoutes][8];
-            row_routes(a, t, j0, slot, w);
+            if (a.top_k > kRowRoutes) row_routes(a, t, j0, slot, w);
+            RowPart<ROW, V> y[kRowRoutes];
+            if (whole) {
 #pragma unroll
-            for (int j = 0; j < kRowRoutes; ++j)
-                if (slot[j] >= 0) row_load8<ROW>(a.rows_in, (int64_t)slot[j] * H + c, n, y[j]);
-#pragma unroll
-            for (int j = 0; j < kRowRoutes; ++j)
-                if (slot[j] >= 0) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sum[i] = a.weights ? __builtin_fmaf(w[j], y[j][i], sum[i]) : sum[i] + y[j][i];
+                for (int j = 0; j < kRowRoutes; ++j) {
+                    y[j].clear();
+                    if (slot[j] >= 0) y[j].load(a.rows_in, (int64_t)slot[j] * H + c, a.far);
                 }
+#pragma unroll
+                for (int j = 0; j < kRowRoutes; ++j)
+                    if (slot[j] >= 0) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) sum[i] = __builtin_fmaf(w[j], y[j].value(i), sum[i]);
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (c + i < H) {
+#pragma unroll
+                        for (int j = 0; j < kRowRoutes; ++j)
+                            if (slot[j] >= 0)
+                                sum[i] = __builtin_fmaf(w[j], load_as_f32(a.rows_in, (int64_t)slot[j] * H + c + i, ROW), sum[i]);
+                    }
+            }
         }
-        row_store8<TOKEN>(a.out, t * H + c, n, sum);
+        if (whole) {
+            row_store<TOKEN, V>(a.out, t * H + c, sum);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (c + i < H) store_out(a.out, t * H + c + i, sum[i], TOKEN);
+        }
     }
 }
 
@@ -208,3 +263,144 @@ __device__ __forceinline__ void gather_rows(const MoeRowsArgs& a) {
 NH_ROWS_KERNELS(scatter_rows, scatter_rows)  // tokens' type, rows' type
 NH_ROWS_KERNELS(gather_rows, gather_rows)
 #undef NH_ROWS_KERNELS
+
+// ---- many routes sorted by expert ----------------------------------------------
+// The stable counting sort of nh_moe_permute over chunks of consecutive routes, a
+// workgroup each (the last one takes the rest, less than two chunks):
+//   count: the chunk's routes per expert, left in the chunk's own part of pos;
+//   scan:  one workgroup turns them into each chunk's first slot per expert;
+//   place: the chunk's waves take consecutive routes; a wave's 64 routes at a time
+//          find their rank among the equal ones by ballots.
+// 49152 routes to 128 experts: 4.8 us each, where one workgroup took 185 for all.
+// pos is its own workspace: a chunk has at least as many routes as there are
+// experts, and place has read its part before it writes there.
+namespace {
+
+__device__ __forceinline__ void sort_chunk(const MoeSortArgs& a, int c, int& r0, int& r1) {
+    r0 = c * a.chunk;
+    r1 = c == a.chunks - 1 ? a.routes : r0 + a.chunk;
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(1024) void nh_moe_sort_count_kernel(MoeSortArgs a) {
+    extern __shared__ int sort_lds[];  // [E]
+    const int E = a.experts;
+    int r0, r1;
+    sort_chunk(a, blockIdx.x, r0, r1);
+    for (int e = threadIdx.x; e < E; e += blockDim.x) sort_lds[e] = 0;
+    __syncthreads();
+    for (int r = r0 + threadIdx.x; r < r1; r += blockDim.x) {
+        const int e = a.indices[r];
+        if (e >= 0 && e < E) atomicAdd(&sort_lds[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += blockDim.x) a.pos[r0 + e] = sort_lds[e];
+}
+
+// Threads by expert (up to 1024 at a time) and by part of the chunks.
+extern "C" __global__ __launch_bounds__(1024) void nh_moe_sort_scan_kernel(MoeSortArgs a) {
+    __shared__ int part[1024], first[1024], wave_sum[16];
+    const int E = a.experts, cols = min(E, 1024), parts = 1024 / cols;
+    const int col = threadIdx.x % cols, p = threadIdx.x / cols, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int per = (a.chunks + parts - 1) / parts, c0 = min(a.chunks, p * per), c1 = p < parts ? min(a.chunks, c0 + per) : c0;
+    int carry = 0;
+    for (int base = 0; base < E; base += cols) {
+        const int e = base + col;
+        constexpr int kAhead = 8;
+        int sum = 0;
+        if (e < E)
+            for (int c = c0; c < c1; c += kAhead) {
+                int v[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) v[u] = c + u < c1 ? a.pos[(int64_t)(c + u) * a.chunk + e] : 0;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) sum += v[u];
+            }
+        part[threadIdx.x] = sum;
+        __syncthreads();
+        int total = 0;  // of expert base + thread
+        if ((int)threadIdx.x < cols && base + (int)threadIdx.x < E)
+            for (int q = 0; q < parts; ++q) total += part[q * cols + threadIdx.x];
+        int incl = total;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int t = __shfl_up(incl, off, kWave);
+            if (lane >= off) incl += t;
+        }
+        if (lane == 63) wave_sum[wave] = incl;
+        __syncthreads();
+        int before = carry, all = 0;
+        for (int w = 0; w < 16; ++w) {
+            before += w < wave ? wave_sum[w] : 0;
+            all += wave_sum[w];
+        }
+        if ((int)threadIdx.x < cols && base + (int)threadIdx.x < E) {
+            first[threadIdx.x] = before + incl - total;
+            a.offsets[base + threadIdx.x] = before + incl - total;
+        }
+        carry += all;
+        __syncthreads();
+        if (e < E && p < parts) {
+            int at = first[col];
+            for (int q = 0; q < p; ++q) at += part[q * cols + col];
+            for (int c = c0; c < c1; c += kAhead) {
+                int v[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) v[u] = c + u < c1 ? a.pos[(int64_t)(c + u) * a.chunk + e] : 0;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                    if (c + u < c1) {
+                        a.pos[(int64_t)(c + u) * a.chunk + e] = at;
+                        at += v[u];
+                    }
+            }
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) a.offsets[E] = carry;
+}
+
+extern "C" __global__ __launch_bounds__(1024) void nh_moe_sort_place_kernel(MoeSortArgs a) {
+    extern __shared__ int sort_lds[];  // [waves][E]: the wave's routes per expert, then its next slot
+    const int E = a.experts, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    int c0, c1;
+    sort_chunk(a, blockIdx.x, c0, c1);
+    const int per = ((c1 - c0 + waves - 1) / waves + 63) & ~63;
+    const int r0 = min(c1, c0 + wave * per), r1 = min(c1, r0 + per);
+    int* mine = sort_lds + wave * E;
+    for (int e = threadIdx.x; e < waves * E; e += blockDim.x) sort_lds[e] = 0;
+    __syncthreads();
+    for (int r = r0 + lane; r < r1; r += 64) {
+        const int e = a.indices[r];
+        if (e >= 0 && e < E) atomicAdd(&mine[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        int at = a.pos[c0 + e];
+        for (int w = 0; w < waves; ++w) {
+            const int n = sort_lds[w * E + e];
+            sort_lds[w * E + e] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+    int bits = 0;
+    while ((1 << bits) < E) ++bits;
+    for (int base = r0; base < r1; base += 64) {  // uniform per wave
+        const int r = base + lane;
+        int e = r < r1 ? a.indices[r] : -1;
+        if (e >= E) e = -1;
+        uint64_t same = __ballot(e >= 0);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t bal = __ballot(e >= 0 && ((e >> b) & 1));
+            same &= ((e >> b) & 1) ? bal : ~bal;
+        }
+        const int leader = e >= 0 ? __ffsll((unsigned long long)same) - 1 : 0;
+        int slot = 0;
+        if (e >= 0 && lane == leader) slot = atomicAdd(&mine[e], __popcll(same));
+        slot = __shfl(slot, leader, kWave) + __popcll(same & ((1ull << lane) - 1));
+        if (r < r1) a.pos[r] = e >= 0 ? slot : -1;
+        if (e >= 0) a.perm[slot] = r;
+    }
+}

@@ -491,7 +491,17 @@ struct MoeRowsArgs {
     int64_t slots;
     int32_t top_k, hidden;
     int32_t threads;         // blockDim
-    int32_t pad_;
+    int32_t far;             // 1: the rows go past the caches
+};
+
+// The sort of many routes: see moe_rows.hip.
+struct MoeSortArgs {
+    const int32_t* indices;  // [routes]
+    int32_t* offsets;        // [experts + 1]
+    int32_t* perm;           // [routes]
+    int32_t* pos;            // [routes]; between the launches each chunk's part holds its counts or first slots
+    int32_t routes, experts;
+    int32_t chunk, chunks;   // routes per chunk, experts at least
 };
 
 // ---- low-rank adapters beside a linear layer (lora.hip) ---------------------

@@ -22,13 +22,14 @@ nh_status check_rows(nh_dtype token, nh_dtype row, size_t tokens, size_t top_k, 
     return NH_OK;
 }
 
-// One workgroup per token; eight values a thread, as many threads as take the row
-// in the fewest turns of at most 512.
+// One workgroup per token; 16 bytes of a row per thread and turn, as many threads
+// as take it in the fewest turns of at most 512.
 nh_status launch_rows(nh_context* ctx, KernelId first, MoeRowsArgs a, nh_dtype token, nh_dtype row, size_t tokens,
                       nh_stream stream, nh_error* err) {
     const KernelId id = (KernelId)(first + (token == NH_BF16 ? 2 : 0) + (row == NH_BF16 ? 1 : 0));
-    const size_t vectors = ((size_t)a.hidden + 7) / 8, turns = (vectors + 511) / 512;
+    const size_t v = row == NH_BF16 ? 8 : 4, vectors = ((size_t)a.hidden + v - 1) / v, turns = (vectors + 511) / 512;
     a.threads = (int)(((vectors + turns - 1) / turns + 63) / 64 * 64);
+    a.far = tokens * (size_t)a.top_k * (size_t)a.hidden * bytes_of(row) >= ((size_t)64 << 20) ? 1 : 0;
     const size_t most = ((1ull << 32) - 1) / (size_t)a.threads;  // workgroups of a launch: fewer than 2^32 threads
     for (size_t t0 = 0; t0 < tokens; t0 += most) {
         a.token0 = (int64_t)t0;

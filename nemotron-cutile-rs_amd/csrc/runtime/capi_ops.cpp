@@ -1100,6 +1100,14 @@ nh_status nh_moe_route_sigmoid_topk(nh_context* ctx, const float* scores, size_t
     return launch(ctx, K_ROUTE_SIGMOID, (unsigned)((tokens + 3) / 4), 256, 0, stream, a, err);
 }
 
+// Routes per chunk of the sort of many: 1024 (a round of 16 waves) and up so that
+// there are at most 256 chunks, and no more than one workgroup scans in time (64 K
+// counts); never fewer than the experts, whose counts lie in a chunk's part of pos.
+static size_t sort_chunk(size_t routes, size_t experts) {
+    const size_t most = std::min<size_t>(256, std::max<size_t>(16, 65536 / experts));
+    return std::max<size_t>({1024, (experts + 63) / 64 * 64, ((routes + most - 1) / most + 1023) / 1024 * 1024});
+}
+
 nh_status nh_moe_permute(nh_context* ctx, const int32_t* indices, size_t tokens, size_t top_k, size_t experts,
                          int32_t* offsets, int32_t* perm, int32_t* pos, nh_stream stream, nh_error* err) {
     clear_error(err);
@@ -1110,12 +1118,22 @@ nh_status nh_moe_permute(nh_context* ctx, const int32_t* indices, size_t tokens,
     nh_status st = bind_device(ctx, err);
     if (st) return st;
     PermuteArgs a{indices, offsets, perm, pos, (int)routes, (int)experts};
-    // one workgroup per expert while their reads of the ids stay small
-    // (experts x routes <= 4M: 16 MiB of L2 reads; the 512-token top-6 layer
-    // with 128 experts reads 1.5 MiB) and the ids are 16-byte aligned, else
-    // the single-workgroup form
-    if (experts * routes <= ((size_t)1 << 22) && aligned16(indices))
+    // Few routes: one workgroup per expert that reads all of them (and stays within
+    // 4 M reads in all, with 16-byte aligned ids).  It takes 6.9 us for 4096 routes,
+    // 8.5 for 8192, 14.4 for 16384 whatever the experts; the three launches over
+    // chunks 12 for 8192 to 131072 of 128 experts.  Others, and 4096 experts' few,
+    // in one workgroup.
+    if (routes <= 12288 && experts * routes <= ((size_t)1 << 22) && aligned16(indices))
         return launch(ctx, K_PERMUTE_EXPERT, (unsigned)experts, 256, 0, stream, a, err);
+    const size_t chunk = sort_chunk(routes, experts);
+    if (routes >= 2 * chunk) {
+        MoeSortArgs s{indices, offsets, perm, pos, (int)routes, (int)experts, (int)chunk, (int)(routes / chunk)};
+        const unsigned waves = experts <= 1024 ? 16 : 4;  // 64 KiB of LDS at most
+        if ((st = launch(ctx, K_MOE_SORT_COUNT, (unsigned)s.chunks, 1024, experts * sizeof(int), stream, s, err)) ||
+            (st = launch(ctx, K_MOE_SORT_SCAN, 1, 1024, 0, stream, s, err)))
+            return st;
+        return launch(ctx, K_MOE_SORT_PLACE, (unsigned)s.chunks, 64 * waves, waves * experts * sizeof(int), stream, s, err);
+    }
     return launch(ctx, K_PERMUTE, 1, 1024, 2 * experts * sizeof(int), stream, a, err);
 }
 

@@ -122,6 +122,9 @@ const char* const kKernelSymbols[K_COUNT] = {  // in KernelId order
     "nh_moe_gather_rows_f32_bf16_kernel",
     "nh_moe_gather_rows_bf16_f32_kernel",
     "nh_moe_gather_rows_bf16_bf16_kernel",
+    "nh_moe_sort_count_kernel",  // K_MOE_SORT_COUNT
+    "nh_moe_sort_scan_kernel",
+    "nh_moe_sort_place_kernel",
     "nh_lora_plan_kernel",  // K_LORA_PLAN
     "nh_lora_finish_kernel",  // K_LORA_FINISH
     "nh_lora_reduce_kernel",  // K_LORA_REDUCE

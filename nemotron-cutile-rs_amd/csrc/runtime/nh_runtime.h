@@ -121,7 +121,10 @@ enum KernelId : int {
     K_BALANCE_BACKWARD,
     K_MOE_SCATTER,               // rows by expert: the tokens' and the rows' types, f32 f32, f32 bf16, bf16 f32, bf16 bf16
     K_MOE_GATHER = K_MOE_SCATTER + 4,
-    K_LORA_PLAN = K_MOE_GATHER + 4,
+    K_MOE_SORT_COUNT = K_MOE_GATHER + 4,  // many routes by expert, in three launches
+    K_MOE_SORT_SCAN,
+    K_MOE_SORT_PLACE,
+    K_LORA_PLAN,
     K_LORA_FINISH,
     K_LORA_REDUCE,
     K_LORA_SHRINK,               // bf16 (f32: + 8) of 16 rows (64: + 4), ranks to 16, 32, 64, 128
