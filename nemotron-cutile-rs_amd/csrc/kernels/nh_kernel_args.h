@@ -520,7 +520,7 @@ struct LoraPlanArgs {
 
 struct LoraArgs {
     const void* x;           // [m][C] activations (shrink, outer), f32 or bf16
-    const void* w;           // [adapters] matrices of rank x C: [rank][C], or [C][rank] (w_cols)
+    const void* w;           // [adapters] matrices: [rank][C], or [C][rank] (expand forward, shrink backward)
     const int32_t* ids;
     const int32_t* slot_row;
     const int32_t* tile_adapter;
@@ -539,9 +539,9 @@ struct LoraArgs {
     int64_t slots;           // of ht
     int32_t m, C, rank, rank_pad, adapters;
     int32_t x_dtype, w_dtype, out_dtype;
-    int32_t w_cols;          // 1: w is [C][rank]
     int32_t splits;          // parts of C that shrink sums apart
-    int32_t per_wave;        // columns of C per wave (shrink, expand), a multiple of 32
+    int32_t per_wave;        // shrink: columns of C per wave, a multiple of 32
+    int32_t columns;         // expand: columns of C per workgroup, a multiple of 256
     int32_t scaled;          // finish, expand: times the adapter's scale
     int32_t accumulate;
 };

@@ -9,28 +9,36 @@ using namespace nh;
 namespace {
 
 constexpr size_t kTileRows = 64;    // of the plan
-constexpr size_t kDirectRows = 64;  // rows that need no plan: one ballot sees all of them
+constexpr size_t kFewRows = 64;  // rows that need no plan: one ballot sees all of them
 
 size_t bytes_of(nh_dtype d) { return d == NH_BF16 ? 2 : 4; }
 int rank_form(size_t rank) { return rank <= 16 ? 0 : rank <= 32 ? 1 : rank <= 64 ? 2 : 3; }
 size_t rank_pad(size_t rank) { return (size_t)16 << rank_form(rank); }
 size_t most_tiles(size_t m, size_t adapters) { return m / kTileRows + std::min(m, adapters + 1); }
 
-// How shrink cuts C: columns per wave (four waves a workgroup) and parts.
+// How shrink cuts C: waves of a workgroup, columns per wave, and parts.
 struct Split {
-    size_t per_wave, parts;
+    size_t waves, per_wave, parts;
 };
 
-Split shrink_split(size_t m, size_t c) {
-    const size_t tiles = m <= kDirectRows ? m : (m + kTileRows - 1) / kTileRows;
-    size_t parts = std::max<size_t>(1, std::min<size_t>(16, (512 + tiles - 1) / tiles));
-    size_t per_wave = std::max<size_t>(128, ((c + 4 * parts - 1) / (4 * parts) + 31) / 32 * 32);
-    return {per_wave, (c + 4 * per_wave - 1) / (4 * per_wave)};
+Split shrink_split(size_t m, size_t c, size_t rank) {
+    const bool few = m <= kFewRows;
+    const size_t tiles = few ? m : (m + kTileRows - 1) / kTileRows;
+    Split s;
+    s.waves = rank > 64 ? 4 : 8;
+    s.parts = std::max<size_t>(1, std::min<size_t>(16, (256 + tiles - 1) / tiles));
+    s.per_wave = std::max<size_t>(few ? 128 : 64, ((c + s.waves * s.parts - 1) / (s.waves * s.parts) + 31) / 32 * 32);
+    s.parts = (c + s.waves * s.per_wave - 1) / (s.waves * s.per_wave);
+    return s;
 }
 
-// Columns that a wave of expand takes: a workgroup's low-rank values are summed
-// anew by each of a tile's workgroups.
-size_t expand_columns(size_t m) { return m <= 16 ? 32 : m <= kDirectRows ? 64 : 128; }
+// Columns that a workgroup of expand takes: every one of a tile's workgroups sums
+// the low-rank values anew.
+size_t expand_columns(size_t m, size_t c) {
+    const size_t tiles = m <= kFewRows ? m : (m + kTileRows - 1) / kTileRows;
+    const size_t groups = std::max<size_t>(1, (m <= kFewRows ? 768 : 1024) / tiles);
+    return std::max<size_t>(256, std::min<size_t>(2048, ((c + groups - 1) / groups + 255) / 256 * 256));
+}
 
 // Most tiles of an outer item: about 32 items of an evenly dealt batch.
 size_t item_tiles(size_t m) { return std::max<size_t>(1, (m / kTileRows + 31) / 32); }
@@ -51,12 +59,12 @@ Layout lora_layout(size_t m, size_t n, size_t k, size_t rank, size_t adapters, b
     };
     const size_t rp = rank_pad(rank), tiles = most_tiles(m, adapters);
     l.slots = tiles * kTileRows;
-    if (m > kDirectRows || backward) {
+    if (m > kFewRows || backward) {
         l.slot_row = take(l.slots * 4);
         l.tile_adapter = take(tiles * 4);
         l.counts = take(8);
     }
-    l.part_x = take(shrink_split(m, k).parts * m * rp * 4);
+    l.part_x = take(shrink_split(m, k, rank).parts * m * rp * 4);
     if (backward) {
         const size_t it = item_tiles(m);
         // of adapters with more than `it` tiles: t / it + 1 < 2 t / it items each, and over 64 it rows, so
@@ -65,7 +73,7 @@ Layout lora_layout(size_t m, size_t n, size_t k, size_t rank, size_t adapters, b
         l.items_most = tiles / it + std::min(m, adapters) + 1;
         l.items = take(l.items_most * 16);
         l.per_adapter = take(adapters * 8);
-        l.part_d = take(shrink_split(m, n).parts * m * rp * 4);
+        l.part_d = take(shrink_split(m, n, rank).parts * m * rp * 4);
         l.ht_h = take(rp * l.slots * 6);
         l.ht_d = take(rp * l.slots * 6);
         l.gpart_a = take(partials * rank * k * 4);
@@ -101,7 +109,7 @@ struct Lora {
     nh_stream stream;
     nh_error* err;
     size_t m, rank, adapters;
-    bool direct;
+    bool few;
     LoraArgs common;
 
     nh_status plan(const Layout& l, uint8_t* ws, const int32_t* ids, bool items) {
@@ -115,34 +123,33 @@ struct Lora {
         p.m = (int)m;
         p.adapters = (int)adapters;
         p.item_tiles = (int)item_tiles(m);
-        return launch(ctx, K_LORA_PLAN, 1, 1024, 17 * (adapters + 1) * 4, stream, p, err);
+        return launch(ctx, K_LORA_PLAN, 1, 1024, 20 * (adapters + 1) * 4, stream, p, err);
     }
 
-    KernelId form(KernelId first, bool bf16) const {
-        return (KernelId)(first + (bf16 ? 0 : 8) + (direct ? 0 : 4) + rank_form(rank));
+    KernelId form(KernelId first, bool bf16, bool back) const {
+        return (KernelId)(first + (bf16 ? 0 : 12) + (few ? 0 : back ? 8 : 4) + rank_form(rank));
     }
-    unsigned tiles() const { return (unsigned)(direct ? m : most_tiles(m, adapters)); }
+    unsigned tiles() const { return (unsigned)(few ? m : most_tiles(m, adapters)); }
 
-    // part = x w^T by parts of C
-    nh_status shrink(const void* x, nh_dtype xd, const void* w, nh_dtype wd, bool w_cols, size_t c, float* part) {
+    // part = x w^T by parts of C; back: w is [C][rank]
+    nh_status shrink(const void* x, nh_dtype xd, const void* w, nh_dtype wd, bool back, size_t c, float* part) {
         LoraArgs a = common;
-        const Split s = shrink_split(m, c);
+        const Split s = shrink_split(m, c, rank);
         a.x = x;
         a.w = w;
         a.part = part;
         a.C = (int)c;
         a.x_dtype = xd;
         a.w_dtype = wd;
-        a.w_cols = w_cols;
         a.per_wave = (int)s.per_wave;
-        const size_t lds = (size_t)4 * (direct ? 16 : kTileRows) * rank_pad(rank) * 4;
-        return launch(ctx, form(K_LORA_SHRINK, xd == NH_BF16 && wd == NH_BF16), tiles(), 256, lds, stream, a, err,
-                      (unsigned)s.parts);
+        const size_t lds = s.waves / 2 * (few ? 16 : kTileRows) * rank_pad(rank) * 4;
+        return launch(ctx, form(K_LORA_SHRINK, xd == NH_BF16 && wd == NH_BF16, back), tiles(), 64 * (unsigned)s.waves, lds,
+                      stream, a, err, (unsigned)s.parts);
     }
 
-    // out = base + (s) h w, h the sum of `splits` parts
-    nh_status expand(const float* part, size_t splits, const void* w, nh_dtype wd, bool w_cols, size_t c, const void* base,
-                     void* out, nh_dtype od, float* h_out, bool scaled) {
+    // out = base + s h w, h the sum of `splits` parts; back: w is [rank][C]
+    nh_status expand(const float* part, size_t splits, const void* w, nh_dtype wd, bool back, size_t c, const void* base,
+                     void* out, nh_dtype od, float* h_out) {
         LoraArgs a = common;
         a.part = const_cast<float*>(part);
         a.splits = (int)splits;
@@ -153,11 +160,11 @@ struct Lora {
         a.C = (int)c;
         a.w_dtype = wd;
         a.out_dtype = od;
-        a.w_cols = w_cols;
-        a.scaled = scaled;
-        a.per_wave = (int)expand_columns(m);
-        return launch(ctx, form(K_LORA_EXPAND, wd == NH_BF16), tiles(), 256, 0, stream, a, err,
-                      (unsigned)((c + 4 * a.per_wave - 1) / (4 * a.per_wave)));
+        a.scaled = 1;
+        const size_t columns = expand_columns(m, c);
+        a.columns = (int)columns;
+        return launch(ctx, form(K_LORA_EXPAND, wd == NH_BF16, back), tiles(), 256, 0, stream, a, err,
+                      (unsigned)((c + columns - 1) / columns));
     }
 
     // low-rank values by slot
@@ -169,11 +176,11 @@ struct Lora {
         a.ht = ht;
         a.scaled = scaled;
         a.x_dtype = bf16 ? DT_BF16 : DT_F32;
-        return launch(ctx, K_LORA_FINISH, tiles(), 256, 0, stream, a, err);
+        return launch(ctx, K_LORA_FINISH, tiles(), 256, 0, stream, a, err, (unsigned)(rank_pad(rank) / 16));
     }
 
-    // grad = ht x over the rows, laid out [rank][c], or [c][rank] (w_cols)
-    nh_status outer(const void* x, nh_dtype xd, const void* ht, bool w_cols, size_t c, float* gpart, float* grad,
+    // grad = ht x over the rows, laid out [rank][c], or [c][rank] (db)
+    nh_status outer(const void* x, nh_dtype xd, const void* ht, bool db, size_t c, float* gpart, float* grad,
                     bool accumulate, size_t items) {
         LoraArgs a = common;
         a.x = x;
@@ -182,9 +189,8 @@ struct Lora {
         a.grad = grad;
         a.C = (int)c;
         a.x_dtype = xd;
-        a.w_cols = w_cols;
         a.accumulate = accumulate;
-        nh_status st = launch(ctx, (KernelId)(K_LORA_OUTER + (xd == NH_BF16 ? 0 : 4) + rank_form(rank)),
+        nh_status st = launch(ctx, (KernelId)(K_LORA_OUTER + (xd == NH_BF16 ? 0 : 8) + (db ? 4 : 0) + rank_form(rank)),
                               (unsigned)((c + 255) / 256), 256, 0, stream, a, err, (unsigned)items);
         if (st) return st;
         return launch(ctx, K_LORA_REDUCE, (unsigned)((rank * c + 255) / 256), 256, 0, stream, a, err, (unsigned)adapters);
@@ -192,8 +198,8 @@ struct Lora {
 };
 
 Lora make_lora(nh_context* ctx, const int32_t* ids, const float* scales, size_t m, size_t rank, size_t adapters,
-               bool direct, const Layout& l, uint8_t* ws, nh_stream stream, nh_error* err) {
-    Lora c{ctx, stream, err, m, rank, adapters, direct, {}};
+               bool few, const Layout& l, uint8_t* ws, nh_stream stream, nh_error* err) {
+    Lora c{ctx, stream, err, m, rank, adapters, few, {}};
     c.common.ids = ids;
     c.common.scales = scales;
     c.common.slot_row = (int32_t*)(ws + l.slot_row);
@@ -241,11 +247,11 @@ nh_status nh_linear_lora(nh_context* ctx, const void* x, nh_dtype x_dtype, const
     const Layout l = lora_layout(m, n, k, rank, adapters, false);
     if ((st = check_workspace(workspace, workspace_bytes, l.bytes, err)) || (st = bind_device(ctx, err))) return st;
     uint8_t* ws = (uint8_t*)workspace;
-    Lora c = make_lora(ctx, adapter_ids, scales, m, rank, adapters, m <= kDirectRows, l, ws, stream, err);
+    Lora c = make_lora(ctx, adapter_ids, scales, m, rank, adapters, m <= kFewRows, l, ws, stream, err);
     float* part = (float*)(ws + l.part_x);
-    if (!c.direct && (st = c.plan(l, ws, adapter_ids, false))) return st;
+    if (!c.few && (st = c.plan(l, ws, adapter_ids, false))) return st;
     if ((st = c.shrink(x, x_dtype, a, w_dtype, false, k, part))) return st;
-    return c.expand(part, shrink_split(m, k).parts, b, w_dtype, true, n, base, out, out_dtype, h_out, true);
+    return c.expand(part, shrink_split(m, k, rank).parts, b, w_dtype, false, n, base, out, out_dtype, h_out);
 }
 
 nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dtype, const int32_t* adapter_ids,
@@ -272,11 +278,11 @@ nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dty
     uint8_t* ws = (uint8_t*)workspace;
     Lora c = make_lora(ctx, adapter_ids, scales, m, rank, adapters, false, l, ws, stream, err);
     float *part_x = (float*)(ws + l.part_x), *part_d = (float*)(ws + l.part_d);
-    const size_t parts_x = shrink_split(m, k).parts, parts_d = shrink_split(m, n).parts;
+    const size_t parts_x = shrink_split(m, k, rank).parts, parts_d = shrink_split(m, n, rank).parts;
     if ((st = c.plan(l, ws, adapter_ids, true))) return st;
     if (again && (st = c.shrink(x, x_dtype, a, w_dtype, false, k, part_x))) return st;
     if ((dx || da) && (st = c.shrink(dout, dout_dtype, b, w_dtype, true, n, part_d))) return st;
-    if (dx && (st = c.expand(part_d, parts_d, a, w_dtype, false, k, dx_base, dx, x_dtype, nullptr, true))) return st;
+    if (dx && (st = c.expand(part_d, parts_d, a, w_dtype, true, k, dx_base, dx, x_dtype, nullptr))) return st;
     if (da && ((st = c.finish(nullptr, part_d, parts_d, true, x_dtype == NH_BF16, ws + l.ht_d)) ||
                (st = c.outer(x, x_dtype, ws + l.ht_d, false, k, (float*)(ws + l.gpart_a), da, accumulate != 0, l.items_most))))
         return st;

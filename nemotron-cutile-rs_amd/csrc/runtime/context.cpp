@@ -128,46 +128,70 @@ const char* const kKernelSymbols[K_COUNT] = {  // in KernelId order
     "nh_lora_plan_kernel",  // K_LORA_PLAN
     "nh_lora_finish_kernel",  // K_LORA_FINISH
     "nh_lora_reduce_kernel",  // K_LORA_REDUCE
-    "nh_lora_shrink_bf16_1_1_kernel",  // K_LORA_SHRINK
-    "nh_lora_shrink_bf16_1_2_kernel",
-    "nh_lora_shrink_bf16_1_4_kernel",
-    "nh_lora_shrink_bf16_1_8_kernel",
-    "nh_lora_shrink_bf16_4_1_kernel",
-    "nh_lora_shrink_bf16_4_2_kernel",
-    "nh_lora_shrink_bf16_4_4_kernel",
-    "nh_lora_shrink_bf16_4_8_kernel",
-    "nh_lora_shrink_f32_1_1_kernel",
-    "nh_lora_shrink_f32_1_2_kernel",
-    "nh_lora_shrink_f32_1_4_kernel",
-    "nh_lora_shrink_f32_1_8_kernel",
-    "nh_lora_shrink_f32_4_1_kernel",
-    "nh_lora_shrink_f32_4_2_kernel",
-    "nh_lora_shrink_f32_4_4_kernel",
-    "nh_lora_shrink_f32_4_8_kernel",
-    "nh_lora_expand_bf16_1_1_kernel",  // K_LORA_EXPAND
-    "nh_lora_expand_bf16_1_2_kernel",
-    "nh_lora_expand_bf16_1_4_kernel",
-    "nh_lora_expand_bf16_1_8_kernel",
-    "nh_lora_expand_bf16_4_1_kernel",
-    "nh_lora_expand_bf16_4_2_kernel",
-    "nh_lora_expand_bf16_4_4_kernel",
-    "nh_lora_expand_bf16_4_8_kernel",
-    "nh_lora_expand_f32_1_1_kernel",
-    "nh_lora_expand_f32_1_2_kernel",
-    "nh_lora_expand_f32_1_4_kernel",
-    "nh_lora_expand_f32_1_8_kernel",
-    "nh_lora_expand_f32_4_1_kernel",
-    "nh_lora_expand_f32_4_2_kernel",
-    "nh_lora_expand_f32_4_4_kernel",
-    "nh_lora_expand_f32_4_8_kernel",
-    "nh_lora_outer_bf16_1_kernel",  // K_LORA_OUTER
-    "nh_lora_outer_bf16_2_kernel",
-    "nh_lora_outer_bf16_4_kernel",
-    "nh_lora_outer_bf16_8_kernel",
-    "nh_lora_outer_f32_1_kernel",
-    "nh_lora_outer_f32_2_kernel",
-    "nh_lora_outer_f32_4_kernel",
-    "nh_lora_outer_f32_8_kernel",
+    "nh_lora_shrink_bf16_few_1_kernel",  // K_LORA_SHRINK
+    "nh_lora_shrink_bf16_few_2_kernel",
+    "nh_lora_shrink_bf16_few_4_kernel",
+    "nh_lora_shrink_bf16_few_8_kernel",
+    "nh_lora_shrink_bf16_tiles_1_kernel",
+    "nh_lora_shrink_bf16_tiles_2_kernel",
+    "nh_lora_shrink_bf16_tiles_4_kernel",
+    "nh_lora_shrink_bf16_tiles_8_kernel",
+    "nh_lora_shrink_bf16_back_1_kernel",
+    "nh_lora_shrink_bf16_back_2_kernel",
+    "nh_lora_shrink_bf16_back_4_kernel",
+    "nh_lora_shrink_bf16_back_8_kernel",
+    "nh_lora_shrink_f32_few_1_kernel",
+    "nh_lora_shrink_f32_few_2_kernel",
+    "nh_lora_shrink_f32_few_4_kernel",
+    "nh_lora_shrink_f32_few_8_kernel",
+    "nh_lora_shrink_f32_tiles_1_kernel",
+    "nh_lora_shrink_f32_tiles_2_kernel",
+    "nh_lora_shrink_f32_tiles_4_kernel",
+    "nh_lora_shrink_f32_tiles_8_kernel",
+    "nh_lora_shrink_f32_back_1_kernel",
+    "nh_lora_shrink_f32_back_2_kernel",
+    "nh_lora_shrink_f32_back_4_kernel",
+    "nh_lora_shrink_f32_back_8_kernel",
+    "nh_lora_expand_bf16_few_1_kernel",  // K_LORA_EXPAND
+    "nh_lora_expand_bf16_few_2_kernel",
+    "nh_lora_expand_bf16_few_4_kernel",
+    "nh_lora_expand_bf16_few_8_kernel",
+    "nh_lora_expand_bf16_tiles_1_kernel",
+    "nh_lora_expand_bf16_tiles_2_kernel",
+    "nh_lora_expand_bf16_tiles_4_kernel",
+    "nh_lora_expand_bf16_tiles_8_kernel",
+    "nh_lora_expand_bf16_back_1_kernel",
+    "nh_lora_expand_bf16_back_2_kernel",
+    "nh_lora_expand_bf16_back_4_kernel",
+    "nh_lora_expand_bf16_back_8_kernel",
+    "nh_lora_expand_f32_few_1_kernel",
+    "nh_lora_expand_f32_few_2_kernel",
+    "nh_lora_expand_f32_few_4_kernel",
+    "nh_lora_expand_f32_few_8_kernel",
+    "nh_lora_expand_f32_tiles_1_kernel",
+    "nh_lora_expand_f32_tiles_2_kernel",
+    "nh_lora_expand_f32_tiles_4_kernel",
+    "nh_lora_expand_f32_tiles_8_kernel",
+    "nh_lora_expand_f32_back_1_kernel",
+    "nh_lora_expand_f32_back_2_kernel",
+    "nh_lora_expand_f32_back_4_kernel",
+    "nh_lora_expand_f32_back_8_kernel",
+    "nh_lora_outer_bf16_a_1_kernel",  // K_LORA_OUTER
+    "nh_lora_outer_bf16_a_2_kernel",
+    "nh_lora_outer_bf16_a_4_kernel",
+    "nh_lora_outer_bf16_a_8_kernel",
+    "nh_lora_outer_bf16_b_1_kernel",
+    "nh_lora_outer_bf16_b_2_kernel",
+    "nh_lora_outer_bf16_b_4_kernel",
+    "nh_lora_outer_bf16_b_8_kernel",
+    "nh_lora_outer_f32_a_1_kernel",
+    "nh_lora_outer_f32_a_2_kernel",
+    "nh_lora_outer_f32_a_4_kernel",
+    "nh_lora_outer_f32_a_8_kernel",
+    "nh_lora_outer_f32_b_1_kernel",
+    "nh_lora_outer_f32_b_2_kernel",
+    "nh_lora_outer_f32_b_4_kernel",
+    "nh_lora_outer_f32_b_8_kernel",
 };
 
 void clear_error(nh_error* err) {

@@ -127,10 +127,10 @@ enum KernelId : int {
     K_LORA_PLAN,
     K_LORA_FINISH,
     K_LORA_REDUCE,
-    K_LORA_SHRINK,               // bf16 (f32: + 8) of 16 rows (64: + 4), ranks to 16, 32, 64, 128
-    K_LORA_EXPAND = K_LORA_SHRINK + 16,
-    K_LORA_OUTER = K_LORA_EXPAND + 16,  // bf16 (f32: + 4), ranks to 16, 32, 64, 128
-    K_COUNT = K_LORA_OUTER + 8
+    K_LORA_SHRINK,               // bf16 (f32: + 12), a few rows (tiles: + 4, backward: + 8), ranks to 16, 32, 64, 128
+    K_LORA_EXPAND = K_LORA_SHRINK + 24,
+    K_LORA_OUTER = K_LORA_EXPAND + 24,  // bf16 (f32: + 8), da (db: + 4), ranks to 16, 32, 64, 128
+    K_COUNT = K_LORA_OUTER + 16
 };
 
 extern const char* const kKernelSymbols[K_COUNT];

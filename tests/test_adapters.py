@@ -256,7 +256,7 @@ def test_accepted_sizes_can_be_launched(rec):
             launches += rec.launches("nh_moe_dispatch", 1 << 50, NH.BF16, S, None, t, k, h, t, far, NH.F32, None)
             launches += rec.launches("nh_moe_combine_rows", far, NH.F32, S, None, None, t, k, h, t, 1 << 50, NH.BF16, None)
         for kernel, gx, gy in launches:
-            threads = 1024 if kernel == "lora_plan" else 512 if "rows" in kernel else 256
+            threads = 1024 if kernel == "lora_plan" else 512 if "rows" in kernel or "shrink" in kernel else 256
             assert gx >= 1 and gx * (threads if "rows" not in kernel else 64) < 1 << 32 and 1 <= gy <= 65535, (kernel, gx, gy)
             seen.add(kernel)
     assert len([k for k in seen if "lora_shrink" in k]) >= 4
@@ -265,7 +265,7 @@ def test_accepted_sizes_can_be_launched(rec):
 @pytest.mark.parametrize("m,plan", [(1, False), (64, False), (65, True), (5000, True)])
 def test_few_rows_need_no_plan(rec, m, plan):
     launches = rec.kernels("nh_linear_lora", *lora_args(m, 512, 512, 16, 4))
-    assert launches == (["lora_plan"] if plan else []) + [f"lora_{f}_bf16_{4 if plan else 1}_1" for f in ("shrink", "expand")]
+    assert launches == (["lora_plan"] if plan else []) + [f"lora_{f}_bf16_{'tiles' if plan else 'few'}_1" for f in ("shrink", "expand")]
 
 
 @pytest.mark.parametrize("rank,form", [(1, 1), (16, 1), (17, 2), (32, 2), (33, 4), (64, 4), (65, 8), (128, 8)])
@@ -273,9 +273,10 @@ def test_few_rows_need_no_plan(rec, m, plan):
                                          (NH.BF16, NH.F32, ("f32", "f32", "bf16")), (NH.F32, NH.F32, ("f32", "f32", "f32"))])
 def test_forms_by_rank_and_type(rec, rank, form, xd, wd, kinds):
     launches = rec.kernels("nh_linear_lora", *lora_args(200, 512, 512, rank, 4, xd=xd, wd=wd))
-    assert launches[1:] == [f"lora_shrink_{kinds[0]}_4_{form}", f"lora_expand_{kinds[1]}_4_{form}"]
+    assert launches[1:] == [f"lora_shrink_{kinds[0]}_tiles_{form}", f"lora_expand_{kinds[1]}_tiles_{form}"]
     launches = rec.kernels("nh_linear_lora_backward", *back_args(200, 512, 512, rank, 4, xd=xd, wd=wd, dd=xd))
-    assert {f"lora_shrink_{kinds[0]}_4_{form}", f"lora_expand_{kinds[1]}_4_{form}", f"lora_outer_{kinds[2]}_{form}"} <= set(launches)
+    assert {f"lora_shrink_{kinds[0]}_back_{form}", f"lora_expand_{kinds[1]}_back_{form}", f"lora_outer_{kinds[2]}_a_{form}",
+            f"lora_outer_{kinds[2]}_b_{form}"} <= set(launches)
 
 
 # ---- the surface ----------------------------------------------------------------------
