@@ -26,8 +26,18 @@ namespace {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(2)));
 
-constexpr int kTileRows = 64;  // slots per tile of the plan
+constexpr int kTileRows = 64;     // slots per tile of the plan
+constexpr int kExpandAhead = 3;   // steps of base in flight
+
+// A choice made where a body is built.
+template <bool B>
+struct Choice {
+    static constexpr bool value = B;
+};
+typedef Choice<true> Yes;
+typedef Choice<false> No;
 
 // ---- operands of a matrix instruction: eight values per lane, of lane l for row
 // or column l % 16 and K 8 (l / 16) .. + 7
@@ -108,18 +118,8 @@ __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Eight f32 values as an operand: PARTS bf16 parts, or as they are.  A value
-// that is not finite is its first part, with zeros behind.
-template <int PARTS>
-struct Split16 {
-    static constexpr int parts = PARTS;
-    Frag16 f[PARTS];
-};
-struct Split32 {
-    static constexpr int parts = 1;
-    Frag32 f[1];
-};
-
+// The next bf16 part of v, which keeps the rest.  A value that is not finite is its
+// first part, with zeros behind.
 __device__ __forceinline__ uint32_t bf16_part(float& v) {
     const uint32_t u = f32_bits(v);
     if ((u & 0x7f800000u) == 0x7f800000u) {
@@ -130,168 +130,250 @@ __device__ __forceinline__ uint32_t bf16_part(float& v) {
     return u >> 16;
 }
 
-template <int PARTS>
-__device__ __forceinline__ void split8(const float (&v)[8], Split16<PARTS>& s) {
-    float r[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = v[i];
-#pragma unroll
-    for (int q = 0; q < PARTS; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = bf16_part(r[2 * i]), hi = bf16_part(r[2 * i + 1]);
-            s.f[q].v[i] = (int)(lo | (hi << 16));
-        }
-}
-__device__ __forceinline__ void split8(const float (&v)[8], Split32& s) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s.f[0].v[i] = v[i];
+// Of lanes 8 apart (in 16) the lower one's second unit for the upper one's first;
+// its own inverse.
+__device__ __forceinline__ void lane_swap(int& first, int& second) {
+    const bool low = (threadIdx.x & 8) == 0;
+    const int x = first, y = second, send = low ? y : x;
+    const int got = __builtin_amdgcn_update_dpp(send, send, 0x128, 0xf, 0xf, false);  // row_ror 8
+    first = low ? x : got;
+    second = low ? got : y;
 }
 
-// ---- the rows of a workgroup ---------------------------------------------------
-// Tile `tile`: its adapter (`adapters`: rows without one) and its rows; returns how
-// many (0: nothing to do), uniform.  64 at a time from the plan, or (FEW) 16 of at
-// most 64 rows in all, where every row that is the 1st, 17th, .. of its adapter
-// leads a tile.
-template <bool FEW>
-__device__ __forceinline__ int lora_tile(const LoraArgs& a, int tile, int* rows, int& adapter) {
-    const int lane = threadIdx.x & 63;
-    if constexpr (FEW) {
-        int e = -1;
-        if (lane < a.m) {
-            e = a.ids[lane];
-            if (e < 0 || e >= a.adapters) e = a.adapters;
-        }
-        adapter = __builtin_amdgcn_readlane(e, tile);
-        const uint64_t same = __ballot(e == adapter);
-        const int before = __popcll(same & ((1ull << tile) - 1));
-        if (before % 16 != 0) return 0;  // uniform
-        const int mine = __popcll(same & ((1ull << lane) - 1)) - before;
-        if (threadIdx.x < 64 && e == adapter && mine >= 0 && mine < 16) rows[mine] = lane;
-        __syncthreads();
-        return min(16, __popcll(same) - before);
-    } else {
-        if (tile >= a.counts[0]) return 0;
-        adapter = a.tile_adapter[tile];
-        const int row = a.slot_row[(int64_t)tile * kTileRows + lane];  // those without a row are the last
-        if (threadIdx.x < 64) rows[lane] = row;
-        __syncthreads();
-        return __popcll(__ballot(row >= 0));
+__device__ __forceinline__ void unit_swap(Frag16& first, Frag16& second) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        int x = first.v[i], y = second.v[i];
+        lane_swap(x, y);
+        first.v[i] = x;
+        second.v[i] = y;
     }
 }
 
+__device__ __forceinline__ void unit_swap(v4u& first, v4u& second) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        int x = (int)first[i], y = (int)second[i];
+        lane_swap(x, y);
+        first[i] = (uint32_t)x;
+        second[i] = (uint32_t)y;
+    }
+}
+
+// ---- the rows of a workgroup ---------------------------------------------------
+// Of at most 64 rows in all every one that is the 1st, 17th, .. of its adapter leads
+// 16: the adapter of row `lead` (`adapters`: none) and the rows, returning how many
+// (0: it leads none), uniform.
+__device__ __forceinline__ int lora_few(const LoraArgs& a, int lead, int* rows, int& adapter) {
+    const int lane = threadIdx.x & 63;
+    int e = -1;
+    if (lane < a.m) {
+        e = a.ids[lane];
+        if (e < 0 || e >= a.adapters) e = a.adapters;
+    }
+    adapter = __builtin_amdgcn_readlane(e, lead);
+    const uint64_t same = __ballot(e == adapter);
+    const int before = __popcll(same & ((1ull << lead) - 1));
+    if (before % 16 != 0) return 0;  // uniform
+    const int mine = __popcll(same & ((1ull << lane) - 1)) - before;
+    if (threadIdx.x < 64 && e == adapter && mine >= 0 && mine < 16) rows[mine] = lane;
+    __syncthreads();
+    return min(16, __popcll(same) - before);
+}
+
+// Consecutive shares of n, to the workgroups of an XCD one after the other
+// (workgroups go round the eight of them, the grid being a multiple): what shares an
+// adapter's matrix reads it into one L2.
+__device__ __forceinline__ int xcd_order(int block, int blocks) { return (block & 7) * (blocks >> 3) + (block >> 3); }
+
 // ---- shrink --------------------------------------------------------------------
-// part[split][row][rank] = sum over the split's columns of x[row][c] w(rank, c).
-// The waves of a workgroup take consecutive parts of the columns, each for all of
-// the tile's rows, so that a matrix is read once per tile, and add up through LDS.
+// part[split][row][rank] = sum over the split's columns of x[row][c] w(rank, c), for
+// 16 rows of an adapter.  The waves take consecutive parts of the columns and add up
+// through LDS; there is one split unless rows are few, so that rows are read once,
+// and the matrix, which all of an adapter's rows share, from the L2s.
 // Ranks past the last and rows past the tile's are computed on the nearest valid
 // operand and not read again; columns past C are zeros in both operands.
-// A matrix of [C][rank] (COLS) goes through LDS, 32 of its rows at a time.
+// bf16 goes through LDS, a wave's part of it: the operands' layout has neighbouring
+// lanes in different rows, and a load costs the address unit a turn for each piece
+// that neighbouring lanes do not continue (8192 x 4096, rank 32: 37 us straight into
+// registers).  So a load has 8 rows of 64 columns, 8 lanes a row, and LDS turns it.
+// A matrix of [C][rank] (COLS) is read as it lies and turned by transposing reads.
+template <class Frag, bool FEW, int RT, bool COLS>
+struct ShrinkForm {
+    static constexpr bool staged = Frag::bf16;
+    static constexpr int RP = 16 * RT;
+    // columns in flight: loads of 10 to 18 KiB a wave
+    static constexpr int block = !Frag::bf16 ? 32 : RT <= 2 ? 128 : 64;
+    static constexpr int pitch = 64 + 8;  // of 16 rows of 64 columns: sixteen rows' reads meet no bank twice
+    // a wave's LDS: 16 rows, and two times 16 more or 32 rows of [C][rank]
+    static constexpr int values = !staged ? 0 : COLS ? 16 * pitch + 64 * RP : 3 * 16 * pitch;
+};
+
 template <class Frag, bool FEW, int RT, bool COLS>
 __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
-    constexpr int RB = FEW ? 1 : 4, RP = 16 * RT, kPlane = 256 * RB * RT;
-    extern __shared__ float lora_lds[];  // half the waves' sums; before: a wave's 32 rows of a [C][rank] matrix each
-    __shared__ int rows[16 * RB];
-    int adapter;
-    const int count = lora_tile<FEW>(a, blockIdx.x, rows, adapter);
+    using F = ShrinkForm<Frag, FEW, RT, COLS>;
+    constexpr int RP = F::RP, kPlane = 16 * RP;
+    extern __shared__ float lora_lds[];  // half the waves' sums; before: each wave's own part
+    __shared__ int rows[16];
+    int adapter, count;
+    unsigned unit = blockIdx.x;
+    if constexpr (FEW) {
+        count = lora_few(a, blockIdx.x, rows, adapter);
+        if (count == 0) return;  // uniform
+    } else {
+        const int tiles = a.counts[0], each = (4 * tiles + 7) / 8, order = blockIdx.x >> 3;
+        unit = (blockIdx.x & 7) * each + order;  // a quarter of a tile
+        if (order >= each || unit >= 4u * tiles) return;
+        const int lane = threadIdx.x & 63;
+        adapter = a.tile_adapter[unit >> 2];
+        const int row = lane < 16 ? a.slot_row[(int64_t)unit * 16 + lane] : -1;  // those without a row are the last
+        if (threadIdx.x < 16) rows[lane] = row;
+        __syncthreads();
+        count = __popcll(__ballot(row >= 0));
+    }
     if (count == 0 || adapter == a.adapters) return;  // uniform
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = blockDim.x >> 7, g = lane >> 4, l16 = lane & 15;
     const int64_t first = ((int64_t)blockIdx.y * (blockDim.x >> 6) + wave) * a.per_wave;
     const int c0 = (int)min((int64_t)a.C, first), c1 = min(a.C, c0 + a.per_wave);
-    int64_t xat[RB], wat[RT];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) xat[b] = (int64_t)rows[min(16 * b + l16, count - 1)] * a.C;
-    const int64_t matrix = (int64_t)adapter * a.rank * a.C;
+    const int64_t matrix = (int64_t)adapter * a.rank * a.C, xat = (int64_t)rows[min(l16, count - 1)] * a.C;
+    int64_t wat[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int rank = min(16 * r + l16, a.rank - 1);
         wat[r] = matrix + (COLS ? rank : (int64_t)rank * a.C);
     }
-    v4f acc[RB][RT];
+    v4f acc[RT];
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) acc[b][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr bool staged = COLS && Frag::bf16;
-    uint16_t* block = (uint16_t*)lora_lds + wave * 32 * RP;
-    // 32 columns from c on: operands, of which the last may be past the end
-    auto load_x = [&](int c, Frag (&x)[RB]) {
+    for (int r = 0; r < RT; ++r) acc[r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    uint16_t* lds = (uint16_t*)lora_lds + wave * F::values;
+    // The operands of 32 columns from c on, of which the last may be past the end.
+    auto load_x = [&](int c, Frag& x) {
         const int at = c + 8 * g;
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            if (16 * b >= count) continue;  // uniform
-            if (at + 8 <= a.C) load8(a.x, xat[b] + at, a.x_dtype, x[b]);
-            else load8(a.x, xat[b] + at, 1, a.x_dtype, a.C - at, x[b]);
-        }
+        if (at + 8 <= a.C) load8(a.x, xat + at, a.x_dtype, x);
+        else load8(a.x, xat + at, 1, a.x_dtype, a.C - at, x);
     };
-    auto load_w = [&](int c, Frag (&w)[RT]) {
-        if constexpr (staged) {
-            // rows c .. c + 31 of the matrix, zeros past C; ranks past the last are not read again
-            const int64_t from = matrix + (int64_t)c * a.rank;
-            const int there = min(32, a.C - c);
-            if (a.rank % 8 == 0) {
-                const int vectors = a.rank >> 3;  // per row
-                for (int i = lane; i < 32 * vectors; i += 64) {
-                    const int row = i / vectors;
-                    Frag16 v;
-                    clear(v);
-                    if (row < there) load8(a.w, from + 8 * i, DT_BF16, v);
-                    *(v4i*)(block + row * RP + 8 * (i - row * vectors)) = v.v;
-                }
-            } else {
-                for (int i = lane; i < 32 * a.rank; i += 64) {
-                    const int row = i / a.rank;
-                    block[row * RP + i - row * a.rank] = row < there ? ((const uint16_t*)a.w)[from + i] : 0;
-                }
-            }
-            wave_lds_sync();
-#pragma unroll
-            for (int r = 0; r < RT; ++r) load_rows(block, RP, [&](int i) { return 16 * r + i; }, w[r]);
-        } else {
-            const int at = c + 8 * g;
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                if constexpr (COLS) {
-                    load8(a.w, wat[r] + (int64_t)at * a.rank, a.rank, a.w_dtype, a.C - at, w[r]);
-                } else {
-                    if (at + 8 <= a.C) load8(a.w, wat[r] + at, a.w_dtype, w[r]);
-                    else load8(a.w, wat[r] + at, 1, a.w_dtype, a.C - at, w[r]);
-                }
-            }
-        }
+    auto load_w = [&](int c, Frag& w, int r) {
+        const int at = c + 8 * g;
+        if constexpr (COLS) load8(a.w, wat[r] + (int64_t)at * a.rank, a.rank, a.w_dtype, a.C - at, w);
+        else if (at + 8 <= a.C) load8(a.w, wat[r] + at, a.w_dtype, w);
+        else load8(a.w, wat[r] + at, 1, a.w_dtype, a.C - at, w);
     };
-    constexpr int UN = staged || RT == 8 || !Frag::bf16 ? 1 : FEW ? 4 : 2;
-    for (int c = c0; c < c1; c += 32 * UN) {
-        Frag x[UN][RB], w[UN][RT];
+    // Rows of a power of two bytes have a column all in one channel of the caches and
+    // the memory, so workgroups start 128 columns apart and go round their own part.
+    const int blocks = Frag::bf16 && COLS && a.rank != RP ? 0 : (c1 - c0) / F::block;
+    int at = blocks > 0 ? (int)(unit * (128u / F::block) % (unsigned)blocks) : 0;
+    if constexpr (F::staged) {
+        constexpr int J = F::block / 64;
+        // of the u-th of a block's loads the lane's row is 8 u + lane / 8
+        const int l8 = 8 * (lane & 7);
+        int64_t from[2], wfrom[RT][2];
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
-            if (c + 32 * u < c1) {
-                load_x(c + 32 * u, x[u]);
-                load_w(c + 32 * u, w[u]);
-            }
+        for (int u = 0; u < 2; ++u) {
+            from[u] = (int64_t)rows[min(8 * u + (lane >> 3), count - 1)] * a.C + l8;
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
-            if (c + 32 * u < c1) {
+            for (int r = 0; r < RT; ++r) wfrom[r][u] = matrix + (int64_t)min(16 * r + 8 * u + (lane >> 3), a.rank - 1) * a.C + l8;
+        }
+        uint16_t* put = lds + (lane >> 3) * F::pitch + l8;
+        const uint16_t* get = lds + l16 * F::pitch + 8 * g;
+        uint16_t* more = lds + 16 * F::pitch;
+        auto turn = [&](const v4i (&v)[2], int region, Frag16 (&f)[2]) {  // 16 rows of 64 columns, as two operands
 #pragma unroll
-                for (int b = 0; b < RB; ++b)
-                    if (16 * b < count) {
+            for (int u = 0; u < 2; ++u) *(v4i*)(put + region * 16 * F::pitch + 8 * u * F::pitch) = v[u];
+            asm volatile("" ::: "memory");  // a wave's LDS accesses go in order
 #pragma unroll
-                        for (int r = 0; r < RT; ++r) acc[b][r] = mma(w[u][r], x[u][b], acc[b][r]);
+            for (int u = 0; u < 2; ++u) f[u].v = *(const v4i*)(get + region * 16 * F::pitch + 32 * u);
+            asm volatile("" ::: "memory");
+        };
+        for (int n = 0; n < blocks; ++n) {
+            const int c = c0 + F::block * at;
+            if (++at == blocks) at = 0;
+            v4i x[J][2], w[J][RT][2];
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    __builtin_memcpy(&x[j][u], (const uint16_t*)a.x + from[u] + c + 64 * j, 16);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        // [C][rank]: 64 rows of RP, 2 RT loads of a KiB
+                        const int64_t p = COLS ? matrix + (int64_t)(c + 64 * j) * RP + 512 * (2 * r + u) + 8 * lane : wfrom[r][u] + c + 64 * j;
+                        __builtin_memcpy(&w[j][r][u], (const uint16_t*)a.w + p, 16);
                     }
+                }
+            __builtin_amdgcn_sched_barrier(0);  // every load of the block ahead of its first wait
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                Frag16 fx[2];
+                turn(x[j], 0, fx);
+                if constexpr (COLS) {
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) *(v4i*)(more + 512 * (2 * r + u) + 8 * lane) = w[j][r][u];
+                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) {
+                            Frag16 fw;
+                            load_rows(more + 32 * u * RP, RP, [&](int i) { return 16 * r + i; }, fw);
+                            acc[r] = mma(fw, fx[u], acc[r]);
+                        }
+                    asm volatile("" ::: "memory");
+                } else {
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        Frag16 fw[2];
+                        turn(w[j][r], 1 + (r & 1), fw);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) acc[r] = mma(fw[u], fx[u], acc[r]);
+                    }
+                }
             }
+        }
+    } else {
+        for (int n = 0; n < blocks; ++n) {
+            const int c = c0 + F::block * at;
+            if (++at == blocks) at = 0;
+            Frag x;
+            load8(a.x, xat + c + 8 * g, a.x_dtype, x);
+            constexpr int kTogether = COLS ? 2 : 4;  // rank tiles whose loads go out at once
+#pragma unroll
+            for (int r0 = 0; r0 < RT; r0 += kTogether) {
+                Frag w[kTogether];
+#pragma unroll
+                for (int r = 0; r < kTogether; ++r)
+                    if (r0 + r < RT) {
+                        if constexpr (COLS) load8(a.w, wat[r0 + r] + (int64_t)(c + 8 * g) * a.rank, a.rank, a.w_dtype, 8, w[r]);
+                        else load8(a.w, wat[r0 + r] + c + 8 * g, a.w_dtype, w[r]);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < kTogether; ++r)
+                    if (r0 + r < RT) acc[r0 + r] = mma(w[r], x, acc[r0 + r]);
+            }
+        }
+    }
+    for (int c = c0 + F::block * blocks; c < c1; c += 32) {
+        Frag x;
+        load_x(c, x);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            Frag w;
+            load_w(c, w, r);
+            acc[r] = mma(w, x, acc[r]);
+        }
     }
     // the waves' sums: the second half's, the first half's onto them, then all in order
-    if (staged) __syncthreads();
+    if (F::staged) __syncthreads();
     float* mine = lora_lds + (wave % half) * kPlane + l16 * RP + 4 * g;
     for (int turn = 0; turn < 2; ++turn) {
         if ((wave >= half) == (turn == 0)) {
 #pragma unroll
-            for (int b = 0; b < RB; ++b)
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    v4f* p = (v4f*)(mine + 16 * b * RP + 16 * r);
-                    *p = turn == 0 ? acc[b][r] : acc[b][r] + *p;
-                }
+            for (int r = 0; r < RT; ++r) {
+                v4f* p = (v4f*)(mine + 16 * r);
+                *p = turn == 0 ? acc[r] : acc[r] + *p;
+            }
         }
         __syncthreads();
     }
@@ -304,196 +386,444 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
 
 // ---- expand --------------------------------------------------------------------
 // out[row][c] = base[row][c] + sum over ranks of (s) h[row][rank] w(rank, c), h the
-// sum of shrink's parts in order.  A wave has 16 rows (of a plan's tile each of the
-// four its own, of a few rows all the same and every fourth step of the columns)
-// and 64 columns a step: four tiles, those of a pair interleaved by fours, so that
-// a lane's results are eight consecutive ones.  A matrix of [rank][C] goes through
-// LDS, a wave's step at a time.
-template <class Frag, class Split, bool FEW, int RT, bool COLS>
-__device__ __forceinline__ void lora_expand_columns(const LoraArgs& a, const int* rows, int count, int adapter,
-                                                    uint16_t* block) {
-    constexpr int KC = (RT + 1) / 2, RP = 16 * RT;  // steps of 32 ranks
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
-    const int own = FEW ? 0 : 16 * wave;
-    if (own >= count) return;  // uniform in the wave
-    const int c0 = (int)min((int64_t)a.C, (int64_t)blockIdx.y * a.columns) + (FEW ? 64 * wave : 0);
-    const int c1 = (int)min((int64_t)a.C, (int64_t)(blockIdx.y + 1) * a.columns);
-    const int row = rows[min(own + l16, count - 1)];
-    const bool mine = own + l16 < count;
-    const int64_t at = (int64_t)row * a.C, matrix = (int64_t)adapter * a.rank * a.C;
-    const bool whole = a.rank % 8 == 0;
-    // the step's matrix operands
-    auto load_w = [&](int c, Frag (&w)[4][KC]) {
-        if constexpr (Frag::bf16 && !COLS) {
-            // ranks by row, eight lanes each; ranks past the last and columns past C are zeros
+// sum of shrink's parts in order, as an operand in registers.  Steps of 64 columns,
+// four MFMA tiles.
+// base and out go by units of 16 bytes: for bf16 the columns of a pair of tiles
+// interleave by fours, so that a lane's results are a unit, and lanes 8 apart swap
+// one of each two units, so that a load or store has whole lines of 128 bytes
+// (8 rows of two units times four) rather than halves.
+template <class Frag, int RT, int OUT>
+struct ExpandForm {
+    static constexpr int KC = (RT + 1) / 2, ranks = 32 * KC;  // steps of 32 ranks
+    static constexpr int parts = !Frag::bf16 ? 1 : OUT == DT_BF16 ? 2 : 3;
+    static constexpr int PT = 4, step = 16 * PT;
+    static constexpr int values = OUT == DT_BF16 ? 8 : 4, units = step / (4 * values);  // of a lane
+    // column of MFMA row i of tile p
+    static __device__ __forceinline__ int column(int p, int i) {
+        return OUT == DT_BF16 ? 32 * (p >> 1) + 8 * (i >> 2) + 4 * (p & 1) + (i & 3) : 16 * p + i;
+    }
+    // the row of 16 and the column of the lane's u-th load or store
+    static __device__ __forceinline__ int unit_row(int u) { return 8 * (u & 1) + (threadIdx.x & 7); }
+    static __device__ __forceinline__ int unit_column(int u) {
+        return 4 * values * ((u & ~1) + ((threadIdx.x >> 3) & 1)) + values * ((threadIdx.x & 63) >> 4);
+    }
+};
+
+// A unit of a row from value `at` on, the first n of its values.
+template <int DT>
+__device__ __forceinline__ v4u unit_load(const void* p, int64_t at, int n) {
+    if constexpr (DT == DT_BF16) {
+        const uint16_t* q = (const uint16_t*)p + at;
+        if (n >= 8) return *(const v4u*)q;
+        uint32_t u[8];
 #pragma unroll
-            for (int r0 = 0; r0 < 32 * KC; r0 += 8) {
-                const int rank = r0 + (lane >> 3), col = c + 8 * (lane & 7);
-                Frag16 v;
-                clear(v);
-                if (rank < a.rank) {
-                    const int64_t p = matrix + (int64_t)rank * a.C + col;
-                    if (col + 8 <= a.C) load8(a.w, p, DT_BF16, v);
-                    else load8(a.w, p, 1, DT_BF16, a.C - col, v);
-                }
-                *(v4i*)(block + rank * 64 + 8 * (lane & 7)) = v.v;
-            }
-            wave_lds_sync();
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-#pragma unroll
-                for (int q = 0; q < KC; ++q)
-                    load_rows(block + 32 * q * 64, 64, [&](int i) { return 32 * (p >> 1) + 2 * i + 4 * (p & 1); }, w[p][q]);
+        for (int i = 0; i < 8; ++i) u[i] = i < n ? q[i] : 0u;
+        return v4u{u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16)};
+    } else {
+        const uint32_t* q = (const uint32_t*)p + at;
+        if (n >= 4) return *(const v4u*)q;
+        return v4u{n > 0 ? q[0] : 0u, n > 1 ? q[1] : 0u, n > 2 ? q[2] : 0u, 0u};
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void unit_store(void* p, int64_t at, int n, v4u v) {
+    if constexpr (DT == DT_BF16) {
+        uint16_t* q = (uint16_t*)p + at;
+        if (n >= 8) {
+            *(v4u*)q = v;
         } else {
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const int col = min(c + 32 * (p >> 1) + 8 * (l16 >> 2) + 4 * (p & 1) + (l16 & 3), a.C - 1);
-#pragma unroll
-                for (int q = 0; q < KC; ++q) {
-                    const int rank = 32 * q + 8 * g;
-                    if constexpr (COLS) {
-                        const int64_t from = matrix + (int64_t)col * a.rank + rank;
-                        if (whole) {
-                            if (rank < a.rank) load8(a.w, from, a.w_dtype, w[p][q]);
-                            else clear(w[p][q]);
-                        } else {
-                            load8(a.w, from, 1, a.w_dtype, a.rank - rank, w[p][q]);
-                        }
-                    } else {
-                        load8(a.w, matrix + (int64_t)rank * a.C + col, a.C, a.w_dtype, a.rank - rank, w[p][q]);
-                    }
-                }
-            }
+            for (int i = 0; i < 8; ++i)
+                if (i < n) q[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
         }
-    };
-    const bool bf16_out = a.out_dtype == DT_BF16;
-    auto load_base = [&](int c, Frag32 (&base)[2]) {
+    } else {
+        uint32_t* q = (uint32_t*)p + at;
+        if (n >= 4) {
+            *(v4u*)q = v;
+        } else {
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const int first = c + 32 * p + 8 * g, there = a.C - first;
-            clear(base[p]);
-            if (!a.base || !mine || there <= 0) continue;
-            if (there >= 8) load8(a.base, at + first, a.out_dtype, base[p]);
-            else load8(a.base, at + first, 1, a.out_dtype, there, base[p]);
-        }
-    };
-    // the low-rank values, while the first step's operands are on their way
-    Frag w[4][KC];
-    Frag32 base[2];
-    if (c0 < c1) {
-        load_w(c0, w);
-        load_base(c0, base);
-    }
-    Split h[KC];
-    const float scale = a.scaled && a.scales ? a.scales[adapter] : 1.0f;
-#pragma unroll
-    for (int q = 0; q < KC; ++q) {
-        float v[8];
-        const int rank = 32 * q + 8 * g;
-        const float* p = a.part + (int64_t)row * RP + rank;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        if (rank < RP) {
-            for (int s = 0; s < a.splits; ++s) {
-                float t[8];
-                __builtin_memcpy(t, p + (int64_t)s * a.m * RP, 32);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = s == 0 ? t[i] : v[i] + t[i];
-            }
-        }
-        const bool first = blockIdx.y == 0 && (!FEW || wave == 0) && a.h_out && mine;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (rank + i >= a.rank) v[i] = 0.0f;
-            else if (first) a.h_out[(int64_t)row * a.rank + rank + i] = v[i];
-            v[i] *= scale;
-            if (rank + i >= a.rank) v[i] = 0.0f;  // a scale without a value
-        }
-        split8(v, h[q]);
-    }
-    constexpr int kStep = FEW ? 256 : 64;
-    for (int c = c0; c < c1; c += kStep) {
-        v4f acc[4];
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            acc[p] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int s = Split::parts - 1; s >= 0; --s)  // the small parts first
-#pragma unroll
-                for (int q = 0; q < KC; ++q) acc[p] = mma(w[p][q], h[q].f[s], acc[p]);
-        }
-        float v[2][8];
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[p][i] = base[p].v[i] + acc[2 * p + (i >> 2)][i & 3];
-        if (c + kStep < c1) {
-            load_w(c + kStep, w);
-            load_base(c + kStep, base);
-        }
-        if (!mine) continue;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const int first = c + 32 * p + 8 * g, there = a.C - first;
-            if (there >= 8) {
-                if (bf16_out) {
-                    const uint32_t u[4] = {f32x2_to_bf16x2(v[p][0], v[p][1]), f32x2_to_bf16x2(v[p][2], v[p][3]),
-                                           f32x2_to_bf16x2(v[p][4], v[p][5]), f32x2_to_bf16x2(v[p][6], v[p][7])};
-                    __builtin_memcpy((uint16_t*)a.out + at + first, u, 16);
-                } else {
-                    __builtin_memcpy((float*)a.out + at + first, v[p], 32);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < there) store_out(a.out, at + first + i, v[p][i], a.out_dtype);
-            }
+            for (int i = 0; i < 4; ++i)
+                if (i < n) q[i] = v[i];
         }
     }
 }
 
-template <class Frag, bool FEW, int RT, bool COLS>
-__device__ __forceinline__ void lora_expand(const LoraArgs& a) {
-    constexpr bool staged = Frag::bf16 && !COLS;
-    __shared__ int rows[FEW ? 16 : kTileRows];
-    __shared__ __align__(16) uint16_t blocks[staged ? 4 * 32 * ((RT + 1) / 2) * 64 : 8];
-    int adapter;
-    const int count = lora_tile<FEW>(a, blockIdx.x, rows, adapter);
-    if (count == 0) return;  // uniform
-    if (adapter == a.adapters) {  // rows without an adapter: the base
-        const int start = (int)min((int64_t)a.C, (int64_t)blockIdx.y * a.columns);
-        const int end = (int)min((int64_t)a.C, (int64_t)(blockIdx.y + 1) * a.columns);
-        if (blockIdx.y == 0 && a.h_out)
-            for (int i = threadIdx.x; i < count * a.rank; i += blockDim.x)
-                a.h_out[(int64_t)rows[i / a.rank] * a.rank + i % a.rank] = 0.0f;
-        if (a.base == a.out) return;
-        for (int r = 0; r < count; ++r) {
-            const int64_t at = (int64_t)rows[r] * a.C;
-            for (int c = start + 8 * threadIdx.x; c < end; c += 8 * blockDim.x) {
-                if (c + 8 <= end && a.base) {  // as they are
-                    uint32_t u[8];
-                    if (a.out_dtype == DT_BF16) {
-                        __builtin_memcpy(u, (const uint16_t*)a.base + at + c, 16);
-                        __builtin_memcpy((uint16_t*)a.out + at + c, u, 16);
-                    } else {
-                        __builtin_memcpy(u, (const float*)a.base + at + c, 32);
-                        __builtin_memcpy((float*)a.out + at + c, u, 32);
+// Row `row`'s low-rank values, the lane's ranks 8 (lane / 16) .. of each 32, as
+// operands; `writes`: to h_out as well.
+template <class Frag, int PARTS, int RT>
+__device__ __forceinline__ void lora_values(const LoraArgs& a, int row, float scale, bool writes,
+                                            Frag (&h)[(RT + 1) / 2][PARTS]) {
+    constexpr int RP = 16 * RT, kAhead = 4;
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int q = 0; q < (RT + 1) / 2; ++q) {
+        const int rank = 32 * q + 8 * g;
+        const float* p = a.part + (int64_t)row * RP + rank;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        if (rank < RP) {
+            for (int s0 = 0; s0 < a.splits; s0 += kAhead) {
+                float t[kAhead][8];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                    if (s0 + u < a.splits) __builtin_memcpy(t[u], p + (int64_t)(s0 + u) * a.m * RP, 32);
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                    if (s0 + u < a.splits) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = s0 + u == 0 ? t[u][i] : v[i] + t[u][i];
                     }
-                } else {
-                    for (int i = c; i < min(c + 8, end); ++i)
-                        store_out(a.out, at + i, a.base ? load_as_f32(a.base, at + i, a.out_dtype) : 0.0f, a.out_dtype);
-                }
             }
         }
-        return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (rank + i < a.rank) {
+                if (writes) a.h_out[(int64_t)row * a.rank + rank + i] = v[i];
+                v[i] *= scale;
+            } else {
+                v[i] = 0.0f;
+            }
+        }
+        if constexpr (Frag::bf16) {
+#pragma unroll
+            for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t lo = bf16_part(v[2 * i]), hi = bf16_part(v[2 * i + 1]);
+                    h[q][s].v[i] = (int)(lo | (hi << 16));
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[q][0].v[i] = v[i];
+        }
     }
-    uint16_t* block = blocks + (staged ? (threadIdx.x >> 6) * 32 * ((RT + 1) / 2) * 64 : 0);
-    if constexpr (!Frag::bf16)
-        lora_expand_columns<Frag, Split32, FEW, RT, COLS>(a, rows, count, adapter, block);
-    else if (a.out_dtype == DT_BF16)
-        lora_expand_columns<Frag, Split16<2>, FEW, RT, COLS>(a, rows, count, adapter, block);
-    else
-        lora_expand_columns<Frag, Split16<3>, FEW, RT, COLS>(a, rows, count, adapter, block);
+}
+
+// 16 rows of a step: the lanes' base units plus the products, stored (WHOLE: no row
+// or column of the step is missing, or a row's stand-in has the same results).
+template <class F, int OUT, bool WHOLE>
+__device__ __forceinline__ void lora_store(const LoraArgs& a, const int64_t (&at)[2], int count, int c, v4u (&x)[F::units],
+                                           const v4f (&acc)[F::PT]) {
+#pragma unroll
+    for (int u = 0; u < F::units; u += 2) unit_swap(x[u], x[u + 1]);
+#pragma unroll
+    for (int u = 0; u < F::units; ++u) {
+        if constexpr (OUT == DT_BF16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[u][i] = f32x2_to_bf16x2(f32_from_bits(x[u][i] << 16) + acc[2 * u + (i >> 1)][2 * (i & 1)],
+                                          f32_from_bits(x[u][i] & 0xffff0000u) + acc[2 * u + (i >> 1)][2 * (i & 1) + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[u][i] = f32_bits(f32_from_bits(x[u][i]) + acc[u][i]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < F::units; u += 2) unit_swap(x[u], x[u + 1]);
+#pragma unroll
+    for (int u = 0; u < F::units; ++u) {
+        const int first = c + F::unit_column(u);
+        if constexpr (WHOLE) unit_store<OUT>(a.out, at[u & 1] + first, 64, x[u]);
+        else if (F::unit_row(u) < count && first < a.C) unit_store<OUT>(a.out, at[u & 1] + first, a.C - first, x[u]);
+    }
+}
+
+template <class F, int OUT>
+__device__ __forceinline__ void lora_base(const LoraArgs& a, const int64_t (&at)[2], int count, int c, v4u (&x)[F::units]) {
+#pragma unroll
+    for (int u = 0; u < F::units; ++u) {
+        const int first = c + F::unit_column(u);
+        x[u] = v4u{0, 0, 0, 0};
+        if (a.base && F::unit_row(u) < count && first < a.C) x[u] = unit_load<OUT>(a.base, at[u & 1] + first, a.C - first);
+    }
+}
+
+// A few rows (at most 16, forward): the waves take every fourth step, each its own
+// part of the matrix, straight into registers a step ahead.
+template <class Frag, int OUT, int RT>
+__device__ __forceinline__ void lora_expand_few(const LoraArgs& a, const int* rows, int count, int adapter) {
+    using F = ExpandForm<Frag, RT, OUT>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+    const int c0 = (int)min((int64_t)a.C, (int64_t)blockIdx.y * a.columns) + F::step * wave;
+    const int c1 = (int)min((int64_t)a.C, (int64_t)(blockIdx.y + 1) * a.columns);
+    const int64_t matrix = (int64_t)adapter * a.rank * a.C;
+    int64_t at[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) at[u] = (int64_t)rows[min(F::unit_row(u), count - 1)] * a.C;
+    const bool whole = a.rank % 8 == 0;
+    Frag w[F::PT][F::KC];
+    auto load_w = [&](int c) {
+#pragma unroll
+        for (int p = 0; p < F::PT; ++p) {
+            const int64_t from = matrix + (int64_t)min(c + F::column(p, l16), a.C - 1) * a.rank;
+#pragma unroll
+            for (int q = 0; q < F::KC; ++q) {
+                const int rank = 32 * q + 8 * g;
+                if (!whole) load8(a.w, from + rank, 1, a.w_dtype, a.rank - rank, w[p][q]);
+                else if (rank < a.rank) load8(a.w, from + rank, a.w_dtype, w[p][q]);
+                else clear(w[p][q]);
+            }
+        }
+    };
+    v4u base[F::units];
+    if (c0 < c1) {
+        load_w(c0);
+        lora_base<F, OUT>(a, at, count, c0, base);
+    }
+    Frag h[F::KC][F::parts];
+    lora_values<Frag, F::parts, RT>(a, rows[min(l16, count - 1)], a.scales ? a.scales[adapter] : 1.0f,
+                                    blockIdx.y == 0 && wave == 0 && a.h_out && l16 < count, h);
+    for (int c = c0; c < c1; c += 4 * F::step) {
+        v4f acc[F::PT];
+#pragma unroll
+        for (int p = 0; p < F::PT; ++p) {
+            acc[p] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = F::parts - 1; s >= 0; --s)  // the small parts first
+#pragma unroll
+                for (int q = 0; q < F::KC; ++q) acc[p] = mma(w[p][q], h[q][s], acc[p]);
+        }
+        v4u x[F::units];
+#pragma unroll
+        for (int u = 0; u < F::units; ++u) x[u] = base[u];
+        if (c + 4 * F::step < c1) {
+            load_w(c + 4 * F::step);
+            lora_base<F, OUT>(a, at, count, c + 4 * F::step, base);
+        }
+        lora_store<F, OUT, false>(a, at, count, c, x, acc);
+    }
+}
+
+// A tile of the plan: 16 rows per wave, every wave the same columns, whose part of
+// the matrix lies in LDS, a step in each of two buffers; one more is on its way, as
+// is the next step's base.  [C][rank] by column, pitch chosen so that sixteen
+// columns' reads meet no bank twice; [rank][C] (backward) as it is for bf16, which
+// reads it transposing, and by column for f32.
+template <class Frag, int RT, bool COLS>
+struct ExpandBlock {
+    static constexpr int ranks = 32 * ((RT + 1) / 2);
+    static constexpr bool by_rank = Frag::bf16 && !COLS;
+    static constexpr int pitch = by_rank ? 64 : Frag::bf16 ? ranks + 8 : ranks + 4;
+    static constexpr int bytes = (by_rank ? ranks : 64) * pitch * (Frag::bf16 ? 2 : 4);
+};
+
+template <class Frag, int OUT, int RT, bool COLS>
+__device__ __forceinline__ void lora_expand_tile(const LoraArgs& a, const int* rows, int count, int adapter, int c0, int c1,
+                                                 uint8_t* lds) {
+    using F = ExpandForm<Frag, RT, OUT>;
+    using B = ExpandBlock<Frag, RT, COLS>;
+    constexpr int kPer = F::ranks * 64 / 8 / 256;  // a thread's eights of a block
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+    const int own = 16 * wave, left = min(16, count - own);  // the wave's rows
+    const int64_t matrix = (int64_t)adapter * a.rank * a.C;
+    int64_t at[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) at[u] = (int64_t)rows[min(own + F::unit_row(u), count - 1)] * a.C;
+    // eights of the block: where they come from (values from the step's first, or -1)
+    // and where they go
+    const bool whole = a.rank % 8 == 0;
+    int from[kPer], to[kPer], col[kPer];
+    const int each = COLS ? (a.rank + 7) / 8 : 8;  // eights of a column's ranks, or of a rank's columns
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = threadIdx.x + 256 * i, major = e / each, minor = 8 * (e - major * each);
+        const bool there = COLS ? major < 64 : major < a.rank;
+        col[i] = COLS ? major : minor;
+        from[i] = there ? (COLS ? major * a.rank + minor : major) : -1;  // of [rank][C]: the rank
+        to[i] = B::by_rank || COLS ? major * B::pitch + minor : minor * B::pitch + major;
+    }
+    Frag raw[kPer];
+    auto load_w = [&](int c, auto all) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int f = max(from[i], 0);  // a thread without an eighth loads the first, which goes nowhere
+            if constexpr (COLS) {
+                const int64_t p = matrix + (int64_t)c * a.rank + f;
+                if (!all.value && c + col[i] >= a.C) clear(raw[i]);
+                else if (all.value || whole) load8(a.w, p, a.w_dtype, raw[i]);
+                else load8(a.w, p, 1, a.w_dtype, from[i] < 0 ? 0 : a.rank - (f - col[i] * a.rank), raw[i]);
+            } else {
+                const int64_t p = matrix + (int64_t)f * a.C + c + col[i];
+                if (all.value || c + col[i] + 8 <= a.C) load8(a.w, p, a.w_dtype, raw[i]);
+                else load8(a.w, p, 1, a.w_dtype, a.C - c - col[i], raw[i]);
+            }
+        }
+    };
+    auto put_w = [&](uint8_t* block) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (from[i] < 0) continue;
+            if constexpr (Frag::bf16) {
+                *(v4i*)((uint16_t*)block + to[i]) = raw[i].v;
+            } else if constexpr (COLS) {
+                *(float4*)((float*)block + to[i]) = make_float4(raw[i].v[0], raw[i].v[1], raw[i].v[2], raw[i].v[3]);
+                *(float4*)((float*)block + to[i] + 4) = make_float4(raw[i].v[4], raw[i].v[5], raw[i].v[6], raw[i].v[7]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ((float*)block)[to[i] + j * B::pitch] = raw[i].v[j];
+            }
+        }
+    };
+    Frag h[F::KC][F::parts];
+    auto products = [&](const uint8_t* block, v4f (&acc)[F::PT]) {
+#pragma unroll
+        for (int p = 0; p < F::PT; ++p) {
+            acc[p] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            Frag w[F::KC];
+#pragma unroll
+            for (int q = 0; q < F::KC; ++q) {
+                if constexpr (B::by_rank) {
+                    load_rows((const uint16_t*)block + 32 * q * B::pitch, B::pitch, [&](int i) { return F::column(p, i); }, w[q]);
+                } else if constexpr (Frag::bf16) {
+                    w[q].v = *(const v4i*)((const uint16_t*)block + F::column(p, l16) * B::pitch + 32 * q + 8 * g);
+                } else {
+                    const float* s = (const float*)block + F::column(p, l16) * B::pitch + 32 * q + 8 * g;
+                    *(float4*)&w[q].v[0] = *(const float4*)s;
+                    *(float4*)&w[q].v[4] = *(const float4*)(s + 4);
+                }
+            }
+#pragma unroll
+            for (int s = F::parts - 1; s >= 0; --s)  // the small parts first
+#pragma unroll
+                for (int q = 0; q < F::KC; ++q) acc[p] = mma(w[q], h[q][s], acc[p]);
+        }
+    };
+    // ranks past the last stay zero in both buffers
+    for (int i = 16 * threadIdx.x; i < 2 * B::bytes; i += 16 * 256) *(v4i*)(lds + i) = v4i{0, 0, 0, 0};
+    // Whole steps without a branch, so that the counts of loads in flight are known and
+    // a wait for one load waits for no store: a row past the tile's is its last one
+    // again, with the same results (and where a step ahead is none, the last one again).
+    // A rank that is no multiple of eight takes the other columns' way.
+    const int steps = !COLS || whole ? (min(c1, a.C / F::step * F::step) - c0) / F::step : 0;
+    auto run = [&](auto based) {
+        constexpr int D = kExpandAhead;
+        v4u base[D][F::units];
+        auto load_base = [&](int step, v4u (&x)[F::units]) {
+            const int c = c0 + min(step, steps - 1) * F::step;
+#pragma unroll
+            for (int u = 0; u < F::units; ++u) {
+                x[u] = v4u{0, 0, 0, 0};
+                if constexpr (based.value) x[u] = unit_load<OUT>(a.base, at[u & 1] + c + F::unit_column(u), 64);
+            }
+        };
+        auto ahead_w = [&](int step) { load_w(c0 + min(step, steps - 1) * F::step, Yes{}); };
+        ahead_w(0);
+#pragma unroll
+        for (int d = 0; d < D; ++d) load_base(d, base[d]);
+        lora_values<Frag, F::parts, RT>(a, rows[min(own + l16, count - 1)], a.scales ? a.scales[adapter] : 1.0f,
+                                        c0 == 0 && a.h_out && l16 < left, h);
+        __syncthreads();
+        put_w(lds);
+        ahead_w(1);
+        __syncthreads();
+        for (int s0 = 0; s0 < steps; s0 += D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                const int step = s0 + d, turn = step & 1;
+                if (step >= steps) break;  // uniform
+                put_w(lds + (turn ^ 1) * B::bytes);
+                ahead_w(step + 2);
+                v4u x[F::units];
+#pragma unroll
+                for (int u = 0; u < F::units; ++u) x[u] = base[d][u];
+                load_base(step + D, base[d]);
+                __builtin_amdgcn_sched_barrier(0);  // the loads ahead of the products
+                v4f acc[F::PT];
+                products(lds + turn * B::bytes, acc);
+                if (left > 0) lora_store<F, OUT, true>(a, at, left, c0 + step * F::step, x, acc);  // uniform in the wave
+                lds_publish();
+            }
+        }
+    };
+    if (steps > 0) {
+        if (a.base) run(Yes{});
+        else run(No{});
+    }
+    if (steps == 0)
+        lora_values<Frag, F::parts, RT>(a, rows[min(own + l16, count - 1)], a.scales ? a.scales[adapter] : 1.0f,
+                                        c0 == 0 && a.h_out && l16 < left, h);
+    for (int c = c0 + steps * F::step; c < c1; c += F::step) {  // uniform
+        load_w(c, No{});
+        v4u x[F::units];
+        lora_base<F, OUT>(a, at, left, c, x);
+        __syncthreads();
+        put_w(lds);
+        __syncthreads();
+        v4f acc[F::PT];
+        products(lds, acc);
+        lora_store<F, OUT, false>(a, at, left, c, x, acc);
+    }
+}
+
+// Rows without an adapter: columns [c0, c1) of their base.
+__device__ __forceinline__ void lora_bare(const LoraArgs& a, const int* rows, int count, int c0, int c1) {
+    if (c0 == 0 && a.h_out)
+        for (int i = threadIdx.x; i < count * a.rank; i += blockDim.x)
+            a.h_out[(int64_t)rows[i / a.rank] * a.rank + i % a.rank] = 0.0f;
+    if (a.base == a.out) return;
+    // 16 bytes at a time as they are, eight rows in flight a thread; row ends value by value
+    const int size = a.out_dtype == DT_BF16 ? 2 : 4, per = 16 / size, wide = (c1 - c0) / per;
+    for (int i = threadIdx.x; i < (count + 7) / 8 * wide; i += blockDim.x) {
+        const int r0 = i / wide * 8, c = c0 + i % wide * per;
+        v4u v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            v[u] = v4u{0, 0, 0, 0};
+            if (a.base && r0 + u < count) v[u] = *(const v4u*)((const uint8_t*)a.base + ((int64_t)rows[r0 + u] * a.C + c) * size);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (r0 + u < count) *(v4u*)((uint8_t*)a.out + ((int64_t)rows[r0 + u] * a.C + c) * size) = v[u];
+    }
+    const int done = c0 + wide * per, rest = c1 - done;
+    for (int i = threadIdx.x; i < count * rest; i += blockDim.x) {
+        const int64_t at = (int64_t)rows[i / rest] * a.C + done + i % rest;
+        store_out(a.out, at, a.base ? load_as_f32(a.base, at, a.out_dtype) : 0.0f, a.out_dtype);
+    }
+}
+
+// A few rows: a workgroup per leading row and `columns` columns.  The plan's tiles:
+// the steps of all tiles, one tile after the other, in as many equal shares as there
+// are workgroups (two a CU), so that however the rows fall onto adapters no CU has
+// more to do than another, and low-rank values are laid out once or twice by each.
+template <class Frag, bool FEW, int RT, bool COLS>
+__device__ __forceinline__ void lora_expand(const LoraArgs& a) {
+    if constexpr (FEW) {
+        __shared__ int rows[16];
+        int adapter;
+        const int count = lora_few(a, blockIdx.x, rows, adapter);
+        if (count == 0) return;  // uniform
+        if (adapter == a.adapters)
+            lora_bare(a, rows, count, (int)min((int64_t)a.C, (int64_t)blockIdx.y * a.columns),
+                      (int)min((int64_t)a.C, (int64_t)(blockIdx.y + 1) * a.columns));
+        else if (a.out_dtype == DT_BF16) lora_expand_few<Frag, DT_BF16, RT>(a, rows, count, adapter);
+        else lora_expand_few<Frag, DT_F32, RT>(a, rows, count, adapter);
+    } else {
+        __shared__ int rows[kTileRows];
+        __shared__ __align__(16) uint8_t lds[2 * ExpandBlock<Frag, RT, COLS>::bytes];
+        constexpr int step = 64;
+        const int lane = threadIdx.x & 63, per = (a.C + step - 1) / step;
+        const int64_t steps = (int64_t)a.counts[0] * per;
+        const int share = xcd_order(blockIdx.x, gridDim.x);
+        int64_t at = steps * share / gridDim.x;
+        const int64_t end = steps * (share + 1) / gridDim.x;
+        while (at < end) {  // uniform
+            const int tile = (int)(at / per), first = (int)(at - (int64_t)tile * per);
+            const int many = (int)min(end - at, (int64_t)(per - first));
+            const int adapter = a.tile_adapter[tile];
+            const int row = a.slot_row[(int64_t)tile * kTileRows + lane];  // those without a row are the last
+            __syncthreads();  // the tile before is done with
+            if (threadIdx.x < 64) rows[lane] = row;
+            __syncthreads();
+            const int count = __popcll(__ballot(row >= 0)), c0 = first * step, c1 = min(a.C, c0 + many * step);
+            if (adapter == a.adapters) lora_bare(a, rows, count, c0, c1);
+            else if (a.out_dtype == DT_BF16) lora_expand_tile<Frag, DT_BF16, RT, COLS>(a, rows, count, adapter, c0, c1, lds);
+            else lora_expand_tile<Frag, DT_F32, RT, COLS>(a, rows, count, adapter, c0, c1, lds);
+            at += many;
+        }
+    }
 }
 
 // ---- outer ---------------------------------------------------------------------
@@ -789,11 +1119,12 @@ extern "C" __global__ __launch_bounds__(256) void nh_lora_reduce_kernel(LoraArgs
 // forward, or the plan's backward (matrices the other way), ranks to 16, 32, 64, 128.
 #define NH_LORA_RANKS(call, ...) call(__VA_ARGS__, 1) call(__VA_ARGS__, 2) call(__VA_ARGS__, 4) call(__VA_ARGS__, 8)
 #define NH_CALL(kind, Frag, rows, FEW, BACK, RT)                                                                     \
-    extern "C" __global__ __launch_bounds__(RT == 8 ? 256 : 512) void                                               \
+    extern "C" __global__ __launch_bounds__(512) void                                                                \
     nh_lora_shrink_##kind##_##rows##_##RT##_kernel(LoraArgs a) {                                                     \
         lora_shrink<Frag, FEW, RT, BACK>(a);                                                                         \
     }                                                                                                                \
-    extern "C" __global__ __launch_bounds__(256) void nh_lora_expand_##kind##_##rows##_##RT##_kernel(LoraArgs a) {    \
+    extern "C" __global__ __launch_bounds__(256, RT == 8 ? 1 : 2) void                                               \
+    nh_lora_expand_##kind##_##rows##_##RT##_kernel(LoraArgs a) {                                                     \
         lora_expand<Frag, FEW, RT, !BACK>(a);                                                                        \
     }
 NH_LORA_RANKS(NH_CALL, bf16, Frag16, few, true, false)

@@ -16,27 +16,26 @@ int rank_form(size_t rank) { return rank <= 16 ? 0 : rank <= 32 ? 1 : rank <= 64
 size_t rank_pad(size_t rank) { return (size_t)16 << rank_form(rank); }
 size_t most_tiles(size_t m, size_t adapters) { return m / kTileRows + std::min(m, adapters + 1); }
 
-// How shrink cuts C: waves of a workgroup, columns per wave, and parts.
+// How shrink cuts C: columns per wave (eight waves a workgroup), and parts, of which
+// there is more than one only while the CUs are not all busy.
+constexpr size_t kShrinkWaves = 8;
 struct Split {
-    size_t waves, per_wave, parts;
+    size_t per_wave, parts;
 };
 
-Split shrink_split(size_t m, size_t c, size_t rank) {
-    const bool few = m <= kFewRows;
-    const size_t tiles = few ? m : (m + kTileRows - 1) / kTileRows;
+Split shrink_split(size_t m, size_t c) {
+    const size_t units = m <= kFewRows ? m : (m + 15) / 16;
     Split s;
-    s.waves = rank > 64 ? 4 : 8;
-    s.parts = std::max<size_t>(1, std::min<size_t>(16, (256 + tiles - 1) / tiles));
-    s.per_wave = std::max<size_t>(few ? 128 : 64, ((c + s.waves * s.parts - 1) / (s.waves * s.parts) + 31) / 32 * 32);
-    s.parts = (c + s.waves * s.per_wave - 1) / (s.waves * s.per_wave);
+    s.parts = std::max<size_t>(1, std::min<size_t>(m <= kFewRows ? 16 : 4, 256 / units));
+    s.per_wave = std::max<size_t>(128, ((c + kShrinkWaves * s.parts - 1) / (kShrinkWaves * s.parts) + 31) / 32 * 32);
+    s.parts = (c + kShrinkWaves * s.per_wave - 1) / (kShrinkWaves * s.per_wave);
     return s;
 }
 
-// Columns that a workgroup of expand takes: every one of a tile's workgroups sums
-// the low-rank values anew.
+// Columns that a workgroup of expand takes of a few rows: each sums the low-rank
+// values anew.
 size_t expand_columns(size_t m, size_t c) {
-    const size_t tiles = m <= kFewRows ? m : (m + kTileRows - 1) / kTileRows;
-    const size_t groups = std::max<size_t>(1, (m <= kFewRows ? 768 : 1024) / tiles);
+    const size_t groups = std::max<size_t>(1, 768 / m);
     return std::max<size_t>(256, std::min<size_t>(2048, ((c + groups - 1) / groups + 255) / 256 * 256));
 }
 
@@ -64,7 +63,7 @@ Layout lora_layout(size_t m, size_t n, size_t k, size_t rank, size_t adapters, b
         l.tile_adapter = take(tiles * 4);
         l.counts = take(8);
     }
-    l.part_x = take(shrink_split(m, k, rank).parts * m * rp * 4);
+    l.part_x = take(shrink_split(m, k).parts * m * rp * 4);
     if (backward) {
         const size_t it = item_tiles(m);
         // of adapters with more than `it` tiles: t / it + 1 < 2 t / it items each, and over 64 it rows, so
@@ -73,7 +72,7 @@ Layout lora_layout(size_t m, size_t n, size_t k, size_t rank, size_t adapters, b
         l.items_most = tiles / it + std::min(m, adapters) + 1;
         l.items = take(l.items_most * 16);
         l.per_adapter = take(adapters * 8);
-        l.part_d = take(shrink_split(m, n, rank).parts * m * rp * 4);
+        l.part_d = take(shrink_split(m, n).parts * m * rp * 4);
         l.ht_h = take(rp * l.slots * 6);
         l.ht_d = take(rp * l.slots * 6);
         l.gpart_a = take(partials * rank * k * 4);
@@ -129,12 +128,10 @@ struct Lora {
     KernelId form(KernelId first, bool bf16, bool back) const {
         return (KernelId)(first + (bf16 ? 0 : 12) + (few ? 0 : back ? 8 : 4) + rank_form(rank));
     }
-    unsigned tiles() const { return (unsigned)(few ? m : most_tiles(m, adapters)); }
-
     // part = x w^T by parts of C; back: w is [C][rank]
     nh_status shrink(const void* x, nh_dtype xd, const void* w, nh_dtype wd, bool back, size_t c, float* part) {
         LoraArgs a = common;
-        const Split s = shrink_split(m, c, rank);
+        const Split s = shrink_split(m, c);
         a.x = x;
         a.w = w;
         a.part = part;
@@ -142,9 +139,14 @@ struct Lora {
         a.x_dtype = xd;
         a.w_dtype = wd;
         a.per_wave = (int)s.per_wave;
-        const size_t lds = s.waves / 2 * (few ? 16 : kTileRows) * rank_pad(rank) * 4;
-        return launch(ctx, form(K_LORA_SHRINK, xd == NH_BF16 && wd == NH_BF16, back), tiles(), 64 * (unsigned)s.waves, lds,
-                      stream, a, err, (unsigned)s.parts);
+        // a unit of 16 rows a workgroup, in whole turns of the XCDs; half the waves' sums,
+        // and before that what lies in LDS to be turned (ShrinkForm of the kernels)
+        const size_t units = few ? m : (4 * most_tiles(m, adapters) + 7) / 8 * 8, rp = rank_pad(rank);
+        const bool bf16 = xd == NH_BF16 && wd == NH_BF16;
+        const size_t turned = !bf16 ? 0 : back ? 16 * 72 + 64 * rp : 3 * 16 * 72;
+        const size_t lds = kShrinkWaves * std::max(16 * rp * 2, 2 * turned);
+        return launch(ctx, form(K_LORA_SHRINK, bf16, back), (unsigned)units, 64 * (unsigned)kShrinkWaves, lds, stream, a, err,
+                      (unsigned)s.parts);
     }
 
     // out = base + s h w, h the sum of `splits` parts; back: w is [rank][C]
@@ -161,10 +163,16 @@ struct Lora {
         a.w_dtype = wd;
         a.out_dtype = od;
         a.scaled = 1;
-        const size_t columns = expand_columns(m, c);
-        a.columns = (int)columns;
-        return launch(ctx, form(K_LORA_EXPAND, wd == NH_BF16, back), tiles(), 256, 0, stream, a, err,
-                      (unsigned)((c + columns - 1) / columns));
+        const KernelId id = form(K_LORA_EXPAND, wd == NH_BF16, back);
+        if (few) {
+            const size_t columns = expand_columns(m, c);
+            a.columns = (int)columns;
+            return launch(ctx, id, (unsigned)m, 256, 0, stream, a, err, (unsigned)((c + columns - 1) / columns));
+        }
+        // two workgroups a CU, or one per step of 64 columns where there are fewer
+        const size_t steps = ((m + kTileRows - 1) / kTileRows + std::min(m, adapters)) * ((c + 63) / 64);
+        const size_t shares = std::min<size_t>(2 * (size_t)ctx->cu_count, steps);
+        return launch(ctx, id, (unsigned)((shares + 7) / 8 * 8), 256, 0, stream, a, err);
     }
 
     // low-rank values by slot
@@ -176,7 +184,7 @@ struct Lora {
         a.ht = ht;
         a.scaled = scaled;
         a.x_dtype = bf16 ? DT_BF16 : DT_F32;
-        return launch(ctx, K_LORA_FINISH, tiles(), 256, 0, stream, a, err, (unsigned)(rank_pad(rank) / 16));
+        return launch(ctx, K_LORA_FINISH, (unsigned)most_tiles(m, adapters), 256, 0, stream, a, err, (unsigned)(rank_pad(rank) / 16));
     }
 
     // grad = ht x over the rows, laid out [rank][c], or [c][rank] (db)
@@ -251,7 +259,7 @@ nh_status nh_linear_lora(nh_context* ctx, const void* x, nh_dtype x_dtype, const
     float* part = (float*)(ws + l.part_x);
     if (!c.few && (st = c.plan(l, ws, adapter_ids, false))) return st;
     if ((st = c.shrink(x, x_dtype, a, w_dtype, false, k, part))) return st;
-    return c.expand(part, shrink_split(m, k, rank).parts, b, w_dtype, false, n, base, out, out_dtype, h_out);
+    return c.expand(part, shrink_split(m, k).parts, b, w_dtype, false, n, base, out, out_dtype, h_out);
 }
 
 nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dtype, const int32_t* adapter_ids,
@@ -278,7 +286,7 @@ nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dty
     uint8_t* ws = (uint8_t*)workspace;
     Lora c = make_lora(ctx, adapter_ids, scales, m, rank, adapters, false, l, ws, stream, err);
     float *part_x = (float*)(ws + l.part_x), *part_d = (float*)(ws + l.part_d);
-    const size_t parts_x = shrink_split(m, k, rank).parts, parts_d = shrink_split(m, n, rank).parts;
+    const size_t parts_x = shrink_split(m, k).parts, parts_d = shrink_split(m, n).parts;
     if ((st = c.plan(l, ws, adapter_ids, true))) return st;
     if (again && (st = c.shrink(x, x_dtype, a, w_dtype, false, k, part_x))) return st;
     if ((dx || da) && (st = c.shrink(dout, dout_dtype, b, w_dtype, true, n, part_d))) return st;
