@@ -28,8 +28,7 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(2)));
 
-constexpr int kTileRows = 64;     // slots per tile of the plan
-constexpr int kExpandAhead = 3;   // steps of base in flight
+constexpr int kTileRows = 64;  // slots per tile of the plan
 
 // A choice made where a body is built.
 template <bool B>
@@ -128,36 +127,6 @@ __device__ __forceinline__ uint32_t bf16_part(float& v) {
     }
     v = v - f32_from_bits(u & 0xffff0000u);  // exact
     return u >> 16;
-}
-
-// Of lanes 8 apart (in 16) the lower one's second unit for the upper one's first;
-// its own inverse.
-__device__ __forceinline__ void lane_swap(int& first, int& second) {
-    const bool low = (threadIdx.x & 8) == 0;
-    const int x = first, y = second, send = low ? y : x;
-    const int got = __builtin_amdgcn_update_dpp(send, send, 0x128, 0xf, 0xf, false);  // row_ror 8
-    first = low ? x : got;
-    second = low ? got : y;
-}
-
-__device__ __forceinline__ void unit_swap(Frag16& first, Frag16& second) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        int x = first.v[i], y = second.v[i];
-        lane_swap(x, y);
-        first.v[i] = x;
-        second.v[i] = y;
-    }
-}
-
-__device__ __forceinline__ void unit_swap(v4u& first, v4u& second) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        int x = (int)first[i], y = (int)second[i];
-        lane_swap(x, y);
-        first[i] = (uint32_t)x;
-        second[i] = (uint32_t)y;
-    }
 }
 
 // ---- the rows of a workgroup ---------------------------------------------------
@@ -387,26 +356,32 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
 // ---- expand --------------------------------------------------------------------
 // out[row][c] = base[row][c] + sum over ranks of (s) h[row][rank] w(rank, c), h the
 // sum of shrink's parts in order, as an operand in registers.  Steps of 64 columns,
-// four MFMA tiles.
-// base and out go by units of 16 bytes: for bf16 the columns of a pair of tiles
-// interleave by fours, so that a lane's results are a unit, and lanes 8 apart swap
-// one of each two units, so that a load or store has whole lines of 128 bytes
-// (8 rows of two units times four) rather than halves.
+// four MFMA tiles; the matrix goes through LDS and so do the products, so that every
+// load and store has neighbouring lanes side by side in a row.
 template <class Frag, int RT, int OUT>
 struct ExpandForm {
     static constexpr int KC = (RT + 1) / 2, ranks = 32 * KC;  // steps of 32 ranks
     static constexpr int parts = !Frag::bf16 ? 1 : OUT == DT_BF16 ? 2 : 3;
     static constexpr int PT = 4, step = 16 * PT;
-    static constexpr int values = OUT == DT_BF16 ? 8 : 4, units = step / (4 * values);  // of a lane
-    // column of MFMA row i of tile p
-    static __device__ __forceinline__ int column(int p, int i) {
-        return OUT == DT_BF16 ? 32 * (p >> 1) + 8 * (i >> 2) + 4 * (p & 1) + (i & 3) : 16 * p + i;
-    }
-    // the row of 16 and the column of the lane's u-th load or store
-    static __device__ __forceinline__ int unit_row(int u) { return 8 * (u & 1) + (threadIdx.x & 7); }
-    static __device__ __forceinline__ int unit_column(int u) {
-        return 4 * values * ((u & ~1) + ((threadIdx.x >> 3) & 1)) + values * ((threadIdx.x & 63) >> 4);
-    }
+    // base and out go by units of 16 bytes, `lanes` of them a row of a step
+    static constexpr int values = OUT == DT_BF16 ? 8 : 4, lanes = step / values, units = 16 * lanes / 64;
+    static __device__ __forceinline__ int unit_row(int u) { return u * (64 / lanes) + (threadIdx.x & 63) / lanes; }
+    static __device__ __forceinline__ int unit_column() { return values * (threadIdx.x & (lanes - 1)); }
+};
+
+// The products of 16 rows of a step in LDS on their way from MFMA's layout.
+constexpr int kSumsPitch = 68;  // sixteen rows' writes and reads meet no bank twice
+constexpr int kSums = 16 * kSumsPitch;
+
+// A step's part of the matrix in LDS: [C][rank] by column, pitch chosen so that
+// sixteen columns' reads meet no bank twice; [rank][C] (backward) as it is for bf16,
+// which reads it transposing, and by column for f32.
+template <class Frag, int RT, bool COLS>
+struct ExpandBlock {
+    static constexpr int ranks = 32 * ((RT + 1) / 2);
+    static constexpr bool by_rank = Frag::bf16 && !COLS;
+    static constexpr int pitch = by_rank ? 64 : Frag::bf16 ? ranks + 8 : ranks + 4;
+    static constexpr int bytes = (by_rank ? ranks : 64) * pitch * (Frag::bf16 ? 2 : 4);
 };
 
 // A unit of a row from value `at` on, the first n of its values.
@@ -504,60 +479,155 @@ __device__ __forceinline__ void lora_values(const LoraArgs& a, int row, float sc
 // 16 rows of a step: the lanes' base units plus the products, stored (WHOLE: no row
 // or column of the step is missing, or a row's stand-in has the same results).
 template <class F, int OUT, bool WHOLE>
-__device__ __forceinline__ void lora_store(const LoraArgs& a, const int64_t (&at)[2], int count, int c, v4u (&x)[F::units],
-                                           const v4f (&acc)[F::PT]) {
+__device__ __forceinline__ void lora_store(const LoraArgs& a, const int64_t (&at)[F::units], int count, int c,
+                                           v4u (&x)[F::units], const v4f (&acc)[F::PT], float* sums) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int u = 0; u < F::units; u += 2) unit_swap(x[u], x[u + 1]);
+    for (int p = 0; p < F::PT; ++p) *(v4f*)(sums + (lane & 15) * kSumsPitch + 16 * p + 4 * (lane >> 4)) = acc[p];
+    asm volatile("" ::: "memory");  // a wave's LDS accesses go in order
 #pragma unroll
     for (int u = 0; u < F::units; ++u) {
+        const float* s = sums + F::unit_row(u) * kSumsPitch + F::unit_column();
         if constexpr (OUT == DT_BF16) {
+            const v4f lo = *(const v4f*)s, hi = *(const v4f*)(s + 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                x[u][i] = f32x2_to_bf16x2(f32_from_bits(x[u][i] << 16) + acc[2 * u + (i >> 1)][2 * (i & 1)],
-                                          f32_from_bits(x[u][i] & 0xffff0000u) + acc[2 * u + (i >> 1)][2 * (i & 1) + 1]);
+                x[u][i] = f32x2_to_bf16x2(f32_from_bits(x[u][i] << 16) + (i < 2 ? lo[2 * i] : hi[2 * i - 4]),
+                                          f32_from_bits(x[u][i] & 0xffff0000u) + (i < 2 ? lo[2 * i + 1] : hi[2 * i - 3]));
         } else {
+            const v4f v = *(const v4f*)s;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[u][i] = f32_bits(f32_from_bits(x[u][i]) + acc[u][i]);
+            for (int i = 0; i < 4; ++i) x[u][i] = f32_bits(f32_from_bits(x[u][i]) + v[i]);
         }
     }
-#pragma unroll
-    for (int u = 0; u < F::units; u += 2) unit_swap(x[u], x[u + 1]);
+    asm volatile("" ::: "memory");
+    const int first = c + F::unit_column();
 #pragma unroll
     for (int u = 0; u < F::units; ++u) {
-        const int first = c + F::unit_column(u);
-        if constexpr (WHOLE) unit_store<OUT>(a.out, at[u & 1] + first, 64, x[u]);
-        else if (F::unit_row(u) < count && first < a.C) unit_store<OUT>(a.out, at[u & 1] + first, a.C - first, x[u]);
+        if constexpr (WHOLE) unit_store<OUT>(a.out, at[u] + first, 64, x[u]);
+        else if (F::unit_row(u) < count && first < a.C) unit_store<OUT>(a.out, at[u] + first, a.C - first, x[u]);
     }
 }
 
 template <class F, int OUT>
-__device__ __forceinline__ void lora_base(const LoraArgs& a, const int64_t (&at)[2], int count, int c, v4u (&x)[F::units]) {
+__device__ __forceinline__ void lora_base(const LoraArgs& a, const int64_t (&at)[F::units], int count, int c,
+                                          v4u (&x)[F::units]) {
+    const int first = c + F::unit_column();
 #pragma unroll
     for (int u = 0; u < F::units; ++u) {
-        const int first = c + F::unit_column(u);
         x[u] = v4u{0, 0, 0, 0};
-        if (a.base && F::unit_row(u) < count && first < a.C) x[u] = unit_load<OUT>(a.base, at[u & 1] + first, a.C - first);
+        if (a.base && F::unit_row(u) < count && first < a.C) x[u] = unit_load<OUT>(a.base, at[u] + first, a.C - first);
+    }
+}
+
+// The part of the matrix of a step from memory to LDS, an eight of values at a time: where a thread's come from, and where they go.
+template <class Frag, int RT, bool COLS>
+struct ExpandLoader {
+    using B = ExpandBlock<Frag, RT, COLS>;
+    static constexpr int per = B::ranks * 64 / 8 / 256;
+    int from[per], to[per], col[per];  // from: values past the step's first, of [rank][C] the rank; -1: none
+    int64_t matrix;
+    bool whole;
+
+    __device__ __forceinline__ void init(const LoraArgs& a, int64_t first) {
+        matrix = first;
+        whole = a.rank % 8 == 0;
+        const int each = COLS ? (a.rank + 7) / 8 : 8;  // eights of a column's ranks, or of a rank's columns
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            const int e = threadIdx.x + 256 * i, major = e / each, minor = 8 * (e - major * each);
+            const bool there = COLS ? major < 64 : major < a.rank;
+            col[i] = COLS ? major : minor;
+            from[i] = there ? (COLS ? major * a.rank + minor : major) : -1;
+            to[i] = B::by_rank || COLS ? major * B::pitch + minor : minor * B::pitch + major;
+        }
+    }
+
+    // WHOLE: all of the step's columns are there and the rank is a multiple of eight;
+    // without a branch (a thread without an eight loads the first, which goes nowhere)
+    template <bool WHOLE>
+    __device__ __forceinline__ void load(const LoraArgs& a, int c, Frag (&raw)[per]) const {
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            const int f = max(from[i], 0);
+            if constexpr (COLS) {
+                const int64_t p = matrix + (int64_t)c * a.rank + f;
+                if (!WHOLE && c + col[i] >= a.C) clear(raw[i]);
+                else if (WHOLE || whole) load8(a.w, p, a.w_dtype, raw[i]);
+                else load8(a.w, p, 1, a.w_dtype, from[i] < 0 ? 0 : a.rank - (f - col[i] * a.rank), raw[i]);
+            } else {
+                const int64_t p = matrix + (int64_t)f * a.C + c + col[i];
+                if (WHOLE || c + col[i] + 8 <= a.C) load8(a.w, p, a.w_dtype, raw[i]);
+                else load8(a.w, p, 1, a.w_dtype, a.C - c - col[i], raw[i]);
+            }
+        }
+    }
+
+    __device__ __forceinline__ void put(uint8_t* block, const Frag (&raw)[per]) const {
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            if (from[i] < 0) continue;
+            if constexpr (Frag::bf16) {
+                *(v4i*)((uint16_t*)block + to[i]) = raw[i].v;
+            } else if constexpr (COLS) {
+                *(float4*)((float*)block + to[i]) = make_float4(raw[i].v[0], raw[i].v[1], raw[i].v[2], raw[i].v[3]);
+                *(float4*)((float*)block + to[i] + 4) = make_float4(raw[i].v[4], raw[i].v[5], raw[i].v[6], raw[i].v[7]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ((float*)block)[to[i] + j * B::pitch] = raw[i].v[j];
+            }
+        }
+    }
+};
+
+// acc: 16 rows' low-rank values times a step's part of the matrix.
+template <class Frag, int RT, bool COLS, class F>
+__device__ __forceinline__ void lora_products(const uint8_t* block, const Frag (&h)[F::KC][F::parts], v4f (&acc)[F::PT]) {
+    using B = ExpandBlock<Frag, RT, COLS>;
+    const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
+#pragma unroll
+    for (int p = 0; p < F::PT; ++p) {
+        acc[p] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        Frag w[F::KC];
+#pragma unroll
+        for (int q = 0; q < F::KC; ++q) {
+            if constexpr (B::by_rank) {
+                load_rows((const uint16_t*)block + 32 * q * B::pitch, B::pitch, [&](int i) { return 16 * p + i; }, w[q]);
+            } else if constexpr (Frag::bf16) {
+                w[q].v = *(const v4i*)((const uint16_t*)block + (16 * p + l16) * B::pitch + 32 * q + 8 * g);
+            } else {
+                const float* s = (const float*)block + (16 * p + l16) * B::pitch + 32 * q + 8 * g;
+                *(float4*)&w[q].v[0] = *(const float4*)s;
+                *(float4*)&w[q].v[4] = *(const float4*)(s + 4);
+            }
+        }
+#pragma unroll
+        for (int s = F::parts - 1; s >= 0; --s)  // the small parts first
+#pragma unroll
+            for (int q = 0; q < F::KC; ++q) acc[p] = mma(w[q], h[q][s], acc[p]);
     }
 }
 
 // A few rows (at most 16, forward): the waves take every fourth step, each its own
-// part of the matrix, straight into registers a step ahead.
+// part of the matrix straight into registers, a step ahead (through LDS 48 rows of
+// their own adapters, 4096 -> 16384, rank 16, took 10.8 us for 9.7).
 template <class Frag, int OUT, int RT>
-__device__ __forceinline__ void lora_expand_few(const LoraArgs& a, const int* rows, int count, int adapter) {
+__device__ __forceinline__ void lora_expand_few(const LoraArgs& a, const int* rows, int count, int adapter, float* sums) {
     using F = ExpandForm<Frag, RT, OUT>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
     const int c0 = (int)min((int64_t)a.C, (int64_t)blockIdx.y * a.columns) + F::step * wave;
     const int c1 = (int)min((int64_t)a.C, (int64_t)(blockIdx.y + 1) * a.columns);
+    if (c0 >= c1) return;  // uniform in the wave
     const int64_t matrix = (int64_t)adapter * a.rank * a.C;
-    int64_t at[2];
+    int64_t at[F::units];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) at[u] = (int64_t)rows[min(F::unit_row(u), count - 1)] * a.C;
+    for (int u = 0; u < F::units; ++u) at[u] = (int64_t)rows[min(F::unit_row(u), count - 1)] * a.C;
     const bool whole = a.rank % 8 == 0;
     Frag w[F::PT][F::KC];
     auto load_w = [&](int c) {
 #pragma unroll
         for (int p = 0; p < F::PT; ++p) {
-            const int64_t from = matrix + (int64_t)min(c + F::column(p, l16), a.C - 1) * a.rank;
+            const int64_t from = matrix + (int64_t)min(c + 16 * p + l16, a.C - 1) * a.rank;
 #pragma unroll
             for (int q = 0; q < F::KC; ++q) {
                 const int rank = 32 * q + 8 * g;
@@ -567,11 +637,9 @@ __device__ __forceinline__ void lora_expand_few(const LoraArgs& a, const int* ro
             }
         }
     };
+    load_w(c0);
     v4u base[F::units];
-    if (c0 < c1) {
-        load_w(c0);
-        lora_base<F, OUT>(a, at, count, c0, base);
-    }
+    lora_base<F, OUT>(a, at, count, c0, base);
     Frag h[F::KC][F::parts];
     lora_values<Frag, F::parts, RT>(a, rows[min(l16, count - 1)], a.scales ? a.scales[adapter] : 1.0f,
                                     blockIdx.y == 0 && wave == 0 && a.h_out && l16 < count, h);
@@ -592,147 +660,74 @@ __device__ __forceinline__ void lora_expand_few(const LoraArgs& a, const int* ro
             load_w(c + 4 * F::step);
             lora_base<F, OUT>(a, at, count, c + 4 * F::step, base);
         }
-        lora_store<F, OUT, false>(a, at, count, c, x, acc);
+        lora_store<F, OUT, false>(a, at, count, c, x, acc, sums);
     }
 }
 
-// A tile of the plan: 16 rows per wave, every wave the same columns, whose part of
-// the matrix lies in LDS, a step in each of two buffers; one more is on its way, as
-// is the next step's base.  [C][rank] by column, pitch chosen so that sixteen
-// columns' reads meet no bank twice; [rank][C] (backward) as it is for bf16, which
-// reads it transposing, and by column for f32.
-template <class Frag, int RT, bool COLS>
-struct ExpandBlock {
-    static constexpr int ranks = 32 * ((RT + 1) / 2);
-    static constexpr bool by_rank = Frag::bf16 && !COLS;
-    static constexpr int pitch = by_rank ? 64 : Frag::bf16 ? ranks + 8 : ranks + 4;
-    static constexpr int bytes = (by_rank ? ranks : 64) * pitch * (Frag::bf16 ? 2 : 4);
-};
-
+// Columns [c0, c1) of a tile of the plan: 16 rows per wave, every wave the same
+// columns.  The step's part of the matrix is in one of two buffers in LDS; those of
+// the next `ahead` steps are on their way, as is their base (loads come back in order:
+// waiting for a younger part of the matrix waits for every older base).
 template <class Frag, int OUT, int RT, bool COLS>
 __device__ __forceinline__ void lora_expand_tile(const LoraArgs& a, const int* rows, int count, int adapter, int c0, int c1,
-                                                 uint8_t* lds) {
+                                                 uint8_t* lds, float* sums) {
     using F = ExpandForm<Frag, RT, OUT>;
     using B = ExpandBlock<Frag, RT, COLS>;
-    constexpr int kPer = F::ranks * 64 / 8 / 256;  // a thread's eights of a block
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
     const int own = 16 * wave, left = min(16, count - own);  // the wave's rows
-    const int64_t matrix = (int64_t)adapter * a.rank * a.C;
-    int64_t at[2];
+    int64_t at[F::units];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) at[u] = (int64_t)rows[min(own + F::unit_row(u), count - 1)] * a.C;
-    // eights of the block: where they come from (values from the step's first, or -1)
-    // and where they go
-    const bool whole = a.rank % 8 == 0;
-    int from[kPer], to[kPer], col[kPer];
-    const int each = COLS ? (a.rank + 7) / 8 : 8;  // eights of a column's ranks, or of a rank's columns
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int e = threadIdx.x + 256 * i, major = e / each, minor = 8 * (e - major * each);
-        const bool there = COLS ? major < 64 : major < a.rank;
-        col[i] = COLS ? major : minor;
-        from[i] = there ? (COLS ? major * a.rank + minor : major) : -1;  // of [rank][C]: the rank
-        to[i] = B::by_rank || COLS ? major * B::pitch + minor : minor * B::pitch + major;
-    }
-    Frag raw[kPer];
-    auto load_w = [&](int c, auto all) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int f = max(from[i], 0);  // a thread without an eighth loads the first, which goes nowhere
-            if constexpr (COLS) {
-                const int64_t p = matrix + (int64_t)c * a.rank + f;
-                if (!all.value && c + col[i] >= a.C) clear(raw[i]);
-                else if (all.value || whole) load8(a.w, p, a.w_dtype, raw[i]);
-                else load8(a.w, p, 1, a.w_dtype, from[i] < 0 ? 0 : a.rank - (f - col[i] * a.rank), raw[i]);
-            } else {
-                const int64_t p = matrix + (int64_t)f * a.C + c + col[i];
-                if (all.value || c + col[i] + 8 <= a.C) load8(a.w, p, a.w_dtype, raw[i]);
-                else load8(a.w, p, 1, a.w_dtype, a.C - c - col[i], raw[i]);
-            }
-        }
-    };
-    auto put_w = [&](uint8_t* block) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (from[i] < 0) continue;
-            if constexpr (Frag::bf16) {
-                *(v4i*)((uint16_t*)block + to[i]) = raw[i].v;
-            } else if constexpr (COLS) {
-                *(float4*)((float*)block + to[i]) = make_float4(raw[i].v[0], raw[i].v[1], raw[i].v[2], raw[i].v[3]);
-                *(float4*)((float*)block + to[i] + 4) = make_float4(raw[i].v[4], raw[i].v[5], raw[i].v[6], raw[i].v[7]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) ((float*)block)[to[i] + j * B::pitch] = raw[i].v[j];
-            }
-        }
-    };
+    for (int u = 0; u < F::units; ++u) at[u] = (int64_t)rows[min(own + F::unit_row(u), count - 1)] * a.C;
+    using L = ExpandLoader<Frag, RT, COLS>;
+    L w;
+    w.init(a, (int64_t)adapter * a.rank * a.C);
     Frag h[F::KC][F::parts];
-    auto products = [&](const uint8_t* block, v4f (&acc)[F::PT]) {
-#pragma unroll
-        for (int p = 0; p < F::PT; ++p) {
-            acc[p] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            Frag w[F::KC];
-#pragma unroll
-            for (int q = 0; q < F::KC; ++q) {
-                if constexpr (B::by_rank) {
-                    load_rows((const uint16_t*)block + 32 * q * B::pitch, B::pitch, [&](int i) { return F::column(p, i); }, w[q]);
-                } else if constexpr (Frag::bf16) {
-                    w[q].v = *(const v4i*)((const uint16_t*)block + F::column(p, l16) * B::pitch + 32 * q + 8 * g);
-                } else {
-                    const float* s = (const float*)block + F::column(p, l16) * B::pitch + 32 * q + 8 * g;
-                    *(float4*)&w[q].v[0] = *(const float4*)s;
-                    *(float4*)&w[q].v[4] = *(const float4*)(s + 4);
-                }
-            }
-#pragma unroll
-            for (int s = F::parts - 1; s >= 0; --s)  // the small parts first
-#pragma unroll
-                for (int q = 0; q < F::KC; ++q) acc[p] = mma(w[q], h[q][s], acc[p]);
-        }
-    };
+    const float scale = a.scales ? a.scales[adapter] : 1.0f;
     // ranks past the last stay zero in both buffers
     for (int i = 16 * threadIdx.x; i < 2 * B::bytes; i += 16 * 256) *(v4i*)(lds + i) = v4i{0, 0, 0, 0};
     // Whole steps without a branch, so that the counts of loads in flight are known and
     // a wait for one load waits for no store: a row past the tile's is its last one
     // again, with the same results (and where a step ahead is none, the last one again).
     // A rank that is no multiple of eight takes the other columns' way.
-    const int steps = !COLS || whole ? (min(c1, a.C / F::step * F::step) - c0) / F::step : 0;
+    const int steps = !COLS || w.whole ? (min(c1, a.C / F::step * F::step) - c0) / F::step : 0;
     auto run = [&](auto based) {
-        constexpr int D = kExpandAhead;
+        constexpr int D = RT <= 2 && Frag::bf16 ? 4 : RT <= 4 ? 3 : 2;  // what the registers hold
         v4u base[D][F::units];
+        Frag raw[D][L::per];
         auto load_base = [&](int step, v4u (&x)[F::units]) {
-            const int c = c0 + min(step, steps - 1) * F::step;
+            const int c = c0 + min(step, steps - 1) * F::step + F::unit_column();
 #pragma unroll
             for (int u = 0; u < F::units; ++u) {
                 x[u] = v4u{0, 0, 0, 0};
-                if constexpr (based.value) x[u] = unit_load<OUT>(a.base, at[u & 1] + c + F::unit_column(u), 64);
+                if constexpr (based.value) x[u] = unit_load<OUT>(a.base, at[u] + c, 64);
             }
         };
-        auto ahead_w = [&](int step) { load_w(c0 + min(step, steps - 1) * F::step, Yes{}); };
-        ahead_w(0);
+        auto ahead_w = [&](int step, Frag (&r)[L::per]) { w.template load<true>(a, c0 + min(step, steps - 1) * F::step, r); };
 #pragma unroll
-        for (int d = 0; d < D; ++d) load_base(d, base[d]);
-        lora_values<Frag, F::parts, RT>(a, rows[min(own + l16, count - 1)], a.scales ? a.scales[adapter] : 1.0f,
-                                        c0 == 0 && a.h_out && l16 < left, h);
+        for (int d = 0; d < D; ++d) {
+            ahead_w(d, raw[d]);
+            load_base(d, base[d]);
+        }
+        lora_values<Frag, F::parts, RT>(a, rows[min(own + l16, count - 1)], scale, c0 == 0 && a.h_out && l16 < left, h);
         __syncthreads();
-        put_w(lds);
-        ahead_w(1);
+        w.put(lds, raw[0]);
+        ahead_w(D, raw[0]);
         __syncthreads();
         for (int s0 = 0; s0 < steps; s0 += D) {
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 const int step = s0 + d, turn = step & 1;
                 if (step >= steps) break;  // uniform
-                put_w(lds + (turn ^ 1) * B::bytes);
-                ahead_w(step + 2);
+                w.put(lds + (turn ^ 1) * B::bytes, raw[(d + 1) % D]);
+                ahead_w(step + 1 + D, raw[(d + 1) % D]);
                 v4u x[F::units];
 #pragma unroll
                 for (int u = 0; u < F::units; ++u) x[u] = base[d][u];
                 load_base(step + D, base[d]);
                 __builtin_amdgcn_sched_barrier(0);  // the loads ahead of the products
                 v4f acc[F::PT];
-                products(lds + turn * B::bytes, acc);
-                if (left > 0) lora_store<F, OUT, true>(a, at, left, c0 + step * F::step, x, acc);  // uniform in the wave
+                lora_products<Frag, RT, COLS, F>(lds + turn * B::bytes, h, acc);
+                if (left > 0) lora_store<F, OUT, true>(a, at, left, c0 + step * F::step, x, acc, sums);  // uniform in the wave
                 lds_publish();
             }
         }
@@ -740,20 +735,20 @@ __device__ __forceinline__ void lora_expand_tile(const LoraArgs& a, const int* r
     if (steps > 0) {
         if (a.base) run(Yes{});
         else run(No{});
+    } else {
+        lora_values<Frag, F::parts, RT>(a, rows[min(own + l16, count - 1)], scale, c0 == 0 && a.h_out && l16 < left, h);
     }
-    if (steps == 0)
-        lora_values<Frag, F::parts, RT>(a, rows[min(own + l16, count - 1)], a.scales ? a.scales[adapter] : 1.0f,
-                                        c0 == 0 && a.h_out && l16 < left, h);
     for (int c = c0 + steps * F::step; c < c1; c += F::step) {  // uniform
-        load_w(c, No{});
+        Frag raw[L::per];
+        w.template load<false>(a, c, raw);
         v4u x[F::units];
         lora_base<F, OUT>(a, at, left, c, x);
         __syncthreads();
-        put_w(lds);
+        w.put(lds, raw);
         __syncthreads();
         v4f acc[F::PT];
-        products(lds, acc);
-        lora_store<F, OUT, false>(a, at, left, c, x, acc);
+        lora_products<Frag, RT, COLS, F>(lds, h, acc);
+        lora_store<F, OUT, false>(a, at, left, c, x, acc, sums);
     }
 }
 
@@ -790,6 +785,8 @@ __device__ __forceinline__ void lora_bare(const LoraArgs& a, const int* rows, in
 // more to do than another, and low-rank values are laid out once or twice by each.
 template <class Frag, bool FEW, int RT, bool COLS>
 __device__ __forceinline__ void lora_expand(const LoraArgs& a) {
+    const int wave = threadIdx.x >> 6;
+    __shared__ __align__(16) float sums[4][kSums];
     if constexpr (FEW) {
         __shared__ int rows[16];
         int adapter;
@@ -798,8 +795,8 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& a) {
         if (adapter == a.adapters)
             lora_bare(a, rows, count, (int)min((int64_t)a.C, (int64_t)blockIdx.y * a.columns),
                       (int)min((int64_t)a.C, (int64_t)(blockIdx.y + 1) * a.columns));
-        else if (a.out_dtype == DT_BF16) lora_expand_few<Frag, DT_BF16, RT>(a, rows, count, adapter);
-        else lora_expand_few<Frag, DT_F32, RT>(a, rows, count, adapter);
+        else if (a.out_dtype == DT_BF16) lora_expand_few<Frag, DT_BF16, RT>(a, rows, count, adapter, sums[wave]);
+        else lora_expand_few<Frag, DT_F32, RT>(a, rows, count, adapter, sums[wave]);
     } else {
         __shared__ int rows[kTileRows];
         __shared__ __align__(16) uint8_t lds[2 * ExpandBlock<Frag, RT, COLS>::bytes];
@@ -819,8 +816,8 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& a) {
             __syncthreads();
             const int count = __popcll(__ballot(row >= 0)), c0 = first * step, c1 = min(a.C, c0 + many * step);
             if (adapter == a.adapters) lora_bare(a, rows, count, c0, c1);
-            else if (a.out_dtype == DT_BF16) lora_expand_tile<Frag, DT_BF16, RT, COLS>(a, rows, count, adapter, c0, c1, lds);
-            else lora_expand_tile<Frag, DT_F32, RT, COLS>(a, rows, count, adapter, c0, c1, lds);
+            else if (a.out_dtype == DT_BF16) lora_expand_tile<Frag, DT_BF16, RT, COLS>(a, rows, count, adapter, c0, c1, lds, sums[wave]);
+            else lora_expand_tile<Frag, DT_F32, RT, COLS>(a, rows, count, adapter, c0, c1, lds, sums[wave]);
             at += many;
         }
     }
@@ -832,11 +829,10 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& a) {
 // gradient, the others a partial sum each.  A wave has 64 columns, 32 rows a step,
 // which bf16 takes through LDS; the next step's rows are on their way meanwhile.
 template <class Frag, int RT, bool COLS>
-__device__ __forceinline__ void lora_outer(const LoraArgs& a) {
+__device__ __forceinline__ void lora_outer(const LoraArgs& a, int number, uint16_t* blocks) {
     constexpr int PARTS = Frag::bf16 ? 3 : 1, CT = 4;
-    __shared__ __align__(16) uint16_t blocks[Frag::bf16 ? 4 * 32 * 64 : 8];
-    if ((int)blockIdx.y >= a.counts[1]) return;
-    const int32_t* item = a.items + 4 * blockIdx.y;
+    if (number >= a.counts[1]) return;
+    const int32_t* item = a.items + 4 * number;
     const int adapter = item[0], tile = item[1], tiles = item[2], partial = item[3];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
     const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * 16 * CT;
@@ -874,7 +870,7 @@ __device__ __forceinline__ void lora_outer(const LoraArgs& a) {
         for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
-                load8(a.ht, ((int64_t)p * (16 * RT) + 16 * r + l16) * a.slots + at, DT_F32, h[r][p]);
+                load8(a.ht, ((s / 32 * PARTS + p) * RT + r) * 512 + 8 * lane, DT_F32, h[r][p]);
         if constexpr (Frag::bf16) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) *(v4i*)(block + (8 * i + (lane >> 3)) * 64 + 8 * (lane & 7)) = ahead[i];
@@ -954,13 +950,19 @@ extern "C" __global__ __launch_bounds__(1024) void nh_lora_plan_kernel(LoraPlanA
         const int e = a.ids[r];
         return e < 0 || e >= a.adapters ? a.adapters : e;
     };
-    // the row's rank among the wave's rows of its adapter so far, or (counted before) its slot
-    auto place = [&](int e) {
+    // the lanes of the same adapter
+    auto match = [&](int e) {
         uint64_t same = __ballot(e >= 0);
+        if (__ballot(e == __builtin_amdgcn_readfirstlane(e)) == ~0ull) return same;  // a run of rows
         for (int b = 0; b < bits; ++b) {
             const uint64_t bal = __ballot(e >= 0 && ((e >> b) & 1));
             same &= ((e >> b) & 1) ? bal : ~bal;
         }
+        return same;
+    };
+    // the row's rank among the wave's rows of its adapter so far, or (counted before) its slot
+    auto place = [&](int e) {
+        const uint64_t same = match(e);
         const int leader = e >= 0 ? __ffsll((unsigned long long)same) - 1 : 0;
         int at = 0;
         if (e >= 0 && lane == leader) at = atomicAdd(&mine[e], __popcll(same));
@@ -972,22 +974,34 @@ extern "C" __global__ __launch_bounds__(1024) void nh_lora_plan_kernel(LoraPlanA
         for (int u = 0; u < kHeld; ++u) e[u] = group(r0 + 64 * u + lane);
     }
     __syncthreads();
-    if (held) {
+    if (held) {  // as place, every round's addition on its way before the first is waited for
+        int leader[kHeld], at[kHeld];
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+            leader[u] = at[u] = rank[u] = 0;
+            if (64 * u >= per) continue;  // uniform
+            const uint64_t same = match(e[u]);
+            leader[u] = e[u] >= 0 ? __ffsll((unsigned long long)same) - 1 : 0;
+            rank[u] = __popcll(same & ((1ull << lane) - 1));
+            if (e[u] >= 0 && lane == leader[u]) at[u] = atomicAdd(&mine[e[u]], __popcll(same));
+        }
 #pragma unroll
         for (int u = 0; u < kHeld; ++u)
-            if (r0 + 64 * u < r1) rank[u] = place(e[u]);
+            if (64 * u < per) rank[u] += __shfl(at[u], leader[u], kWave);
     } else {
         for (int r = r0; r < r1; r += 64) place(group(r + lane));
     }
     __syncthreads();
-    for (int i = tid; i < G; i += blockDim.x) {
-        int sum = 0;
-        for (int w = 0; w < waves; ++w) {
-            const int n = plan_lds[w * G + i];
-            plan_lds[w * G + i] = sum;
-            sum += n;
+    for (int i = tid >> 4; i < G; i += 64) {  // 16 lanes a group: a wave's rows each
+        const int w = tid & 15, n = plan_lds[w * G + i];
+        int sum = n;
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) {
+            const int t = __shfl_up(sum, off, 16);
+            if (w >= off) sum += t;
         }
-        total[i] = sum;
+        plan_lds[w * G + i] = sum - n;
+        if (w == 15) total[i] = sum;
     }
     __syncthreads();
     if (wave == 0) {
@@ -1053,66 +1067,110 @@ extern "C" __global__ __launch_bounds__(1024) void nh_lora_plan_kernel(LoraPlanA
     }
 }
 
-// The low-rank values by slot, for the outer products: h as given or the sum of
-// shrink's parts, times the adapter's scale; zeros where there is no row or rank.
-// A tile per workgroup, 16 ranks at a time turned in LDS.
-extern "C" __global__ __launch_bounds__(256) void nh_lora_finish_kernel(LoraArgs a) {
-    __shared__ float turned[16][kTileRows + 1];
+// The low-rank values for the outer products: h as given or the sum of shrink's
+// parts, times the adapter's scale, zeros where there is no row or rank; as operands
+// whose K runs over slots: per 32 slots, part and 16 ranks the eight values of each
+// lane of a wave, so that a wave loads them in one piece.  A tile per workgroup, 16
+// ranks at a time turned in LDS.
+namespace {
+
+__device__ __forceinline__ void lora_finish(const LoraArgs& a, int r0, float (&turned)[16][kTileRows + 1]) {
     const int tile = blockIdx.x;
     if (tile >= a.counts[0]) return;
     const int adapter = a.tile_adapter[tile];
     if (adapter == a.adapters) return;
     const float scale = a.scaled && a.scales ? a.scales[adapter] : 1.0f;
-    const bool bf16 = a.x_dtype == DT_BF16;
     const int slot = threadIdx.x >> 2, r4 = 4 * (threadIdx.x & 3), row = a.slot_row[(int64_t)tile * kTileRows + slot];
-    for (int r0 = 16 * blockIdx.y; r0 < a.rank_pad; r0 += 16 * gridDim.y) {
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (row >= 0) {
-            if (a.h) {
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (row >= 0) {
+        if (a.h) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (r0 + r4 + i < a.rank) v[i] = a.h[(int64_t)row * a.rank + r0 + r4 + i];
-            } else {
-                const float* p = a.part + (int64_t)row * a.rank_pad + r0 + r4;
-                for (int s = 0; s < a.splits; ++s) {
-                    const v4f t = *(const v4f*)(p + (int64_t)s * a.m * a.rank_pad);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = s == 0 ? t[i] : v[i] + t[i];
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) turned[r4 + i][slot] = row >= 0 && r0 + r4 + i < a.rank ? v[i] * scale : 0.0f;
-        __syncthreads();
-        const int rank = threadIdx.x >> 4, s4 = 4 * (threadIdx.x & 15);
-        const int64_t at = (r0 + rank) * a.slots + (int64_t)tile * kTileRows + s4;
-        float u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = turned[rank][s4 + i];
-        if (bf16) {
-#pragma unroll
-            for (int q = 0; q < 3; ++q) {
-                const uint32_t p0 = bf16_part(u[0]), p1 = bf16_part(u[1]), p2 = bf16_part(u[2]), p3 = bf16_part(u[3]);
-                *(uint2*)((uint16_t*)a.ht + (int64_t)q * a.rank_pad * a.slots + at) = make_uint2(p0 | (p1 << 16), p2 | (p3 << 16));
-            }
+            for (int i = 0; i < 4; ++i)
+                if (r0 + r4 + i < a.rank) v[i] = a.h[(int64_t)row * a.rank + r0 + r4 + i];
         } else {
-            *(float4*)((float*)a.ht + at) = make_float4(u[0], u[1], u[2], u[3]);
+            const float* p = a.part + (int64_t)row * a.rank_pad + r0 + r4;
+            for (int s = 0; s < a.splits; ++s) {
+                const v4f t = *(const v4f*)(p + (int64_t)s * a.m * a.rank_pad);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = s == 0 ? t[i] : v[i] + t[i];
+            }
         }
-        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) turned[r4 + i][slot] = row >= 0 && r0 + r4 + i < a.rank ? v[i] * scale : 0.0f;
+    __syncthreads();
+    // four slots of a rank: lane 16 (slot / 8) + rank of the operand of 32 slots
+    const int rank = threadIdx.x >> 4, s4 = 4 * (threadIdx.x & 15);
+    const int64_t block = (int64_t)tile * 2 + (s4 >> 5), tiles = a.rank_pad / 16;
+    const int in = ((s4 >> 3 & 3) * 16 + rank) * 8 + (s4 & 7);
+    float u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = turned[rank][s4 + i];
+    if (a.x_dtype == DT_BF16) {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            const uint32_t p0 = bf16_part(u[0]), p1 = bf16_part(u[1]), p2 = bf16_part(u[2]), p3 = bf16_part(u[3]);
+            *(uint2*)((uint16_t*)a.ht + ((block * 3 + q) * tiles + r0 / 16) * 512 + in) = make_uint2(p0 | (p1 << 16), p2 | (p3 << 16));
+        }
+    } else {
+        *(float4*)((float*)a.ht + (block * tiles + r0 / 16) * 512 + in) = make_float4(u[0], u[1], u[2], u[3]);
     }
 }
 
 // An adapter's partial sums in order; zeros for one without rows.
-extern "C" __global__ __launch_bounds__(256) void nh_lora_reduce_kernel(LoraArgs a) {
-    const int adapter = blockIdx.y, items = a.per_adapter[2 * adapter];
+__device__ __forceinline__ void lora_reduce(const LoraArgs& a, int adapter) {
+    const int items = a.per_adapter[2 * adapter];
     if (items == 1 || (items == 0 && a.accumulate)) return;
-    const int64_t size = (int64_t)a.rank * a.C, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t size = (int64_t)a.rank * a.C, i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
     if (i >= size) return;
     float* to = a.grad + adapter * size + i;
-    float v = 0.0f;
     const float* p = a.gpart + (int64_t)a.per_adapter[2 * adapter + 1] * size + i;
-    for (int s = 0; s < items; ++s) v += p[s * size];
-    *to = a.accumulate ? *to + v : v;
+    if (i + 4 <= size) {
+        v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int kAhead = 8;
+        for (int s0 = 0; s0 < items; s0 += kAhead) {
+            v4f t[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (s0 + u < items) __builtin_memcpy(&t[u], p + (s0 + u) * size, 16);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (s0 + u < items) v += t[u];
+        }
+        if (a.accumulate) {
+            v4f old;
+            __builtin_memcpy(&old, to, 16);
+            v += old;
+        }
+        __builtin_memcpy(to, &v, 16);
+    } else {
+        for (int j = 0; i + j < size; ++j) {
+            float v = 0.0f;
+            for (int s = 0; s < items; ++s) v += p[s * size + j];
+            to[j] = a.accumulate ? to[j] + v : v;
+        }
+    }
+}
+
+// Which of the two a workgroup is for, and its number among that one's.
+__device__ __forceinline__ bool lora_second(const LoraPairArgs& p, int& number) {
+    number = p.many == 2 ? blockIdx.y >> 1 : blockIdx.y;
+    return (p.many == 2 ? blockIdx.y & 1 : p.first) != 0;
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void nh_lora_finish_kernel(LoraPairArgs p) {
+    __shared__ float turned[16][kTileRows + 1];
+    int number;
+    if (lora_second(p, number)) lora_finish(p.v[1], 16 * number, turned);
+    else lora_finish(p.v[0], 16 * number, turned);
+}
+
+extern "C" __global__ __launch_bounds__(256) void nh_lora_reduce_kernel(LoraPairArgs p) {
+    int number;
+    if (lora_second(p, number)) lora_reduce(p.v[1], number);
+    else lora_reduce(p.v[0], number);
 }
 
 // Compute kind (bf16, or f32 whatever the operands), a few rows or the plan's tiles
@@ -1134,13 +1192,14 @@ NH_LORA_RANKS(NH_CALL, f32, Frag32, few, true, false)
 NH_LORA_RANKS(NH_CALL, f32, Frag32, tiles, false, false)
 NH_LORA_RANKS(NH_CALL, f32, Frag32, back, false, true)
 #undef NH_CALL
-#define NH_CALL(kind, Frag, name, COLS, RT)                                                                           \
-    extern "C" __global__ __launch_bounds__(256) void nh_lora_outer_##kind##_##name##_##RT##_kernel(LoraArgs a) {      \
-        lora_outer<Frag, RT, COLS>(a);                                                                               \
+#define NH_CALL(kind, Frag, RT)                                                                                       \
+    extern "C" __global__ __launch_bounds__(256) void nh_lora_outer_##kind##_##RT##_kernel(LoraPairArgs p) {          \
+        __shared__ __align__(16) uint16_t blocks[Frag::bf16 ? 4 * 32 * 64 : 8];                                      \
+        int number;                                                                                                  \
+        if (lora_second(p, number)) lora_outer<Frag, RT, true>(p.v[1], number, blocks);                              \
+        else lora_outer<Frag, RT, false>(p.v[0], number, blocks);                                                    \
     }
-NH_LORA_RANKS(NH_CALL, bf16, Frag16, a, false)
-NH_LORA_RANKS(NH_CALL, bf16, Frag16, b, true)
-NH_LORA_RANKS(NH_CALL, f32, Frag32, a, false)
-NH_LORA_RANKS(NH_CALL, f32, Frag32, b, true)
+NH_LORA_RANKS(NH_CALL, bf16, Frag16)
+NH_LORA_RANKS(NH_CALL, f32, Frag32)
 #undef NH_CALL
 #undef NH_LORA_RANKS

@@ -533,10 +533,9 @@ struct LoraArgs {
     float* h_out;            // [m][rank] or null
     const void* base;        // [m][C] or null: 0
     void* out;               // [m][C]
-    void* ht;                // outer: low-rank values [rank_pad][slots] (f32), or three such planes of bf16
+    void* ht;                // outer: low-rank values as operands, see nh_lora_finish_kernel
     float* gpart;            // outer: partial sums [partials][rank * C]
     float* grad;             // [adapters] matrices, laid out as w
-    int64_t slots;           // of ht
     int32_t m, C, rank, rank_pad, adapters;
     int32_t x_dtype, w_dtype, out_dtype;
     int32_t splits;          // parts of C that shrink sums apart
@@ -544,6 +543,13 @@ struct LoraArgs {
     int32_t columns;         // expand: columns of C per workgroup, a multiple of 256
     int32_t scaled;          // finish: times the adapter's scale
     int32_t accumulate;
+};
+
+// The gradients' products, of dh with x (da) and of h with dout (db), in one launch:
+// blockIdx.y counts them in turn where both are wanted.
+struct LoraPairArgs {
+    LoraArgs v[2];
+    int32_t first, many;     // 0 and 2, 0 and 1, or 1 and 1
 };
 
 }  // namespace nh

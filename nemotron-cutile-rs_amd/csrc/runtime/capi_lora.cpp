@@ -26,7 +26,7 @@ struct Split {
 Split shrink_split(size_t m, size_t c) {
     const size_t units = m <= kFewRows ? m : (m + 15) / 16;
     Split s;
-    s.parts = std::max<size_t>(1, std::min<size_t>(m <= kFewRows ? 16 : 4, 256 / units));
+    s.parts = std::max<size_t>(1, std::min<size_t>(m <= kFewRows ? 16 : 4, 512 / units));
     s.per_wave = std::max<size_t>(128, ((c + kShrinkWaves * s.parts - 1) / (kShrinkWaves * s.parts) + 31) / 32 * 32);
     s.parts = (c + kShrinkWaves * s.per_wave - 1) / (kShrinkWaves * s.per_wave);
     return s;
@@ -175,33 +175,52 @@ struct Lora {
         return launch(ctx, id, (unsigned)((shares + 7) / 8 * 8), 256, 0, stream, a, err);
     }
 
-    // low-rank values by slot
-    nh_status finish(const float* h, const float* part, size_t splits, bool scaled, bool bf16, void* ht) {
-        LoraArgs a = common;
-        a.h = h;
-        a.part = const_cast<float*>(part);
-        a.splits = (int)splits;
-        a.ht = ht;
-        a.scaled = scaled;
-        a.x_dtype = bf16 ? DT_BF16 : DT_F32;
-        return launch(ctx, K_LORA_FINISH, (unsigned)most_tiles(m, adapters), 256, 0, stream, a, err, (unsigned)(rank_pad(rank) / 16));
-    }
+    // The gradients of one or both matrices from the low-rank values that belong to the
+    // other side: da from x and dh, db from dout and h.
+    struct Gradient {
+        const void* x;
+        nh_dtype dtype;
+        const float *h, *part;  // low-rank values: h as given, or the sum of shrink's parts
+        size_t splits, c;
+        void* ht;
+        float *gpart, *grad;
+    };
 
-    // grad = ht x over the rows, laid out [rank][c], or [c][rank] (db)
-    nh_status outer(const void* x, nh_dtype xd, const void* ht, bool db, size_t c, float* gpart, float* grad,
-                    bool accumulate, size_t items) {
-        LoraArgs a = common;
-        a.x = x;
-        a.ht = const_cast<void*>(ht);
-        a.gpart = gpart;
-        a.grad = grad;
-        a.C = (int)c;
-        a.x_dtype = xd;
-        a.accumulate = accumulate;
-        nh_status st = launch(ctx, (KernelId)(K_LORA_OUTER + (xd == NH_BF16 ? 0 : 8) + (db ? 4 : 0) + rank_form(rank)),
-                              (unsigned)((c + 255) / 256), 256, 0, stream, a, err, (unsigned)items);
+    nh_status gradients(const Gradient (&g)[2], bool accumulate, size_t items) {
+        LoraPairArgs p{};
+        for (int i = 0; i < 2; ++i) {
+            LoraArgs& a = p.v[i] = common;
+            a.h = g[i].h;
+            a.part = const_cast<float*>(g[i].part);
+            a.splits = (int)g[i].splits;
+            a.ht = g[i].ht;
+            a.scaled = 1;
+            a.x = g[i].x;
+            a.x_dtype = g[i].dtype;
+            a.gpart = g[i].gpart;
+            a.grad = g[i].grad;
+            a.C = (int)g[i].c;
+            a.accumulate = accumulate;
+        }
+        auto launch_pair = [&](KernelId id, int first, int many, size_t gx, size_t gy) {
+            p.first = first;
+            p.many = many;
+            return launch(ctx, id, (unsigned)gx, 256, 0, stream, p, err, (unsigned)(gy * many));
+        };
+        auto outer_id = [&](int i) { return (KernelId)(K_LORA_OUTER + (g[i].dtype == NH_BF16 ? 0 : 4) + rank_form(rank)); };
+        auto columns = [&](int i) { return (g[i].c + 255) / 256; };
+        const bool both = g[0].grad && g[1].grad;
+        const int first = g[0].grad ? 0 : 1, many = both ? 2 : 1, last = first + many - 1;
+        const size_t c = std::max(g[first].c, g[last].c);
+        nh_status st = launch_pair(K_LORA_FINISH, first, many, most_tiles(m, adapters), rank_pad(rank) / 16);
         if (st) return st;
-        return launch(ctx, K_LORA_REDUCE, (unsigned)((rank * c + 255) / 256), 256, 0, stream, a, err, (unsigned)adapters);
+        if (both && outer_id(0) != outer_id(1)) {
+            if ((st = launch_pair(outer_id(0), 0, 1, columns(0), items)) || (st = launch_pair(outer_id(1), 1, 1, columns(1), items)))
+                return st;
+        } else if ((st = launch_pair(outer_id(first), first, many, (c + 255) / 256, items))) {
+            return st;
+        }
+        return launch_pair(K_LORA_REDUCE, first, many, (rank * c + 1023) / 1024, adapters);
     }
 };
 
@@ -215,7 +234,6 @@ Lora make_lora(nh_context* ctx, const int32_t* ids, const float* scales, size_t 
     c.common.counts = (int32_t*)(ws + l.counts);
     c.common.items = (int32_t*)(ws + l.items);
     c.common.per_adapter = (int32_t*)(ws + l.per_adapter);
-    c.common.slots = (int64_t)l.slots;
     c.common.m = (int)m;
     c.common.rank = (int)rank;
     c.common.rank_pad = (int)rank_pad(rank);
@@ -291,13 +309,11 @@ nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dty
     if (again && (st = c.shrink(x, x_dtype, a, w_dtype, false, k, part_x))) return st;
     if ((dx || da) && (st = c.shrink(dout, dout_dtype, b, w_dtype, true, n, part_d))) return st;
     if (dx && (st = c.expand(part_d, parts_d, a, w_dtype, true, k, dx_base, dx, x_dtype, nullptr))) return st;
-    if (da && ((st = c.finish(nullptr, part_d, parts_d, true, x_dtype == NH_BF16, ws + l.ht_d)) ||
-               (st = c.outer(x, x_dtype, ws + l.ht_d, false, k, (float*)(ws + l.gpart_a), da, accumulate != 0, l.items_most))))
-        return st;
-    if (db && ((st = c.finish(h, part_x, parts_x, true, dout_dtype == NH_BF16, ws + l.ht_h)) ||
-               (st = c.outer(dout, dout_dtype, ws + l.ht_h, true, n, (float*)(ws + l.gpart_b), db, accumulate != 0, l.items_most))))
-        return st;
-    return NH_OK;
+    if (!da && !db) return NH_OK;
+    const Lora::Gradient g[2] = {
+        {x, x_dtype, nullptr, part_d, parts_d, k, ws + l.ht_d, (float*)(ws + l.gpart_a), da},
+        {dout, dout_dtype, h, part_x, parts_x, n, ws + l.ht_h, (float*)(ws + l.gpart_b), db}};
+    return c.gradients(g, accumulate != 0, l.items_most);
 }
 
 }  // extern "C"

@@ -176,22 +176,14 @@ const char* const kKernelSymbols[K_COUNT] = {  // in KernelId order
     "nh_lora_expand_f32_back_2_kernel",
     "nh_lora_expand_f32_back_4_kernel",
     "nh_lora_expand_f32_back_8_kernel",
-    "nh_lora_outer_bf16_a_1_kernel",  // K_LORA_OUTER
-    "nh_lora_outer_bf16_a_2_kernel",
-    "nh_lora_outer_bf16_a_4_kernel",
-    "nh_lora_outer_bf16_a_8_kernel",
-    "nh_lora_outer_bf16_b_1_kernel",
-    "nh_lora_outer_bf16_b_2_kernel",
-    "nh_lora_outer_bf16_b_4_kernel",
-    "nh_lora_outer_bf16_b_8_kernel",
-    "nh_lora_outer_f32_a_1_kernel",
-    "nh_lora_outer_f32_a_2_kernel",
-    "nh_lora_outer_f32_a_4_kernel",
-    "nh_lora_outer_f32_a_8_kernel",
-    "nh_lora_outer_f32_b_1_kernel",
-    "nh_lora_outer_f32_b_2_kernel",
-    "nh_lora_outer_f32_b_4_kernel",
-    "nh_lora_outer_f32_b_8_kernel",
+    "nh_lora_outer_bf16_1_kernel",  // K_LORA_OUTER
+    "nh_lora_outer_bf16_2_kernel",
+    "nh_lora_outer_bf16_4_kernel",
+    "nh_lora_outer_bf16_8_kernel",
+    "nh_lora_outer_f32_1_kernel",
+    "nh_lora_outer_f32_2_kernel",
+    "nh_lora_outer_f32_4_kernel",
+    "nh_lora_outer_f32_8_kernel",
 };
 
 void clear_error(nh_error* err) {

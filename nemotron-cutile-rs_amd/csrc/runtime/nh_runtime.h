@@ -129,8 +129,8 @@ enum KernelId : int {
     K_LORA_REDUCE,
     K_LORA_SHRINK,               // bf16 (f32: + 12), a few rows (tiles: + 4, backward: + 8), ranks to 16, 32, 64, 128
     K_LORA_EXPAND = K_LORA_SHRINK + 24,
-    K_LORA_OUTER = K_LORA_EXPAND + 24,  // bf16 (f32: + 8), da (db: + 4), ranks to 16, 32, 64, 128
-    K_COUNT = K_LORA_OUTER + 16
+    K_LORA_OUTER = K_LORA_EXPAND + 24,  // bf16 (f32: + 4), ranks to 16, 32, 64, 128
+    K_COUNT = K_LORA_OUTER + 8
 };
 
 extern const char* const kKernelSymbols[K_COUNT];
