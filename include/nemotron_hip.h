@@ -611,7 +611,7 @@ nh_status nh_moe_balance_loss_backward_host(const float *logits, const int32_t *
  * at any address of their element type.  Sums run in f32, over j in order, and
  * are rounded once: results do not change from run to run.  Errors:
  * INVALID_SHAPE (top_k or hidden == 0), INVALID_PARAMS (dtype, a null operand, an
- * output over an input but where it says so), UNSUPPORTED outside
+ * output over another operand but where it says so), UNSUPPORTED outside
  * nh_supports_moe_rows (tokens * top_k, slots and hidden < 2^31, tokens * hidden
  * and slots * hidden < 2^40).  No counterpart in the reference.
  *
@@ -671,7 +671,7 @@ nh_status nh_moe_combine_rows_backward_host(const void *dout, nh_dtype out_dtype
  * (nh_linear_lora_workspace_size bytes, 16-byte aligned) is free again once the
  * call has run; calls that may run at once need one each.  Errors: INVALID_SHAPE
  * (n, k, rank or adapters == 0), INVALID_ROW_COUNT (m == 0), INVALID_PARAMS
- * (dtype, a null operand, out over x or partly over base), LENGTH_MISMATCH
+ * (dtype, a null operand, an output over an operand but for out on base), LENGTH_MISMATCH
  * "workspace", UNSUPPORTED outside nh_supports_linear_lora (m < 2^24, n and k <=
  * 2^20, m n and m k < 2^40, rank <= 128, adapters <= 1024) or for a misaligned
  * workspace.  No counterpart in the reference. */
@@ -690,8 +690,9 @@ nh_status nh_linear_lora(nh_context *ctx, const void *x, nh_dtype x_dtype, const
  * db), a (dx, db without h) and b (dx, da) may be NULL where nothing asks for
  * them.  h is nh_linear_lora's h_out, or NULL: computed again (for db).  With
  * accumulate != 0 da and db are added to; otherwise adapters without rows get
- * zeros.  Workspace nh_linear_lora_backward_workspace_size bytes, errors as
- * above (dx over x or dout, or partly over dx_base). */
+ * zeros.  An infinity in x or dout makes its adapter's da and db infinite or NaN.
+ * Workspace nh_linear_lora_backward_workspace_size bytes, errors as above (dx on
+ * dx_base alone may overlap). */
 size_t nh_linear_lora_backward_workspace_size(size_t m, size_t n, size_t k, size_t rank, size_t adapters);
 nh_status nh_linear_lora_backward(nh_context *ctx, const void *x, nh_dtype x_dtype, const int32_t *adapter_ids,
                                   const void *a, const void *b, nh_dtype w_dtype, const float *scales, const float *h,

@@ -267,9 +267,11 @@ nh_status nh_linear_lora(nh_context* ctx, const void* x, nh_dtype x_dtype, const
     if ((st = check_lora(m, n, k, rank, adapters, {x_dtype, w_dtype, out_dtype}, err)) ||
         (st = check_given({x, adapter_ids, a, b, out}, err)))
         return st;
-    const size_t out_bytes = m * n * bytes_of(out_dtype);
-    if (overlap(out, out_bytes, x, m * k * bytes_of(x_dtype)) || (base != out && overlap(out, out_bytes, base, base ? out_bytes : 0)))
-        return set_error(err, NH_INVALID_PARAMS, "out must not overlap x, nor base in part");
+    const size_t out_bytes = m * n * bytes_of(out_dtype), matrix = adapters * rank * bytes_of(w_dtype);
+    if (!apart({{out, out_bytes}, {h_out, m * rank * 4}},
+               {{x, m * k * bytes_of(x_dtype)}, {base != out ? base : nullptr, out_bytes}, {adapter_ids, m * 4}, {a, matrix * k},
+                {b, matrix * n}, {scales, adapters * 4}}))
+        return set_error(err, NH_INVALID_PARAMS, "out and h_out must not overlap another operand, but for base as a whole");
     const Layout l = lora_layout(m, n, k, rank, adapters, false);
     if ((st = check_workspace(workspace, workspace_bytes, l.bytes, err)) || (st = bind_device(ctx, err))) return st;
     uint8_t* ws = (uint8_t*)workspace;
@@ -295,10 +297,11 @@ nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dty
     if (((da || again) && (st = check_given({x}, err))) || ((dx || again) && (st = check_given({a}, err))) ||
         ((dx || da) && (st = check_given({b}, err))))
         return st;
-    const size_t x_bytes = m * k * bytes_of(x_dtype);
-    if (dx && (overlap(dx, x_bytes, x, x ? x_bytes : 0) || overlap(dx, x_bytes, dout, m * n * bytes_of(dout_dtype)) ||
-               (dx_base != dx && overlap(dx, x_bytes, dx_base, dx_base ? x_bytes : 0))))
-        return set_error(err, NH_INVALID_PARAMS, "dx must not overlap x or dout, nor dx_base in part");
+    const size_t x_bytes = m * k * bytes_of(x_dtype), matrix = adapters * rank;
+    if (!apart({{dx, x_bytes}, {da, matrix * k * 4}, {db, matrix * n * 4}},
+               {{x, x_bytes}, {dx_base != dx ? dx_base : nullptr, x_bytes}, {dout, m * n * bytes_of(dout_dtype)}, {adapter_ids, m * 4},
+                {a, matrix * k * bytes_of(w_dtype)}, {b, matrix * n * bytes_of(w_dtype)}, {scales, adapters * 4}, {h, m * rank * 4}}))
+        return set_error(err, NH_INVALID_PARAMS, "dx, da and db must not overlap another operand, but for dx_base as a whole");
     const Layout l = lora_layout(m, n, k, rank, adapters, true);
     if ((st = check_workspace(workspace, workspace_bytes, l.bytes, err)) || (st = bind_device(ctx, err))) return st;
     uint8_t* ws = (uint8_t*)workspace;

@@ -57,8 +57,10 @@ nh_status nh_moe_dispatch(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
     nh_status st = check_rows(x_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
     if (st) return st;
     if (tokens != 0 && slots != 0 && (st = check_given({x, pos, rows}, err))) return st;
-    if (overlap(rows, slots * hidden * bytes_of(rows_dtype), x, tokens * hidden * bytes_of(x_dtype)))
-        return set_error(err, NH_INVALID_PARAMS, "rows must not overlap x");
+    const size_t routes = tokens * top_k * 4;
+    if (!apart({{rows, slots * hidden * bytes_of(rows_dtype)}},
+               {{x, tokens * hidden * bytes_of(x_dtype)}, {pos, routes}, {weights, routes}}))
+        return set_error(err, NH_INVALID_PARAMS, "rows must not overlap another operand");
     if ((st = bind_device(ctx, err))) return st;
     if (tokens == 0 || slots == 0) return NH_OK;
     MoeRowsArgs a{};
@@ -82,9 +84,10 @@ nh_status nh_moe_dispatch_backward(nh_context* ctx, const void* drows, nh_dtype 
     if (tokens != 0 && ((st = check_given({pos, dx}, err)) || (slots != 0 && (st = check_given({drows}, err))) ||
                         (dweights && (st = check_given({x}, err)))))
         return st;
-    const size_t token_bytes = tokens * hidden * bytes_of(x_dtype);
-    if (overlap(dx, token_bytes, drows, slots * hidden * bytes_of(rows_dtype)) || (dweights && overlap(dx, token_bytes, x, token_bytes)))
-        return set_error(err, NH_INVALID_PARAMS, "dx must not overlap drows or x");
+    const size_t token_bytes = tokens * hidden * bytes_of(x_dtype), routes = tokens * top_k * 4;
+    if (!apart({{dx, token_bytes}, {dweights, routes}},
+               {{drows, slots * hidden * bytes_of(rows_dtype)}, {dweights ? x : nullptr, token_bytes}, {pos, routes}, {weights, routes}}))
+        return set_error(err, NH_INVALID_PARAMS, "dx and dweights must not overlap another operand");
     if ((st = bind_device(ctx, err))) return st;
     if (tokens == 0) return NH_OK;
     MoeRowsArgs a{};
@@ -107,10 +110,10 @@ nh_status nh_moe_combine_rows(nh_context* ctx, const void* rows, nh_dtype rows_d
     nh_status st = check_rows(out_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
     if (st) return st;
     if (tokens != 0 && ((st = check_given({pos, out}, err)) || (slots != 0 && (st = check_given({rows}, err))))) return st;
-    const size_t token_bytes = tokens * hidden * bytes_of(out_dtype);
-    if (overlap(out, token_bytes, rows, slots * hidden * bytes_of(rows_dtype)) ||
-        (shared && shared != out && overlap(out, token_bytes, shared, token_bytes)))
-        return set_error(err, NH_INVALID_PARAMS, "out must not overlap rows, nor shared in part");
+    const size_t token_bytes = tokens * hidden * bytes_of(out_dtype), routes = tokens * top_k * 4;
+    if (!apart({{out, token_bytes}}, {{rows, slots * hidden * bytes_of(rows_dtype)}, {shared != out ? shared : nullptr, token_bytes},
+                                      {pos, routes}, {weights, routes}}))
+        return set_error(err, NH_INVALID_PARAMS, "out must not overlap another operand, but for shared as a whole");
     if ((st = bind_device(ctx, err))) return st;
     if (tokens == 0) return NH_OK;
     MoeRowsArgs a{};
@@ -135,10 +138,11 @@ nh_status nh_moe_combine_rows_backward(nh_context* ctx, const void* dout, nh_dty
     if (tokens != 0 && ((st = check_given({dout, pos}, err)) || (slots != 0 && (st = check_given({drows}, err))) ||
                         (dweights && slots != 0 && (st = check_given({rows}, err)))))
         return st;
-    const size_t row_bytes = slots * hidden * bytes_of(rows_dtype);
-    if (overlap(drows, row_bytes, dout, tokens * hidden * bytes_of(out_dtype)) ||
-        (dweights && rows != drows && overlap(drows, row_bytes, rows, row_bytes)))
-        return set_error(err, NH_INVALID_PARAMS, "drows must not overlap dout, nor rows in part");
+    const size_t row_bytes = slots * hidden * bytes_of(rows_dtype), routes = tokens * top_k * 4;
+    if (!apart({{drows, row_bytes}, {dweights, routes}},
+               {{dout, tokens * hidden * bytes_of(out_dtype)}, {dweights && rows != drows ? rows : nullptr, row_bytes},
+                {pos, routes}, {weights, routes}}))
+        return set_error(err, NH_INVALID_PARAMS, "drows and dweights must not overlap another operand, but for rows as a whole");
     if ((st = bind_device(ctx, err))) return st;
     if (tokens == 0) return NH_OK;
     MoeRowsArgs a{};

@@ -232,6 +232,22 @@ inline bool overlap(const void* a, size_t an, const void* b, size_t bn) {
     return an != 0 && bn != 0 && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
 }
 
+// An operand's bytes; one that is not given has none.
+struct Span {
+    const void* at;
+    size_t bytes;
+};
+// Whether no output shares bytes with an input or with another output.
+inline bool apart(std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+    for (const Span& o : outs) {
+        for (const Span& i : ins)
+            if (o.at && i.at && overlap(o.at, o.bytes, i.at, i.bytes)) return false;
+        for (const Span& p : outs)
+            if (&p != &o && o.at && p.at && overlap(o.at, o.bytes, p.at, p.bytes)) return false;
+    }
+    return true;
+}
+
 inline bool mul_ok(size_t a, size_t b, size_t* out) { return !__builtin_mul_overflow(a, b, out); }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 

@@ -150,6 +150,13 @@ def test_rows_refusals(rec, name):
         assert status((out, args[2] + 2), (out + 1, None), (2, None)) == NH.OK
     if name == "nh_moe_dispatch_backward":
         assert status((out, args[2])) == NH.INVALID_PARAMS and status((2, None), (out + 1, None)) == NH.OK
+    for at in range(size):  # over positions and weights, and a second output over anything
+        if args[at] in (P1, P2, P3) and (name, at) != ("nh_moe_combine_rows_backward", 2):
+            assert status((out, args[at])) == NH.INVALID_PARAMS
+        if name.endswith("_backward") and args[at] in (P1, P2, P3):
+            assert status((out + 1, args[at])) == NH.INVALID_PARAMS
+    if name.endswith("_backward"):
+        assert status((out + 1, P4)) == NH.INVALID_PARAMS and status((5, P5)) == NH.INVALID_PARAMS
     if name == "nh_moe_combine_rows":
         assert status((4, P4)) == NH.OK and status((4, P4 + 2)) == NH.INVALID_PARAMS
     host = [a for a in args]
@@ -195,6 +202,9 @@ def test_lora_refusals(rec):
     for operand in ("x", "ids", "a", "b", "out"):
         assert f(**{operand: None}) == NH.INVALID_PARAMS
     assert f(base=None) == f(base=OUT) == f(s=P2) == f(h=P2) == NH.OK
+    for operand in (X, S, W, W2, P4, OUT):
+        assert f(h=operand) == f(h=operand + 4) == NH.INVALID_PARAMS
+    assert f(s=P2, h=P2) == f(out=S) == f(out=W) == f(out=W2 + 16) == NH.INVALID_PARAMS
     assert f(base=OUT + 2) == f(out=X) == f(out=X + 4800) == NH.INVALID_PARAMS
     g = lambda **o: NH.call_status("nh_linear_lora_backward", rec.ctx, *back_args(*size, **o))[0]  # noqa: E731
     for operand in ("x", "ids", "a", "b", "dout"):
@@ -204,6 +214,9 @@ def test_lora_refusals(rec):
     assert g(da=None, db=None, x=None, h=None) == g(dx=None, db=None, a=None, h=None) == NH.OK
     assert g(dx=None, da=None, a=None, b=None, x=P1) == g(dx=None, da=None, db=P3, b=None, h=None) == NH.OK
     assert g(dx=None, da=None, h=None, x=None) == g(dx=None, da=None, h=None, a=None) == NH.INVALID_PARAMS
+    for operand in (X, S, W, W2, P4, P5, OUT):
+        assert g(da=operand) == g(db=operand) == NH.INVALID_PARAMS and (operand == OUT or g(dx=operand) == NH.INVALID_PARAMS)
+    assert g(da=P3) == g(dx=P2) == NH.INVALID_PARAMS
     assert g(dx=X) == g(dx=P4) == g(dx_base=OUT + 2) == NH.INVALID_PARAMS and g(dx_base=OUT) == NH.OK
 
 
