@@ -253,6 +253,14 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
             for (int u = 0; u < 2; ++u) f[u].v = *(const v4i*)(get + region * 16 * F::pitch + 32 * u);
             asm volatile("" ::: "memory");
         };
+        v4i next[J][2];  // the next block's rows, which come from memory
+        auto load_rows_at = [&](int c) {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) __builtin_memcpy(&next[j][u], (const uint16_t*)a.x + from[u] + c + 64 * j, 16);
+        };
+        if (blocks > 0) load_rows_at(c0 + F::block * at);
         for (int n = 0; n < blocks; ++n) {
             const int c = c0 + F::block * at;
             if (++at == blocks) at = 0;
@@ -261,7 +269,7 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
             for (int j = 0; j < J; ++j)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    __builtin_memcpy(&x[j][u], (const uint16_t*)a.x + from[u] + c + 64 * j, 16);
+                    x[j][u] = next[j][u];
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
                         // [C][rank]: 64 rows of RP, 2 RT loads of a KiB
@@ -269,7 +277,9 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
                         __builtin_memcpy(&w[j][r][u], (const uint16_t*)a.w + p, 16);
                     }
                 }
+            if constexpr (!FEW) load_rows_at(c0 + F::block * at);  // the last block's: the first again
             __builtin_amdgcn_sched_barrier(0);  // every load of the block ahead of its first wait
+            if constexpr (FEW) if (n + 1 < blocks) load_rows_at(c0 + F::block * at);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 Frag16 fx[2];
@@ -828,9 +838,16 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& a) {
 // item of the plan is some of an adapter's tiles; one that has them all writes the
 // gradient, the others a partial sum each.  A wave has 64 columns, 32 rows a step,
 // which bf16 takes through LDS; the next step's rows are on their way meanwhile.
+// Workgroups from the grid's end on write the zeros of adapters without rows.
 template <class Frag, int RT, bool COLS>
-__device__ __forceinline__ void lora_outer(const LoraArgs& a, int number, uint16_t* blocks) {
+__device__ __forceinline__ void lora_outer(const LoraArgs& a, int number, int numbers, uint16_t* blocks) {
     constexpr int PARTS = Frag::bf16 ? 3 : 1, CT = 4;
+    const int other = numbers - 1 - number;
+    if (other < a.adapters && !a.accumulate && a.per_adapter[2 * other] == 0) {
+        const int64_t size = (int64_t)a.rank * a.C, share = (int64_t)a.rank * 256;  // this workgroup's columns' worth
+        const int64_t from = blockIdx.x * share, to = min(size, from + share);
+        for (int64_t i = from + threadIdx.x; i < to; i += 256) a.grad[other * size + i] = 0.0f;
+    }
     if (number >= a.counts[1]) return;
     const int32_t* item = a.items + 4 * number;
     const int adapter = item[0], tile = item[1], tiles = item[2], partial = item[3];
@@ -1117,10 +1134,10 @@ __device__ __forceinline__ void lora_finish(const LoraArgs& a, int r0, float (&t
     }
 }
 
-// An adapter's partial sums in order; zeros for one without rows.
+// An adapter's partial sums in order.
 __device__ __forceinline__ void lora_reduce(const LoraArgs& a, int adapter) {
     const int items = a.per_adapter[2 * adapter];
-    if (items == 1 || (items == 0 && a.accumulate)) return;
+    if (items < 2) return;
     const int64_t size = (int64_t)a.rank * a.C, i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
     if (i >= size) return;
     float* to = a.grad + adapter * size + i;
@@ -1196,8 +1213,8 @@ NH_LORA_RANKS(NH_CALL, f32, Frag32, back, false, true)
     extern "C" __global__ __launch_bounds__(256) void nh_lora_outer_##kind##_##RT##_kernel(LoraPairArgs p) {          \
         __shared__ __align__(16) uint16_t blocks[Frag::bf16 ? 4 * 32 * 64 : 8];                                      \
         int number;                                                                                                  \
-        if (lora_second(p, number)) lora_outer<Frag, RT, true>(p.v[1], number, blocks);                              \
-        else lora_outer<Frag, RT, false>(p.v[0], number, blocks);                                                    \
+        if (lora_second(p, number)) lora_outer<Frag, RT, true>(p.v[1], number, gridDim.y / p.many, blocks);          \
+        else lora_outer<Frag, RT, false>(p.v[0], number, gridDim.y / p.many, blocks);                                \
     }
 NH_LORA_RANKS(NH_CALL, bf16, Frag16)
 NH_LORA_RANKS(NH_CALL, f32, Frag32)

@@ -220,6 +220,7 @@ struct Lora {
         } else if ((st = launch_pair(outer_id(first), first, many, (c + 255) / 256, items))) {
             return st;
         }
+        if (m <= kTileRows * item_tiles(m)) return NH_OK;  // one item an adapter
         return launch_pair(K_LORA_REDUCE, first, many, (rank * c + 1023) / 1024, adapters);
     }
 };
@@ -316,7 +317,7 @@ nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dty
     const Lora::Gradient g[2] = {
         {x, x_dtype, nullptr, part_d, parts_d, k, ws + l.ht_d, (float*)(ws + l.gpart_a), da},
         {dout, dout_dtype, h, part_x, parts_x, n, ws + l.ht_h, (float*)(ws + l.gpart_b), db}};
-    return c.gradients(g, accumulate != 0, l.items_most);
+    return c.gradients(g, accumulate != 0, std::max(l.items_most, adapters));
 }
 
 }  // extern "C"
