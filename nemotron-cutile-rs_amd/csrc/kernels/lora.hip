@@ -131,23 +131,36 @@ __device__ __forceinline__ uint32_t bf16_part(float& v) {
 
 // ---- the rows of a workgroup ---------------------------------------------------
 // Of at most 64 rows in all every one that is the 1st, 17th, .. of its adapter leads
-// 16: the adapter of row `lead` (`adapters`: none) and the rows, returning how many
-// (0: it leads none), uniform.
-__device__ __forceinline__ int lora_few(const LoraArgs& a, int lead, int* rows, int& adapter) {
+// 16: the adapter (`adapters`: none) and the rows of the 16 that a workgroup is for,
+// returning how many (0: none), uniform.  With a workgroup for each row (many
+// adapters) that is the row to lead; with fewer the number of the leader, which costs
+// a ballot per bit of the adapters first (0.25 us of a launch).
+__device__ __forceinline__ int lora_few(const LoraArgs& a, int number, int* rows, int& adapter) {
     const int lane = threadIdx.x & 63;
     int e = -1;
     if (lane < a.m) {
         e = a.ids[lane];
         if (e < 0 || e >= a.adapters) e = a.adapters;
     }
+    const uint64_t lower = (1ull << lane) - 1;
+    int lead = number;
+    if ((int)gridDim.x < a.m) {
+        uint64_t same = __ballot(e >= 0);  // the lanes of the same adapter
+        for (int bit = 1; bit <= a.adapters; bit <<= 1) {
+            const uint64_t with = __ballot(e & bit);
+            same &= (e & bit) ? with : ~with;
+        }
+        const uint64_t leads = __ballot(e >= 0 && __popcll(same & lower) % 16 == 0);
+        if (number >= __popcll(leads)) return 0;  // uniform
+        lead = __ffsll((unsigned long long)__ballot(((leads >> lane) & 1) && __popcll(leads & lower) == number)) - 1;
+    }
     adapter = __builtin_amdgcn_readlane(e, lead);
-    const uint64_t same = __ballot(e == adapter);
-    const int before = __popcll(same & ((1ull << lead) - 1));
+    const uint64_t group = __ballot(e == adapter);
+    const int before = __popcll(group & ((1ull << lead) - 1)), mine = __popcll(group & lower) - before;
     if (before % 16 != 0) return 0;  // uniform
-    const int mine = __popcll(same & ((1ull << lane) - 1)) - before;
     if (threadIdx.x < 64 && e == adapter && mine >= 0 && mine < 16) rows[mine] = lane;
     __syncthreads();
-    return min(16, __popcll(same) - before);
+    return min(16, __popcll(group) - before);
 }
 
 // Consecutive shares of n, to the workgroups of an XCD one after the other

@@ -8,23 +8,31 @@ using namespace nh;
 
 namespace {
 
-constexpr size_t kTileRows = 64;    // of the plan
-constexpr size_t kFewRows = 64;  // rows that need no plan: one ballot sees all of them
+constexpr size_t kTileRows = 64;  // of the plan
+// Rows that need no plan: one ballot sees all of them, and each 16 of an adapter are a
+// workgroup's.  Without the plan 1, 16, 48 and 64 rows of 4096 -> 16384 (the last of
+// one adapter of rank 64) take 7.4, 8.9, 12.8 and 15.0 us, with it 12.1, 18.8, 25.1
+// and 19.1.
+constexpr size_t kFewRows = 64;
 
 size_t bytes_of(nh_dtype d) { return d == NH_BF16 ? 2 : 4; }
 int rank_form(size_t rank) { return rank <= 16 ? 0 : rank <= 32 ? 1 : rank <= 64 ? 2 : 3; }
 size_t rank_pad(size_t rank) { return (size_t)16 << rank_form(rank); }
 size_t most_tiles(size_t m, size_t adapters) { return m / kTileRows + std::min(m, adapters + 1); }
 
+// A few rows: the most 16s of rows of an adapter (or of none).
+size_t few_units(size_t m, size_t adapters) { return std::min(m, m / 16 + adapters + 1); }
+
 // How shrink cuts C: columns per wave (eight waves a workgroup), and parts, of which
-// there is more than one only while the CUs are not all busy.
+// there is more than one only while the CUs are not all busy: in 1, 2 and 4 parts 300
+// rows of 2701 -> 1999 take 22.5, 18.7 and 16.3 us.  A wave has 128 columns at least.
 constexpr size_t kShrinkWaves = 8;
 struct Split {
     size_t per_wave, parts;
 };
 
-Split shrink_split(size_t m, size_t c) {
-    const size_t units = m <= kFewRows ? m : (m + 15) / 16;
+Split shrink_split(size_t m, size_t adapters, size_t c) {
+    const size_t units = m <= kFewRows ? few_units(m, adapters) : (m + 15) / 16;
     Split s;
     s.parts = std::max<size_t>(1, std::min<size_t>(m <= kFewRows ? 16 : 4, 512 / units));
     s.per_wave = std::max<size_t>(128, ((c + kShrinkWaves * s.parts - 1) / (kShrinkWaves * s.parts) + 31) / 32 * 32);
@@ -32,14 +40,17 @@ Split shrink_split(size_t m, size_t c) {
     return s;
 }
 
-// Columns that a workgroup of expand takes of a few rows: each sums the low-rank
-// values anew.
-size_t expand_columns(size_t m, size_t c) {
-    const size_t groups = std::max<size_t>(1, 768 / m);
-    return std::max<size_t>(256, std::min<size_t>(2048, ((c + groups - 1) / groups + 255) / 256 * 256));
+// Columns that a workgroup of expand takes of a few rows, for about 768 workgroups:
+// each sums the low-rank values anew.  With 384, 768 and 1536 workgroups 48 rows of 64
+// adapters (4096 -> 16384, rank 16) take 14.7, 12.8 and 14.0 us, one row the same.
+size_t expand_columns(size_t m, size_t adapters, size_t c) {
+    const size_t shares = std::max<size_t>(1, 768 / few_units(m, adapters));
+    return std::max<size_t>(256, std::min<size_t>(2048, ((c + shares - 1) / shares + 255) / 256 * 256));
 }
 
-// Most tiles of an outer item: about 32 items of an evenly dealt batch.
+// Most tiles of an outer item: about 32 items of an evenly dealt batch (8192 rows of
+// 4096, rank 32: for 16, 32 and 64 items the products and the sums of parts take 59 +
+// 6, 41 + 8 and 48 + 12 us).
 size_t item_tiles(size_t m) { return std::max<size_t>(1, (m / kTileRows + 31) / 32); }
 
 struct Layout {
@@ -63,7 +74,7 @@ Layout lora_layout(size_t m, size_t n, size_t k, size_t rank, size_t adapters, b
         l.tile_adapter = take(tiles * 4);
         l.counts = take(8);
     }
-    l.part_x = take(shrink_split(m, k).parts * m * rp * 4);
+    l.part_x = take(shrink_split(m, adapters, k).parts * m * rp * 4);
     if (backward) {
         const size_t it = item_tiles(m);
         // of adapters with more than `it` tiles: t / it + 1 < 2 t / it items each, and over 64 it rows, so
@@ -72,7 +83,7 @@ Layout lora_layout(size_t m, size_t n, size_t k, size_t rank, size_t adapters, b
         l.items_most = tiles / it + std::min(m, adapters) + 1;
         l.items = take(l.items_most * 16);
         l.per_adapter = take(adapters * 8);
-        l.part_d = take(shrink_split(m, n).parts * m * rp * 4);
+        l.part_d = take(shrink_split(m, adapters, n).parts * m * rp * 4);
         l.ht_h = take(rp * l.slots * 6);
         l.ht_d = take(rp * l.slots * 6);
         l.gpart_a = take(partials * rank * k * 4);
@@ -131,7 +142,7 @@ struct Lora {
     // part = x w^T by parts of C; back: w is [C][rank]
     nh_status shrink(const void* x, nh_dtype xd, const void* w, nh_dtype wd, bool back, size_t c, float* part) {
         LoraArgs a = common;
-        const Split s = shrink_split(m, c);
+        const Split s = shrink_split(m, adapters, c);
         a.x = x;
         a.w = w;
         a.part = part;
@@ -141,7 +152,7 @@ struct Lora {
         a.per_wave = (int)s.per_wave;
         // a unit of 16 rows a workgroup, in whole turns of the XCDs; half the waves' sums,
         // and before that what lies in LDS to be turned (ShrinkForm of the kernels)
-        const size_t units = few ? m : (4 * most_tiles(m, adapters) + 7) / 8 * 8, rp = rank_pad(rank);
+        const size_t units = few ? few_units(m, adapters) : (4 * most_tiles(m, adapters) + 7) / 8 * 8, rp = rank_pad(rank);
         const bool bf16 = xd == NH_BF16 && wd == NH_BF16;
         const size_t turned = !bf16 ? 0 : back ? 16 * 72 + 64 * rp : 3 * 16 * 72;
         const size_t lds = kShrinkWaves * std::max(16 * rp * 2, 2 * turned);
@@ -165,9 +176,9 @@ struct Lora {
         a.scaled = 1;
         const KernelId id = form(K_LORA_EXPAND, wd == NH_BF16, back);
         if (few) {
-            const size_t columns = expand_columns(m, c);
+            const size_t columns = expand_columns(m, adapters, c);
             a.columns = (int)columns;
-            return launch(ctx, id, (unsigned)m, 256, 0, stream, a, err, (unsigned)((c + columns - 1) / columns));
+            return launch(ctx, id, (unsigned)few_units(m, adapters), 256, 0, stream, a, err, (unsigned)((c + columns - 1) / columns));
         }
         // two workgroups a CU, or one per step of 64 columns where there are fewer
         const size_t steps = ((m + kTileRows - 1) / kTileRows + std::min(m, adapters)) * ((c + 63) / 64);
@@ -280,7 +291,7 @@ nh_status nh_linear_lora(nh_context* ctx, const void* x, nh_dtype x_dtype, const
     float* part = (float*)(ws + l.part_x);
     if (!c.few && (st = c.plan(l, ws, adapter_ids, false))) return st;
     if ((st = c.shrink(x, x_dtype, a, w_dtype, false, k, part))) return st;
-    return c.expand(part, shrink_split(m, k).parts, b, w_dtype, false, n, base, out, out_dtype, h_out);
+    return c.expand(part, shrink_split(m, adapters, k).parts, b, w_dtype, false, n, base, out, out_dtype, h_out);
 }
 
 nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dtype, const int32_t* adapter_ids,
@@ -308,7 +319,7 @@ nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dty
     uint8_t* ws = (uint8_t*)workspace;
     Lora c = make_lora(ctx, adapter_ids, scales, m, rank, adapters, false, l, ws, stream, err);
     float *part_x = (float*)(ws + l.part_x), *part_d = (float*)(ws + l.part_d);
-    const size_t parts_x = shrink_split(m, k).parts, parts_d = shrink_split(m, n).parts;
+    const size_t parts_x = shrink_split(m, adapters, k).parts, parts_d = shrink_split(m, adapters, n).parts;
     if ((st = c.plan(l, ws, adapter_ids, true))) return st;
     if (again && (st = c.shrink(x, x_dtype, a, w_dtype, false, k, part_x))) return st;
     if ((dx || da) && (st = c.shrink(dout, dout_dtype, b, w_dtype, true, n, part_d))) return st;

@@ -113,7 +113,8 @@ SHAPES = [  # m, n, k, rank, adapters, ids
     (300, 513, 700, 64, 5, "runs"), (500, 40, 96, 100, 3, "runs"), (80, 31, 33, 4, 2, "none"), (1000, 65, 72, 17, 1024, "each"),
     (2200, 130, 70, 12, 2, "runs"), (3, 4200, 5000, 16, 2, "each"), (40, 2700, 9000, 24, 3, "each"),
     (150, 3100, 4500, 16, 2, "runs"), (97, 5000, 2600, 40, 2, "runs"), (70, 2049, 2303, 72, 1, "one"),
-    (9000, 33, 40, 5, 1024, "each"), (8200, 40, 70, 16, 3, "runs"), (20011, 24, 16, 3, 7, "each")]
+    (9000, 33, 40, 5, 1024, "each"), (63, 300, 130, 40, 3, "each"), (64, 1030, 90, 16, 2, "runs"), (8200, 40, 70, 16, 3, "runs"),
+    (20011, 24, 16, 3, 7, "each")]
 TYPES = [("bf16", "bf16", "bf16"), ("f32", "f32", "f32"), ("bf16", "f32", "bf16"), ("bf16", "bf16", "f32"),
          ("f32", "bf16", "bf16")]
 
