@@ -242,7 +242,7 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
     };
     // Rows of a power of two bytes have a column all in one channel of the caches and
     // the memory, so workgroups start 128 columns apart and go round their own part.
-    const int blocks = Frag::bf16 && COLS && a.rank != RP ? 0 : (c1 - c0) / F::block;
+    const int blocks = Frag::bf16 && COLS && a.rank % 8 != 0 ? 0 : (c1 - c0) / F::block;
     int at = blocks > 0 ? (int)(unit * (128u / F::block) % (unsigned)blocks) : 0;
     if constexpr (F::staged) {
         constexpr int J = F::block / 64;
@@ -266,6 +266,21 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
             for (int u = 0; u < 2; ++u) f[u].v = *(const v4i*)(get + region * 16 * F::pitch + 32 * u);
             asm volatile("" ::: "memory");
         };
+        // [C][rank]: 64 rows are 8 rank eights in a row, which go to rows of RP, the rest of
+        // them zeros; the eight of load q, and where (its row by a multiplication: of fewer than
+        // 1024 by at most 16 it is exact)
+        const int eights = a.rank / 8, most = 8 * a.rank - 1;
+        const uint32_t inverse = COLS && eights > 0 ? 65536u / eights + 1 : 0;
+        auto eight = [&](int q) { return min(64 * q + lane, most); };
+        auto eight_at = [&](int q) {
+            const int row = (int)((uint32_t)eight(q) * inverse >> 16);
+            return row * RP + 8 * (eight(q) - row * eights);
+        };
+        if (COLS && a.rank < RP) {
+#pragma unroll
+            for (int q = 0; q < 2 * RT; ++q) *(v4i*)(more + 512 * q + 8 * lane) = v4i{0, 0, 0, 0};
+            asm volatile("" ::: "memory");
+        }
         v4i next[J][2];  // the next block's rows, which come from memory
         auto load_rows_at = [&](int c) {
 #pragma unroll
@@ -285,8 +300,7 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
                     x[j][u] = next[j][u];
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
-                        // [C][rank]: 64 rows of RP, 2 RT loads of a KiB
-                        const int64_t p = COLS ? matrix + (int64_t)(c + 64 * j) * RP + 512 * (2 * r + u) + 8 * lane : wfrom[r][u] + c + 64 * j;
+                        const int64_t p = COLS ? matrix + (int64_t)(c + 64 * j) * a.rank + 8 * eight(2 * r + u) : wfrom[r][u] + c + 64 * j;
                         __builtin_memcpy(&w[j][r][u], (const uint16_t*)a.w + p, 16);
                     }
                 }
@@ -301,7 +315,7 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
 #pragma unroll
                     for (int r = 0; r < RT; ++r)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) *(v4i*)(more + 512 * (2 * r + u) + 8 * lane) = w[j][r][u];
+                        for (int u = 0; u < 2; ++u) *(v4i*)(more + eight_at(2 * r + u)) = w[j][r][u];
                     asm volatile("" ::: "memory");
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
