@@ -12,7 +12,7 @@
 // run on the bf16 matrix cores: an f32 low-rank value is cut into three bf16
 // parts of eight significant bits each (by truncation, so v = hi + mid + lo
 // exactly while lo is normal), whose products with bf16 are exact in the f32
-// sums; bf16 results take the first two parts (off by 2^-16 of a term, 2^-7 of
+// sums; bf16 results take the first two parts (off by under 2^-15 of a term, 2^-7 of
 // the result's own rounding).  Otherwise the f32 matrix cores take every value as
 // it is.  Every sum has a fixed order: results do not change from run to run.
 //
@@ -144,7 +144,7 @@ __device__ __forceinline__ int lora_few(const LoraArgs& a, int number, int* rows
     }
     const uint64_t lower = (1ull << lane) - 1;
     int lead = number;
-    if ((int)gridDim.x < a.m) {
+    if (a.numbered) {
         uint64_t same = __ballot(e >= 0);  // the lanes of the same adapter
         for (int bit = 1; bit <= a.adapters; bit <<= 1) {
             const uint64_t with = __ballot(e & bit);
@@ -179,7 +179,12 @@ __device__ __forceinline__ int xcd_order(int block, int blocks) { return (block 
 // lanes in different rows, and a load costs the address unit a turn for each piece
 // that neighbouring lanes do not continue (8192 x 4096, rank 32: 37 us straight into
 // registers).  So a load has 8 rows of 64 columns, 8 lanes a row, and LDS turns it.
-// A matrix of [C][rank] (COLS) is read as it lies and turned by transposing reads.
+// A matrix of [C][rank] (COLS) is read as it lies and turned by transposing reads,
+// for ranks that are multiples of 8.
+// 4096 rows of 4096, rank 64: 25 us, of which a launch without loads or turning takes
+// 10, one without the matrix's loads 18, one without the rows' 18.5; 8192 rows, rank
+// 32: 28 us (67 MB of rows, 134 MB of matrix from the L2s).  What bounds it is a
+// workgroup's chain (plan, rows, four blocks, the sum over waves), one round of them.
 template <class Frag, bool FEW, int RT, bool COLS>
 struct ShrinkForm {
     static constexpr bool staged = Frag::bf16;
@@ -394,7 +399,9 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
 // out[row][c] = base[row][c] + sum over ranks of (s) h[row][rank] w(rank, c), h the
 // sum of shrink's parts in order, as an operand in registers.  Steps of 64 columns,
 // four MFMA tiles; the matrix goes through LDS and so do the products, so that every
-// load and store has neighbouring lanes side by side in a row.
+// load and store has neighbouring lanes side by side in a row.  Memory bounds it: 4096
+// rows -> 21504, rank 64, 93 us (3.8 TB/s; a plain copy by the same tiles and steps 77),
+// 8192 rows -> 4096, rank 32, 35 us (3.9 TB/s).
 template <class Frag, int RT, int OUT>
 struct ExpandForm {
     static constexpr int KC = (RT + 1) / 2, ranks = 32 * KC;  // steps of 32 ranks
@@ -866,6 +873,7 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& a) {
 // gradient, the others a partial sum each.  A wave has 64 columns, 32 rows a step,
 // which bf16 takes through LDS; the next step's rows are on their way meanwhile.
 // Workgroups from the grid's end on write the zeros of adapters without rows.
+// Both sides of 8192 x 4096, rank 32: 41 us (134 MB of rows read once, 3.3 TB/s).
 template <class Frag, int RT, bool COLS>
 __device__ __forceinline__ void lora_outer(const LoraArgs& a, int number, int numbers, uint16_t* blocks) {
     constexpr int PARTS = Frag::bf16 ? 3 : 1, CT = 4;
@@ -976,7 +984,9 @@ __device__ __forceinline__ void lora_outer(const LoraArgs& a, int number, int nu
 // each adapter's from a tile of its own on; the waves take consecutive parts of the
 // rows.  A wave ranks 64 rows at a time among its rows of the same adapter by
 // ballots, and keeps the ranks of up to 512 rows; of more rows they are found
-// again.  Then tiles, and items of up to item_tiles of them.
+// again.  Then tiles, and items of up to item_tiles of them.  One CU's instructions
+// bound it: 300 rows 4.2 us, 4096 8.8, 8192 10.9; two launches of many workgroups would
+// start twice.
 extern "C" __global__ __launch_bounds__(1024) void nh_lora_plan_kernel(LoraPlanArgs a) {
     extern __shared__ int plan_lds[];  // [waves][G] rows of the wave, then its next slot; [G] totals, tiles and items before
     const int G = a.adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
@@ -1161,7 +1171,7 @@ __device__ __forceinline__ void lora_finish(const LoraArgs& a, int r0, float (&t
     }
 }
 
-// An adapter's partial sums in order.
+// An adapter's partial sums in order (8192 x 4096, rank 32, both: 8.2 us).
 __device__ __forceinline__ void lora_reduce(const LoraArgs& a, int adapter) {
     const int items = a.per_adapter[2 * adapter];
     if (items < 2) return;

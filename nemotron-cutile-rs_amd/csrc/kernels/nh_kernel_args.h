@@ -541,6 +541,7 @@ struct LoraArgs {
     int32_t splits;          // parts of C that shrink sums apart
     int32_t per_wave;        // shrink: columns of C per wave, a multiple of 32
     int32_t columns;         // expand: columns of C per workgroup, a multiple of 256
+    int32_t numbered;        // a few rows: workgroups are for the 16s of rows in turn, not for a row each
     int32_t scaled;          // finish: times the adapter's scale
     int32_t accumulate;
 };

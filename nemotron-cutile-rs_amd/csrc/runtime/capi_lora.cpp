@@ -250,6 +250,7 @@ Lora make_lora(nh_context* ctx, const int32_t* ids, const float* scales, size_t 
     c.common.rank = (int)rank;
     c.common.rank_pad = (int)rank_pad(rank);
     c.common.adapters = (int)adapters;
+    c.common.numbered = few && few_units(m, adapters) < m;
     return c;
 }
 
