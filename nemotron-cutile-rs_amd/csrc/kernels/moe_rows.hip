@@ -161,7 +161,8 @@ __device__ __forceinline__ void scatter_rows(const MoeRowsArgs& a) {
         row_routes(a, t, j0, slot, w);
 #pragma unroll
         for (int j = 0; j < kRowRoutes; ++j) d[j] = 0.0f;
-        for (int c = V * threadIdx.x; c < H; c += V * blockDim.x) {
+        for (uint32_t u = V * threadIdx.x; u < (uint32_t)H; u += V * blockDim.x) {  // u may pass 2^31
+            const int c = (int)u;
             // rows_in may be rows_out: the thread's own values, read first
             if (a.dweights) row_dots<TOKEN, ROW, V>(a, a.tokens, t, c, slot, d);
             if (H - c >= V) {
@@ -202,12 +203,13 @@ __device__ __forceinline__ void gather_rows(const MoeRowsArgs& a) {
             row_routes(a, t, j0, slot, w);
 #pragma unroll
             for (int j = 0; j < kRowRoutes; ++j) d[j] = 0.0f;
-            for (int c = V * threadIdx.x; c < H; c += V * blockDim.x) row_dots<TOKEN, ROW, V>(a, a.dot, t, c, slot, d);
+            for (uint32_t u = V * threadIdx.x; u < (uint32_t)H; u += V * blockDim.x) row_dots<TOKEN, ROW, V>(a, a.dot, t, (int)u, slot, d);
             row_dweights(a, t, j0, d, red);
         }
     }
     row_routes(a, t, 0, slot, w);
-    for (int c = V * threadIdx.x; c < H; c += V * blockDim.x) {
+    for (uint32_t u = V * threadIdx.x; u < (uint32_t)H; u += V * blockDim.x) {  // u may pass 2^31
+        const int c = (int)u;
         float sum[V];
         const bool whole = H - c >= V;
 #pragma unroll
@@ -215,7 +217,7 @@ __device__ __forceinline__ void gather_rows(const MoeRowsArgs& a) {
         if (a.shared) {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (c + i < H) sum[i] = load_as_f32(a.shared, t * H + c + i, TOKEN);
+                if (i < H - c) sum[i] = load_as_f32(a.shared, t * H + c + i, TOKEN);
         }
         for (int j0 = 0; j0 < a.top_k; j0 += kRowRoutes) {
             if (a.top_k > kRowRoutes) row_routes(a, t, j0, slot, w);
@@ -235,7 +237,7 @@ __device__ __forceinline__ void gather_rows(const MoeRowsArgs& a) {
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (c + i < H) {
+                    if (i < H - c) {
 #pragma unroll
                         for (int j = 0; j < kRowRoutes; ++j)
                             if (slot[j] >= 0)
@@ -248,7 +250,7 @@ __device__ __forceinline__ void gather_rows(const MoeRowsArgs& a) {
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (c + i < H) store_out(a.out, t * H + c + i, sum[i], TOKEN);
+                if (i < H - c) store_out(a.out, t * H + c + i, sum[i], TOKEN);
         }
     }
 }
@@ -276,8 +278,9 @@ NH_ROWS_KERNELS(gather_rows, gather_rows)
 // experts, and place has read its part before it writes there.
 namespace {
 
-__device__ __forceinline__ void sort_chunk(const MoeSortArgs& a, int c, int& r0, int& r1) {
-    r0 = c * a.chunk;
+// (Sums of routes may pass 2^31.)
+__device__ __forceinline__ void sort_chunk(const MoeSortArgs& a, int c, uint32_t& r0, uint32_t& r1) {
+    r0 = (uint32_t)c * a.chunk;
     r1 = c == a.chunks - 1 ? a.routes : r0 + a.chunk;
 }
 
@@ -286,11 +289,11 @@ __device__ __forceinline__ void sort_chunk(const MoeSortArgs& a, int c, int& r0,
 extern "C" __global__ __launch_bounds__(1024) void nh_moe_sort_count_kernel(MoeSortArgs a) {
     extern __shared__ int sort_lds[];  // [E]
     const int E = a.experts;
-    int r0, r1;
+    uint32_t r0, r1;
     sort_chunk(a, blockIdx.x, r0, r1);
     for (int e = threadIdx.x; e < E; e += blockDim.x) sort_lds[e] = 0;
     __syncthreads();
-    for (int r = r0 + threadIdx.x; r < r1; r += blockDim.x) {
+    for (uint32_t r = r0 + threadIdx.x; r < r1; r += blockDim.x) {
         const int e = a.indices[r];
         if (e >= 0 && e < E) atomicAdd(&sort_lds[e], 1);
     }
@@ -364,14 +367,14 @@ extern "C" __global__ __launch_bounds__(1024) void nh_moe_sort_scan_kernel(MoeSo
 extern "C" __global__ __launch_bounds__(1024) void nh_moe_sort_place_kernel(MoeSortArgs a) {
     extern __shared__ int sort_lds[];  // [waves][E]: the wave's routes per expert, then its next slot
     const int E = a.experts, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    int c0, c1;
+    uint32_t c0, c1;
     sort_chunk(a, blockIdx.x, c0, c1);
-    const int per = ((c1 - c0 + waves - 1) / waves + 63) & ~63;
-    const int r0 = min(c1, c0 + wave * per), r1 = min(c1, r0 + per);
+    const uint32_t per = ((c1 - c0 + waves - 1) / waves + 63) & ~63u;
+    const uint32_t r0 = min(c1, c0 + wave * per), r1 = min(c1, r0 + per);
     int* mine = sort_lds + wave * E;
     for (int e = threadIdx.x; e < waves * E; e += blockDim.x) sort_lds[e] = 0;
     __syncthreads();
-    for (int r = r0 + lane; r < r1; r += 64) {
+    for (uint32_t r = r0 + lane; r < r1; r += 64) {
         const int e = a.indices[r];
         if (e >= 0 && e < E) atomicAdd(&mine[e], 1);
     }
@@ -387,8 +390,8 @@ extern "C" __global__ __launch_bounds__(1024) void nh_moe_sort_place_kernel(MoeS
     __syncthreads();
     int bits = 0;
     while ((1 << bits) < E) ++bits;
-    for (int base = r0; base < r1; base += 64) {  // uniform per wave
-        const int r = base + lane;
+    for (uint32_t base = r0; base < r1; base += 64) {  // uniform per wave
+        const uint32_t r = base + lane;
         int e = r < r1 ? a.indices[r] : -1;
         if (e >= E) e = -1;
         uint64_t same = __ballot(e >= 0);
@@ -401,6 +404,6 @@ extern "C" __global__ __launch_bounds__(1024) void nh_moe_sort_place_kernel(MoeS
         if (e >= 0 && lane == leader) slot = atomicAdd(&mine[e], __popcll(same));
         slot = __shfl(slot, leader, kWave) + __popcll(same & ((1ull << lane) - 1));
         if (r < r1) a.pos[r] = e >= 0 ? slot : -1;
-        if (e >= 0) a.perm[slot] = r;
+        if (e >= 0) a.perm[slot] = (int)r;
     }
 }

@@ -30,7 +30,7 @@ def read_ends(ctx, buf, rows, cols, n, dtype=np.uint16):
     return np.concatenate([get(ctx, buf, 0, (half, cols), dtype), get(ctx, buf, (rows - (n - half)) * cols * size, (n - half, cols), dtype)])
 
 
-@pytest.mark.parametrize("tokens,hidden", [((1 << 19) + 37, 4100), (3, (1 << 30) + 1)])
+@pytest.mark.parametrize("tokens,hidden", [((1 << 19) + 37, 4100), (3, (1 << 30) + 1), (1, (1 << 31) - 1)])
 def test_rows(ctx, free, tokens, hidden):  # noqa: F811
     note(f"far rows {tokens} x {hidden}")
     rng = np.random.default_rng(0)
@@ -57,7 +57,7 @@ def test_rows(ctx, free, tokens, hidden):  # noqa: F811
         assert near(read_ends(ctx, rows, tokens, hidden, n)[::-1], wn * v, 1)  # pos turns them round
     else:
         assert near(get(ctx, rows, 2 * hidden - 2000, (1, 1000), np.uint16), wn * v, 1)
-        assert (get(ctx, rows, rows.nbytes - 2000, 1000, np.uint16) == 0).all()
+        assert (get(ctx, rows, rows.nbytes - 4000, 1000, np.uint16) == 0).all()
     NH.call("nh_moe_combine_rows", ctx.handle, rows.ptr, NH.BF16, pos.ptr, None, x.ptr, *sizes, out.ptr, NH.BF16, None)
     ctx.synchronize()
     if n:
@@ -65,6 +65,35 @@ def test_rows(ctx, free, tokens, hidden):  # noqa: F811
         assert (get(ctx, out, (tokens // 2) * hidden * 2, hidden, np.uint16) == 0).all()
     else:
         assert near(get(ctx, out, out.nbytes - 2000, (1, 1000), np.uint16), (1 + wn) * v, 2)
+
+
+def test_dweights_of_the_longest_rows(ctx, free):  # noqa: F811
+    hidden = (1 << 31) - 1
+    note("far dweights")
+    rows, out = zeros(ctx, (1, hidden), np.uint16, free), zeros(ctx, (1, hidden), np.uint16, free)
+    for b, v in ((rows, 2.0), (out, 3.0)):
+        put(ctx, b, b.nbytes - 20, A.held(np.full(10, v), "bf16")[0])
+    pos, dw = ctx.upload(np.zeros(1, np.int32)), ctx.upload(np.zeros(1, np.float32))
+    NH.call("nh_moe_combine_rows_backward", ctx.handle, out.ptr, NH.BF16, rows.ptr, NH.BF16, pos.ptr, None, 1, 1, hidden, 1,
+            rows.ptr, dw.ptr, None)
+    assert dw.numpy()[0] == 60.0  # exact in f32
+    assert np.array_equal(get(ctx, rows, rows.nbytes - 40, 20, np.uint16), get(ctx, out, out.nbytes - 40, 20, np.uint16))
+
+
+def test_sort_of_the_most_routes(ctx, free):  # noqa: F811
+    n = (1 << 31) - 1
+    note("far sort")
+    ids, perm, pos = [zeros(ctx, (n,), np.int32, free) for _ in range(3)]
+    offsets = ctx.upload(np.full(4, -7, np.int32))
+    put(ctx, ids, 4 * (n - 5), np.array([2, 9, 1, -1, 0], np.int32))
+    NH.call("nh_moe_permute", ctx.handle, ids.ptr, n, 1, 3, offsets.ptr, perm.ptr, pos.ptr, None)
+    ctx.synchronize()
+    assert offsets.numpy().tolist() == [0, n - 4, n - 3, n - 2]
+    assert get(ctx, perm, 4 * (n - 7), 5, np.int32).tolist() == [n - 7, n - 6, n - 1, n - 3, n - 5]
+    assert get(ctx, pos, 4 * (n - 7), 7, np.int32).tolist() == [n - 7, n - 6, n - 3, -1, n - 4, -1, n - 5]
+    for at in (0, 12345678, 1 << 30, (1 << 31) - (1 << 23) - 3):  # chunk ends among them
+        assert np.array_equal(get(ctx, pos, 4 * at, 70, np.int32), np.arange(at, at + 70))
+        assert np.array_equal(get(ctx, perm, 4 * at, 70, np.int32), np.arange(at, at + 70))
 
 
 @pytest.mark.parametrize("m,n,k,adapters", [((1 << 20) + 75, 2100, 2056, 2), (2100, 1 << 20, 72, 3), (2100, 72, 1 << 20, 3)])
