@@ -12,9 +12,10 @@
 // run on the bf16 matrix cores: an f32 low-rank value is cut into three bf16
 // parts of eight significant bits each (by truncation, so v = hi + mid + lo
 // exactly while lo is normal), whose products with bf16 are exact in the f32
-// sums; bf16 results take the first two parts (off by under 2^-15 of a term, 2^-7 of
-// the result's own rounding).  Otherwise the f32 matrix cores take every value as
-// it is.  Every sum has a fixed order: results do not change from run to run.
+// sums.  All three go in, whatever the result's type: where terms or the base cancel,
+// what two parts leave out (2^-15 of a term) is more than a bf16 result's own
+// rounding.  Otherwise the f32 matrix cores take every value as it is.  Every sum
+// has a fixed order: results do not change from run to run.
 //
 // A row's products see its own values only; what stands in rows without an
 // adapter, or in another adapter's matrices, reaches no other row.
@@ -405,7 +406,7 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
 template <class Frag, int RT, int OUT>
 struct ExpandForm {
     static constexpr int KC = (RT + 1) / 2, ranks = 32 * KC;  // steps of 32 ranks
-    static constexpr int parts = !Frag::bf16 ? 1 : OUT == DT_BF16 ? 2 : 3;
+    static constexpr int parts = Frag::bf16 ? 3 : 1;
     static constexpr int PT = 4, step = 16 * PT;
     // base and out go by units of 16 bytes, `lanes` of them a row of a step
     static constexpr int values = OUT == DT_BF16 ? 8 : 4, lanes = step / values, units = 16 * lanes / 64;

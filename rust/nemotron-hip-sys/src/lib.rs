@@ -1606,8 +1606,8 @@ extern "C" {
     /// dispatched rows and adapter_ids their experts. Products of bf16 values are exact; h and every sum
     /// are f32, of a fixed order: results do not change from run to run. The order depends on m and on how
     /// many rows share an adapter, so a row's last bits may differ between batches. Where the matrices are
-    /// bf16, B_l's products take h in bf16 parts of 16 significant bits (24 for an f32 out); an infinity in
-    /// B_l then makes its outputs infinite or NaN. Operands start at any address of their element type. The
+    /// bf16, B_l's products take h in three bf16 parts that make all of it up; an infinity in B_l then
+    /// makes its outputs infinite or NaN. Operands start at any address of their element type. The
     /// workspace (nh_linear_lora_workspace_size bytes, 16-byte aligned) is free again once the call has
     /// run; calls that may run at once need one each. Errors: INVALID_SHAPE (n, k, rank or adapters == 0),
     /// INVALID_ROW_COUNT (m == 0), INVALID_PARAMS (dtype, a null operand, an output over an operand but for
