@@ -666,7 +666,7 @@ nh_status nh_moe_combine_rows_backward_host(const void *dout, nh_dtype out_dtype
  * results do not change from run to run.  The order depends on m and on how many
  * rows share an adapter, so a row's last bits may differ between batches.  Where
  * the matrices are bf16, B_l's products take h in three bf16 parts that make all of
- * it up; an infinity in B_l then makes its outputs infinite or NaN.
+ * it up.  Infinities and NaN come out as the formulas have them.
  * Operands start at any address of their element type.  The workspace
  * (nh_linear_lora_workspace_size bytes, 16-byte aligned) is free again once the
  * call has run; calls that may run at once need one each.  Errors: INVALID_SHAPE
@@ -690,8 +690,7 @@ nh_status nh_linear_lora(nh_context *ctx, const void *x, nh_dtype x_dtype, const
  * db), a (dx, db without h) and b (dx, da) may be NULL where nothing asks for
  * them.  h is nh_linear_lora's h_out, or NULL: computed again (for db).  With
  * accumulate != 0 da and db are added to; otherwise adapters without rows get
- * zeros.  dx takes dh as out takes h.  An infinity in x or dout makes its adapter's
- * da and db infinite or NaN.
+ * zeros.  dx takes dh as out takes h, and so do da and db.
  * Workspace nh_linear_lora_backward_workspace_size bytes, errors as above (dx on
  * dx_base alone may overlap). */
 size_t nh_linear_lora_backward_workspace_size(size_t m, size_t n, size_t k, size_t rank, size_t adapters);

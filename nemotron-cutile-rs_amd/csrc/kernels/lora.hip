@@ -94,6 +94,43 @@ __device__ __forceinline__ v4f mma(const Frag32& a, const Frag32& b, v4f acc) {
     return acc;
 }
 
+// acc of products with the parts of h after the first, which are zero where few bits or
+// no finite value are left: beside an infinity they say NaN.  An operand that is not
+// finite makes the first part's product infinite or NaN as the formula has it (only
+// values under 2^-133 have no first part), so what comes ahead of it is held finite
+// (med3 of a NaN is the least of the others).
+__device__ __forceinline__ v4f held_finite(v4f acc) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = __builtin_amdgcn_fmed3f(acc[i], -3.402823466e38f, 3.402823466e38f);
+    return acc;
+}
+
+// The same where the sum goes on: operands for those parts, with zeros for what is not finite.
+__device__ __forceinline__ Frag16 finite_values(const Frag16& f) {
+    Frag16 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t u = (uint32_t)f.v[i], e = u & 0x7f807f80u;
+        const uint32_t lo = (e & 0xffffu) == 0x7f80u ? 0u : u, hi = e >> 16 == 0x7f80u ? 0u : u;
+        r.v[i] = (int)((lo & 0xffffu) | (hi & 0xffff0000u));
+    }
+    return r;
+}
+__device__ __forceinline__ const Frag32& finite_values(const Frag32& f) { return f; }
+
+// The sum of w h over K, of h's parts the small ones first.
+template <class Frag, int KC, int PARTS>
+__device__ __forceinline__ v4f mma_parts(const Frag (&w)[KC], const Frag (&h)[KC][PARTS]) {
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = PARTS - 1; s >= 0; --s) {
+#pragma unroll
+        for (int q = 0; q < KC; ++q) acc = mma(w[q], h[q][s], acc);
+        if (s == 1) acc = held_finite(acc);
+    }
+    return acc;
+}
+
 // A block of bf16 rows in LDS, `pitch` values from one to the next, as operands
 // whose K runs down the rows: lane l gets rows 8 (l / 16) .. + 7 of column
 // col(l % 16).  A transposing read gives each of 16 lanes four rows of its column,
@@ -118,16 +155,18 @@ __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// The next bf16 part of v, which keeps the rest.  A value that is not finite is its
-// first part, with zeros behind.
-__device__ __forceinline__ uint32_t bf16_part(float& v) {
-    const uint32_t u = f32_bits(v);
-    if ((u & 0x7f800000u) == 0x7f800000u) {
-        v = 0.0f;
-        return (u >> 16) | ((u & 0x7fffffu) ? 0x40u : 0u);
-    }
-    v = v - f32_from_bits(u & 0xffff0000u);  // exact
-    return u >> 16;
+// The three bf16 parts of two values, a pair a part.  A value that is not finite is its
+// first part, with zeros behind (canonical: a NaN's upper half is one as well).
+__device__ __forceinline__ void bf16_parts(float a, float b, uint32_t (&parts)[3]) {
+    auto pair = [](float lo, float hi) { return f32_bits(lo) >> 16 | (f32_bits(hi) & 0xffff0000u); };
+    auto rest = [](float v) { return v - f32_from_bits(f32_bits(v) & 0xffff0000u); };  // exact
+    a = __builtin_canonicalizef(a);
+    b = __builtin_canonicalizef(b);
+    parts[0] = pair(a, b);
+    a = __builtin_isfinite(a) ? rest(a) : 0.0f;
+    b = __builtin_isfinite(b) ? rest(b) : 0.0f;
+    parts[1] = pair(a, b);
+    parts[2] = pair(rest(a), rest(b));
 }
 
 // ---- the rows of a workgroup ---------------------------------------------------
@@ -508,12 +547,12 @@ __device__ __forceinline__ void lora_values(const LoraArgs& a, int row, float sc
         }
         if constexpr (Frag::bf16) {
 #pragma unroll
-            for (int s = 0; s < PARTS; ++s)
+            for (int i = 0; i < 4; ++i) {
+                uint32_t parts[3];
+                bf16_parts(v[2 * i], v[2 * i + 1], parts);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t lo = bf16_part(v[2 * i]), hi = bf16_part(v[2 * i + 1]);
-                    h[q][s].v[i] = (int)(lo | (hi << 16));
-                }
+                for (int s = 0; s < PARTS; ++s) h[q][s].v[i] = (int)parts[s];
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[q][0].v[i] = v[i];
@@ -632,7 +671,6 @@ __device__ __forceinline__ void lora_products(const uint8_t* block, const Frag (
     const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
 #pragma unroll
     for (int p = 0; p < F::PT; ++p) {
-        acc[p] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         Frag w[F::KC];
 #pragma unroll
         for (int q = 0; q < F::KC; ++q) {
@@ -646,10 +684,7 @@ __device__ __forceinline__ void lora_products(const uint8_t* block, const Frag (
                 *(float4*)&w[q].v[4] = *(const float4*)(s + 4);
             }
         }
-#pragma unroll
-        for (int s = F::parts - 1; s >= 0; --s)  // the small parts first
-#pragma unroll
-            for (int q = 0; q < F::KC; ++q) acc[p] = mma(w[q], h[q][s], acc[p]);
+        acc[p] = mma_parts(w, h);
     }
 }
 
@@ -691,13 +726,7 @@ __device__ __forceinline__ void lora_expand_few(const LoraArgs& a, const int* ro
     for (int c = c0; c < c1; c += 4 * F::step) {
         v4f acc[F::PT];
 #pragma unroll
-        for (int p = 0; p < F::PT; ++p) {
-            acc[p] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int s = F::parts - 1; s >= 0; --s)  // the small parts first
-#pragma unroll
-                for (int q = 0; q < F::KC; ++q) acc[p] = mma(w[p][q], h[q][s], acc[p]);
-        }
+        for (int p = 0; p < F::PT; ++p) acc[p] = mma_parts(w[p], h);
         v4u x[F::units];
 #pragma unroll
         for (int u = 0; u < F::units; ++u) x[u] = base[u];
@@ -892,10 +921,6 @@ __device__ __forceinline__ void lora_outer(const LoraArgs& a, int number, int nu
     if (first >= a.C) return;
     const int c0 = (int)first;
     v4f acc[CT][RT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) acc[c][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     const int64_t s0 = (int64_t)tile * kTileRows, s1 = s0 + (int64_t)tiles * kTileRows;
     uint16_t* block = blocks + (Frag::bf16 ? wave * 32 * 64 : 0);
     // bf16: a lane loads eight columns of four rows
@@ -915,41 +940,63 @@ __device__ __forceinline__ void lora_outer(const LoraArgs& a, int number, int nu
             ahead[i] = v.v;
         }
     };
-    if constexpr (Frag::bf16) load_rows32(s0);
-    for (int64_t s = s0; s < s1; s += 32) {
-        const int64_t at = s + 8 * g;
-        Frag x[CT], h[RT][PARTS];
+    auto sum = [&](auto careful) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int c = 0; c < CT; ++c)
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-                load8(a.ht, ((s / 32 * PARTS + p) * RT + r) * 512 + 8 * lane, DT_F32, h[r][p]);
-        if constexpr (Frag::bf16) {
+            for (int r = 0; r < RT; ++r) acc[c][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (Frag::bf16) load_rows32(s0);
+        for (int64_t s = s0; s < s1; s += 32) {
+            const int64_t at = s + 8 * g;
+            Frag x[CT], h[RT][PARTS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) *(v4i*)(block + (8 * i + (lane >> 3)) * 64 + 8 * (lane & 7)) = ahead[i];
-            wave_lds_sync();
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int c = 0; c < CT; ++c) load_rows(block, 64, [&](int i) { return 16 * c + i; }, x[c]);
-            if (s + 32 < s1) load_rows32(s + 32);
-        } else {
-            int row[8];
+                for (int p = 0; p < PARTS; ++p)
+                    load8(a.ht, ((s / 32 * PARTS + p) * RT + r) * 512 + 8 * lane, DT_F32, h[r][p]);
+            if constexpr (Frag::bf16) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) row[i] = a.slot_row[at + i];
+                for (int i = 0; i < 4; ++i) *(v4i*)(block + (8 * i + (lane >> 3)) * 64 + 8 * (lane & 7)) = ahead[i];
+                wave_lds_sync();
+#pragma unroll
+                for (int c = 0; c < CT; ++c) load_rows(block, 64, [&](int i) { return 16 * c + i; }, x[c]);
+                if (s + 32 < s1) load_rows32(s + 32);
+            } else {
+                int row[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) row[i] = a.slot_row[at + i];
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const int col = min(c0 + 16 * c + l16, a.C - 1);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        x[c].v[i] = row[i] >= 0 ? load_as_f32(a.x, (int64_t)row[i] * a.C + col, a.x_dtype) : 0.0f;
+                }
+            }
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                const int col = min(c0 + 16 * c + l16, a.C - 1);
+                Frag rest = x[c];
+                if constexpr (careful.value) rest = finite_values(x[c]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    x[c].v[i] = row[i] >= 0 ? load_as_f32(a.x, (int64_t)row[i] * a.C + col, a.x_dtype) : 0.0f;
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; --p) {
+                        const Frag& v = p == 0 ? x[c] : rest;
+                        acc[c][r] = COLS ? mma(h[r][p], v, acc[c][r]) : mma(v, h[r][p], acc[c][r]);
+                    }
             }
         }
+    };
+    sum(No{});
+    if constexpr (Frag::bf16) {  // a sum that is not finite: again, with what is not finite in the first parts' products alone
+        bool fine = true;
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int p = PARTS - 1; p >= 0; --p)
-                    acc[c][r] = COLS ? mma(h[r][p], x[c], acc[c][r]) : mma(x[c], h[r][p], acc[c][r]);
+                for (int i = 0; i < 4; ++i) fine &= __builtin_isfinite(acc[c][r][i]);
+        if (__ballot(!fine)) sum(Yes{});  // uniform
     }
     const bool add = partial < 0 && a.accumulate;
     float* to = partial < 0 ? a.grad + (int64_t)adapter * a.rank * a.C : a.gpart + (int64_t)partial * a.rank * a.C;
@@ -1162,11 +1209,12 @@ __device__ __forceinline__ void lora_finish(const LoraArgs& a, int r0, float (&t
 #pragma unroll
     for (int i = 0; i < 4; ++i) u[i] = turned[rank][s4 + i];
     if (a.x_dtype == DT_BF16) {
+        uint32_t lo[3], hi[3];
+        bf16_parts(u[0], u[1], lo);
+        bf16_parts(u[2], u[3], hi);
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {
-            const uint32_t p0 = bf16_part(u[0]), p1 = bf16_part(u[1]), p2 = bf16_part(u[2]), p3 = bf16_part(u[3]);
-            *(uint2*)((uint16_t*)a.ht + ((block * 3 + q) * tiles + r0 / 16) * 512 + in) = make_uint2(p0 | (p1 << 16), p2 | (p3 << 16));
-        }
+        for (int q = 0; q < 3; ++q)
+            *(uint2*)((uint16_t*)a.ht + ((block * 3 + q) * tiles + r0 / 16) * 512 + in) = make_uint2(lo[q], hi[q]);
     } else {
         *(float4*)((float*)a.ht + (block * tiles + r0 / 16) * 512 + in) = make_float4(u[0], u[1], u[2], u[3]);
     }

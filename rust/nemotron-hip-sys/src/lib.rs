@@ -1606,10 +1606,10 @@ extern "C" {
     /// dispatched rows and adapter_ids their experts. Products of bf16 values are exact; h and every sum
     /// are f32, of a fixed order: results do not change from run to run. The order depends on m and on how
     /// many rows share an adapter, so a row's last bits may differ between batches. Where the matrices are
-    /// bf16, B_l's products take h in three bf16 parts that make all of it up; an infinity in B_l then
-    /// makes its outputs infinite or NaN. Operands start at any address of their element type. The
-    /// workspace (nh_linear_lora_workspace_size bytes, 16-byte aligned) is free again once the call has
-    /// run; calls that may run at once need one each. Errors: INVALID_SHAPE (n, k, rank or adapters == 0),
+    /// bf16, B_l's products take h in three bf16 parts that make all of it up. Infinities and NaN come out
+    /// as the formulas have them. Operands start at any address of their element type. The workspace
+    /// (nh_linear_lora_workspace_size bytes, 16-byte aligned) is free again once the call has run; calls
+    /// that may run at once need one each. Errors: INVALID_SHAPE (n, k, rank or adapters == 0),
     /// INVALID_ROW_COUNT (m == 0), INVALID_PARAMS (dtype, a null operand, an output over an operand but for
     /// out on base), LENGTH_MISMATCH "workspace", UNSUPPORTED outside nh_supports_linear_lora (m < 2^24, n
     /// and k <= 2^20, m n and m k < 2^40, rank <= 128, adapters <= 1024) or for a misaligned workspace. No
@@ -1657,9 +1657,8 @@ extern "C" {
     /// db may be NULL (not all), then it is not computed and x (da, db), a (dx, db without h) and b (dx,
     /// da) may be NULL where nothing asks for them. h is nh_linear_lora's h_out, or NULL: computed again
     /// (for db). With accumulate != 0 da and db are added to; otherwise adapters without rows get zeros. dx
-    /// takes dh as out takes h. An infinity in x or dout makes its adapter's da and db infinite or NaN.
-    /// Workspace nh_linear_lora_backward_workspace_size bytes, errors as above (dx on dx_base alone may
-    /// overlap).
+    /// takes dh as out takes h, and so do da and db. Workspace nh_linear_lora_backward_workspace_size
+    /// bytes, errors as above (dx on dx_base alone may overlap).
     pub fn nh_linear_lora_backward_workspace_size(
         m: usize,
         n: usize,
