@@ -289,7 +289,9 @@ nh_status nh_moe_route_softmax_topk_host(const float *scores, size_t scores_len,
                                          size_t top_k, int32_t *indices, size_t indices_len, float *weights,
                                          size_t weights_len, nh_error *err);
 /* R2: counts -> offsets[E+1] (exclusive scan), perm (slot -> route, stable
- * by route id inside an expert), pos (route -> slot). */
+ * by route id inside an expert), pos (route -> slot).  An id outside [0, E) is
+ * not placed (pos -1; the _host form: OUT_OF_RANGE).  pos may be indices itself;
+ * any other overlap of an output with another operand is INVALID_PARAMS. */
 nh_status nh_moe_permute(nh_context *ctx, const int32_t *indices, size_t tokens, size_t top_k, size_t experts,
                          int32_t *offsets, int32_t *perm, int32_t *pos, nh_stream stream, nh_error *err);
 nh_status nh_moe_permute_host(const int32_t *indices, size_t tokens, size_t top_k, size_t experts,

@@ -357,6 +357,9 @@ nh_status nh_moe_permute_host(const int32_t* indices, size_t tokens, size_t top_
     clear_error(err);
     if (experts == 0 || top_k == 0) return set_error(err, NH_INVALID_SHAPE, "experts and top_k must be non-zero");
     const size_t routes = tokens * top_k;
+    if (!apart({{offsets, (experts + 1) * 4}, {perm, routes * 4}, {pos, routes * 4}},
+               {{pos == indices ? nullptr : indices, routes * 4}}))
+        return set_error(err, NH_INVALID_PARAMS, "offsets, perm and pos must not overlap another operand, but for pos on indices as a whole");
     std::vector<int32_t> count(experts, 0);
     for (size_t r = 0; r < routes; ++r) {
         if (indices[r] < 0 || (size_t)indices[r] >= experts)

@@ -1115,6 +1115,9 @@ nh_status nh_moe_permute(nh_context* ctx, const int32_t* indices, size_t tokens,
     size_t routes;
     if (!mul_ok(tokens, top_k, &routes) || routes > (size_t)kMaxGrid || experts > 4096)
         return set_error(err, NH_UNSUPPORTED, "device permutation needs routes < 2^31 and experts <= 4096");
+    const bool in_place = pos == indices;
+    if (!apart({{offsets, (experts + 1) * 4}, {perm, routes * 4}, {pos, routes * 4}}, {{in_place ? nullptr : indices, routes * 4}}))
+        return set_error(err, NH_INVALID_PARAMS, "offsets, perm and pos must not overlap another operand, but for pos on indices as a whole");
     nh_status st = bind_device(ctx, err);
     if (st) return st;
     PermuteArgs a{indices, offsets, perm, pos, (int)routes, (int)experts};
@@ -1122,7 +1125,9 @@ nh_status nh_moe_permute(nh_context* ctx, const int32_t* indices, size_t tokens,
     // 4 M reads in all, with 16-byte aligned ids).  It takes 6.9 us for 4096 routes,
     // 8.5 for 8192, 14.4 for 16384 whatever the experts; the three launches over
     // chunks 12 for 8192 to 131072 of 128 experts.  Others, and 4096 experts' few,
-    // in one workgroup.
+    // in one workgroup, and so are ids that pos is to replace: it reads each before
+    // anything is written there, the other forms read them again or write counts first.
+    if (in_place) return launch(ctx, K_PERMUTE, 1, 1024, 2 * experts * sizeof(int), stream, a, err);
     if (routes <= 12288 && experts * routes <= ((size_t)1 << 22) && aligned16(indices))
         return launch(ctx, K_PERMUTE_EXPERT, (unsigned)experts, 256, 0, stream, a, err);
     const size_t chunk = sort_chunk(routes, experts);

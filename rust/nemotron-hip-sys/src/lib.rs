@@ -727,7 +727,9 @@ extern "C" {
     ) -> nh_status;
 
     /// R2: counts -> offsets[E+1] (exclusive scan), perm (slot -> route, stable by route id inside an
-    /// expert), pos (route -> slot).
+    /// expert), pos (route -> slot). An id outside [0, E) is not placed (pos -1; the _host form:
+    /// OUT_OF_RANGE). pos may be indices itself; any other overlap of an output with another operand is
+    /// INVALID_PARAMS.
     pub fn nh_moe_permute(
         ctx: *mut nh_context,
         indices: *const i32,
