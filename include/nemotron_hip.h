@@ -638,7 +638,7 @@ nh_status nh_moe_combine_rows_backward(nh_context *ctx, const void *dout, nh_dty
                                        nh_dtype rows_dtype, const int32_t *pos, const float *weights, size_t tokens,
                                        size_t top_k, size_t hidden, size_t slots, void *drows, float *dweights,
                                        nh_stream stream, nh_error *err);
-/* Host twins (sums in f64). */
+/* Host twins (sums in f64; any shape, the same operands refused). */
 nh_status nh_moe_dispatch_host(const void *x, nh_dtype x_dtype, const int32_t *pos, const float *weights, size_t tokens,
                                size_t top_k, size_t hidden, size_t slots, void *rows, nh_dtype rows_dtype,
                                nh_error *err);
@@ -701,7 +701,7 @@ nh_status nh_linear_lora_backward(nh_context *ctx, const void *x, nh_dtype x_dty
                                   const void *dout, nh_dtype dout_dtype, size_t m, size_t n, size_t k, size_t rank,
                                   size_t adapters, const void *dx_base, void *dx, float *da, float *db, int accumulate,
                                   void *workspace, size_t workspace_bytes, nh_stream stream, nh_error *err);
-/* Host twins (sums in f64, h rounded to f32), any shape. */
+/* Host twins (sums in f64, h rounded to f32; any shape, the same operands refused). */
 nh_status nh_linear_lora_host(const void *x, nh_dtype x_dtype, const int32_t *adapter_ids, const void *a, const void *b,
                               nh_dtype w_dtype, const float *scales, size_t m, size_t n, size_t k, size_t rank,
                               size_t adapters, const void *base, void *out, nh_dtype out_dtype, float *h_out,

@@ -3,7 +3,7 @@
 #include <exception>
 #include <vector>
 
-#include "../runtime/nh_runtime.h"
+#include "adapters_operands.h"
 
 using namespace nh;
 
@@ -102,7 +102,9 @@ nh_status nh_moe_dispatch_host(const void* x, nh_dtype x_dtype, const int32_t* p
     clear_error(err);
     nh_status st = check_rows(x_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
     if (st) return st;
-    if (tokens != 0 && slots != 0 && (st = check_given({x, pos, rows}, err))) return st;
+    if ((tokens != 0 && slots != 0 && (st = check_given({x, pos, rows}, err))) ||
+        (st = dispatch_apart(x, x_dtype, pos, weights, tokens, top_k, hidden, slots, rows, rows_dtype, err)))
+        return st;
     if (slots != 0) scatter(x, x_dtype, nullptr, rows, rows_dtype, pos, weights, tokens, top_k, hidden, slots, nullptr);
     return NH_OK;
 }
@@ -116,6 +118,8 @@ nh_status nh_moe_dispatch_backward_host(const void* drows, nh_dtype rows_dtype, 
     if (tokens != 0 && ((st = check_given({pos, dx}, err)) || (slots != 0 && (st = check_given({drows}, err))) ||
                         (dweights && (st = check_given({x}, err)))))
         return st;
+    if ((st = dispatch_backward_apart(drows, rows_dtype, x, x_dtype, pos, weights, tokens, top_k, hidden, slots, dx, dweights, err)))
+        return st;
     gather(drows, rows_dtype, nullptr, x, dx, x_dtype, pos, weights, tokens, top_k, hidden, slots, dweights);
     return NH_OK;
 }
@@ -127,6 +131,8 @@ nh_status nh_moe_combine_rows_host(const void* rows, nh_dtype rows_dtype, const 
     nh_status st = check_rows(out_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
     if (st) return st;
     if (tokens != 0 && ((st = check_given({pos, out}, err)) || (slots != 0 && (st = check_given({rows}, err))))) return st;
+    if ((st = combine_rows_apart(rows, rows_dtype, pos, weights, shared, tokens, top_k, hidden, slots, out, out_dtype, err)))
+        return st;
     gather(rows, rows_dtype, shared, nullptr, out, out_dtype, pos, weights, tokens, top_k, hidden, slots, nullptr);
     return NH_OK;
 }
@@ -140,6 +146,9 @@ nh_status nh_moe_combine_rows_backward_host(const void* dout, nh_dtype out_dtype
     if (tokens != 0 && ((st = check_given({dout, pos}, err)) || (slots != 0 && (st = check_given({drows}, err))) ||
                         (dweights && slots != 0 && (st = check_given({rows}, err)))))
         return st;
+    if ((st = combine_rows_backward_apart(dout, out_dtype, rows, rows_dtype, pos, weights, tokens, top_k, hidden, slots, drows,
+                                          dweights, err)))
+        return st;
     scatter(dout, out_dtype, rows, drows, rows_dtype, pos, weights, tokens, top_k, hidden, slots, dweights);
     return NH_OK;
 }
@@ -151,7 +160,8 @@ nh_status nh_linear_lora_host(const void* x, nh_dtype x_dtype, const int32_t* ad
     clear_error(err);
     nh_status st;
     if ((st = check_lora(m, n, k, rank, adapters, {x_dtype, w_dtype, out_dtype}, err)) ||
-        (st = check_given({x, adapter_ids, a, b, out}, err)))
+        (st = check_given({x, adapter_ids, a, b, out}, err)) ||
+        (st = lora_apart(x, x_dtype, adapter_ids, a, b, w_dtype, scales, m, n, k, rank, adapters, base, out, out_dtype, h_out, err)))
         return st;
     return guarded(err, [&]() -> nh_status {
         std::vector<float> h(rank);
@@ -191,7 +201,9 @@ nh_status nh_linear_lora_backward_host(const void* x, nh_dtype x_dtype, const in
     if (!dx && !da && !db) return set_error(err, NH_INVALID_PARAMS, "null operand");
     const bool again = db && !h;
     if (((da || again) && (st = check_given({x}, err))) || ((dx || again) && (st = check_given({a}, err))) ||
-        ((dx || da) && (st = check_given({b}, err))))
+        ((dx || da) && (st = check_given({b}, err))) ||
+        (st = lora_backward_apart(x, x_dtype, adapter_ids, a, b, w_dtype, scales, h, dout, dout_dtype, m, n, k, rank, adapters,
+                                  dx_base, dx, da, db, err)))
         return st;
     return guarded(err, [&]() -> nh_status {
         std::vector<double> ga(da ? rank * k : 0), gb(db ? rank * n : 0);

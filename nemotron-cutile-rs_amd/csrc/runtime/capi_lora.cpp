@@ -2,7 +2,7 @@
 #include <algorithm>
 #include <cstdint>
 
-#include "nh_runtime.h"
+#include "../host/adapters_operands.h"
 
 using namespace nh;
 
@@ -15,7 +15,6 @@ constexpr size_t kTileRows = 64;  // of the plan
 // and 19.1.
 constexpr size_t kFewRows = 64;
 
-size_t bytes_of(nh_dtype d) { return d == NH_BF16 ? 2 : 4; }
 int rank_form(size_t rank) { return rank <= 16 ? 0 : rank <= 32 ? 1 : rank <= 64 ? 2 : 3; }
 size_t rank_pad(size_t rank) { return (size_t)16 << rank_form(rank); }
 size_t most_tiles(size_t m, size_t adapters) { return m / kTileRows + std::min(m, adapters + 1); }
@@ -278,13 +277,9 @@ nh_status nh_linear_lora(nh_context* ctx, const void* x, nh_dtype x_dtype, const
     clear_error(err);
     nh_status st;
     if ((st = check_lora(m, n, k, rank, adapters, {x_dtype, w_dtype, out_dtype}, err)) ||
-        (st = check_given({x, adapter_ids, a, b, out}, err)))
+        (st = check_given({x, adapter_ids, a, b, out}, err)) ||
+        (st = lora_apart(x, x_dtype, adapter_ids, a, b, w_dtype, scales, m, n, k, rank, adapters, base, out, out_dtype, h_out, err)))
         return st;
-    const size_t out_bytes = m * n * bytes_of(out_dtype), matrix = adapters * rank * bytes_of(w_dtype);
-    if (!apart({{out, out_bytes}, {h_out, m * rank * 4}},
-               {{x, m * k * bytes_of(x_dtype)}, {base != out ? base : nullptr, out_bytes}, {adapter_ids, m * 4}, {a, matrix * k},
-                {b, matrix * n}, {scales, adapters * 4}}))
-        return set_error(err, NH_INVALID_PARAMS, "out and h_out must not overlap another operand, but for base as a whole");
     const Layout l = lora_layout(m, n, k, rank, adapters, false);
     if ((st = check_workspace(workspace, workspace_bytes, l.bytes, err)) || (st = bind_device(ctx, err))) return st;
     uint8_t* ws = (uint8_t*)workspace;
@@ -308,13 +303,10 @@ nh_status nh_linear_lora_backward(nh_context* ctx, const void* x, nh_dtype x_dty
     if (!dx && !da && !db) return set_error(err, NH_INVALID_PARAMS, "null operand");
     const bool again = db && !h;  // h is computed here
     if (((da || again) && (st = check_given({x}, err))) || ((dx || again) && (st = check_given({a}, err))) ||
-        ((dx || da) && (st = check_given({b}, err))))
+        ((dx || da) && (st = check_given({b}, err))) ||
+        (st = lora_backward_apart(x, x_dtype, adapter_ids, a, b, w_dtype, scales, h, dout, dout_dtype, m, n, k, rank, adapters,
+                                  dx_base, dx, da, db, err)))
         return st;
-    const size_t x_bytes = m * k * bytes_of(x_dtype), matrix = adapters * rank;
-    if (!apart({{dx, x_bytes}, {da, matrix * k * 4}, {db, matrix * n * 4}},
-               {{x, x_bytes}, {dx_base != dx ? dx_base : nullptr, x_bytes}, {dout, m * n * bytes_of(dout_dtype)}, {adapter_ids, m * 4},
-                {a, matrix * k * bytes_of(w_dtype)}, {b, matrix * n * bytes_of(w_dtype)}, {scales, adapters * 4}, {h, m * rank * 4}}))
-        return set_error(err, NH_INVALID_PARAMS, "dx, da and db must not overlap another operand, but for dx_base as a whole");
     const Layout l = lora_layout(m, n, k, rank, adapters, true);
     if ((st = check_workspace(workspace, workspace_bytes, l.bytes, err)) || (st = bind_device(ctx, err))) return st;
     uint8_t* ws = (uint8_t*)workspace;

@@ -2,13 +2,11 @@
 #include <algorithm>
 #include <cstdint>
 
-#include "nh_runtime.h"
+#include "../host/adapters_operands.h"
 
 using namespace nh;
 
 namespace {
-
-size_t bytes_of(nh_dtype d) { return d == NH_BF16 ? 2 : 4; }
 
 nh_status check_rows(nh_dtype token, nh_dtype row, size_t tokens, size_t top_k, size_t hidden, size_t slots,
                      nh_error* err) {
@@ -57,11 +55,9 @@ nh_status nh_moe_dispatch(nh_context* ctx, const void* x, nh_dtype x_dtype, cons
     nh_status st = check_rows(x_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
     if (st) return st;
     if (tokens != 0 && slots != 0 && (st = check_given({x, pos, rows}, err))) return st;
-    const size_t routes = tokens * top_k * 4;
-    if (!apart({{rows, slots * hidden * bytes_of(rows_dtype)}},
-               {{x, tokens * hidden * bytes_of(x_dtype)}, {pos, routes}, {weights, routes}}))
-        return set_error(err, NH_INVALID_PARAMS, "rows must not overlap another operand");
-    if ((st = bind_device(ctx, err))) return st;
+    if ((st = dispatch_apart(x, x_dtype, pos, weights, tokens, top_k, hidden, slots, rows, rows_dtype, err)) ||
+        (st = bind_device(ctx, err)))
+        return st;
     if (tokens == 0 || slots == 0) return NH_OK;
     MoeRowsArgs a{};
     a.tokens = x;
@@ -84,11 +80,10 @@ nh_status nh_moe_dispatch_backward(nh_context* ctx, const void* drows, nh_dtype 
     if (tokens != 0 && ((st = check_given({pos, dx}, err)) || (slots != 0 && (st = check_given({drows}, err))) ||
                         (dweights && (st = check_given({x}, err)))))
         return st;
-    const size_t token_bytes = tokens * hidden * bytes_of(x_dtype), routes = tokens * top_k * 4;
-    if (!apart({{dx, token_bytes}, {dweights, routes}},
-               {{drows, slots * hidden * bytes_of(rows_dtype)}, {dweights ? x : nullptr, token_bytes}, {pos, routes}, {weights, routes}}))
-        return set_error(err, NH_INVALID_PARAMS, "dx and dweights must not overlap another operand");
-    if ((st = bind_device(ctx, err))) return st;
+    if ((st = dispatch_backward_apart(drows, rows_dtype, x, x_dtype, pos, weights, tokens, top_k, hidden, slots, dx, dweights,
+                                      err)) ||
+        (st = bind_device(ctx, err)))
+        return st;
     if (tokens == 0) return NH_OK;
     MoeRowsArgs a{};
     a.rows_in = drows;
@@ -110,11 +105,9 @@ nh_status nh_moe_combine_rows(nh_context* ctx, const void* rows, nh_dtype rows_d
     nh_status st = check_rows(out_dtype, rows_dtype, tokens, top_k, hidden, slots, err);
     if (st) return st;
     if (tokens != 0 && ((st = check_given({pos, out}, err)) || (slots != 0 && (st = check_given({rows}, err))))) return st;
-    const size_t token_bytes = tokens * hidden * bytes_of(out_dtype), routes = tokens * top_k * 4;
-    if (!apart({{out, token_bytes}}, {{rows, slots * hidden * bytes_of(rows_dtype)}, {shared != out ? shared : nullptr, token_bytes},
-                                      {pos, routes}, {weights, routes}}))
-        return set_error(err, NH_INVALID_PARAMS, "out must not overlap another operand, but for shared as a whole");
-    if ((st = bind_device(ctx, err))) return st;
+    if ((st = combine_rows_apart(rows, rows_dtype, pos, weights, shared, tokens, top_k, hidden, slots, out, out_dtype, err)) ||
+        (st = bind_device(ctx, err)))
+        return st;
     if (tokens == 0) return NH_OK;
     MoeRowsArgs a{};
     a.rows_in = rows;
@@ -138,12 +131,10 @@ nh_status nh_moe_combine_rows_backward(nh_context* ctx, const void* dout, nh_dty
     if (tokens != 0 && ((st = check_given({dout, pos}, err)) || (slots != 0 && (st = check_given({drows}, err))) ||
                         (dweights && slots != 0 && (st = check_given({rows}, err)))))
         return st;
-    const size_t row_bytes = slots * hidden * bytes_of(rows_dtype), routes = tokens * top_k * 4;
-    if (!apart({{drows, row_bytes}, {dweights, routes}},
-               {{dout, tokens * hidden * bytes_of(out_dtype)}, {dweights && rows != drows ? rows : nullptr, row_bytes},
-                {pos, routes}, {weights, routes}}))
-        return set_error(err, NH_INVALID_PARAMS, "drows and dweights must not overlap another operand, but for rows as a whole");
-    if ((st = bind_device(ctx, err))) return st;
+    if ((st = combine_rows_backward_apart(dout, out_dtype, rows, rows_dtype, pos, weights, tokens, top_k, hidden, slots, drows,
+                                          dweights, err)) ||
+        (st = bind_device(ctx, err)))
+        return st;
     if (tokens == 0) return NH_OK;
     MoeRowsArgs a{};
     a.tokens = dout;

@@ -1540,7 +1540,7 @@ extern "C" {
         stream: nh_stream,
         err: *mut nh_error,
     ) -> nh_status;
-    /// Host twins (sums in f64).
+    /// Host twins (sums in f64; any shape, the same operands refused).
     pub fn nh_moe_dispatch_host(
         x: *const c_void,
         x_dtype: nh_dtype,
@@ -1695,7 +1695,7 @@ extern "C" {
         stream: nh_stream,
         err: *mut nh_error,
     ) -> nh_status;
-    /// Host twins (sums in f64, h rounded to f32), any shape.
+    /// Host twins (sums in f64, h rounded to f32; any shape, the same operands refused).
     pub fn nh_linear_lora_host(
         x: *const c_void,
         x_dtype: nh_dtype,
