@@ -10,14 +10,15 @@
 // dw = 0.  Slots that no route names are left as they were.
 //
 // Bound by the rows' bytes: each value of a row is read or written once, each of
-// a token once.  One workgroup per token, so that pos and the weights are
-// uniform and a weight's gradient is one sum of the workgroup; 16 bytes of a row
-// per thread and turn, all of a token's routes in flight, as many threads as take
+// a token once per eight routes, but for gather with dw, which goes over the rows
+// twice (for all dw first, then for out).  One workgroup per token, so that pos and
+// the weights are uniform and a weight's gradient is one sum of the workgroup; 16
+// bytes of a row per thread and turn, eight routes in flight, as many threads as take
 // the row in the fewest turns.  Rows of 64 MiB and more in all go past the caches,
 // which they would only sweep.  8192 x 2688 bf16, 6 routes each: dispatch (308 MB)
-// 55 us, 64 through the caches; combine (308 MB) 59, 86 so; combine backward with
-// the weights' gradients (573 MB) 108; dispatch backward 59: 5.2 to 5.6 TB/s, the
-// rate of a copy.
+// 55 us, 74 through the caches; combine (308 MB) 60, with a dispatch of the same rows
+// ahead of it 118 and 158 for the two; combine backward with dw (573 MB) 108; dispatch
+// backward 59: 5.2 to 5.6 TB/s, the rate of a copy; with dw 92.
 // Sums run in f32, over j in route order; results do not change from run to run.
 #include "nh_device.h"
 

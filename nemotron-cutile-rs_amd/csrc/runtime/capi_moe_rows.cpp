@@ -22,12 +22,19 @@ nh_status check_rows(nh_dtype token, nh_dtype row, size_t tokens, size_t top_k, 
 
 // One workgroup per token; 16 bytes of a row per thread and turn, as many threads
 // as take it in the fewest turns of at most 512.
+// Rows go past the caches from 64 MiB on, but for a gather with the weights' gradients,
+// which reads them twice.  Through them and past them, us, 2688 wide, 6 routes, bf16,
+// rows of 32, 64 and 264 MiB: dispatch 9.5, 8.6; 21, 15; 74, 56.  Combine 9.1, 9.8; 18.0,
+// 17.6; 63, 62, with the dispatch of the same rows 19, 18; 36, 33; 158, 118.  Combine
+// backward 21, 18; 35, 30; 124, 113.  Dispatch backward with the weights' gradients 15, 18;
+// 28, 31; 92, 111.
 nh_status launch_rows(nh_context* ctx, KernelId first, MoeRowsArgs a, nh_dtype token, nh_dtype row, size_t tokens,
                       nh_stream stream, nh_error* err) {
     const KernelId id = (KernelId)(first + (token == NH_BF16 ? 2 : 0) + (row == NH_BF16 ? 1 : 0));
     const size_t v = row == NH_BF16 ? 8 : 4, vectors = ((size_t)a.hidden + v - 1) / v, turns = (vectors + 511) / 512;
     a.threads = (int)(((vectors + turns - 1) / turns + 63) / 64 * 64);
-    a.far = tokens * (size_t)a.top_k * (size_t)a.hidden * bytes_of(row) >= ((size_t)64 << 20) ? 1 : 0;
+    const bool twice = first == K_MOE_GATHER && a.dweights;
+    a.far = !twice && tokens * (size_t)a.top_k * (size_t)a.hidden * bytes_of(row) >= ((size_t)64 << 20) ? 1 : 0;
     const size_t most = ((1ull << 32) - 1) / (size_t)a.threads;  // workgroups of a launch: fewer than 2^32 threads
     for (size_t t0 = 0; t0 < tokens; t0 += most) {
         a.token0 = (int64_t)t0;
