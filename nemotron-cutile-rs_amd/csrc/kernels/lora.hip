@@ -1181,7 +1181,7 @@ __device__ __forceinline__ void lora_finish(const LoraArgs& a, int r0, float (&t
     if (tile >= a.counts[0]) return;
     const int adapter = a.tile_adapter[tile];
     if (adapter == a.adapters) return;
-    const float scale = a.scaled && a.scales ? a.scales[adapter] : 1.0f;
+    const float scale = a.scales ? a.scales[adapter] : 1.0f;
     const int slot = threadIdx.x >> 2, r4 = 4 * (threadIdx.x & 3), row = a.slot_row[(int64_t)tile * kTileRows + slot];
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (row >= 0) {

@@ -490,8 +490,8 @@ struct MoeRowsArgs {
     int64_t token0;          // first token of this launch
     int64_t slots;
     int32_t top_k, hidden;
-    int32_t threads;         // blockDim
     int32_t far;             // 1: the rows go past the caches
+    int32_t pad_;
 };
 
 // The sort of many routes: see moe_rows.hip.
@@ -542,8 +542,8 @@ struct LoraArgs {
     int32_t per_wave;        // shrink: columns of C per wave, a multiple of 32
     int32_t columns;         // expand: columns of C per workgroup, a multiple of 256
     int32_t numbered;        // a few rows: workgroups are for the 16s of rows in turn, not for a row each
-    int32_t scaled;          // finish: times the adapter's scale
     int32_t accumulate;
+    int32_t pad_;
 };
 
 // The gradients' products, of dh with x (da) and of h with dout (db), in one launch:

@@ -23,8 +23,11 @@ size_t most_tiles(size_t m, size_t adapters) { return m / kTileRows + std::min(m
 size_t few_units(size_t m, size_t adapters) { return std::min(m, m / 16 + adapters + 1); }
 
 // How shrink cuts C: columns per wave (eight waves a workgroup), and parts, of which
-// there is more than one only while the CUs are not all busy: in 1, 2 and 4 parts 300
-// rows of 2701 -> 1999 take 22.5, 18.7 and 16.3 us.  A wave has 128 columns at least.
+// there is more than one only while the CUs are not all busy.  A wave has 128 columns at
+// least.  A few rows are a few workgroups: 16 rows of 21504, rank 64, take 40, 26, 22, 18,
+// 17 and 21 us in 1, 2, 4, 8, 16 and 32 parts, one row of 16384, rank 16, 17, 12, 9.9, 9.5,
+// 9.8, 9.8.  The plan's tiles gain to 4: 300 rows of 2701 -> 1999 bf16, rank 20, 24, 20, 18
+// and 18 in 1, 2, 4 and 8; 1024 rows of 4096, rank 32, 24, 23, 24, 24.
 constexpr size_t kShrinkWaves = 8;
 struct Split {
     size_t per_wave, parts;
@@ -41,15 +44,17 @@ Split shrink_split(size_t m, size_t adapters, size_t c) {
 
 // Columns that a workgroup of expand takes of a few rows, for about 768 workgroups:
 // each sums the low-rank values anew.  With 384, 768 and 1536 workgroups 48 rows of 64
-// adapters (4096 -> 16384, rank 16) take 14.7, 12.8 and 14.0 us, one row the same.
+// adapters (4096 -> 16384, rank 16) take 15.6, 12.8 and 14.0 us, 16 rows of them 10.5, 9.7
+// and 9.6, 64 rows of one adapter (4096 -> 21504, rank 64) 14.7, 15.8 and 15.8, one row the
+// same.
 size_t expand_columns(size_t m, size_t adapters, size_t c) {
     const size_t shares = std::max<size_t>(1, 768 / few_units(m, adapters));
     return std::max<size_t>(256, std::min<size_t>(2048, ((c + shares - 1) / shares + 255) / 256 * 256));
 }
 
-// Most tiles of an outer item: about 32 items of an evenly dealt batch (8192 rows of
-// 4096, rank 32: for 16, 32 and 64 items the products and the sums of parts take 59 +
-// 6, 41 + 8 and 48 + 12 us).
+// Most tiles of an outer item: about 32 items of an evenly dealt batch.  da and db of
+// 4096 -> 4096 in 16, 32 and 64 items, us: 4096 rows, rank 32, 53, 57, 71; 8192 rows, rank 8,
+// 86, 67, 75, rank 32 97, 83, 100, rank 64 121, 135, 163; 32768 rows, rank 16, 299, 230, 239.
 size_t item_tiles(size_t m) { return std::max<size_t>(1, (m / kTileRows + 31) / 32); }
 
 struct Layout {
@@ -172,7 +177,6 @@ struct Lora {
         a.C = (int)c;
         a.w_dtype = wd;
         a.out_dtype = od;
-        a.scaled = 1;
         const KernelId id = form(K_LORA_EXPAND, wd == NH_BF16, back);
         if (few) {
             const size_t columns = expand_columns(m, adapters, c);
@@ -204,7 +208,6 @@ struct Lora {
             a.part = const_cast<float*>(g[i].part);
             a.splits = (int)g[i].splits;
             a.ht = g[i].ht;
-            a.scaled = 1;
             a.x = g[i].x;
             a.x_dtype = g[i].dtype;
             a.gpart = g[i].gpart;

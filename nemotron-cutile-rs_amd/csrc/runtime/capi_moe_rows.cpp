@@ -32,13 +32,13 @@ nh_status launch_rows(nh_context* ctx, KernelId first, MoeRowsArgs a, nh_dtype t
                       nh_stream stream, nh_error* err) {
     const KernelId id = (KernelId)(first + (token == NH_BF16 ? 2 : 0) + (row == NH_BF16 ? 1 : 0));
     const size_t v = row == NH_BF16 ? 8 : 4, vectors = ((size_t)a.hidden + v - 1) / v, turns = (vectors + 511) / 512;
-    a.threads = (int)(((vectors + turns - 1) / turns + 63) / 64 * 64);
+    const size_t threads = ((vectors + turns - 1) / turns + 63) / 64 * 64;
     const bool twice = first == K_MOE_GATHER && a.dweights;
     a.far = !twice && tokens * (size_t)a.top_k * (size_t)a.hidden * bytes_of(row) >= ((size_t)64 << 20) ? 1 : 0;
-    const size_t most = ((1ull << 32) - 1) / (size_t)a.threads;  // workgroups of a launch: fewer than 2^32 threads
+    const size_t most = ((1ull << 32) - 1) / threads;  // workgroups of a launch: fewer than 2^32 threads
     for (size_t t0 = 0; t0 < tokens; t0 += most) {
         a.token0 = (int64_t)t0;
-        const nh_status st = launch(ctx, id, (unsigned)std::min(most, tokens - t0), (unsigned)a.threads, 0, stream, a, err);
+        const nh_status st = launch(ctx, id, (unsigned)std::min(most, tokens - t0), (unsigned)threads, 0, stream, a, err);
         if (st) return st;
     }
     return NH_OK;
