@@ -665,8 +665,8 @@ nh_status nh_moe_combine_rows_backward_host(const void *dout, nh_dtype out_dtype
  * adapters, x holds the dispatched rows and adapter_ids their experts.
  *
  * Products of bf16 values are exact; h and every sum are f32, of a fixed order:
- * results do not change from run to run.  The order depends on m and on how many
- * rows share an adapter, so a row's last bits may differ between batches.  Where
+ * results do not change from run to run.  The order depends on the whole batch (m,
+ * the adapters of all rows), so a row's last bits may differ between batches.  Where
  * the matrices are bf16, B_l's products take h in three bf16 parts that make all of
  * it up.  Infinities and NaN come out as the formulas have them.
  * Operands start at any address of their element type.  The workspace

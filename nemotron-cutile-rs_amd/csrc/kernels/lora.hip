@@ -440,8 +440,8 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& a) {
 // sum of shrink's parts in order, as an operand in registers.  Steps of 64 columns,
 // four MFMA tiles; the matrix goes through LDS and so do the products, so that every
 // load and store has neighbouring lanes side by side in a row.  Memory bounds it: 4096
-// rows -> 21504, rank 64, 93 us (3.8 TB/s; a plain copy by the same tiles and steps 77),
-// 8192 rows -> 4096, rank 32, 35 us (3.9 TB/s).
+// rows -> 21504, rank 64, 94 us (3.8 TB/s; a plain copy by the same tiles and steps 77),
+// 8192 rows -> 4096, rank 32, 36 us (3.7 TB/s).
 template <class Frag, int RT, int OUT>
 struct ExpandForm {
     static constexpr int KC = (RT + 1) / 2, ranks = 32 * KC;  // steps of 32 ranks
@@ -903,7 +903,7 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& a) {
 // gradient, the others a partial sum each.  A wave has 64 columns, 32 rows a step,
 // which bf16 takes through LDS; the next step's rows are on their way meanwhile.
 // Workgroups from the grid's end on write the zeros of adapters without rows.
-// Both sides of 8192 x 4096, rank 32: 41 us (134 MB of rows read once, 3.3 TB/s).
+// Both sides of 8192 x 4096, rank 32: 42 us (134 MB of rows read once, 3.2 TB/s).
 template <class Frag, int RT, bool COLS>
 __device__ __forceinline__ void lora_outer(const LoraArgs& a, int number, int numbers, uint16_t* blocks) {
     constexpr int PARTS = Frag::bf16 ? 3 : 1, CT = 4;
@@ -1033,8 +1033,9 @@ __device__ __forceinline__ void lora_outer(const LoraArgs& a, int number, int nu
 // rows.  A wave ranks 64 rows at a time among its rows of the same adapter by
 // ballots, and keeps the ranks of up to 512 rows; of more rows they are found
 // again.  Then tiles, and items of up to item_tiles of them.  One CU's instructions
-// bound it: 300 rows 4.2 us, 4096 8.8, 8192 10.9; two launches of many workgroups would
-// start twice.
+// bound it: 300 rows 4.2 us, 4096 8.7, 8192 11.2, where two launches of many workgroups
+// would start twice; past those, with the calls around it, 16384 rows 49 of mixed ids and
+// 29 in runs, 49152 115 and 58.
 extern "C" __global__ __launch_bounds__(1024) void nh_lora_plan_kernel(LoraPlanArgs a) {
     extern __shared__ int plan_lds[];  // [waves][G] rows of the wave, then its next slot; [G] totals, tiles and items before
     const int G = a.adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
@@ -1220,7 +1221,7 @@ __device__ __forceinline__ void lora_finish(const LoraArgs& a, int r0, float (&t
     }
 }
 
-// An adapter's partial sums in order (8192 x 4096, rank 32, both: 8.2 us).
+// An adapter's partial sums in order (8192 x 4096, rank 32, both: 8.4 us).
 __device__ __forceinline__ void lora_reduce(const LoraArgs& a, int adapter) {
     const int items = a.per_adapter[2 * adapter];
     if (items < 2) return;

@@ -274,7 +274,7 @@ NH_ROWS_KERNELS(gather_rows, gather_rows)
 //   scan:  one workgroup turns them into each chunk's first slot per expert;
 //   place: the chunk's waves take consecutive routes; a wave's 64 routes at a time
 //          find their rank among the equal ones by ballots.
-// 49152 routes to 128 experts: 4.8 us each, where one workgroup took 185 for all.
+// 49152 routes to 128 experts: 4.8 us each alone, 10.5 for the three, 185 in one workgroup.
 // pos is its own workspace: a chunk has at least as many routes as there are
 // experts, and place has read its part before it writes there.
 namespace {

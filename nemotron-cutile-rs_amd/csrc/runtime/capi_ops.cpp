@@ -1123,8 +1123,8 @@ nh_status nh_moe_permute(nh_context* ctx, const int32_t* indices, size_t tokens,
     PermuteArgs a{indices, offsets, perm, pos, (int)routes, (int)experts};
     // Few routes: one workgroup per expert that reads all of them (and stays within
     // 4 M reads in all, with 16-byte aligned ids).  It takes 6.9 us for 4096 routes,
-    // 8.5 for 8192, 14.4 for 16384 whatever the experts; the three launches over
-    // chunks 12 for 8192 to 131072 of 128 experts.  Others, and 4096 experts' few,
+    // 8.5 for 8192, 11.0 for 12288, 14.4 for 16384 whatever the experts; the three
+    // launches over chunks 10 to 13 for 12600 to 120000 of 128 experts.  Others, and 4096 experts' few,
     // in one workgroup, and so are ids that pos is to replace: it reads each before
     // anything is written there, the other forms read them again or write counts first.
     if (in_place) return launch(ctx, K_PERMUTE, 1, 1024, 2 * experts * sizeof(int), stream, a, err);

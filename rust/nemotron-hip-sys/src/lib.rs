@@ -1606,12 +1606,12 @@ extern "C" {
     /// itself may be base. Rows without an adapter get their base. h_out, f32 [m][rank], receives h for the
     /// backward pass (0 in rows without an adapter) unless it is NULL. For experts' adapters, x holds the
     /// dispatched rows and adapter_ids their experts. Products of bf16 values are exact; h and every sum
-    /// are f32, of a fixed order: results do not change from run to run. The order depends on m and on how
-    /// many rows share an adapter, so a row's last bits may differ between batches. Where the matrices are
-    /// bf16, B_l's products take h in three bf16 parts that make all of it up. Infinities and NaN come out
-    /// as the formulas have them. Operands start at any address of their element type. The workspace
-    /// (nh_linear_lora_workspace_size bytes, 16-byte aligned) is free again once the call has run; calls
-    /// that may run at once need one each. Errors: INVALID_SHAPE (n, k, rank or adapters == 0),
+    /// are f32, of a fixed order: results do not change from run to run. The order depends on the whole
+    /// batch (m, the adapters of all rows), so a row's last bits may differ between batches. Where the
+    /// matrices are bf16, B_l's products take h in three bf16 parts that make all of it up. Infinities and
+    /// NaN come out as the formulas have them. Operands start at any address of their element type. The
+    /// workspace (nh_linear_lora_workspace_size bytes, 16-byte aligned) is free again once the call has
+    /// run; calls that may run at once need one each. Errors: INVALID_SHAPE (n, k, rank or adapters == 0),
     /// INVALID_ROW_COUNT (m == 0), INVALID_PARAMS (dtype, a null operand, an output over an operand but for
     /// out on base), LENGTH_MISMATCH "workspace", UNSUPPORTED outside nh_supports_linear_lora (m < 2^24, n
     /// and k <= 2^20, m n and m k < 2^40, rank <= 128, adapters <= 1024) or for a misaligned workspace. No
